@@ -540,6 +540,55 @@ int vybdq_moe_forward_exl3(uint64_t x, int x_dt, uint64_t logits, int logits_dt,
 int vybdq_quant_q8_act(uint64_t X, uint64_t Xq, uint64_t Xs, int64_t M, int64_t K, int x_dt,
                        uint64_t stream);
 
+/* ---- key/value cache in 8 bits: append and attention --------------------------------------- */
+
+/* The cache of one layer, in pages of `page` consecutive tokens of one sequence (a power of two in 16 .. 256), for
+   each of Hkv heads of D = 64, 128, 192 or 256 dims; codes are e4m3 (OCP, no infinities):
+     K  [n_pages][Hkv][page][D]         V  [n_pages][Hkv][page / 4][D][4] (slot s, dim d at [s / 4][d][s % 4])
+     Ks, Vs float32 [n_pages][Hkv]      powers of two; value = code * scale
+   The batch, read on the device (calls can be captured; the tables may change between replays): sequence b < B has
+   rows q_start[b] .. q_start[b + 1] - 1 (int32 [B + 1], rising, within 0 .. T) of k, v and q; they are the last of its
+   ctx[b] tokens (int32 [B]); table int32 [B][W] names the page of its tokens i page .. i page + page - 1. The pages
+   that a call appends to must differ between sequences; pages that are only read may be shared.
+   max_new and max_ctx are the caller's bounds on a sequence's rows and tokens (0: unknown). They choose the launch
+   shape; results are right for any value, but for vybdq_kv_attn's last bits (the split of the keys).
+   What the device finds wrong with the tables is skipped, or NaN in the outputs concerned, and reported by the next
+   vybdq_kv_status(); nothing outside the cache and the outputs is read or written whatever they hold.
+
+   vybdq_kv_append: writes the rows' keys and values to the cache, k rotated to its token's position, and the rotated q
+   (or q = 0) to q_out [T][Hq][D]. k, v, q: x_dt (F32, F16 or BF16), row strides ldk, ldv, ldq in elements (heads of a row
+   consecutive: slices of one q|k|v projection's output). Rotation of the first R dims (R % 16 == 0, 0: none) by
+   cos, sin float32 [n_pos][R / 2], row = the token's position: pairs (i, i + R / 2), or (2 i, 2 i + 1) with
+   interleaved; float32, each product and sum rounded once. A page's scale is 2^e with the least e that holds its
+   values (|y| <= 448 * 2^e, e in [-60, 60]); code = y / scale to nearest, ties to even. Rows that begin inside a page keep
+   its earlier tokens: e then does not shrink, and where it grows their codes are rounded anew to the larger scale.
+   Slots behind the last row stay as they are. A token with an infinity or NaN in a head's rotated k or its v is stored
+   so that exactly the attention rows that see it are NaN. K, V, cos, sin, q_out and every row 16-byte aligned. */
+int vybdq_kv_append(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs, int64_t n_pages, int64_t Hkv, int64_t D, int64_t page,
+                    uint64_t k, uint64_t v, uint64_t q, uint64_t q_out, int x_dt, int64_t ldk, int64_t ldv, int64_t ldq,
+                    int64_t Hq, uint64_t cos, uint64_t sin, int64_t R, int64_t n_pos, int interleaved, uint64_t table,
+                    int64_t W, uint64_t q_start, uint64_t ctx, int64_t T, int64_t B, int64_t max_new, uint64_t stream);
+
+/* Workspace bytes that vybdq_kv_attn splits keys in, for any batch at this D; -1 for an unsupported D. */
+int64_t vybdq_kv_attn_workspace_size(int64_t D);
+
+/* out [T][Hq][D] = softmax over the keys j that row i of its sequence sees of (scale q_i . k_j), times v_j; query head h
+   reads key head h / (Hq / Hkv). With p_i = ctx - rows + i the row's position, it sees j < ctx, j <= p_i if causal, and
+   j > p_i - window if window > 0. A row that sees nothing is 0, with lse -infinity. lse (float32 [T][Hq], or 0): the natural
+   log of the sum of exp(scale q . k). q, out: x_dt, q's row stride ldq. Softmax and sums are float32 in one pass;
+   operands are fp16 (codes exactly; q scaled by a power of two per row; float32 q and its weights in two fp16 terms).
+   ws: 256-byte aligned, of vybdq_kv_attn_workspace_size(D) bytes, zero-filled once before the first call (arrival
+   counters that every completed call leaves at zero); a smaller one splits less, 0 not at all. Calls that share a
+   workspace must not overlap. One launch. */
+int vybdq_kv_attn(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs, int64_t n_pages, int64_t Hkv, int64_t D, int64_t page,
+                  uint64_t q, int x_dt, int64_t ldq, int64_t Hq, uint64_t out, uint64_t lse, uint64_t table, int64_t W,
+                  uint64_t q_start, uint64_t ctx, int64_t T, int64_t B, int64_t max_new, int64_t max_ctx, double scale,
+                  int causal, int64_t window, uint64_t ws, int64_t ws_bytes, uint64_t stream);
+
+/* Synchronises the current device, then returns 0 or the error of a batch whose tables were wrong (rows, ctx, pages,
+   positions) in vybdq_kv_append or vybdq_kv_attn since the previous call on this device, and clears it. */
+int vybdq_kv_status(void);
+
 #ifdef __cplusplus
 }
 #endif

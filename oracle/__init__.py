@@ -33,6 +33,8 @@ repository root):
                             grid as native/gguf/iq2s_tables.py holds it
   producers RMSNorm / SwiGLU with the q8 copy (rms_blkg VYB_RMSQ8, silu32q VYB_SWQ8)
                             native/kernels/layer.vyb:989-1066,1551-1590, vmath.vyb:7-40
+  kvcache  the paged 8-bit key/value cache: append with rotation, attention (this library's own
+           format, include/vybdq.h; no counterpart in the reference)
 
 Pinning (what checks each function, all under tests/):
   q4_0 decode      the reference's frozen GGUF fixture block (interleaved order) and
@@ -68,5 +70,8 @@ Pinning (what checks each function, all under tests/):
                    rational sums; the reference's exp within its stated 1e-9 of libm;
                    RMSNorm closed form; the q8 copy is xq8
                    (tests/test_producers_oracle.py).                     -> pinned
+  kvcache          e4m3 against torch's conversions, scales and rotation against their
+                   formulas, attention against torch in float64
+                   (tests/test_kvcache_oracle.py).                       -> pinned
 Every function above is pinned; none is "parity unpinned".
 """

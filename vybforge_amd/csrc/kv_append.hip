@@ -1,0 +1,435 @@
+// Appending keys and values to the paged 8-bit cache (layout: kv.h), with the position rotation of q and k on
+// the way, gfx950.
+//
+//   y_a = x_a c - x_b s, y_b = x_b c + x_a s   for the pairs (a, b) of the first R dims: (i, i + R / 2), or
+//     (2 i, 2 i + 1) interleaved; c, s = cos, sin [position][i], float32. Contraction is off: every product and
+//     sum rounds once to float32, so codes do not depend on how a compiler fuses them.
+//   e = the least integer with amax <= 448 * 2^e over a page's new tokens of one head (k rotated), in
+//     [-60, 60]; where the page keeps earlier tokens, at least its old e. scale = 2^e, code = e4m3(y * 2^-e),
+//     ties to even. If e grows, the kept codes become e4m3(code * 2^(e_old - e)): a change of exponent, exact but
+//     for values that fall among e4m3's subnormals (below 2^-15 of the page's largest), which is why the scale
+//     is a power of two.
+// A token of which a rotated k or a v of a head is an infinity or NaN gets codes that no finite token has there:
+// k NaN, v zero. Its score is then NaN for the rows that see it, and a row that does not see it multiplies zeros.
+//
+// One workgroup per (page that a sequence's rows reach, key/value head): it alone writes that page's codes and
+// scales, reads the new k and v for the largest magnitude, then reads them again (from L2) to write codes, and
+// rotates the query heads of its key head for the same tokens. A page of 64 tokens of 8 heads of 128 (bf16) moves
+// 0.56 MB with 32 query heads, so a prefill step is bound by HBM; a decode step is a launch and three dependent
+// round trips (rows, table, page).
+#include "kv.h"
+
+#include <mutex>
+#include <string>
+
+namespace vybdq {
+
+static __device__ __align__(256) uint32_t kv_status_word[64] = {0};
+
+namespace {
+std::mutex g_kv_mu;
+uint32_t *g_kv_status[64];
+}  // namespace
+
+// the current device's status word (hipGetSymbolAddress once per device)
+int kv_status_address(uint32_t *&ptr) {
+  int dev = -1;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64)
+    return set_error(VYBDQ_ERR_HIP, "vybdq_kv: no current HIP device");
+  std::lock_guard<std::mutex> lock(g_kv_mu);
+  if (!g_kv_status[dev]) {
+    void *p = nullptr;
+    const hipError_t e = hipGetSymbolAddress(&p, HIP_SYMBOL(kv_status_word));
+    if (e != hipSuccess || !p)
+      return set_error(VYBDQ_ERR_HIP, std::string("vybdq_kv: hipGetSymbolAddress failed: ") + hipGetErrorString(e));
+    g_kv_status[dev] = static_cast<uint32_t *>(p);
+  }
+  ptr = g_kv_status[dev];
+  return VYBDQ_OK;
+}
+
+struct KvAppendArgs {
+  KvCacheArgs c;
+  KvBatchArgs b;
+  const void *k, *v, *q;
+  void *q_out;
+  const float *cosv, *sinv;
+  int64_t ldk, ldv, ldq;
+  int32_t G, R, n_pos, inter;
+  int32_t per_seq;  // 1: workgroup (b, head) takes every page of sequence b; 0: one page per workgroup
+};
+
+template <int DT>
+__device__ __forceinline__ void load_n(const void *p, int64_t i, float (&x)[8]) {
+  if constexpr (DT == VYBDQ_F32) {
+    const f4 *s = reinterpret_cast<const f4 *>(static_cast<const float *>(p) + i);
+    const f4 a = s[0], b = s[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] = a[j];
+      x[4 + j] = b[j];
+    }
+  } else if constexpr (DT == VYBDQ_F16) {
+    const h8 a = *reinterpret_cast<const h8 *>(static_cast<const _Float16 *>(p) + i);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = static_cast<float>(a[j]);
+  } else {
+    const u4 a = *reinterpret_cast<const u4 *>(static_cast<const uint16_t *>(p) + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t w = a[j];
+      x[2 * j] = __uint_as_float(w << 16);
+      x[2 * j + 1] = __uint_as_float(w & 0xffff0000u);
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void load_n(const void *p, int64_t i, float (&x)[4]) {
+  if constexpr (DT == VYBDQ_F32) {
+    const f4 a = *reinterpret_cast<const f4 *>(static_cast<const float *>(p) + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = a[j];
+  } else if constexpr (DT == VYBDQ_F16) {
+    const h4 a = *reinterpret_cast<const h4 *>(static_cast<const _Float16 *>(p) + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = static_cast<float>(a[j]);
+  } else {
+    const u2 a = *reinterpret_cast<const u2 *>(static_cast<const uint16_t *>(p) + i);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t w = a[j];
+      x[2 * j] = __uint_as_float(w << 16);
+      x[2 * j + 1] = __uint_as_float(w & 0xffff0000u);
+    }
+  }
+}
+
+// Dims d .. d + 7 (d % 8 == 0, R % 16 == 0) of the row at element `at`, rotated to position pos.
+template <int DT>
+__device__ __forceinline__ void rotated8(const KvAppendArgs &a, const void *p, int64_t at, int d, int pos, float (&x)[8]) {
+#pragma clang fp contract(off)
+  load_n<DT>(p, at + d, x);
+  if (d >= a.R) return;
+  const int half = a.R >> 1;
+  const float *c = a.cosv + static_cast<int64_t>(pos) * half;
+  const float *s = a.sinv + static_cast<int64_t>(pos) * half;
+  if (a.inter) {
+    const f4 c4 = *reinterpret_cast<const f4 *>(c + (d >> 1)), s4 = *reinterpret_cast<const f4 *>(s + (d >> 1));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float u = x[2 * j], w = x[2 * j + 1];
+      const float uc = u * c4[j], ws = w * s4[j], wc = w * c4[j], us = u * s4[j];
+      x[2 * j] = uc - ws;
+      x[2 * j + 1] = wc + us;
+    }
+  } else {
+    const bool upper = d >= half;  // half % 8 == 0: eight dims lie on one side
+    float o[8], cs[8], sn[8];
+    load_n<DT>(p, at + (upper ? d - half : d + half), o);
+    load_n<VYBDQ_F32>(c, upper ? d - half : d, cs);
+    load_n<VYBDQ_F32>(s, upper ? d - half : d, sn);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float xc = x[j] * cs[j], os = o[j] * sn[j];
+      x[j] = upper ? xc + os : xc - os;
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void store8(void *p, int64_t i, const float (&x)[8]) {
+  if constexpr (DT == VYBDQ_F32) {
+    f4 *o = reinterpret_cast<f4 *>(static_cast<float *>(p) + i);
+    o[0] = f4{x[0], x[1], x[2], x[3]};
+    o[1] = f4{x[4], x[5], x[6], x[7]};
+  } else if constexpr (DT == VYBDQ_F16) {
+    h8 o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = static_cast<_Float16>(x[j]);
+    *reinterpret_cast<h8 *>(static_cast<_Float16 *>(p) + i) = o;
+  } else {
+    u4 o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      o[j] = f32_to_bf16(x[2 * j]) | (static_cast<uint32_t>(f32_to_bf16(x[2 * j + 1])) << 16);
+    *reinterpret_cast<u4 *>(static_cast<uint16_t *>(p) + i) = o;
+  }
+}
+
+// Four values times a power of two as e4m3 codes, rounded to nearest even and held to +-448.
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float inv) {
+  auto cl = [&](float x) { return __builtin_amdgcn_fmed3f(x * inv, -kKvCodeMax, kKvCodeMax); };
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(cl(a), cl(b), 0, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(cl(c), cl(d), lo, true);
+}
+
+// Four codes brought to a larger scale (f = 2^(e_old - e)). A NaN code stays one.
+__device__ __forceinline__ uint32_t recode4(uint32_t w, float f) {
+  const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+  const int a = __builtin_amdgcn_cvt_pk_fp8_f32(lo.x * f, lo.y * f, 0, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(hi.x * f, hi.y * f, a, true);
+}
+
+// The least e with amax <= 448 * 2^e (448 = 1.75 * 2^8), within the allowed exponents; a zero has the smallest.
+__device__ __forceinline__ int page_exp(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  const int x = static_cast<int>(u >> 23) - 127;
+  const int e = (u & 0x7fffffu) <= 0x600000u ? x - 8 : x - 7;
+  return e < kKvExpMin ? kKvExpMin : (e > kKvExpMax ? kKvExpMax : e);
+}
+
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v = fmaxf(v, __shfl_xor(v, m));
+  return v;
+}
+
+// |x| where x is finite, else 0 and `bad`
+__device__ __forceinline__ float magnitude(float x, bool &bad) {
+  const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
+  if (u < 0x7f800000u) return __uint_as_float(u);
+  bad = true;
+  return 0.0f;
+}
+
+template <int DT, int D>
+__global__ void __launch_bounds__(256) k_kv_append(const KvAppendArgs a) {
+  __shared__ float red[2][4];
+  __shared__ int bad_token[256];  // by the token's place among the page's new ones
+  constexpr int D8 = D / 8, D4 = D / 4;
+  const int tid = threadIdx.x, P = 1 << a.c.ps;
+  const int Hkv = a.c.Hkv, h = blockIdx.x % Hkv;
+  const int64_t u = blockIdx.x / Hkv;
+  int b = static_cast<int>(u);
+  int64_t j = 0;
+  if (!a.per_seq) {
+    // sequence b's pages are units first(b) ..: n rows reach at most ceil(n / P) + 1 pages, and
+    // floor((s + n) / P) - floor(s / P) + 2 is no less
+    auto first = [&](int i) { return (static_cast<int64_t>(a.b.q_start[i]) >> a.c.ps) + 2 * static_cast<int64_t>(i); };
+    b = kv_find(a.b.B, u, first);
+    j = u - first(b);
+  }
+  const KvSeq sq = kv_seq(a.b, b);
+  if (!sq.ok || sq.n == 0 || j < 0) return;
+  if (sq.ctx < sq.n || (static_cast<int64_t>(sq.ctx) + P - 1) >> a.c.ps > a.b.W) {
+    if (tid == 0) kv_flag(a.b.status, kKvBadCtx);
+    return;
+  }
+  const int p0 = sq.ctx - sq.n;  // position of the first row
+  if (a.R && sq.ctx > a.n_pos) {
+    if (tid == 0) kv_flag(a.b.status, kKvBadAngle);
+    return;
+  }
+  const int last = (sq.ctx - 1) >> a.c.ps;
+  for (int64_t i = (p0 >> a.c.ps) + j; i <= last; ++i) {
+    const int base = static_cast<int>(i) << a.c.ps;
+    const int lo = p0 > base ? p0 : base, hi = sq.ctx < base + P ? sq.ctx : base + P;
+    const int keep = lo - base, nt = hi - lo;
+    const int64_t row0 = sq.s0 + (lo - p0);
+    const int pg = a.b.table[static_cast<int64_t>(b) * a.b.W + i];
+    const bool valid = pg >= 0 && pg < a.c.n_pages;
+    if (!valid && tid == 0) kv_flag(a.b.status, kKvBadPage);
+
+    if (valid) {
+      const int64_t ph = static_cast<int64_t>(pg) * Hkv + h;
+      uint8_t *Kp = a.c.K + ph * P * D, *Vp = a.c.V + ph * P * D;
+      // 1. the largest finite magnitude of the new tokens, and the tokens that hold something else
+      for (int t = tid; t < nt; t += 256) bad_token[t] = 0;
+      __syncthreads();
+      float mk = 0.f, mv = 0.f;
+      for (int it = tid; it < nt * D8; it += 256) {
+        const int t = it / D8, d = it % D8 * 8;
+        float x[8];
+        bool bad = false;
+        rotated8<DT>(a, a.k, (row0 + t) * a.ldk + h * D, d, lo + t, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mk = fmaxf(mk, magnitude(x[e], bad));
+        load_n<DT>(a.v, (row0 + t) * a.ldv + h * D + d, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mv = fmaxf(mv, magnitude(x[e], bad));
+        if (bad) bad_token[t] = 1;
+      }
+      mk = wave_max(mk);
+      mv = wave_max(mv);
+      if ((tid & 63) == 0) {
+        red[0][tid >> 6] = mk;
+        red[1][tid >> 6] = mv;
+      }
+      // the old exponents, read before any thread writes the new ones
+      const int eko = keep ? static_cast<int>((__float_as_uint(a.c.Ks[ph]) >> 23) & 0xffu) - 127 : kKvExpMin;
+      const int evo = keep ? static_cast<int>((__float_as_uint(a.c.Vs[ph]) >> 23) & 0xffu) - 127 : kKvExpMin;
+      __syncthreads();
+      mk = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+      mv = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+      const int ekn = page_exp(mk), evn = page_exp(mv);
+      const int eko_c = eko > kKvExpMax ? kKvExpMax : (eko < kKvExpMin ? kKvExpMin : eko);
+      const int evo_c = evo > kKvExpMax ? kKvExpMax : (evo < kKvExpMin ? kKvExpMin : evo);
+      const int ek = ekn > eko_c ? ekn : eko_c, ev = evn > evo_c ? evn : evo_c;
+      const bool grow_k = keep && ek > eko_c, grow_v = keep && ev > evo_c;
+      if (tid == 0) {
+        a.c.Ks[ph] = exp2i(ek);
+        a.c.Vs[ph] = exp2i(ev);
+      }
+      const float ik = exp2i(-ek), iv = exp2i(-ev);
+      const float fk = exp2i(eko_c - ek), fv = exp2i(evo_c - ev);  // no less than 2^-120
+
+      // 2. K: slots of eight dims; the kept ones only where the scale grows
+      for (int it = tid + (grow_k ? 0 : keep * D8); it < (keep + nt) * D8; it += 256) {
+        const int s = it / D8, d = it % D8 * 8;
+        u2 *dst = reinterpret_cast<u2 *>(Kp + s * D + d);
+        if (s < keep) {
+          const u2 w = *dst;
+          *dst = u2{recode4(w.x, fk), recode4(w.y, fk)};
+        } else if (bad_token[s - keep]) {
+          *dst = u2{0x7f7f7f7fu, 0x7f7f7f7fu};
+        } else {
+          const int t = s - keep;
+          float x[8];
+          rotated8<DT>(a, a.k, (row0 + t) * a.ldk + h * D, d, lo + t, x);
+          *dst = u2{codes4(x[0], x[1], x[2], x[3], ik), codes4(x[4], x[5], x[6], x[7], ik)};
+        }
+      }
+      // 3. V: four slots of four dims, 16 bytes; bytes of slots behind the new ones stay
+      for (int it = tid + (grow_v ? 0 : keep >> 2) * D4; it < ((keep + nt + 3) >> 2) * D4; it += 256) {
+        const int g = it / D4, d = it % D4 * 4;
+        u4 *dst = reinterpret_cast<u4 *>(Vp + (g * D + d) * 4);
+        const bool whole = 4 * g >= keep && 4 * g + 4 <= keep + nt;
+        u4 w = whole ? u4{0, 0, 0, 0} : *dst;
+        if (grow_v && 4 * g < keep) {
+          // the kept slots' bytes at the new scale (bytes of the others are written below, or put back)
+          const int cnt = keep - 4 * g;
+          const uint32_t m = cnt >= 4 ? 0xffffffffu : (1u << (8 * cnt)) - 1;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = (recode4(w[e], fv) & m) | (w[e] & ~m);
+        }
+        uint32_t row[4] = {0, 0, 0, 0}, fresh = 0;  // codes of slot 4 g + r's four dims
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int t = 4 * g + r - keep;
+          if (t >= 0 && t < nt) {
+            fresh |= 0xffu << (8 * r);
+            if (!bad_token[t]) {
+              float x[4];
+              load_n<DT>(a.v, (row0 + t) * a.ldv + h * D + d, x);
+              row[r] = codes4(x[0], x[1], x[2], x[3], iv);
+            }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t col = ((row[0] >> (8 * e)) & 0xffu) | (((row[1] >> (8 * e)) & 0xffu) << 8) |
+                               (((row[2] >> (8 * e)) & 0xffu) << 16) | (((row[3] >> (8 * e)) & 0xffu) << 24);
+          w[e] = (w[e] & ~fresh) | col;
+        }
+        *dst = w;
+      }
+    }
+    // 4. the query heads of this key head
+    if (a.q) {
+      for (int it = tid; it < nt * a.G * D8; it += 256) {
+        const int t = it / (a.G * D8), r = it % (a.G * D8);
+        const int hq = h * a.G + r / D8, d = r % D8 * 8;
+        float x[8];
+        rotated8<DT>(a, a.q, (row0 + t) * a.ldq + static_cast<int64_t>(hq) * D, d, lo + t, x);
+        store8<DT>(a.q_out, ((row0 + t) * Hkv * a.G + hq) * D + d, x);
+      }
+    }
+    if (!a.per_seq) break;
+    __syncthreads();  // bad_token and red are the next page's
+  }
+}
+
+template <int DT>
+static void launch_append(int D, const KvAppendArgs &a, unsigned grid, hipStream_t s) {
+  switch (D) {
+    case 64: hipLaunchKernelGGL((k_kv_append<DT, 64>), dim3(grid), dim3(256), 0, s, a); break;
+    case 128: hipLaunchKernelGGL((k_kv_append<DT, 128>), dim3(grid), dim3(256), 0, s, a); break;
+    case 192: hipLaunchKernelGGL((k_kv_append<DT, 192>), dim3(grid), dim3(256), 0, s, a); break;
+    default: hipLaunchKernelGGL((k_kv_append<DT, 256>), dim3(grid), dim3(256), 0, s, a); break;
+  }
+}
+
+}  // namespace vybdq
+
+using namespace vybdq;
+
+extern "C" int vybdq_kv_append(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs, int64_t n_pages, int64_t Hkv, int64_t D,
+                               int64_t page, uint64_t k, uint64_t v, uint64_t q, uint64_t q_out, int x_dt, int64_t ldk,
+                               int64_t ldv, int64_t ldq, int64_t Hq, uint64_t cosv, uint64_t sinv, int64_t R,
+                               int64_t n_pos, int interleaved, uint64_t table, int64_t W, uint64_t q_start,
+                               uint64_t ctx, int64_t T, int64_t B, int64_t max_new, uint64_t stream) {
+  VYBDQ_REQUIRE(dt_valid_in(x_dt), VYBDQ_ERR_ARG, "x_dt must be F32, F16 or BF16");
+  VYBDQ_REQUIRE(D == 64 || D == 128 || D == 192 || D == 256, VYBDQ_ERR_SHAPE, "D must be 64, 128, 192 or 256");
+  VYBDQ_REQUIRE(page >= 16 && page <= 256 && (page & (page - 1)) == 0, VYBDQ_ERR_SHAPE,
+                "page must be a power of two in 16 .. 256");
+  VYBDQ_REQUIRE(n_pages >= 1 && n_pages < (int64_t(1) << 31), VYBDQ_ERR_SHAPE, "n_pages must be in 1 .. 2^31 - 1");
+  VYBDQ_REQUIRE(Hkv >= 1 && Hkv <= 1024, VYBDQ_ERR_SHAPE, "Hkv must be in 1 .. 1024");
+  VYBDQ_REQUIRE(T >= 0 && T < (int64_t(1) << 30) && B >= 0 && B < (int64_t(1) << 20), VYBDQ_ERR_SHAPE,
+                "T must be below 2^30 and B below 2^20");
+  VYBDQ_REQUIRE(W >= 1 && W * page < (int64_t(1) << 31), VYBDQ_ERR_SHAPE, "W must be at least 1 and W * page below 2^31");
+  VYBDQ_REQUIRE(R >= 0 && R <= D && R % 16 == 0, VYBDQ_ERR_SHAPE, "R must be a multiple of 16 in 0 .. D");
+  VYBDQ_REQUIRE(!q || (Hq >= Hkv && Hq % Hkv == 0 && Hq <= 16384), VYBDQ_ERR_SHAPE, "Hq must be a multiple of Hkv");
+  if (T == 0 || B == 0) return VYBDQ_OK;
+  VYBDQ_REQUIRE(K && V && Ks && Vs && k && v && table && q_start && ctx, VYBDQ_ERR_ARG, "null pointer");
+  VYBDQ_REQUIRE(!q || q_out, VYBDQ_ERR_ARG, "q needs q_out");
+  VYBDQ_REQUIRE(R == 0 || (cosv && sinv && n_pos >= 1), VYBDQ_ERR_ARG, "a rotation needs cos and sin");
+  const int es = dt_size(x_dt);
+  VYBDQ_REQUIRE(ldk >= Hkv * D && ldv >= Hkv * D && (!q || ldq >= Hq * D), VYBDQ_ERR_SHAPE,
+                "a row stride is smaller than a row");
+  VYBDQ_REQUIRE((K | V | k | v | q | q_out | cosv | sinv) % 16 == 0 && ldk * es % 16 == 0 && ldv * es % 16 == 0 &&
+                    (!q || ldq * es % 16 == 0),
+                VYBDQ_ERR_ALIGN, "codes, rows, cos and sin must be 16-byte aligned");
+  VYBDQ_REQUIRE((Ks | Vs | table | q_start | ctx) % 4 == 0, VYBDQ_ERR_ALIGN,
+                "scales, table, q_start and ctx must be 4-byte aligned");
+  KvAppendArgs a{};
+  int ps = 4;
+  while ((1 << ps) < page) ++ps;
+  a.c = {reinterpret_cast<uint8_t *>(K), reinterpret_cast<uint8_t *>(V), reinterpret_cast<float *>(Ks),
+         reinterpret_cast<float *>(Vs), static_cast<int32_t>(n_pages), static_cast<int32_t>(Hkv), ps};
+  a.b = {reinterpret_cast<const int32_t *>(table), reinterpret_cast<const int32_t *>(q_start),
+         reinterpret_cast<const int32_t *>(ctx), nullptr, W, static_cast<int32_t>(T), static_cast<int32_t>(B)};
+  a.k = reinterpret_cast<const void *>(k);
+  a.v = reinterpret_cast<const void *>(v);
+  a.q = reinterpret_cast<const void *>(q);
+  a.q_out = reinterpret_cast<void *>(q_out);
+  a.cosv = reinterpret_cast<const float *>(cosv);
+  a.sinv = reinterpret_cast<const float *>(sinv);
+  a.ldk = ldk;
+  a.ldv = ldv;
+  a.ldq = ldq;
+  a.G = q ? static_cast<int32_t>(Hq / Hkv) : 0;
+  a.R = static_cast<int32_t>(R);
+  a.n_pos = static_cast<int32_t>(n_pos < (int64_t(1) << 30) ? n_pos : (int64_t(1) << 30));
+  a.inter = interleaved != 0;
+  a.per_seq = max_new == 1;
+  const int64_t units = a.per_seq ? B : (T >> ps) + 2 * B;
+  VYBDQ_REQUIRE(units * Hkv < (int64_t(1) << 31), VYBDQ_ERR_SHAPE, "too many pages in one call");
+  const int rc = kv_status_address(a.b.status);
+  if (rc) return rc;
+  const unsigned grid = static_cast<unsigned>(units * Hkv);
+  hipStream_t s = as_stream(stream);
+  VYBDQ_DISPATCH_IN(x_dt, DT, launch_append<DT>(static_cast<int>(D), a, grid, s));
+  return check_launch("vybdq_kv_append");
+}
+
+extern "C" int vybdq_kv_status(void) {
+  uint32_t *st = nullptr;
+  const int rc = kv_status_address(st);
+  if (rc) return rc;
+  uint32_t v = 0;
+  hipError_t e = hipDeviceSynchronize();
+  if (e == hipSuccess) e = hipMemcpy(&v, st, 4, hipMemcpyDeviceToHost);
+  if (e == hipSuccess && v) {
+    const uint32_t zero = 0;
+    e = hipMemcpy(st, &zero, 4, hipMemcpyHostToDevice);
+  }
+  if (e != hipSuccess) return set_error(VYBDQ_ERR_HIP, std::string("vybdq_kv_status: ") + hipGetErrorString(e));
+  if (v & kKvBadRows) return set_error(VYBDQ_ERR_SHAPE, "q_start was not a rising sequence within the rows");
+  if (v & kKvBadCtx) return set_error(VYBDQ_ERR_SHAPE, "a sequence's ctx was below its rows or past its pages");
+  if (v & kKvBadPage) return set_error(VYBDQ_ERR_SHAPE, "a page of the table was outside the cache");
+  if (v & kKvBadAngle) return set_error(VYBDQ_ERR_SHAPE, "a position was past the rows of cos and sin");
+  return VYBDQ_OK;
+}

@@ -578,3 +578,166 @@ class MoeExl3Layer:
              _ptr(self.table), _ptr(sg), _ptr(su), _ptr(sd), _ptr(out), _dt(out.dtype), _ptr(idx), _ptr(w), T, self.H,
              self.I, self.E, self.topk, float(self.scale), float(self.limit), ws, nb, _stream())
         return (out, idx, w) if routing else out
+
+
+# ---- key/value cache in 8 bits -----------------------------------------------------------------
+
+KV_HEAD_DIMS = (64, 128, 192, 256)
+
+
+class KvCache:
+    """One layer's paged key/value cache in e4m3 with a power-of-two scale per page and head (layout: include/vybdq.h).
+
+    k: float8_e4m3fn [n_pages, Hkv, page, D]; v: float8_e4m3fn [n_pages, Hkv, page // 4, D, 4]; k_scale, v_scale:
+    float32 [n_pages, Hkv]. KvCache.empty makes them; pages need no clearing before their first use."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        _need(k.dim() == 4, "k must be [n_pages, Hkv, page, D]")
+        n, Hkv, page, D = k.shape
+        _need(D in KV_HEAD_DIMS, f"D must be one of {KV_HEAD_DIMS}")
+        _need(16 <= page <= 256 and page & (page - 1) == 0, "page must be a power of two in 16 .. 256")
+        _need(n >= 1 and Hkv >= 1, "the cache needs pages and heads")
+        _need(tuple(v.shape) == (n, Hkv, page // 4, D, 4), f"v must be {(n, Hkv, page // 4, D, 4)}")
+        _need(k.dtype == v.dtype == torch.float8_e4m3fn, "codes must be float8_e4m3fn")
+        for s in (k_scale, v_scale):
+            _need(tuple(s.shape) == (n, Hkv) and s.dtype == torch.float32, f"scales must be float32 {(n, Hkv)}")
+        _need(k.device == v.device == k_scale.device == v_scale.device, "the cache's tensors must be on one device")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_pages, self.n_heads, self.page, self.head_dim, self.index = n, Hkv, page, D, k.get_device()
+        self._args = (_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), n, Hkv, D, page)
+
+    @classmethod
+    def empty(cls, n_pages, n_heads, head_dim, page=64, device="cuda"):
+        code = lambda *shape: torch.empty(shape, dtype=torch.float8_e4m3fn, device=device)
+        scale = lambda: torch.ones(n_pages, n_heads, dtype=torch.float32, device=device)
+        return cls(code(n_pages, n_heads, page, head_dim), code(n_pages, n_heads, page // 4, head_dim, 4), scale(),
+                   scale())
+
+
+def _kv_rows(x, shape, cache, what):
+    """Device address and row stride of x [T, H, D], whose heads are consecutive within a row."""
+    if x.shape != shape:
+        raise ValueError(f"{what} must be {list(shape)}")
+    T, H, D = shape
+    st = x.stride()
+    if st[2] != 1 or (st[1] != D and H != 1):
+        raise ValueError(f"{what}: the heads of a row must be consecutive")
+    if x.get_device() != cache.index:
+        raise ValueError(f"{what} must be on the cache's device")
+    return x.data_ptr(), st[0] if T > 1 else H * D
+
+
+def _kv_batch(cache, table, q_start, ctx):
+    """W, B, the addresses of the batch's int32 tables (read on the device by the calls), and the stream."""
+    if table.dim() != 2:
+        raise ValueError("page_table must be [B, W]")
+    B, W = table.shape
+    if q_start.shape != (B + 1,) or ctx.shape != (B,):
+        raise ValueError(f"page_table holds {B} sequences: q_start must be [{B + 1}] and ctx [{B}]")
+    i32, at = torch.int32, cache.index
+    if table.dtype != i32 or q_start.dtype != i32 or ctx.dtype != i32:
+        raise ValueError("page_table, q_start and ctx must be int32")
+    if not (table.is_contiguous() and q_start.is_contiguous() and ctx.is_contiguous()):
+        raise ValueError("page_table, q_start and ctx must be contiguous")
+    if table.get_device() != at or q_start.get_device() != at or ctx.get_device() != at:
+        raise ValueError("page_table, q_start and ctx must be on the cache's device")
+    return W, B, table.data_ptr(), q_start.data_ptr(), ctx.data_ptr()
+
+
+def _kv_stream(cache):
+    now = torch._C._cuda_getDevice()
+    if now != cache.index:
+        raise ValueError(f"the cache is on device {cache.index}, the current device is {now}")
+    return torch._C._cuda_getCurrentRawStream(now)
+
+
+def kv_append(cache, k, v, page_table, q_start, ctx, q=None, cos=None, sin=None, interleaved=False, max_new=None,
+              q_out=None):
+    """Append k, v [T, Hkv, D] to the cache, k rotated to its tokens' positions (vybdq_kv_append); returns the
+    rotated q [T, Hq, D], or None without q.
+
+    Sequence b's rows q_start[b] .. q_start[b + 1] - 1 are the last of its ctx[b] tokens; page_table int32 [B, W]. k, v and q
+    may be slices of one projection's output (heads of a row consecutive). cos, sin: float32 [n_pos, R / 2] (None: no
+    rotation). max_new: most rows that a sequence has, if the host knows it (1 for a decode step)."""
+    T, Hkv, D, dt = k.shape[0], cache.n_heads, cache.head_dim, k.dtype
+    W, B, tp, sp, cp = _kv_batch(cache, page_table, q_start, ctx)
+    kp, ldk = _kv_rows(k, (T, Hkv, D), cache, "k")
+    vp, ldv = _kv_rows(v, (T, Hkv, D), cache, "v")
+    if v.dtype != dt:
+        raise ValueError("v must have k's dtype")
+    qp = op = ldq = Hq = 0
+    if q is not None:
+        if q.dim() != 3 or q.dtype != dt:
+            raise ValueError("q must be [T, Hq, D] of k's dtype")
+        Hq = q.shape[1]
+        if Hq % Hkv or not Hq:
+            raise ValueError("Hq must be a multiple of the cache's heads")
+        qp, ldq = _kv_rows(q, (T, Hq, D), cache, "q")
+        if q_out is None:
+            q_out = torch.empty((T, Hq, D), dtype=dt, device=q.device)
+        elif q_out.shape != (T, Hq, D) or q_out.dtype != dt or q_out.get_device() != cache.index:
+            raise ValueError(f"q_out must be [{T}, {Hq}, {D}] of q's dtype")
+        op = _ptr(q_out)
+    elif q_out is not None:
+        raise ValueError("q_out needs q")
+    cosp = sinp = R = n_pos = 0
+    if cos is not None and sin is not None:
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+            raise ValueError("cos and sin must be float32 [n_pos, R / 2]")
+        if cos.get_device() != cache.index or sin.get_device() != cache.index:
+            raise ValueError("cos and sin must be on the cache's device")
+        n_pos, R = cos.shape
+        R *= 2
+        cosp, sinp = _ptr(cos), _ptr(sin)
+    elif cos is not None or sin is not None:
+        raise ValueError("cos and sin come together")
+    if max_new is None:
+        max_new = 1 if T == B else T
+    call("vybdq_kv_append", *cache._args, kp, vp, qp, op, _dt(dt), ldk, ldv, ldq, Hq, cosp, sinp, R, n_pos,
+         1 if interleaved else 0, tp, W, sp, cp, T, B, max_new, _kv_stream(cache))
+    return q_out
+
+
+class KvAttention:
+    """Attention over a KvCache (vybdq_kv_attn), with its workspace. Calls of one object must not overlap (one stream, or
+    streams that wait for each other; so for the replays of graphs that captured them)."""
+
+    def __init__(self, n_heads, n_kv_heads, head_dim, device="cuda"):
+        _need(head_dim in KV_HEAD_DIMS, f"head_dim must be one of {KV_HEAD_DIMS}")
+        _need(n_kv_heads >= 1 and n_heads >= 1 and n_heads % n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads")
+        self.Hq, self.Hkv, self.D, self.scale = n_heads, n_kv_heads, head_dim, head_dim ** -0.5
+        self.ws_bytes = _lib.lib.vybdq_kv_attn_workspace_size(head_dim)
+        # zero-filled once: the arrival counters at its start must be zero (each call leaves them so)
+        self.ws = torch.zeros(self.ws_bytes + 256, dtype=torch.uint8, device=device)
+        self.ws_ptr, self.index = (self.ws.data_ptr() + 255) // 256 * 256, self.ws.get_device()
+
+    def __call__(self, q, cache, page_table, q_start, ctx, scale=None, causal=True, window=0, max_new=None,
+                 max_ctx=None, out=None, lse=False):
+        """out [T, Hq, D] (and lse float32 [T, Hq] with lse=True) for q [T, Hq, D].
+
+        scale: of q . k, 1 / sqrt(D) by default. window: keys that a row sees at most, itself included (0: all).
+        max_new, max_ctx: most rows and tokens that a sequence has, if the host knows them."""
+        T, Hq, D, dt = q.shape[0], self.Hq, self.D, q.dtype
+        if cache.n_heads != self.Hkv or cache.head_dim != D:
+            raise ValueError(f"the cache must hold {self.Hkv} heads of {D}")
+        if self.index != cache.index:
+            raise ValueError("the workspace must be on the cache's device")
+        W, B, tp, sp, cp = _kv_batch(cache, page_table, q_start, ctx)
+        qp, ldq = _kv_rows(q, (T, Hq, D), cache, "q")
+        if out is None:
+            out = torch.empty((T, Hq, D), dtype=dt, device=q.device)
+        elif out.shape != (T, Hq, D) or out.dtype != dt or out.get_device() != cache.index:
+            raise ValueError(f"out must be [{T}, {Hq}, {D}] of q's dtype")
+        stats = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if lse else None
+        if max_new is None:
+            max_new = 1 if T == B else T
+        call("vybdq_kv_attn", *cache._args, qp, _dt(dt), ldq, Hq, _ptr(out), _ptr(stats), tp, W, sp, cp, T, B, max_new,
+             max_ctx or 0, self.scale if scale is None else scale, 1 if causal else 0, window, self.ws_ptr, self.ws_bytes,
+             _kv_stream(cache))
+        return (out, stats) if lse else out
+
+
+def kv_status():
+    """Synchronise, and raise if a batch's tables were wrong in kv_append or KvAttention since the last call
+    (vybdq_kv_status)."""
+    call("vybdq_kv_status")
