@@ -292,6 +292,19 @@ def test_attention_split_keys(dev, rng, x, n):
     run_attention(dev, rng, [(n, 3001)], 4, 1, 64, 64, x, max_new=n)
 
 
+@pytest.mark.parametrize("variant", [0, 1, 3, 4])
+@pytest.mark.parametrize("splits", [1, 2, 7])
+@pytest.mark.parametrize("x,D", [("bf16", 128), ("f32", 256), ("f16", 64), ("f32", 128), ("bf16", 192)])
+def test_attention_every_variant(dev, rng, monkeypatch, variant, splits, x, D):
+    """Kernel variants and key splits other than the chosen ones, on odd lengths, with and without a window; more keys than
+    a batch of 64 steps."""
+    monkeypatch.setenv("VYBDQ_KV_VARIANT", str(variant))
+    monkeypatch.setenv("VYBDQ_KV_SPLITS", str(splits))
+    lens = [(1, 2300), (70, 333), (0, 50), (33, 33), (5, 90)]
+    run_attention(dev, rng, lens, 3, 1, D, 16, x)
+    run_attention(dev, rng, lens, 4, 2, D, 64, x, window=77, causal=False)
+
+
 @pytest.mark.parametrize("q_scale", [1e-30, 1e-4, 30.0])
 @pytest.mark.parametrize("x", ["bf16", "f32"])
 def test_attention_query_magnitudes(dev, rng, x, q_scale):

@@ -37,7 +37,6 @@ struct KvAttnArgs {
   int64_t ldq;
   int32_t G, dt;       // dt: F32, F16 or BF16 of q and out
   int32_t causal, window;
-  int32_t per_seq;     // 1: a workgroup takes every tile of one sequence; 0: one tile
   float scale2;        // scale * log2(e)
 };
 
@@ -64,9 +63,10 @@ __device__ __forceinline__ float col_sum(float v) {
   return v + __shfl_xor(v, 32);
 }
 
-// 16 consecutive elements of a row as float32
-__device__ __forceinline__ void load16(const void *p, int dt, int64_t i, float (&x)[16]) {
-  if (dt == VYBDQ_F32) {
+// 16 consecutive elements of a row as float32. TWO: float32 elements, else fp16 or bf16.
+template <bool TWO>
+__device__ __forceinline__ void load16(const void *p, bool bf16, int64_t i, float (&x)[16]) {
+  if constexpr (TWO) {
     const f4 *s = reinterpret_cast<const f4 *>(static_cast<const float *>(p) + i);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -82,387 +82,713 @@ __device__ __forceinline__ void load16(const void *p, int dt, int64_t i, float (
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t w = v[e];
-        if (dt == VYBDQ_F16) {
-          x[8 * j + 2 * e] = half_bits_to_f32(w & 0xffffu);
-          x[8 * j + 2 * e + 1] = half_bits_to_f32(w >> 16);
-        } else {
-          x[8 * j + 2 * e] = __uint_as_float(w << 16);
-          x[8 * j + 2 * e + 1] = __uint_as_float(w & 0xffff0000u);
-        }
+        const float h0 = half_bits_to_f32(w & 0xffffu), h1 = half_bits_to_f32(w >> 16);
+        x[8 * j + 2 * e] = bf16 ? __uint_as_float(w << 16) : h0;
+        x[8 * j + 2 * e + 1] = bf16 ? __uint_as_float(w & 0xffff0000u) : h1;
       }
     }
   }
 }
 
-// N consecutive outputs (N a multiple of 4), rounded once to the output type
-template <int N>
-__device__ __forceinline__ void store_n(void *p, int dt, int64_t i, const float (&x)[N]) {
-  if (dt == VYBDQ_F32) {
-    f4 *o = reinterpret_cast<f4 *>(static_cast<float *>(p) + i);
+// N consecutive outputs (N even), rounded once to the output type
+template <bool TWO, int N>
+__device__ __forceinline__ void store_n(void *p, bool bf16, int64_t i, const float (&x)[N]) {
+  if constexpr (TWO) {
+    f2 *o = reinterpret_cast<f2 *>(static_cast<float *>(p) + i);
 #pragma unroll
-    for (int j = 0; j < N / 4; ++j) o[j] = f4{x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]};
+    for (int j = 0; j < N / 2; ++j) o[j] = f2{x[2 * j], x[2 * j + 1]};
   } else {
-    u2 *o = reinterpret_cast<u2 *>(static_cast<uint16_t *>(p) + i);
+    uint32_t *o = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p) + i);
 #pragma unroll
-    for (int j = 0; j < N / 4; ++j) {
-      uint16_t r[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        r[e] = dt == VYBDQ_F16 ? __builtin_bit_cast(uint16_t, static_cast<_Float16>(x[4 * j + e]))
-                               : f32_to_bf16(x[4 * j + e]);
-      o[j] = u2{r[0] | (static_cast<uint32_t>(r[1]) << 16), r[2] | (static_cast<uint32_t>(r[3]) << 16)};
+    for (int j = 0; j < N / 2; ++j) {
+      const uint32_t b = f32_to_bf16(x[2 * j]) | (static_cast<uint32_t>(f32_to_bf16(x[2 * j + 1])) << 16);
+      const h2 f = {static_cast<_Float16>(x[2 * j]), static_cast<_Float16>(x[2 * j + 1])};
+      o[j] = bf16 ? b : __builtin_bit_cast(uint32_t, f);
     }
   }
 }
 
-constexpr float kKvRef = 12.0f;   // a row's reference is 2^-12 of its largest weight when it is taken
-constexpr float kKvMove = 15.0f;  // and is taken anew once a weight would pass 2^15
+// Variants. 0, 1: k_kv_attn_keys, 16 or 32 query rows to a workgroup; 3, 4: k_kv_attn_rows, 64 or 128.
+constexpr int kKvVariants = 5;
+constexpr int kv_variant_rows(int variant) { return variant == 0 ? 16 : variant == 1 ? 32 : variant == 4 ? 128 : 64; }
+// workgroups of a variant on a CU (registers, LDS)
+constexpr int kv_variant_per_cu(int variant, int64_t D) {
+  return variant < 3 ? (D <= 128 ? 2 : 1) : variant == 4 ? 2 : D <= 128 ? 4 : D == 192 ? 3 : 2;
+}
+
+constexpr float kKvRef = 12.0f;    // a row's reference is 2^-12 of its largest weight when it is taken
+constexpr float kKvMove = 15.0f;   // and is taken anew once a weight would pass 2^15
+constexpr float kKvNone = -1e30f;  // the reference of a row that has seen nothing (finite: no inf - inf)
 #define KV_NEG_INF (-__builtin_inff())
 
-// LDS floats a workgroup joins its WT waves through: one column tile at a time
-template <int D, int WT>
-constexpr int kv_join_floats() {
-  return WT > 1 ? WT * 16 * (D + 4 + 2) : 1;
+// What the kernels only read, through the constant address space: uniform reads become scalar loads.
+template <class T>
+__device__ __forceinline__ T kv_const(const T *p, int64_t i) {
+  return ((const T __attribute__((address_space(4))) *)p)[i];
 }
 
-template <int D, int NCT, int WT, int WR, bool SPLIT2>
-__global__ void __launch_bounds__(64 * WT * WR) k_kv_attn(const KvAttnArgs a) {
-  constexpr int C = D / 64, R = 16 * NCT * WR, NW = WT * WR, NQ = SPLIT2 ? 2 : 1;
-  __shared__ float join[kv_join_floats<D, WT>()];
-  __shared__ bool is_last;
-  const int lane = threadIdx.x & 63, col = lane & 15, g4 = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wt = WT > 1 ? wave % WT : 0, wr = WR > 1 ? wave / WT : 0;
-  const int Hkv = a.c.Hkv, h = blockIdx.x % Hkv, S = gridDim.y, split = blockIdx.y;
-  const int unit = blockIdx.x / Hkv, G = a.G, ps = a.c.ps, P = 1 << ps;
-  int b = unit;
-  int64_t tile = 0;
-  if (!a.per_seq) {
-    // sequence b's tiles are units first(b) ..: ceil(n G / R) of them, and floor((s + n) G / R) - floor(s G / R) + 1
-    // is no less. The last units first: with a causal mask they have the most keys.
-    const int64_t u = static_cast<int64_t>(gridDim.x / Hkv) - 1 - unit;
-    auto first = [&](int i) { return static_cast<int64_t>(a.b.q_start[i]) * G / R + i; };
-    b = kv_find(a.b.B, u, first);
-    tile = u - first(b);
-    if (tile < 0) return;
-  }
-  const KvSeq sq = kv_seq(a.b, b);
-  const int64_t rows = static_cast<int64_t>(sq.n) * G;
-  if (rows == 0) return;
-  // tokens past the table's pages: the sequence's rows are NaN
-  const bool past = sq.ctx > (a.b.W << ps);
-  if (past && (threadIdx.x & 63) == 0) kv_flag(a.b.status, kKvBadCtx);
-  const int ctx = sq.ctx > 0 && !past ? sq.ctx : 0, p0 = ctx - sq.n;
-  const int32_t *table = a.b.table + static_cast<int64_t>(b) * a.b.W;
+// A tile of query rows: rows r0 .. of sequence b's n G (row = token * G + head of the group), and its keys.
+struct KvTile {
+  KvSeq sq;
+  int rows, r0;        // (T G < 2^31)
+  int ctx, p0;         // tokens; position of the first row
+  int k0, steps;       // keys that some row of the tile sees lie in k0 .. k0 + 32 steps - 1
+  int free0, free1;    // keys that every row sees: no mask
+  const int32_t *table;
+  bool past;           // tokens past the table's pages: the rows are NaN
+};
 
-  for (int64_t r0 = tile * R; r0 < rows; r0 += R) {
-    // a tile beyond the first that the launch did not plan for is not split: split 0 takes all its keys
-    const bool whole = S == 1 || (a.per_seq && r0 > 0);
-    if (whole && split > 0) return;
-    // keys that some row of the tile sees: [k0, k1), in steps of 32
-    const int i_lo = static_cast<int>(r0 / G);
-    const int i_hi = static_cast<int>((r0 + R < rows ? r0 + R : rows) - 1) / G;
-    int k1 = a.causal ? p0 + i_hi + 1 : ctx;
-    k1 = k1 > 0 ? k1 : 0;
-    int k0 = a.window ? p0 + i_lo - a.window + 1 : 0;
-    k0 = (k0 > 0 ? k0 : 0) & ~31;
-    const int steps = k1 > k0 ? (k1 - k0 + 31) >> 5 : 0;
-    const int t0 = whole ? 0 : static_cast<int>(static_cast<int64_t>(steps) * split / S);
-    const int t1 = whole ? steps : static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / S);
-    // keys that every row sees need no mask
-    const int free0 = a.window ? p0 + i_hi - a.window + 1 : 0, free1 = a.causal ? p0 + i_lo + 1 : ctx;
+__device__ __forceinline__ bool kv_tile_seq(const KvAttnArgs &a, int b, KvTile &t) {
+  t.sq = kv_seq(a.b, b);
+  t.rows = t.sq.n * a.G;
+  t.past = t.sq.ctx > (a.b.W << a.c.ps);
+  if (t.past && (threadIdx.x & 63) == 0) kv_flag(a.b.status, kKvBadCtx);
+  t.ctx = t.sq.ctx > 0 && !t.past ? t.sq.ctx : 0;
+  t.p0 = t.ctx - t.sq.n;
+  t.table = a.b.table + static_cast<int64_t>(b) * a.b.W;
+  return t.rows > 0;
+}
 
-    // this lane's query rows
-    h8 qf[NCT][2 * C][NQ];
-    float qc[NCT], m[NCT], l[NCT];
-    int lo_r[NCT], hi_r[NCT];
-    f4 acc[NCT][4 * C];
+// Tile u of the batch. Sequence b's tiles are units first(b) ..: ceil(n G / R) of them, and
+// floor((s + n) G / R) - floor(s G / R) + 1 is no less.
+__device__ __forceinline__ bool kv_tile_unit(const KvAttnArgs &a, int R, int u, KvTile &t) {
+  auto first = [&](int i) { return static_cast<int64_t>(static_cast<uint32_t>(a.b.q_start[i]) * static_cast<uint32_t>(a.G) / R + i); };
+  const int b = kv_find(a.b.B, u, first);
+  const int64_t r0 = (u - first(b)) * R;
+  t.r0 = static_cast<int>(r0 < a.b.T * a.G ? r0 : -1);
+  return t.r0 >= 0 && kv_tile_seq(a, b, t) && t.r0 < t.rows;
+}
+
+__device__ __forceinline__ void kv_tile_keys(const KvAttnArgs &a, int R, KvTile &t) {
+  const int i_lo = t.r0 / a.G, i_hi = ((t.rows - t.r0 > R ? t.r0 + R : t.rows) - 1) / a.G;
+  int k1 = a.causal ? t.p0 + i_hi + 1 : t.ctx;
+  k1 = k1 > 0 ? k1 : 0;
+  const int first = a.window ? t.p0 + i_lo - a.window + 1 : 0;
+  t.k0 = (first > 0 ? first : 0) & ~31;
+  t.steps = k1 > t.k0 ? (k1 - t.k0 + 31) >> 5 : 0;
+  t.free0 = a.window ? t.p0 + i_hi - a.window + 1 : 0;
+  t.free1 = a.causal ? t.p0 + i_lo + 1 : t.ctx;
+}
+
+// The 16 query rows r .. r + 15 as operands of S^T = K Q^T, one row per column: lane (col, g4) holds dims
+// 64 c + 16 g4 + 8 x + 0 .. 7 in f[2 c + x], scaled by the power of two that brings the row's largest value
+// into [2^14, 2^15). qc: the factor from their products with K codes to scale * log2(e) q . (K code).
+template <int C, bool TWO>
+struct KvRows {
+  h8 f[2 * C][TWO ? 2 : 1];
+  float qc;
+  int lo, hi;  // keys lo .. hi - 1 are seen
+};
+
+template <int C, bool TWO>
+__device__ __forceinline__ void kv_load_rows(const KvAttnArgs &a, const KvTile &t, int r, int h, KvRows<C, TWO> &q) {
+  constexpr int D = 64 * C;
+  const int lane = threadIdx.x & 63, g4 = lane >> 4;
+  r += lane & 15;
+  const bool have = r < t.rows;
+  const int rr = have ? r : 0;  // rows past the last: the first one's values, not stored
+  const int i = rr / a.G, hq = h * a.G + rr % a.G;
+  q.hi = !have ? 0 : a.causal ? t.p0 + i + 1 : t.ctx;
+  q.lo = a.window ? t.p0 + i - a.window + 1 : 0;
+  const int64_t at = (t.sq.s0 + i) * a.ldq + hq * D + 16 * g4;
+  const bool bf16 = a.dt == VYBDQ_BF16;
+  float x[C][16], amax = 0.f;
+  bool bad = false;
 #pragma unroll
-    for (int ct = 0; ct < NCT; ++ct) {
-      const int64_t r = r0 + (wr * NCT + ct) * 16 + col;
-      const bool have = r < rows;
-      const int64_t rr = have ? r : 0;
-      const int i = static_cast<int>(rr / G), hq = h * G + static_cast<int>(rr % G);
-      hi_r[ct] = !have ? 0 : a.causal ? p0 + i + 1 : ctx;
-      lo_r[ct] = a.window ? p0 + i - a.window + 1 : 0;
-      const int64_t at = (sq.s0 + i) * a.ldq + static_cast<int64_t>(hq) * D + 16 * g4;
-      float amax = 0.f;
-      bool bad = false;
+  for (int c = 0; c < C; ++c) {
+    load16<TWO>(a.q, bf16, at + 64 * c, x[c]);
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        float x[16];
-        load16(a.q, a.dt, at + 64 * c, x);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          bad |= (__float_as_uint(x[e]) & 0x7fffffffu) >= 0x7f800000u;
-          amax = fmaxf(amax, fabsf(x[e]));
-        }
-      }
-      float inv;
-      const float sc = block_scale(col_max(amax), inv);
-      // an infinity or NaN in any of the row's four lanes makes its scores NaN
-      qc[ct] = sc * a.scale2 + col_sum(bad ? __builtin_nanf("") : 0.f);
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        float x[16];
-        load16(a.q, a.dt, at + 64 * c, x);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float v = x[e] * inv;
-          const _Float16 f = static_cast<_Float16>(v);
-          qf[ct][2 * c + e / 8][0][e % 8] = f;
-          if constexpr (SPLIT2) qf[ct][2 * c + e / 8][NQ - 1][e % 8] = static_cast<_Float16>(v - static_cast<float>(f));
-        }
-      }
-      m[ct] = KV_NEG_INF;
-      l[ct] = past ? __builtin_nanf("") : 0.f;
-#pragma unroll
-      for (int t = 0; t < 4 * C; ++t) acc[ct][t] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int e = 0; e < 16; ++e) {
+      bad |= (__float_as_uint(x[c][e]) & 0x7fffffffu) >= 0x7f800000u;
+      amax = fmaxf(amax, fabsf(x[c][e]));
     }
+  }
+  float inv;
+  const float sc = block_scale(col_max(amax), inv);
+  // an infinity or NaN in any of the row's four lanes makes its scores NaN
+  q.qc = sc * a.scale2 + col_sum(bad ? __builtin_nanf("") : 0.f);
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float v = x[c][e] * inv;
+      const _Float16 f = static_cast<_Float16>(v);
+      q.f[2 * c + e / 8][0][e % 8] = f;
+      if constexpr (TWO) q.f[2 * c + e / 8][1][e % 8] = static_cast<_Float16>(v - static_cast<float>(f));
+    }
+}
 
-    for (int st = t0 + wt; st < t1; st += WT) {
-      const int tok = k0 + 32 * st;
-      // the two blocks of 16 keys: where they lie, and their scales
-      const uint8_t *kb[2], *vb[2];
-      float ks[2], ev[2], iv[2];
-      bool drop[2];
+// Weights of one tile of scores. s[ct][n]: the products of 2 blocks of 16 keys with the rows of column tile ct; ks, ev, iv: the
+// blocks' K scale, V exponent and 2^-ev. Updates m, l and acc, returns the weights as operands of O^T = V^T P^T.
+template <int NCT, int C, bool TWO>
+__device__ __forceinline__ void kv_weights(const f4 (&s)[NCT][2], const KvRows<C, TWO> (&q)[NCT], const float (&ks)[2],
+                                           const float (&ev)[2], const float (&iv)[2], int tok, bool masked, float (&m)[NCT],
+                                           float (&l)[NCT], f4 (&acc)[NCT][4 * C], h8 (&p)[NCT][TWO ? 2 : 1]) {
+  const int g4 = (threadIdx.x & 63) >> 4;
+  float t[NCT][8];
+  auto exponents = [&]() {  // t - m
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const int t = tok + 16 * n, at = t >> ps;
-        const bool in = t < ctx;
-        const int pg = in ? table[at] : 0;
-        drop[n] = pg < 0 || pg >= a.c.n_pages;
-        const int64_t ph = static_cast<int64_t>(drop[n] ? 0 : pg) * Hkv + h;
-        const int64_t off = ((ph << ps) + (t & (P - 1))) * D;
-        kb[n] = a.c.K + off;
-        vb[n] = a.c.V + off;
-        const uint32_t e = in && !drop[n] ? (__float_as_uint(a.c.Vs[ph]) >> 23) & 0xffu : 127u;
-        ks[n] = drop[n] ? __builtin_nanf("") : in ? a.c.Ks[ph] : 1.0f;
-        ev[n] = static_cast<float>(static_cast<int>(e) - 127);
-        iv[n] = __uint_as_float((254u - e) << 23);
-        if (drop[n] && lane == 0) kv_flag(a.b.status, kKvBadPage);
+        const float ck = q[ct].qc * ks[n], add = ev[n] - m[ct];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[ct][4 * n + e] = __builtin_fmaf(s[ct][n][e], ck, add);
       }
-      u4 kw[2][C], vw[2][C];
+    if (masked) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-          kw[n][c] = *reinterpret_cast<const u4 *>(kb[n] + col * D + 64 * c + 16 * g4);
-          vw[n][c] = *reinterpret_cast<const u4 *>(vb[n] + 4 * (g4 * D + 64 * c + 4 * col));
-        }
-      f4 s[NCT][2];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-#pragma unroll
-        for (int ct = 0; ct < NCT; ++ct) s[ct][n] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const h8 kf = kv_dec8(kw[n][c][2 * x], kw[n][c][2 * x + 1]);
-#pragma unroll
-            for (int ct = 0; ct < NCT; ++ct)
-#pragma unroll
-              for (int y = 0; y < NQ; ++y)
-                s[ct][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[ct][2 * c + x][y], s[ct][n], 0, 0, 0);
-          }
-      }
-      // slots behind the sequence's end were never written: their V codes may be anything, NaN included
-      if (tok + 32 > ctx || drop[0] || drop[1]) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const int left = drop[n] ? 0 : ctx - (tok + 16 * n + 4 * g4);
-          const uint32_t keep = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1;
-#pragma unroll
-          for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) vw[n][c][e] &= keep;
-        }
-      }
-      const bool masked = tok < free0 || tok + 32 > free1;
-      h8 pf[NCT][NQ];
-#pragma unroll
-      for (int ct = 0; ct < NCT; ++ct) {
-        float t[8];
-        float top = KV_NEG_INF;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float ck = qc[ct] * ks[n];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            t[4 * n + e] = __builtin_fmaf(s[ct][n][e], ck, ev[n]);
-            if (masked) {
-              const int key = tok + 16 * n + 4 * g4 + e;
-              t[4 * n + e] = key >= lo_r[ct] && key < hi_r[ct] ? t[4 * n + e] : KV_NEG_INF;
-            }
-            top = fmaxf(top, t[4 * n + e]);
-          }
-        }
-        if (__ballot(top > m[ct] + kKvMove)) {
-          const float now = fmaxf(m[ct], col_max(top) - kKvRef);
-          const float f = now == KV_NEG_INF ? 1.0f : __builtin_amdgcn_exp2f(m[ct] - now);
-          m[ct] = now;
-          l[ct] *= f;
-#pragma unroll
-          for (int d = 0; d < 4 * C; ++d) acc[ct][d] *= f;
-        }
-        const float ref = m[ct] == KV_NEG_INF ? 0.f : m[ct];
+      for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float w = __builtin_amdgcn_exp2f(t[4 * n + e] - ref);
-            l[ct] = __builtin_fmaf(w, iv[n], l[ct]);
-            const _Float16 f = static_cast<_Float16>(w);
-            pf[ct][0][4 * n + e] = f;
-            if constexpr (SPLIT2) pf[ct][NQ - 1][4 * n + e] = static_cast<_Float16>(w - static_cast<float>(f));
+            const int key = tok + 16 * n + 4 * g4 + e;
+            t[ct][4 * n + e] = key >= q[ct].lo && key < q[ct].hi ? t[ct][4 * n + e] : KV_NEG_INF;
+          }
+    }
+  };
+  exponents();
+  float top[NCT], any = KV_NEG_INF;
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    top[ct] = t[ct][0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) top[ct] = fmaxf(top[ct], t[ct][e]);
+    any = fmaxf(any, top[ct]);
+  }
+  if (__ballot(any > kKvMove)) {
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct) {
+      // the largest exponent itself, not its difference to the old reference (which may be kKvNone)
+      float big = KV_NEG_INF;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          big = fmaxf(big, t[ct][4 * n + e] == KV_NEG_INF ? KV_NEG_INF : __builtin_fmaf(s[ct][n][e], q[ct].qc * ks[n], ev[n]));
+      const float now = fmaxf(m[ct], col_max(big) - kKvRef);
+      const float f = __builtin_amdgcn_exp2f(m[ct] - now);
+      m[ct] = now;
+      l[ct] *= f;
+#pragma unroll
+      for (int d = 0; d < 4 * C; ++d) acc[ct][d] *= f;
+    }
+    exponents();
+  }
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float w = __builtin_amdgcn_exp2f(t[ct][4 * n + e]);
+        l[ct] = __builtin_fmaf(w, iv[n], l[ct]);  // not of the rounded weight: lse is a float32 result
+        const _Float16 f = static_cast<_Float16>(w);
+        p[ct][0][4 * n + e] = f;
+        if constexpr (TWO) p[ct][1][4 * n + e] = static_cast<_Float16>(w - static_cast<float>(f));
+      }
+}
+
+// Where a tile's results go: the output, or the workspace as one of S partial results. COHERENT: partials that another
+// workgroup of the same launch reads (stored through the XCD's L2), else plain stores for the next launch.
+template <int D, int R, bool TWO, bool COHERENT>
+struct KvSink {
+  const KvAttnArgs &a;
+  const KvTile &t;
+  int h;
+  bool whole;
+  float *part;  // this split's: m, l interleaved [R], acc [R][D]
+
+  // N dims d .. of tile row r: sums x over weights of sum lr, reference mr
+  template <int N>
+  __device__ __forceinline__ void finish(int r, float mr, float lr, int d, const float (&x)[N]) const {
+    const int rr = t.r0 + r;
+    if (rr >= t.rows) return;
+    const int64_t at = (t.sq.s0 + rr / a.G) * (static_cast<int64_t>(a.c.Hkv) * a.G) + h * a.G + rr % a.G;
+    const float f = lr == 0.f ? 0.f : 1.0f / lr;
+    float y[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) y[e] = x[e] * f;
+    store_n<TWO, N>(a.out, a.dt == VYBDQ_BF16, at * D + d, y);
+    if (a.lse && d == 0) a.lse[at] = lr == 0.f ? KV_NEG_INF : (mr + __builtin_amdgcn_logf(lr)) * 0.6931471805599453f;
+  }
+  template <int N>
+  __device__ __forceinline__ void put(int r, float mr, float lr, int d, const float (&x)[N]) const {
+    if (whole) {
+      finish<N>(r, mr, lr, d, x);
+    } else if (t.r0 + r < t.rows && !COHERENT) {
+      f2 *o = reinterpret_cast<f2 *>(part + 2 * R + r * D + d);
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) o[e] = f2{x[2 * e], x[2 * e + 1]};
+      if (d == 0) reinterpret_cast<f2 *>(part)[r] = f2{mr, lr};
+    } else if (t.r0 + r < t.rows) {
+      uint64_t *o = reinterpret_cast<uint64_t *>(part + 2 * R + r * D + d);
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e)
+        __hip_atomic_store(o + e, __float_as_uint(x[2 * e]) | (static_cast<uint64_t>(__float_as_uint(x[2 * e + 1])) << 32),
+                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (d == 0)
+        __hip_atomic_store(reinterpret_cast<uint64_t *>(part) + r,
+                           __float_as_uint(mr) | (static_cast<uint64_t>(__float_as_uint(lr)) << 32), __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+
+  // All S splits' results of the tile, joined in split order by the last workgroup to arrive. The partials are stored
+  // through the XCD's L2 and have completed before the arrival is counted; they are read by device-coherent loads.
+  __device__ __forceinline__ void join(int S, bool &is_last) const {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      uint32_t *count = a.arrivals + blockIdx.x;
+      const uint32_t old = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      is_last = old == static_cast<uint32_t>(S - 1);
+      if (is_last) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!is_last) return;
+    constexpr int64_t kSize = static_cast<int64_t>(R) * (D + 2);
+    const float *all = a.part + blockIdx.x * S * kSize;
+    const int n_rows = t.rows - t.r0 < R ? t.rows - t.r0 : R;
+    for (int it = threadIdx.x; it < n_rows * (D / 4); it += blockDim.x) {
+      const int r = it / (D / 4), d = it % (D / 4) * 4;
+      float mr = kKvNone, lr = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int w0 = 0; w0 < S; w0 += 8) {  // 24 independent loads to a round trip
+        uint64_t ml[8], v[8][2];
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+          const float *pw = all + (w0 + w < S ? w0 + w : S - 1) * kSize;
+          ml[w] = __hip_atomic_load(reinterpret_cast<const uint64_t *>(pw) + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            v[w][e] = __hip_atomic_load(reinterpret_cast<const uint64_t *>(pw + 2 * R + r * D + d) + e, __ATOMIC_RELAXED,
+                                        __HIP_MEMORY_SCOPE_AGENT);
+        }
+        float now = mr;
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+          if (w0 + w < S) now = fmaxf(now, __uint_as_float(static_cast<uint32_t>(ml[w])));
+        const float f0 = __builtin_amdgcn_exp2f(mr - now);
+        lr *= f0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] *= f0;
+        mr = now;
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+          if (w0 + w < S) {
+            const float f = __builtin_amdgcn_exp2f(__uint_as_float(static_cast<uint32_t>(ml[w])) - now);
+            lr = __builtin_fmaf(f, __uint_as_float(static_cast<uint32_t>(ml[w] >> 32)), lr);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              x[2 * e] = __builtin_fmaf(f, __uint_as_float(static_cast<uint32_t>(v[w][e])), x[2 * e]);
+              x[2 * e + 1] = __builtin_fmaf(f, __uint_as_float(static_cast<uint32_t>(v[w][e] >> 32)), x[2 * e + 1]);
+            }
           }
       }
+      finish<4>(r, mr, lr, d, x);
+    }
+  }
+};
+
+// ---- few rows: the waves of a workgroup take turns over the keys ---------------------------------
+
+// One step of 32 keys on its way: the codes in registers, where the step lies, its blocks' scales.
+template <int C>
+struct KvStep {
+  u4 k[2][C], v[2][C];
+  float ks[2], vs[2];
+  bool bad[2];
+};
+
+// WR groups of 16 rows; the 4 / WR waves of a group take turns over the keys. (The groups' waves read the same codes; the
+// second reads come from the CU's own cache.)
+template <int D, int WR, bool TWO>
+__global__ void __launch_bounds__(256) k_kv_attn_keys(const KvAttnArgs a) {
+  constexpr int C = D / 64, R = 16 * WR, WT = 4 / WR, NQ = TWO ? 2 : 1;
+  __shared__ float acc_w[4][16][D + 4];
+  __shared__ float ml_w[4][2][16];
+  __shared__ bool is_last;
+  const int lane = threadIdx.x & 63, col = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave % WR, wt = wave / WR;
+  const int Hkv = a.c.Hkv, h = blockIdx.x % Hkv, b = blockIdx.x / Hkv, S = gridDim.y, split = blockIdx.y;
+  const int ps = a.c.ps, in_page = (1 << ps) - 1;
+  KvTile t;
+  if (!kv_tile_seq(a, b, t)) return;
+  const uint32_t koff = col * D + 16 * g4, voff = 4 * (g4 * D + 4 * col);
+  const int last_page = t.ctx > 0 ? (t.ctx - 1) >> ps : 0;
+
+  for (t.r0 = 0; t.r0 < t.rows; t.r0 += R) {
+    // a tile beyond the first, which the launch did not plan for, is not split: split 0 takes all its keys
+    const bool whole = S == 1 || t.r0 > 0;
+    if (whole && split > 0) return;
+    kv_tile_keys(a, R, t);
+    const int t0 = whole ? 0 : t.steps * split / S;
+    const int t1 = whole ? t.steps : t.steps * (split + 1) / S;
+
+    // pages of a step's two blocks; a block behind the sequence's end takes the last page (its keys are masked)
+    auto page_of = [&](int st, int n) {
+      const int at = (t.k0 + 32 * st + 16 * n) >> ps;
+      return kv_const(t.table, at < last_page ? at : last_page);
+    };
+    auto fetch = [&](KvStep<C> &x, int st, const int (&pg)[2]) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        x.bad[n] = static_cast<uint32_t>(pg[n]) >= static_cast<uint32_t>(a.c.n_pages);
+        const int64_t ph = static_cast<int64_t>(x.bad[n] ? 0 : pg[n]) * Hkv + h;
+        x.ks[n] = kv_const(a.c.Ks, ph);
+        x.vs[n] = kv_const(a.c.Vs, ph);
+        const int64_t at = ((ph << ps) + ((t.k0 + 32 * st + 16 * n) & in_page)) * D;
+        const uint8_t *kb = a.c.K + at, *vb = a.c.V + at;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          x.k[n][c] = *reinterpret_cast<const u4 *>(kb + (koff + 64 * c));
+          x.v[n][c] = *reinterpret_cast<const u4 *>(vb + (voff + 256 * c));
+        }
+      }
+    };
+
+    int st = t0 + wt;
+    const bool work = st < t1;
+    int pg[2] = {0, 0};
+    KvStep<C> even, odd;
+    if (work) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) pg[n] = page_of(st, n);
+      fetch(even, st, pg);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) pg[n] = page_of(st + WT, n);
+    }
+
+    KvRows<C, TWO> q[1];
+    float m[1] = {kKvNone}, l[1] = {t.past ? __builtin_nanf("") : 0.f};
+    f4 acc[1][4 * C];
+    kv_load_rows<C, TWO>(a, t, t.r0 + 16 * wr, h, q[0]);
+#pragma unroll
+    for (int d = 0; d < 4 * C; ++d) acc[0][d] = f4{0.f, 0.f, 0.f, 0.f};
+
+    auto use = [&](KvStep<C> &x, int st) {
+      const int tok = t.k0 + 32 * st;
+      f4 s[1][2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        s[0][n] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const h8 kf = kv_dec8(x.k[n][c][2 * y], x.k[n][c][2 * y + 1]);
+#pragma unroll
+            for (int z = 0; z < NQ; ++z) s[0][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[0].f[2 * c + y][z], s[0][n], 0, 0, 0);
+          }
+      }
+      float ks[2], ev[2], iv[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const uint32_t e = x.bad[n] ? 127u : (__float_as_uint(x.vs[n]) >> 23) & 0xffu;
+        ks[n] = x.bad[n] ? __builtin_nanf("") : x.ks[n];
+        ev[n] = static_cast<float>(static_cast<int>(e) - 127);
+        iv[n] = __uint_as_float((254u - e) << 23);
+      }
+      // slots behind the sequence's end were never written: their V codes may be anything, NaN included
+      if (tok + 32 > t.ctx || x.bad[0] || x.bad[1]) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int left = x.bad[n] ? 0 : t.ctx - (tok + 16 * n + 4 * g4);
+          const uint32_t keep = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1;
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x.v[n][c][e] &= keep;
+          if (x.bad[n] && lane == 0) kv_flag(a.b.status, kKvBadPage);
+        }
+      }
+      h8 p[1][NQ];
+      kv_weights<1, C, TWO>(s, q, ks, ev, iv, tok, tok < t.free0 || tok + 32 > t.free1, m, l, acc, p);
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-          const h8 vf = kv_dec8(vw[0][c][d], vw[1][c][d]);
+          const h8 vf = kv_dec8(x.v[0][c][d], x.v[1][c][d]);
 #pragma unroll
-          for (int ct = 0; ct < NCT; ++ct)
-#pragma unroll
-            for (int y = 0; y < NQ; ++y)
-              acc[ct][4 * c + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[ct][y], acc[ct][4 * c + d], 0, 0, 0);
+          for (int z = 0; z < NQ; ++z) acc[0][4 * c + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p[0][z], acc[0][4 * c + d], 0, 0, 0);
         }
+    };
+
+    // two steps to a turn, the next one's codes on their way while one is used, the page numbers one step further ahead
+    while (st < t1) {
+      const bool two = st + WT < t1;
+      if (two) {
+        fetch(odd, st + WT, pg);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) pg[n] = page_of(st + 2 * WT, n);
+      }
+      use(even, st);
+      if (!two) break;
+      if (st + 2 * WT < t1) {
+        fetch(even, st + 2 * WT, pg);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) pg[n] = page_of(st + 3 * WT, n);
+      }
+      use(odd, st + WT);
+      st += 2 * WT;
     }
 
-    // ---- the tile's rows: joined over the waves, then stored, or left for the last split
-    float *part = a.part + (static_cast<int64_t>(blockIdx.x) * S + split) * (R * (D + 2));
-    auto put = [&](int r, float mr, float lr, int d, const auto &x) {  // dims d .. of tile row r
-      constexpr int N = sizeof(x) / 4;
-      if (whole) {
-        const int64_t rr = r0 + r;
-        if (rr >= rows) return;
-        const int64_t at = (sq.s0 + rr / G) * (static_cast<int64_t>(Hkv) * G) + h * G + rr % G;
-        const float f = lr == 0.f ? 0.f : 1.0f / lr;
-        float y[N];
+    // the waves' results, joined through LDS
+    const KvSink<D, R, TWO, true> sink{a, t, h, whole, a.part + (static_cast<int64_t>(blockIdx.x) * S + split) * (R * (D + 2))};
+    l[0] = col_sum(l[0]);
+    if (t.r0 > 0) __syncthreads();
 #pragma unroll
-        for (int e = 0; e < N; ++e) y[e] = x[e] * f;
-        store_n<N>(a.out, a.dt, at * D + d, y);
-        if (a.lse && d == 0) a.lse[at] = lr == 0.f ? KV_NEG_INF : (mr + __builtin_amdgcn_logf(lr)) * 0.6931471805599453f;
-      } else if (r0 + r < rows) {
-        uint64_t *o = reinterpret_cast<uint64_t *>(part + 2 * R + r * D + d);
+    for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int e = 0; e < N / 2; ++e)
-          __hip_atomic_store(o + e, __float_as_uint(x[2 * e]) | (static_cast<uint64_t>(__float_as_uint(x[2 * e + 1])) << 32),
-                             __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (d == 0)
-          __hip_atomic_store(reinterpret_cast<uint64_t *>(part) + r,
-                             __float_as_uint(mr) | (static_cast<uint64_t>(__float_as_uint(lr)) << 32), __ATOMIC_RELAXED,
-                             __HIP_MEMORY_SCOPE_AGENT);
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<f4 *>(&acc_w[wave][col][64 * c + 16 * g4 + 4 * e]) =
+            f4{acc[0][4 * c][e], acc[0][4 * c + 1][e], acc[0][4 * c + 2][e], acc[0][4 * c + 3][e]};
+    if (g4 == 0) {
+      ml_w[wave][0][col] = m[0];
+      ml_w[wave][1][col] = l[0];
+    }
+    __syncthreads();
+    for (int it = threadIdx.x; it < R * (D / 4); it += 256) {
+      const int r = it / (D / 4), d = it % (D / 4) * 4, r16 = r & 15, w0 = r >> 4;
+      float mr = kKvNone, lr = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < WT; ++w) mr = fmaxf(mr, ml_w[w0 + w * WR][0][r16]);
+#pragma unroll
+      for (int w = 0; w < WT; ++w) {
+        const float f = __builtin_amdgcn_exp2f(ml_w[w0 + w * WR][0][r16] - mr);
+        lr = __builtin_fmaf(f, ml_w[w0 + w * WR][1][r16], lr);
+        const f4 v = *reinterpret_cast<const f4 *>(&acc_w[w0 + w * WR][r16][d]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(f, v[e], x[e]);
       }
-    };
+      sink.template put<4>(r, mr, lr, d, x);
+    }
+    if (!whole) sink.join(S, is_last);
+  }
+}
+
+// ---- many rows: the waves own rows and share the keys through LDS ----------------------------------
+
+// A step's codes are converted once per workgroup: a wave reads its share of them from the cache, converts it and writes
+// operand registers to LDS (1 KB each, lane by lane, so reads and writes are free of bank conflicts), from where every
+// wave feeds its matrix instructions. Two buffers, one barrier a step: a step is written while the one before it is
+// used, and its codes were asked for one step earlier still. The pages and scales of 128 blocks of 16 keys at a time
+// go through LDS as well (scalar loads would be waited for with every wait for LDS data).
+// The last units first: with a causal mask they have the most keys.
+template <int D, int NCT, int NW, bool TWO>
+__global__ void __launch_bounds__(64 * NW, NCT > 1 || D == 256 || (TWO && D == 192) ? 2 : TWO || D == 192 ? 3 : 4) k_kv_attn_rows(const KvAttnArgs a) {
+  constexpr int C = D / 64, R = 16 * NCT * NW, NQ = TWO ? 2 : 1;
+  // 64 dims of a block of 16 keys are a unit: the step's 2 C units of K, then 2 C of V, are dealt to the waves in turn
+  constexpr int kMine = (4 * C + NW - 1) / NW;
+  __shared__ h8 tile[2][8 * C][64];  // K of block n: 2 (n C + c) + y; V: 4 C + 4 c + d, its first four values of block 0
+  __shared__ u4 meta[2][128];        // a block's page, K scale, V exponent e and 2^-e
+  const int lane = threadIdx.x & 63, col = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int Hkv = a.c.Hkv, h = blockIdx.x % Hkv, S = gridDim.y, split = blockIdx.y;
+  const int ps = a.c.ps, in_page = (1 << ps) - 1;
+  KvTile t;
+  if (!kv_tile_unit(a, R, gridDim.x / Hkv - 1 - blockIdx.x / Hkv, t)) return;
+  kv_tile_keys(a, R, t);
+  const int t0 = t.steps * split / S, t1 = t.steps * (split + 1) / S;
+  const int last_page = t.ctx > 0 ? (t.ctx - 1) >> ps : 0;
+  const uint32_t koff = col * D + 16 * g4, voff = 4 * (g4 * D + 4 * col);
+
+  // Blocks 128 batch .. of this split. A block behind the sequence's end takes the last page (its keys are masked); one
+  // outside the cache reads page 0 with a NaN scale.
+  auto ask = [&](int batch) {
+    for (int i = threadIdx.x; i < 128; i += 64 * NW) {
+      const int at = ((t.k0 >> 4) + 2 * t0 + 128 * batch + i) >> (ps - 4);
+      const int pg = t.table[at < last_page ? at : last_page];
+      const bool bad = static_cast<uint32_t>(pg) >= static_cast<uint32_t>(a.c.n_pages);
+      if (bad) kv_flag(a.b.status, kKvBadPage);
+      const int64_t ph = static_cast<int64_t>(bad ? 0 : pg) * Hkv + h;
+      const int e = bad ? 0 : static_cast<int>((__float_as_uint(a.c.Vs[ph]) >> 23) & 0xffu) - 127;
+      meta[batch & 1][i] = u4{static_cast<uint32_t>(bad ? 0 : pg), bad ? 0x7fc00000u : __float_as_uint(a.c.Ks[ph]),
+                              __float_as_uint(static_cast<float>(e)), static_cast<uint32_t>(127 - e) << 23};
+    }
+  };
+  auto block_meta = [&](int st, int n) -> const u4 & { return meta[(st - t0) >> 6 & 1][(2 * (st - t0) + n) & 127]; };
+  // this wave's unit i: is it one, is it K's (known at compile time for all but a mixed turn), which block and dims
+  auto unit = [&](int i) { return wave + i * NW; };
+  auto mine = [&](int i) { return 4 * C % NW == 0 || unit(i) < 4 * C; };
+  auto is_k = [&](int i) { return (i + 1) * NW <= 2 * C || (i * NW < 2 * C && unit(i) < 2 * C); };
+  auto block_of = [&](int i) { return (is_k(i) ? unit(i) : unit(i) - 2 * C) / C; };
+  auto dims_of = [&](int i) { return unit(i) % C; };
+  u2 coming[kMine];  // page and K scale of the blocks that are fetched next
+  u4 code[kMine];
+  uint32_t ks[kMine];
+  auto peek = [&](int st) {
 #pragma unroll
-    for (int ct = 0; ct < NCT; ++ct) {
-      l[ct] = col_sum(l[ct]);
-      if constexpr (WT == 1) {
+    for (int i = 0; i < kMine; ++i)
+      if (mine(i)) coming[i] = *reinterpret_cast<const u2 *>(&block_meta(st, block_of(i)));
+  };
+  auto fetch = [&](int st) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          float x[16];  // dims 64 c + 16 g4 + 4 e + d
+    for (int i = 0; i < kMine; ++i) {
+      if (!mine(i)) continue;
+      const int pg = __builtin_amdgcn_readfirstlane(coming[i].x);
+      ks[i] = __builtin_amdgcn_readfirstlane(coming[i].y);
+      const int64_t at = (((static_cast<int64_t>(pg) * Hkv + h) << ps) + ((t.k0 + 32 * st + 16 * block_of(i)) & in_page)) * D;
+      const uint8_t *base = (is_k(i) ? a.c.K + 64 * dims_of(i) : a.c.V + 256 * dims_of(i)) + at;
+      code[i] = *reinterpret_cast<const u4 *>(base + (is_k(i) ? koff : voff));
+    }
+    if (st + 1 < t1) peek(st + 1);
+  };
+  auto write = [&](int st) {
+    const int buf = st & 1, tok = t.k0 + 32 * st;
 #pragma unroll
-          for (int d = 0; d < 4; ++d)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * e + d] = acc[ct][4 * c + d][e];
-          put((wr * NCT + ct) * 16 + col, m[ct], l[ct], 64 * c + 16 * g4, x);
-        }
+    for (int i = 0; i < kMine; ++i) {
+      if (!mine(i)) continue;
+      if (is_k(i)) {
+        tile[buf][2 * unit(i)][lane] = kv_dec8(code[i].x, code[i].y);
+        tile[buf][2 * unit(i) + 1][lane] = kv_dec8(code[i].z, code[i].w);
       } else {
-        float *acc_w = join + wave * (16 * (D + 4)), *m_w = join + WT * 16 * (D + 4), *l_w = m_w + WT * 16;
-        if (ct > 0 || r0 > tile * R) __syncthreads();
+        const int n = block_of(i), c = dims_of(i);
+        const bool bad = (ks[i] & 0x7fffffffu) > 0x7f800000u;
+        if (tok + 32 > t.ctx || bad) {
+          // slots behind the sequence's end were never written: their V codes may be anything, NaN included
+          const int left = bad ? 0 : t.ctx - (tok + 16 * n + 4 * g4);
+          const uint32_t keep = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1;
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<f4 *>(acc_w + col * (D + 4) + 64 * c + 16 * g4 + 4 * e) =
-                f4{acc[ct][4 * c][e], acc[ct][4 * c + 1][e], acc[ct][4 * c + 2][e], acc[ct][4 * c + 3][e]};
-        if (g4 == 0) {
-          m_w[wt * 16 + col] = m[ct];
-          l_w[wt * 16 + col] = l[ct];
+          for (int d = 0; d < 4; ++d) code[i][d] &= keep;
         }
-        __syncthreads();
-        for (int it = threadIdx.x; it < 16 * (D / 4); it += 64 * NW) {
-          const int r = it / (D / 4), d = it % (D / 4) * 4;
-          float mr = KV_NEG_INF, lr = 0.f;
 #pragma unroll
-          for (int w = 0; w < WT; ++w) mr = fmaxf(mr, m_w[w * 16 + r]);
-          const float ref = mr == KV_NEG_INF ? 0.f : mr;
-          float x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int w = 0; w < WT; ++w) {
-            const float f = __builtin_amdgcn_exp2f(m_w[w * 16 + r] - ref);
-            lr = __builtin_fmaf(f, l_w[w * 16 + r], lr);
-            const f4 v = *reinterpret_cast<const f4 *>(join + w * (16 * (D + 4)) + r * (D + 4) + d);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(f, v[e], x[e]);
-          }
-          put(ct * 16 + r, mr, lr, d, x);
+        for (int d = 0; d < 4; ++d) {
+          h2 x, y;
+          kv_dec4(code[i][d], x, y);
+          reinterpret_cast<h4 *>(&tile[buf][4 * C + 4 * c + d][lane])[n] = h4{x.x, x.y, y.x, y.y};
         }
       }
     }
-    if (!whole) {
-      // arrival: the partials are stored through the XCD's L2 and have completed before it is counted; the last
-      // one resets the counter and reads the others' with device-coherent loads
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        const uint32_t old = __hip_atomic_fetch_add(a.arrivals + blockIdx.x, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        is_last = old == static_cast<uint32_t>(S - 1);
-        if (is_last) __hip_atomic_store(a.arrivals + blockIdx.x, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
-      __syncthreads();
-      if (is_last) {
-        const float *all = a.part + static_cast<int64_t>(blockIdx.x) * S * (R * (D + 2));
-        const int n_rows = rows - r0 < R ? static_cast<int>(rows - r0) : R;
-        for (int it = threadIdx.x; it < n_rows * (D / 2); it += 64 * NW) {
-          const int r = it / (D / 2), d = it % (D / 2) * 2;
-          float mr = KV_NEG_INF, lr = 0.f, x0 = 0.f, x1 = 0.f;
-          for (int w0 = 0; w0 < S; w0 += 8) {
-            uint64_t ml[8], v[8];
+  };
+
+  if (t0 < t1) ask(0);
+  __syncthreads();
+  if (t0 < t1) {
+    peek(t0);
+    fetch(t0);
+  }
+  KvRows<C, TWO> q[NCT];
+  float m[NCT], l[NCT];
+  f4 acc[NCT][4 * C];
 #pragma unroll
-            for (int w = 0; w < 8; ++w)
-              if (w0 + w < S) {
-                const float *pw = all + static_cast<int64_t>(w0 + w) * (R * (D + 2));
-                ml[w] = __hip_atomic_load(reinterpret_cast<const uint64_t *>(pw) + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                v[w] = __hip_atomic_load(reinterpret_cast<const uint64_t *>(pw + 2 * R + r * D + d), __ATOMIC_RELAXED,
-                                         __HIP_MEMORY_SCOPE_AGENT);
-              }
-            float now = mr;
+  for (int ct = 0; ct < NCT; ++ct) {
+    kv_load_rows<C, TWO>(a, t, t.r0 + (wave * NCT + ct) * 16, h, q[ct]);
+    m[ct] = kKvNone;
+    l[ct] = t.past ? __builtin_nanf("") : 0.f;
 #pragma unroll
-            for (int w = 0; w < 8; ++w)
-              if (w0 + w < S) now = fmaxf(now, __uint_as_float(static_cast<uint32_t>(ml[w])));
-            const float ref = now == KV_NEG_INF ? 0.f : now;
-            const float f0 = __builtin_amdgcn_exp2f(mr - ref);
-            lr *= f0;
-            x0 *= f0;
-            x1 *= f0;
-            mr = now;
+    for (int d = 0; d < 4 * C; ++d) acc[ct][d] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (t0 < t1) {
+    write(t0);
+    if (t0 + 1 < t1) fetch(t0 + 1);
+  }
+  __syncthreads();
+
+  for (int st = t0; st < t1; ++st) {
+    const int buf = st & 1, tok = t.k0 + 32 * st;
+    const u4 m0 = block_meta(st, 0), m1 = block_meta(st, 1);
+    h8 kf[2 * C];
 #pragma unroll
-            for (int w = 0; w < 8; ++w)
-              if (w0 + w < S) {
-                const float f = __builtin_amdgcn_exp2f(__uint_as_float(static_cast<uint32_t>(ml[w])) - ref);
-                lr = __builtin_fmaf(f, __uint_as_float(static_cast<uint32_t>(ml[w] >> 32)), lr);
-                x0 = __builtin_fmaf(f, __uint_as_float(static_cast<uint32_t>(v[w])), x0);
-                x1 = __builtin_fmaf(f, __uint_as_float(static_cast<uint32_t>(v[w] >> 32)), x1);
-              }
-          }
-          const int64_t rr = r0 + r;
-          const int64_t at = (sq.s0 + rr / G) * (static_cast<int64_t>(Hkv) * G) + h * G + rr % G;
-          const float f = lr == 0.f ? 0.f : 1.0f / lr;
-          if (a.dt == VYBDQ_F32) *reinterpret_cast<f2 *>(static_cast<float *>(a.out) + at * D + d) = f2{x0 * f, x1 * f};
-          else {
-            const uint16_t u = a.dt == VYBDQ_F16 ? __builtin_bit_cast(uint16_t, static_cast<_Float16>(x0 * f)) : f32_to_bf16(x0 * f);
-            const uint16_t v = a.dt == VYBDQ_F16 ? __builtin_bit_cast(uint16_t, static_cast<_Float16>(x1 * f)) : f32_to_bf16(x1 * f);
-            *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.out) + at * D + d) = u | (static_cast<uint32_t>(v) << 16);
-          }
-          if (a.lse && d == 0) a.lse[at] = lr == 0.f ? KV_NEG_INF : (mr + __builtin_amdgcn_logf(lr)) * 0.6931471805599453f;
-        }
+    for (int c = 0; c < 2 * C; ++c) kf[c] = tile[buf][c][lane];
+    if (st + 1 < t1) {
+      write(st + 1);
+      if (((st - t0) & 63) == 32 && st - t0 + 32 < t1 - t0) ask(((st - t0) >> 6) + 1);
+      if (st + 2 < t1) fetch(st + 2);
+    }
+    f4 s[NCT][2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) s[ct][n] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 2 * C; ++c)
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+          for (int z = 0; z < NQ; ++z)
+            s[ct][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[c], q[ct].f[c][z], s[ct][n], 0, 0, 0);
+      if (n == 0) {
+#pragma unroll
+        for (int c = 0; c < 2 * C; ++c) kf[c] = tile[buf][2 * C + c][lane];
       }
     }
-    if (!a.per_seq) break;
+    const float sk[2] = {__uint_as_float(m0.y), __uint_as_float(m1.y)}, ev[2] = {__uint_as_float(m0.z), __uint_as_float(m1.z)},
+                iv[2] = {__uint_as_float(m0.w), __uint_as_float(m1.w)};
+    h8 vf[2 * C];
+#pragma unroll
+    for (int d = 0; d < 2 * C; ++d) vf[d] = tile[buf][4 * C + d][lane];
+    h8 p[NCT][NQ];
+    kv_weights<NCT, C, TWO>(s, q, sk, ev, iv, tok, tok < t.free0 || tok + 32 > t.free1, m, l, acc, p);
+#pragma unroll
+    for (int d = 0; d < 4 * C; ++d) {
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+        for (int z = 0; z < NQ; ++z) acc[ct][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d % (2 * C)], p[ct][z], acc[ct][d], 0, 0, 0);
+      if (d < 2 * C) vf[d] = tile[buf][6 * C + d][lane];
+    }
+    __syncthreads();
+  }
+
+  const KvSink<D, R, TWO, false> sink{a, t, h, S == 1, a.part + (static_cast<int64_t>(blockIdx.x) * S + split) * (R * (D + 2))};
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    l[ct] = col_sum(l[ct]);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float x[16];  // dims 64 c + 16 g4 + 4 e + d
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * e + d] = acc[ct][4 * c + d][e];
+      sink.template put<16>((wave * NCT + ct) * 16 + col, m[ct], l[ct], 64 * c + 16 * g4, x);
+    }
+  }
+}
+
+// The splits' results of k_kv_attn_rows, joined in split order: workgroup (tile and head, 8 rows), each thread four dims at a
+// time. In the same launch, as k_kv_attn_keys does it, one workgroup would read all S R (D + 2) floats alone.
+template <int D, int R, bool TWO>
+__global__ void __launch_bounds__(256) k_kv_attn_join(const KvAttnArgs a, int S) {
+  constexpr int64_t kSize = static_cast<int64_t>(R) * (D + 2);
+  const int Hkv = a.c.Hkv, h = blockIdx.x % Hkv;
+  KvTile t;
+  if (!kv_tile_unit(a, R, gridDim.x / Hkv - 1 - blockIdx.x / Hkv, t)) return;
+  const float *all = a.part + blockIdx.x * S * kSize;
+  const KvSink<D, R, TWO, false> sink{a, t, h, true, nullptr};
+  for (int it = threadIdx.x; it < 8 * (D / 4); it += 256) {
+    const int r = blockIdx.y * 8 + it / (D / 4), d = it % (D / 4) * 4;
+    if (t.r0 + r >= t.rows) return;
+    float mr = kKvNone, lr = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int w0 = 0; w0 < S; w0 += 4) {  // 8 independent loads to a round trip
+      f2 ml[4];
+      f4 v[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float *pw = all + (w0 + w < S ? w0 + w : S - 1) * kSize;
+        ml[w] = reinterpret_cast<const f2 *>(pw)[r];
+        v[w] = *reinterpret_cast<const f4 *>(pw + 2 * R + r * D + d);
+      }
+      float now = mr;
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        if (w0 + w < S) now = fmaxf(now, ml[w].x);
+      const float f0 = __builtin_amdgcn_exp2f(mr - now);
+      mr = now;
+      lr *= f0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] *= f0;
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        if (w0 + w < S) {
+          const float f = __builtin_amdgcn_exp2f(ml[w].x - now);
+          lr = __builtin_fmaf(f, ml[w].y, lr);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(f, v[w][e], x[e]);
+        }
+    }
+    sink.template finish<4>(r, mr, lr, d, x);
   }
 }
 

@@ -1,6 +1,7 @@
 // vybdq_kv_attn: checks, the choice of variant and key split, and the dispatch (kernel: kv_attn.h).
 #include "kv_attn.h"
 
+#include <cstdlib>
 #include <string>
 
 namespace vybdq {
@@ -9,8 +10,75 @@ namespace vybdq {
 void kv_attn_launch_h(int D, int variant, const KvAttnArgs &a, dim3 grid, hipStream_t s);
 void kv_attn_launch_f(int D, int variant, const KvAttnArgs &a, dim3 grid, hipStream_t s);
 
-constexpr int64_t kKvPartRows = 65536;   // rows of split results that a workspace holds
+constexpr int64_t kKvPartRows = 131072;  // rows of split results that a workspace holds
 constexpr int64_t kKvArrivalBytes = 16384;
+
+struct KvShape {
+  int64_t D, Hkv, G, T, B, new_rows, steps;  // new_rows: most rows of a sequence; steps: of 32 keys, at most
+  bool two, causal;
+  int64_t part_rows;  // rows of split results that the workspace holds
+};
+struct KvPlan {
+  int variant;
+  int64_t units, splits;
+};
+
+// Key splits of a variant. Times in us as measured (MI355X):
+// - k_kv_attn_keys: a workgroup takes a step of 32 keys in (0.08 + 0.0011 D) WR us when it is not held up by the others
+//   (one sequence of 131072 keys, 8 heads of 128: 8 splits 108 us, 16 splits 60, 32 splits 47 = 5.8 TB/s), together they
+//   take 1 / 5.5 TB/s, not quite hiding one under the other, and the last one joins its tile's splits in about 0.02 D / 128 us a row and split (192 splits: 67 us).
+//   48 sequences of 2 k to 8 k keys: 1 split 117 us, 2 113, 4 105, 8 109.
+// - k_kv_attn_rows: rounds of workgroups, each about 6 steps of its own besides its keys, and a launch to join them.
+static int64_t kv_splits(const KvShape &s, int variant, int64_t wgs) {
+  const int64_t R = kv_variant_rows(variant), held = s.part_rows / R / wgs;
+  const int64_t slots = device_cu_count() * kv_variant_per_cu(variant, s.D);
+  if (const char *e = tuning_env("VYBDQ_KV_SPLITS")) return atoi(e) < 1 || held < 1 ? 1 : atoi(e) < held ? atoi(e) : held;
+  int64_t S = 1;
+  double best = 1e30;
+  const int64_t rows = s.new_rows * s.G < R ? s.new_rows * s.G : R;
+  const double read = static_cast<double>(wgs) * s.steps * 64 * s.D / 5.5e6;
+  for (int64_t n = 1; n <= 256 && (n == 1 || (n <= held && 4 * n <= s.steps)); ++n) {
+    const double rounds = static_cast<double>((wgs * n + slots - 1) / slots);
+    double time;
+    if (variant < 3) {
+      const double alone = rounds * s.steps / n * (0.08 + 0.0011 * s.D) * (R / 16);
+      time = (alone > read ? alone : read) + 0.3 * alone + (n > 1 ? 0.5 + 0.02 * n * rows * s.D / 128 : 0);
+    } else {
+      time = rounds * (static_cast<double>(s.steps) / n + 6) + (n > 1 ? 6 : 0);
+    }
+    if (time < best) {
+      best = time;
+      S = n;
+    }
+  }
+  return S;
+}
+
+// Variant by the rows that share keys. Up to 32 (a decode step, drafted tokens): k_kv_attn_keys, whose waves need not
+// wait for each other (16 sequences of 8 tokens, 4 heads a key head, 6000 keys: D = 128 46 us against 53 with
+// k_kv_attn_rows, D = 256 98 against 123); more: k_kv_attn_rows, whose waves share the conversion (16 tokens: 34 us against
+// 68). Its tiles of 128 rows need half the cache reads, those of 64 keep more waves and even out better: 128 rows only
+// where D = 128 leaves room for their registers and they still fill the chip (512 tokens behind 3584, 4 sequences: 158 us
+// against 183; a prompt of 2048: 67 against 60, of 4096: 182 against 184).
+static KvPlan kv_plan(const KvShape &s) {
+  const int64_t rows = s.new_rows * s.G;
+  int variant = rows <= 16 ? 0 : rows <= 32 ? 1 : 3;
+  bool given = false;
+  if (const char *e = tuning_env("VYBDQ_KV_VARIANT")) {
+    variant = atoi(e) < 0 || atoi(e) >= kKvVariants ? variant : atoi(e);
+    given = true;
+  }
+  auto make = [&](int v) {
+    const int64_t units = v < 2 ? s.B : s.T * s.G / kv_variant_rows(v) + s.B, wgs = units * s.Hkv;
+    return KvPlan{v, units, wgs * 4 <= kKvArrivalBytes ? kv_splits(s, v, wgs) : 1};
+  };
+  if (s.D == 128 && !s.two && (given ? variant == 4 : variant == 3)) {
+    const KvPlan p = make(4);
+    const double seen = s.causal ? 1.0 - 0.5 * s.new_rows / (32.0 * s.steps) : 1.0;
+    if (given || p.units * s.Hkv * p.splits * seen >= 0.75 * device_cu_count() * kv_variant_per_cu(4, s.D)) return p;
+  }
+  return make(variant == 4 ? 3 : variant);
+}
 
 }  // namespace vybdq
 
@@ -35,6 +103,7 @@ extern "C" int vybdq_kv_attn(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs, i
                 "Hq must be a multiple of Hkv, Hkv in 1 .. 1024 and Hq at most 16384");
   VYBDQ_REQUIRE(T >= 0 && T < (int64_t(1) << 30) && B >= 0 && B < (int64_t(1) << 20), VYBDQ_ERR_SHAPE,
                 "T must be below 2^30 and B below 2^20");
+  VYBDQ_REQUIRE(T * Hq < (int64_t(1) << 31), VYBDQ_ERR_SHAPE, "T * Hq must be below 2^31");
   VYBDQ_REQUIRE(W >= 1 && W * page < (int64_t(1) << 30), VYBDQ_ERR_SHAPE, "W must be at least 1 and W * page below 2^30");
   VYBDQ_REQUIRE(window >= 0 && window < (int64_t(1) << 30), VYBDQ_ERR_SHAPE, "window must be in 0 .. 2^30 - 1");
   if (T == 0 || B == 0) return VYBDQ_OK;
@@ -49,28 +118,13 @@ extern "C" int vybdq_kv_attn(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs, i
   while ((1 << ps) < page) ++ps;
   const int G = static_cast<int>(Hq / Hkv);
   const bool two = x_dt == VYBDQ_F32;
-  // Variant: 0, 1: 16 or 32 query rows, the waves of a workgroup take turns over the keys; 2: rows spread over
-  // the waves (kv_attn_*.hip).
-  const int64_t rows = max_new >= 1 ? max_new * G : T * G;
-  const int variant = rows <= 16 ? 0 : rows <= 32 ? 1 : 2;
-  const int64_t R = variant == 0 ? 16 : variant == 1 ? 32 : two && D > 128 ? 64 : 128;
+  const int64_t cap = W * page, tokens = max_ctx >= 1 && max_ctx < cap ? max_ctx : cap;
+  const int64_t most = max_new >= 1 && max_new < T ? max_new : T;
+  const KvShape shape{D, Hkv, G, T, B, most, (tokens + 31) / 32, two, causal != 0,
+                      ws && ws_bytes > kKvArrivalBytes ? (ws_bytes - kKvArrivalBytes) / ((D + 2) * 4) : 0};
+  KvPlan plan = kv_plan(shape);
+  VYBDQ_REQUIRE(plan.units * Hkv < (int64_t(1) << 31), VYBDQ_ERR_SHAPE, "too many rows in one call");
   KvAttnArgs a{};
-  a.per_seq = variant < 2;
-  const int64_t units = a.per_seq ? B : T * G / R + B;
-  VYBDQ_REQUIRE(units * Hkv < (int64_t(1) << 31), VYBDQ_ERR_SHAPE, "too many rows in one call");
-  // Keys split over workgroups until the chip is full: at least 8 steps of 32 keys each, and what the workspace holds
-  const int64_t wgs = units * Hkv, cap = W * page;
-  const int64_t tokens = max_ctx >= 1 && max_ctx < cap ? max_ctx : cap;
-  const int64_t steps = (tokens + 31) / 32;
-  int64_t S = 1;
-  if (ws && ws_bytes > kKvArrivalBytes && wgs * 4 <= kKvArrivalBytes) {
-    const int64_t held = (ws_bytes - kKvArrivalBytes) / (R * (D + 2) * 4);
-    const int64_t want = 4 * static_cast<int64_t>(device_cu_count()) / (variant == 2 ? 2 : 1);
-    S = want / wgs;
-    if (S > steps / 8) S = steps / 8;
-    if (S > held / wgs) S = held / wgs;
-    if (S < 1) S = 1;
-  }
   const int rc = kv_status_address(a.b.status);
   if (rc) return rc;
   uint32_t *status = a.b.status;
@@ -89,8 +143,8 @@ extern "C" int vybdq_kv_attn(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs, i
   a.causal = causal != 0;
   a.window = static_cast<int32_t>(window);
   a.scale2 = static_cast<float>(scale * 1.4426950408889634);
-  const dim3 grid(static_cast<unsigned>(wgs), static_cast<unsigned>(S));
-  if (two) kv_attn_launch_f(static_cast<int>(D), variant, a, grid, as_stream(stream));
-  else kv_attn_launch_h(static_cast<int>(D), variant, a, grid, as_stream(stream));
+  const dim3 grid(static_cast<unsigned>(plan.units * Hkv), static_cast<unsigned>(plan.splits));
+  if (two) kv_attn_launch_f(static_cast<int>(D), plan.variant, a, grid, as_stream(stream));
+  else kv_attn_launch_h(static_cast<int>(D), plan.variant, a, grid, as_stream(stream));
   return check_launch("vybdq_kv_attn");
 }
