@@ -12,11 +12,11 @@
 // A token of which a rotated k or a v of a head is an infinity or NaN gets codes that no finite token has there:
 // k NaN, v zero. Its score is then NaN for the rows that see it, and a row that does not see it multiplies zeros.
 //
-// One workgroup per (page that a sequence's rows reach, key/value head): it alone writes that page's codes and
-// scales, reads the new k and v for the largest magnitude, then reads them again (from L2) to write codes, and
-// rotates the query heads of its key head for the same tokens. A page of 64 tokens of 8 heads of 128 (bf16) moves
-// 0.56 MB with 32 query heads, so a prefill step is bound by HBM; a decode step is a launch and three dependent
-// round trips (rows, table, page).
+// One workgroup per (page that a sequence's rows reach, key/value head): it alone writes that page's codes and scales.
+// A thread reads 16 dims of a token's k (both halves of its pairs) and 4 dims of four slots of v and keeps them in registers
+// until the page's largest magnitude is known (512 threads: all of a page of 64 tokens of 128 dims); of a larger page the
+// rest is read again (from L2). Query heads are rotated by workgroups of their own (gridDim.y), which need not wait for a page's
+// magnitude.
 #include "kv.h"
 
 #include <mutex>
@@ -105,35 +105,39 @@ __device__ __forceinline__ void load_n(const void *p, int64_t i, float (&x)[4]) 
   }
 }
 
-// Dims d .. d + 7 (d % 8 == 0, R % 16 == 0) of the row at element `at`, rotated to position pos.
-template <int DT>
-__device__ __forceinline__ void rotated8(const KvAppendArgs &a, const void *p, int64_t at, int d, int pos, float (&x)[8]) {
-#pragma clang fp contract(off)
-  load_n<DT>(p, at + d, x);
-  if (d >= a.R) return;
+// Piece i of a row's D / 16: 16 dims that hold both members of their pairs, 8 from dim lo and 8 from dim hi.
+struct KvPiece {
+  int lo, hi;
+};
+__device__ __forceinline__ KvPiece kv_piece(const KvAppendArgs &a, int i) {
   const int half = a.R >> 1;
-  const float *c = a.cosv + static_cast<int64_t>(pos) * half;
-  const float *s = a.sinv + static_cast<int64_t>(pos) * half;
+  if (!a.inter && 8 * i < half) return {8 * i, half + 8 * i};
+  return {16 * i, 16 * i + 8};  // (pairs of neighbours, or dims behind R)
+}
+
+// Piece i of the row at element `at`, rotated to position pos.
+template <int DT>
+__device__ __forceinline__ void rotated16(const KvAppendArgs &a, const void *p, int64_t at, int i, int pos, float (&x)[2][8]) {
+#pragma clang fp contract(off)
+  const KvPiece d = kv_piece(a, i);
+  load_n<DT>(p, at + d.lo, x[0]);
+  load_n<DT>(p, at + d.hi, x[1]);
+  if (16 * i >= a.R) return;
+  const int64_t row = static_cast<int64_t>(pos) * (a.R >> 1) + 8 * i;
+  float c[8], s[8];
+  load_n<VYBDQ_F32>(a.cosv, row, c);
+  load_n<VYBDQ_F32>(a.sinv, row, s);
+  auto turn = [](float &u, float &w, float cj, float sj) {
+    const float uc = u * cj, ws = w * sj, wc = w * cj, us = u * sj;
+    u = uc - ws;
+    w = wc + us;
+  };
   if (a.inter) {
-    const f4 c4 = *reinterpret_cast<const f4 *>(c + (d >> 1)), s4 = *reinterpret_cast<const f4 *>(s + (d >> 1));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float u = x[2 * j], w = x[2 * j + 1];
-      const float uc = u * c4[j], ws = w * s4[j], wc = w * c4[j], us = u * s4[j];
-      x[2 * j] = uc - ws;
-      x[2 * j + 1] = wc + us;
-    }
+    for (int j = 0; j < 8; ++j) turn(x[j >> 2][2 * (j & 3)], x[j >> 2][2 * (j & 3) + 1], c[j], s[j]);
   } else {
-    const bool upper = d >= half;  // half % 8 == 0: eight dims lie on one side
-    float o[8], cs[8], sn[8];
-    load_n<DT>(p, at + (upper ? d - half : d + half), o);
-    load_n<VYBDQ_F32>(c, upper ? d - half : d, cs);
-    load_n<VYBDQ_F32>(s, upper ? d - half : d, sn);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float xc = x[j] * cs[j], os = o[j] * sn[j];
-      x[j] = upper ? xc + os : xc - os;
-    }
+    for (int j = 0; j < 8; ++j) turn(x[0][j], x[1][j], c[j], s[j]);
   }
 }
 
@@ -196,14 +200,14 @@ __device__ __forceinline__ float magnitude(float x, bool &bad) {
 }
 
 template <int DT, int D>
-__global__ void __launch_bounds__(256) k_kv_append(const KvAppendArgs a) {
-  __shared__ float red[2][4];
+__global__ void __launch_bounds__(512, 4) k_kv_append(const KvAppendArgs a) {
+  __shared__ float red[2][8];
   __shared__ int bad_token[256];  // by the token's place among the page's new ones
-  constexpr int D8 = D / 8, D4 = D / 4;
-  const int tid = threadIdx.x, P = 1 << a.c.ps;
+  constexpr int D16 = D / 16, D4 = D / 4;
+  const int tid = threadIdx.x, nthr = blockDim.x, P = 1 << a.c.ps;
   const int Hkv = a.c.Hkv, h = blockIdx.x % Hkv;
-  const int64_t u = blockIdx.x / Hkv;
-  int b = static_cast<int>(u);
+  const int u = blockIdx.x / Hkv;
+  int b = u;
   int64_t j = 0;
   if (!a.per_seq) {
     // sequence b's pages are units first(b) ..: n rows reach at most ceil(n / P) + 1 pages, and
@@ -218,39 +222,93 @@ __global__ void __launch_bounds__(256) k_kv_append(const KvAppendArgs a) {
     if (tid == 0) kv_flag(a.b.status, kKvBadCtx);
     return;
   }
-  const int p0 = sq.ctx - sq.n;  // position of the first row
   if (a.R && sq.ctx > a.n_pos) {
     if (tid == 0) kv_flag(a.b.status, kKvBadAngle);
     return;
   }
+  const int p0 = sq.ctx - sq.n;  // position of the first row
   const int last = (sq.ctx - 1) >> a.c.ps;
   for (int64_t i = (p0 >> a.c.ps) + j; i <= last; ++i) {
     const int base = static_cast<int>(i) << a.c.ps;
     const int lo = p0 > base ? p0 : base, hi = sq.ctx < base + P ? sq.ctx : base + P;
     const int keep = lo - base, nt = hi - lo;
     const int64_t row0 = sq.s0 + (lo - p0);
+
+    if (blockIdx.y > 0) {  // query heads
+      const int per_token = a.G * D16;
+      for (int it = (blockIdx.y - 1) * nthr + tid; it < nt * per_token; it += (gridDim.y - 1) * nthr) {
+        const int t = it / per_token, r = it % per_token;
+        const int hq = h * a.G + r / D16, d = r % D16;
+        float x[2][8];
+        rotated16<DT>(a, a.q, (row0 + t) * a.ldq + static_cast<int64_t>(hq) * D, d, lo + t, x);
+        const int64_t at = ((row0 + t) * Hkv * a.G + hq) * D;
+        const KvPiece p = kv_piece(a, d);
+        store8<DT>(a.q_out, at + p.lo, x[0]);
+        store8<DT>(a.q_out, at + p.hi, x[1]);
+      }
+      if (!a.per_seq) break;
+      continue;
+    }
+
     const int pg = a.b.table[static_cast<int64_t>(b) * a.b.W + i];
     const bool valid = pg >= 0 && pg < a.c.n_pages;
     if (!valid && tid == 0) kv_flag(a.b.status, kKvBadPage);
-
     if (valid) {
       const int64_t ph = static_cast<int64_t>(pg) * Hkv + h;
       uint8_t *Kp = a.c.K + ph * P * D, *Vp = a.c.V + ph * P * D;
-      // 1. the largest finite magnitude of the new tokens, and the tokens that hold something else
-      for (int t = tid; t < nt; t += 256) bad_token[t] = 0;
+      // the old exponents, read before any thread writes the new ones
+      auto old_exp = [&](const float *s) {
+        const int e = keep ? static_cast<int>((__float_as_uint(s[ph]) >> 23) & 0xffu) - 127 : kKvExpMin;
+        return e > kKvExpMax ? kKvExpMax : (e < kKvExpMin ? kKvExpMin : e);
+      };
+      const int eko = old_exp(a.c.Ks), evo = old_exp(a.c.Vs);
+      for (int t = tid; t < nt; t += nthr) bad_token[t] = 0;
       __syncthreads();
-      float mk = 0.f, mv = 0.f;
-      for (int it = tid; it < nt * D8; it += 256) {
-        const int t = it / D8, d = it % D8 * 8;
-        float x[8];
+      // 1. the largest finite magnitude of the new tokens, and the tokens that hold something else
+      const int nk = nt * D16, g0 = keep >> 2, nv = (((keep + nt + 3) >> 2) - g0) * D4;
+      auto load_k = [&](int it, float (&x)[2][8]) {
+        const int t = it / D16;
+        rotated16<DT>(a, a.k, (row0 + t) * a.ldk + h * D, it % D16, lo + t, x);
+      };
+      auto load_v = [&](int it, float (&x)[4][4]) {  // slots 4 g .., dims d ..; slots that are not new: zero
+        const int t0 = 4 * (g0 + it / D4) - keep, d = it % D4 * 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int t = t0 + r;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[r][e] = 0.f;
+          if (t >= 0 && t < nt) load_n<DT>(a.v, (row0 + t) * a.ldv + h * D + d, x[r]);
+        }
+      };
+      float kx[2][8], vx[4][4], mk = 0.f, mv = 0.f;  // this thread's first pieces, held until their codes are known
+      auto see_k = [&](int it, const float (&x)[2][8]) {
         bool bad = false;
-        rotated8<DT>(a, a.k, (row0 + t) * a.ldk + h * D, d, lo + t, x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mk = fmaxf(mk, magnitude(x[e], bad));
-        load_n<DT>(a.v, (row0 + t) * a.ldv + h * D + d, x);
+        for (int e = 0; e < 16; ++e) mk = fmaxf(mk, magnitude(x[e >> 3][e & 7], bad));
+        if (bad) bad_token[it / D16] = 1;
+      };
+      auto see_v = [&](int it, const float (&x)[4][4]) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mv = fmaxf(mv, magnitude(x[e], bad));
-        if (bad) bad_token[t] = 1;
+        for (int r = 0; r < 4; ++r) {
+          bool bad = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mv = fmaxf(mv, magnitude(x[r][e], bad));
+          if (bad) bad_token[4 * (g0 + it / D4) - keep + r] = 1;
+        }
+      };
+      if (tid < nk) load_k(tid, kx);
+      if (tid < nv) load_v(tid, vx);
+      if (tid < nk) see_k(tid, kx);
+      if (tid < nv) see_v(tid, vx);
+      for (int it = tid + nthr; it < nk; it += nthr) {
+        float x[2][8];
+        load_k(it, x);
+        see_k(it, x);
+      }
+      for (int it = tid + nthr; it < nv; it += nthr) {
+        float x[4][4];
+        load_v(it, x);
+        see_v(it, x);
       }
       mk = wave_max(mk);
       mv = wave_max(mv);
@@ -258,83 +316,82 @@ __global__ void __launch_bounds__(256) k_kv_append(const KvAppendArgs a) {
         red[0][tid >> 6] = mk;
         red[1][tid >> 6] = mv;
       }
-      // the old exponents, read before any thread writes the new ones
-      const int eko = keep ? static_cast<int>((__float_as_uint(a.c.Ks[ph]) >> 23) & 0xffu) - 127 : kKvExpMin;
-      const int evo = keep ? static_cast<int>((__float_as_uint(a.c.Vs[ph]) >> 23) & 0xffu) - 127 : kKvExpMin;
       __syncthreads();
-      mk = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-      mv = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
-      const int ekn = page_exp(mk), evn = page_exp(mv);
-      const int eko_c = eko > kKvExpMax ? kKvExpMax : (eko < kKvExpMin ? kKvExpMin : eko);
-      const int evo_c = evo > kKvExpMax ? kKvExpMax : (evo < kKvExpMin ? kKvExpMin : evo);
-      const int ek = ekn > eko_c ? ekn : eko_c, ev = evn > evo_c ? evn : evo_c;
-      const bool grow_k = keep && ek > eko_c, grow_v = keep && ev > evo_c;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        mk = fmaxf(mk, w < nthr >> 6 ? red[0][w] : 0.f);
+        mv = fmaxf(mv, w < nthr >> 6 ? red[1][w] : 0.f);
+      }
+      const int ekn = page_exp(mk), evn = page_exp(mv), ek = ekn > eko ? ekn : eko, ev = evn > evo ? evn : evo;
       if (tid == 0) {
         a.c.Ks[ph] = exp2i(ek);
         a.c.Vs[ph] = exp2i(ev);
       }
       const float ik = exp2i(-ek), iv = exp2i(-ev);
-      const float fk = exp2i(eko_c - ek), fv = exp2i(evo_c - ev);  // no less than 2^-120
 
-      // 2. K: slots of eight dims; the kept ones only where the scale grows
-      for (int it = tid + (grow_k ? 0 : keep * D8); it < (keep + nt) * D8; it += 256) {
-        const int s = it / D8, d = it % D8 * 8;
-        u2 *dst = reinterpret_cast<u2 *>(Kp + s * D + d);
-        if (s < keep) {
-          const u2 w = *dst;
-          *dst = u2{recode4(w.x, fk), recode4(w.y, fk)};
-        } else if (bad_token[s - keep]) {
-          *dst = u2{0x7f7f7f7fu, 0x7f7f7f7fu};
-        } else {
-          const int t = s - keep;
-          float x[8];
-          rotated8<DT>(a, a.k, (row0 + t) * a.ldk + h * D, d, lo + t, x);
-          *dst = u2{codes4(x[0], x[1], x[2], x[3], ik), codes4(x[4], x[5], x[6], x[7], ik)};
-        }
-      }
-      // 3. V: four slots of four dims, 16 bytes; bytes of slots behind the new ones stay
-      for (int it = tid + (grow_v ? 0 : keep >> 2) * D4; it < ((keep + nt + 3) >> 2) * D4; it += 256) {
-        const int g = it / D4, d = it % D4 * 4;
-        u4 *dst = reinterpret_cast<u4 *>(Vp + (g * D + d) * 4);
-        const bool whole = 4 * g >= keep && 4 * g + 4 <= keep + nt;
-        u4 w = whole ? u4{0, 0, 0, 0} : *dst;
-        if (grow_v && 4 * g < keep) {
-          // the kept slots' bytes at the new scale (bytes of the others are written below, or put back)
-          const int cnt = keep - 4 * g;
-          const uint32_t m = cnt >= 4 ? 0xffffffffu : (1u << (8 * cnt)) - 1;
+      // 2. codes of the new tokens
+      auto put_k = [&](int it, const float (&x)[2][8]) {
+        const int t = it / D16;
+        const KvPiece d = kv_piece(a, it % D16);
+        const bool bad = bad_token[t];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = (recode4(w[e], fv) & m) | (w[e] & ~m);
+        for (int e = 0; e < 2; ++e) {
+          const u2 w = {codes4(x[e][0], x[e][1], x[e][2], x[e][3], ik), codes4(x[e][4], x[e][5], x[e][6], x[e][7], ik)};
+          *reinterpret_cast<u2 *>(Kp + (keep + t) * D + (e ? d.hi : d.lo)) = bad ? u2{0x7f7f7f7fu, 0x7f7f7f7fu} : w;
         }
-        uint32_t row[4] = {0, 0, 0, 0}, fresh = 0;  // codes of slot 4 g + r's four dims
+      };
+      auto put_v = [&](int it, const float (&x)[4][4]) {  // 16 bytes; those of slots that are not new stay
+        const int g = g0 + it / D4, t0 = 4 * g - keep;
+        u4 *dst = reinterpret_cast<u4 *>(Vp + (g * D + it % D4 * 4) * 4);
+        uint32_t row[4], fresh = 0;  // the codes of a slot's four dims
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int t = 4 * g + r - keep;
-          if (t >= 0 && t < nt) {
-            fresh |= 0xffu << (8 * r);
-            if (!bad_token[t]) {
-              float x[4];
-              load_n<DT>(a.v, (row0 + t) * a.ldv + h * D + d, x);
-              row[r] = codes4(x[0], x[1], x[2], x[3], iv);
-            }
-          }
+          const bool is_new = t0 + r >= 0 && t0 + r < nt;
+          row[r] = is_new && !bad_token[t0 + r] ? codes4(x[r][0], x[r][1], x[r][2], x[r][3], iv) : 0;
+          fresh |= is_new ? 0xffu << (8 * r) : 0;
         }
+        u4 w = {0, 0, 0, 0};
+        if (fresh != 0xffffffffu) w = *dst;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t col = ((row[0] >> (8 * e)) & 0xffu) | (((row[1] >> (8 * e)) & 0xffu) << 8) |
-                               (((row[2] >> (8 * e)) & 0xffu) << 16) | (((row[3] >> (8 * e)) & 0xffu) << 24);
-          w[e] = (w[e] & ~fresh) | col;
+          const uint32_t c = ((row[0] >> (8 * e)) & 0xffu) | (((row[1] >> (8 * e)) & 0xffu) << 8) |
+                             (((row[2] >> (8 * e)) & 0xffu) << 16) | (((row[3] >> (8 * e)) & 0xffu) << 24);
+          w[e] = (w[e] & ~fresh) | c;
         }
         *dst = w;
+      };
+      // where the scale grows, the kept tokens' codes first (a group of four slots may hold kept and new ones)
+      if (keep && ek > eko) {
+        const float f = exp2i(eko - ek);  // no less than 2^-120
+        for (int it = tid; it < keep * (D / 8); it += nthr) {
+          u2 *dst = reinterpret_cast<u2 *>(Kp) + it;
+          *dst = u2{recode4(dst->x, f), recode4(dst->y, f)};
+        }
       }
-    }
-    // 4. the query heads of this key head
-    if (a.q) {
-      for (int it = tid; it < nt * a.G * D8; it += 256) {
-        const int t = it / (a.G * D8), r = it % (a.G * D8);
-        const int hq = h * a.G + r / D8, d = r % D8 * 8;
-        float x[8];
-        rotated8<DT>(a, a.q, (row0 + t) * a.ldq + static_cast<int64_t>(hq) * D, d, lo + t, x);
-        store8<DT>(a.q_out, ((row0 + t) * Hkv * a.G + hq) * D + d, x);
+      if (keep && ev > evo) {
+        const float f = exp2i(evo - ev);
+        for (int it = tid; it < ((keep + 3) >> 2) * D4; it += nthr) {
+          u4 *dst = reinterpret_cast<u4 *>(Vp) + it;
+          const int left = keep - it / D4 * 4;
+          const uint32_t m = left >= 4 ? 0xffffffffu : (1u << (8 * left)) - 1;
+          u4 w = *dst;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = (recode4(w[e], f) & m) | (w[e] & ~m);
+          *dst = w;
+        }
+        __syncthreads();
+      }
+      if (tid < nk) put_k(tid, kx);
+      if (tid < nv) put_v(tid, vx);
+      for (int it = tid + nthr; it < nk; it += nthr) {
+        float x[2][8];
+        load_k(it, x);
+        put_k(it, x);
+      }
+      for (int it = tid + nthr; it < nv; it += nthr) {
+        float x[4][4];
+        load_v(it, x);
+        put_v(it, x);
       }
     }
     if (!a.per_seq) break;
@@ -343,12 +400,12 @@ __global__ void __launch_bounds__(256) k_kv_append(const KvAppendArgs a) {
 }
 
 template <int DT>
-static void launch_append(int D, const KvAppendArgs &a, unsigned grid, hipStream_t s) {
+static void launch_append(int D, const KvAppendArgs &a, dim3 grid, int threads, hipStream_t s) {
   switch (D) {
-    case 64: hipLaunchKernelGGL((k_kv_append<DT, 64>), dim3(grid), dim3(256), 0, s, a); break;
-    case 128: hipLaunchKernelGGL((k_kv_append<DT, 128>), dim3(grid), dim3(256), 0, s, a); break;
-    case 192: hipLaunchKernelGGL((k_kv_append<DT, 192>), dim3(grid), dim3(256), 0, s, a); break;
-    default: hipLaunchKernelGGL((k_kv_append<DT, 256>), dim3(grid), dim3(256), 0, s, a); break;
+    case 64: hipLaunchKernelGGL((k_kv_append<DT, 64>), grid, dim3(threads), 0, s, a); break;
+    case 128: hipLaunchKernelGGL((k_kv_append<DT, 128>), grid, dim3(threads), 0, s, a); break;
+    case 192: hipLaunchKernelGGL((k_kv_append<DT, 192>), grid, dim3(threads), 0, s, a); break;
+    default: hipLaunchKernelGGL((k_kv_append<DT, 256>), grid, dim3(threads), 0, s, a); break;
   }
 }
 
@@ -409,9 +466,14 @@ extern "C" int vybdq_kv_append(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs,
   VYBDQ_REQUIRE(units * Hkv < (int64_t(1) << 31), VYBDQ_ERR_SHAPE, "too many pages in one call");
   const int rc = kv_status_address(a.b.status);
   if (rc) return rc;
-  const unsigned grid = static_cast<unsigned>(units * Hkv);
+  // threads: a page's pieces of 16 dims (a decode step's 8 to 16: one wave, so that all workgroups of a batch are resident);
+  // query heads: about four pieces to a thread
+  const int64_t rows = max_new >= 1 && max_new < page ? max_new : T < page ? T : page;
+  const int threads = rows * (D / 16) <= 64 ? 64 : rows * (D / 16) <= 256 ? 256 : 512;
+  const int64_t q_wgs = q ? (rows * a.G * (D / 16) + 4 * threads - 1) / (4 * threads) : 0;
+  const dim3 grid(static_cast<unsigned>(units * Hkv), static_cast<unsigned>(1 + (q_wgs < 64 ? q_wgs : 64)));
   hipStream_t s = as_stream(stream);
-  VYBDQ_DISPATCH_IN(x_dt, DT, launch_append<DT>(static_cast<int>(D), a, grid, s));
+  VYBDQ_DISPATCH_IN(x_dt, DT, launch_append<DT>(static_cast<int>(D), a, grid, threads, s));
   return check_launch("vybdq_kv_append");
 }
 

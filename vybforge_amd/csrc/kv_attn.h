@@ -403,7 +403,7 @@ struct KvStep {
 // WR groups of 16 rows; the 4 / WR waves of a group take turns over the keys. (The groups' waves read the same codes; the
 // second reads come from the CU's own cache.)
 template <int D, int WR, bool TWO>
-__global__ void __launch_bounds__(256) k_kv_attn_keys(const KvAttnArgs a) {
+__global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_kv_attn_keys(const KvAttnArgs a) {
   constexpr int C = D / 64, R = 16 * WR, WT = 4 / WR, NQ = TWO ? 2 : 1;
   __shared__ float acc_w[4][16][D + 4];
   __shared__ float ml_w[4][2][16];
@@ -448,15 +448,14 @@ __global__ void __launch_bounds__(256) k_kv_attn_keys(const KvAttnArgs a) {
     };
 
     int st = t0 + wt;
-    const bool work = st < t1;
     int pg[2] = {0, 0};
     KvStep<C> even, odd;
-    if (work) {
+    if (st < t1) {
 #pragma unroll
       for (int n = 0; n < 2; ++n) pg[n] = page_of(st, n);
       fetch(even, st, pg);
 #pragma unroll
-      for (int n = 0; n < 2; ++n) pg[n] = page_of(st + WT, n);
+      for (int n = 0; n < 2; ++n) pg[n] = page_of(st + WT < t1 ? st + WT : t1 - 1, n);
     }
 
     KvRows<C, TWO> q[1];
@@ -514,21 +513,18 @@ __global__ void __launch_bounds__(256) k_kv_attn_keys(const KvAttnArgs a) {
         }
     };
 
-    // two steps to a turn, the next one's codes on their way while one is used, the page numbers one step further ahead
+    // two steps to a turn, the next one's codes on their way while one is used, the page numbers one step further ahead (behind
+    // the last step they are the last step's again: a load under a condition would have to be waited for where the ways meet)
+    auto held = [&](int x) { return x < t1 ? x : t1 - 1; };
     while (st < t1) {
-      const bool two = st + WT < t1;
-      if (two) {
-        fetch(odd, st + WT, pg);
+      fetch(odd, held(st + WT), pg);
 #pragma unroll
-        for (int n = 0; n < 2; ++n) pg[n] = page_of(st + 2 * WT, n);
-      }
+      for (int n = 0; n < 2; ++n) pg[n] = page_of(held(st + 2 * WT), n);
       use(even, st);
-      if (!two) break;
-      if (st + 2 * WT < t1) {
-        fetch(even, st + 2 * WT, pg);
+      if (st + WT >= t1) break;
+      fetch(even, held(st + 2 * WT), pg);
 #pragma unroll
-        for (int n = 0; n < 2; ++n) pg[n] = page_of(st + 3 * WT, n);
-      }
+      for (int n = 0; n < 2; ++n) pg[n] = page_of(held(st + 3 * WT), n);
       use(odd, st + WT);
       st += 2 * WT;
     }
@@ -632,7 +628,7 @@ __global__ void __launch_bounds__(64 * NW, NCT > 1 || D == 256 || (TWO && D == 1
       const uint8_t *base = (is_k(i) ? a.c.K + 64 * dims_of(i) : a.c.V + 256 * dims_of(i)) + at;
       code[i] = *reinterpret_cast<const u4 *>(base + (is_k(i) ? koff : voff));
     }
-    if (st + 1 < t1) peek(st + 1);
+    peek(st + 1 < t1 ? st + 1 : st);
   };
   auto write = [&](int st) {
     const int buf = st & 1, tok = t.k0 + 32 * st;
@@ -681,21 +677,21 @@ __global__ void __launch_bounds__(64 * NW, NCT > 1 || D == 256 || (TWO && D == 1
   }
   if (t0 < t1) {
     write(t0);
-    if (t0 + 1 < t1) fetch(t0 + 1);
+    fetch(t0 + 1 < t1 ? t0 + 1 : t0);
   }
   __syncthreads();
 
+  // (The last steps write and fetch as well, the last step again, which nothing reads: a load under a condition would have to
+  // be waited for where the two ways meet.)
   for (int st = t0; st < t1; ++st) {
     const int buf = st & 1, tok = t.k0 + 32 * st;
     const u4 m0 = block_meta(st, 0), m1 = block_meta(st, 1);
     h8 kf[2 * C];
 #pragma unroll
     for (int c = 0; c < 2 * C; ++c) kf[c] = tile[buf][c][lane];
-    if (st + 1 < t1) {
-      write(st + 1);
-      if (((st - t0) & 63) == 32 && st - t0 + 32 < t1 - t0) ask(((st - t0) >> 6) + 1);
-      if (st + 2 < t1) fetch(st + 2);
-    }
+    write(st + 1);
+    if (((st - t0) & 63) == 32 && st - t0 + 32 < t1 - t0) ask(((st - t0) >> 6) + 1);
+    fetch(st + 2 < t1 ? st + 2 : t1 - 1);
     f4 s[NCT][2];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {

@@ -614,34 +614,35 @@ class KvCache:
                    scale())
 
 
+# The checks of a decode step's calls are written out (a helper's messages would be formatted on every call): they
+# take about half of such a call's host time.
+
 def _kv_rows(x, shape, cache, what):
     """Device address and row stride of x [T, H, D], whose heads are consecutive within a row."""
     if x.shape != shape:
         raise ValueError(f"{what} must be {list(shape)}")
-    T, H, D = shape
-    st = x.stride()
-    if st[2] != 1 or (st[1] != D and H != 1):
+    row, head, one = x.stride()
+    if one != 1 or (head != shape[2] and shape[1] != 1):
         raise ValueError(f"{what}: the heads of a row must be consecutive")
     if x.get_device() != cache.index:
         raise ValueError(f"{what} must be on the cache's device")
-    return x.data_ptr(), st[0] if T > 1 else H * D
+    return x.data_ptr(), row if shape[0] > 1 else shape[1] * shape[2]
 
 
 def _kv_batch(cache, table, q_start, ctx):
-    """W, B, the addresses of the batch's int32 tables (read on the device by the calls), and the stream."""
+    """B, W and the addresses of the batch's int32 tables (read on the device by the calls)."""
     if table.dim() != 2:
         raise ValueError("page_table must be [B, W]")
     B, W = table.shape
     if q_start.shape != (B + 1,) or ctx.shape != (B,):
         raise ValueError(f"page_table holds {B} sequences: q_start must be [{B + 1}] and ctx [{B}]")
-    i32, at = torch.int32, cache.index
-    if table.dtype != i32 or q_start.dtype != i32 or ctx.dtype != i32:
+    if not table.dtype == q_start.dtype == ctx.dtype == torch.int32:
         raise ValueError("page_table, q_start and ctx must be int32")
     if not (table.is_contiguous() and q_start.is_contiguous() and ctx.is_contiguous()):
         raise ValueError("page_table, q_start and ctx must be contiguous")
-    if table.get_device() != at or q_start.get_device() != at or ctx.get_device() != at:
+    if not table.get_device() == q_start.get_device() == ctx.get_device() == cache.index:
         raise ValueError("page_table, q_start and ctx must be on the cache's device")
-    return W, B, table.data_ptr(), q_start.data_ptr(), ctx.data_ptr()
+    return B, W, table.data_ptr(), q_start.data_ptr(), ctx.data_ptr()
 
 
 def _kv_stream(cache):
@@ -660,9 +661,10 @@ def kv_append(cache, k, v, page_table, q_start, ctx, q=None, cos=None, sin=None,
     may be slices of one projection's output (heads of a row consecutive). cos, sin: float32 [n_pos, R / 2] (None: no
     rotation). max_new: most rows that a sequence has, if the host knows it (1 for a decode step)."""
     T, Hkv, D, dt = k.shape[0], cache.n_heads, cache.head_dim, k.dtype
-    W, B, tp, sp, cp = _kv_batch(cache, page_table, q_start, ctx)
-    kp, ldk = _kv_rows(k, (T, Hkv, D), cache, "k")
-    vp, ldv = _kv_rows(v, (T, Hkv, D), cache, "v")
+    B, W, tp, sp, cp = _kv_batch(cache, page_table, q_start, ctx)
+    shape = (T, Hkv, D)
+    kp, ldk = _kv_rows(k, shape, cache, "k")
+    vp, ldv = _kv_rows(v, shape, cache, "v")
     if v.dtype != dt:
         raise ValueError("v must have k's dtype")
     qp = op = ldq = Hq = 0
@@ -672,29 +674,34 @@ def kv_append(cache, k, v, page_table, q_start, ctx, q=None, cos=None, sin=None,
         Hq = q.shape[1]
         if Hq % Hkv or not Hq:
             raise ValueError("Hq must be a multiple of the cache's heads")
-        qp, ldq = _kv_rows(q, (T, Hq, D), cache, "q")
+        shape = (T, Hq, D)
+        qp, ldq = _kv_rows(q, shape, cache, "q")
         if q_out is None:
-            q_out = torch.empty((T, Hq, D), dtype=dt, device=q.device)
-        elif q_out.shape != (T, Hq, D) or q_out.dtype != dt or q_out.get_device() != cache.index:
+            q_out = q.new_empty(shape)
+        elif q_out.shape != shape or q_out.dtype != dt or q_out.get_device() != cache.index:
             raise ValueError(f"q_out must be [{T}, {Hq}, {D}] of q's dtype")
-        op = _ptr(q_out)
+        elif not q_out.is_contiguous():
+            raise ValueError("q_out must be contiguous")
+        op = q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out needs q")
     cosp = sinp = R = n_pos = 0
     if cos is not None and sin is not None:
-        if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        if cos.dim() != 2 or cos.shape != sin.shape or not cos.dtype == sin.dtype == torch.float32:
             raise ValueError("cos and sin must be float32 [n_pos, R / 2]")
-        if cos.get_device() != cache.index or sin.get_device() != cache.index:
+        if not cos.get_device() == sin.get_device() == cache.index:
             raise ValueError("cos and sin must be on the cache's device")
+        if not (cos.is_contiguous() and sin.is_contiguous()):
+            raise ValueError("cos and sin must be contiguous")
         n_pos, R = cos.shape
         R *= 2
-        cosp, sinp = _ptr(cos), _ptr(sin)
+        cosp, sinp = cos.data_ptr(), sin.data_ptr()
     elif cos is not None or sin is not None:
         raise ValueError("cos and sin come together")
     if max_new is None:
         max_new = 1 if T == B else T
-    call("vybdq_kv_append", *cache._args, kp, vp, qp, op, _dt(dt), ldk, ldv, ldq, Hq, cosp, sinp, R, n_pos,
-         1 if interleaved else 0, tp, W, sp, cp, T, B, max_new, _kv_stream(cache))
+    call("vybdq_kv_append", *cache._args, kp, vp, qp, op, _dt(dt), ldk, ldv, ldq, Hq, cosp, sinp, R, n_pos, interleaved, tp, W,
+         sp, cp, T, B, max_new, _kv_stream(cache))
     return q_out
 
 
@@ -722,17 +729,20 @@ class KvAttention:
             raise ValueError(f"the cache must hold {self.Hkv} heads of {D}")
         if self.index != cache.index:
             raise ValueError("the workspace must be on the cache's device")
-        W, B, tp, sp, cp = _kv_batch(cache, page_table, q_start, ctx)
-        qp, ldq = _kv_rows(q, (T, Hq, D), cache, "q")
+        B, W, tp, sp, cp = _kv_batch(cache, page_table, q_start, ctx)
+        shape = (T, Hq, D)
+        qp, ldq = _kv_rows(q, shape, cache, "q")
         if out is None:
-            out = torch.empty((T, Hq, D), dtype=dt, device=q.device)
-        elif out.shape != (T, Hq, D) or out.dtype != dt or out.get_device() != cache.index:
+            out = q.new_empty(shape)
+        elif out.shape != shape or out.dtype != dt or out.get_device() != cache.index:
             raise ValueError(f"out must be [{T}, {Hq}, {D}] of q's dtype")
+        elif not out.is_contiguous():
+            raise ValueError("out must be contiguous")
         stats = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if lse else None
         if max_new is None:
             max_new = 1 if T == B else T
-        call("vybdq_kv_attn", *cache._args, qp, _dt(dt), ldq, Hq, _ptr(out), _ptr(stats), tp, W, sp, cp, T, B, max_new,
-             max_ctx or 0, self.scale if scale is None else scale, 1 if causal else 0, window, self.ws_ptr, self.ws_bytes,
+        call("vybdq_kv_attn", *cache._args, qp, _dt(dt), ldq, Hq, out.data_ptr(), _ptr(stats), tp, W, sp, cp, T, B, max_new,
+             max_ctx or 0, self.scale if scale is None else scale, causal, window, self.ws_ptr, self.ws_bytes,
              _kv_stream(cache))
         return (out, stats) if lse else out
 
