@@ -292,7 +292,7 @@ def test_attention_split_keys(dev, rng, x, n):
     run_attention(dev, rng, [(n, 3001)], 4, 1, 64, 64, x, max_new=n)
 
 
-@pytest.mark.parametrize("variant", [0, 1, 3, 4])
+@pytest.mark.parametrize("variant", [0, 1, 2, 3])
 @pytest.mark.parametrize("splits", [1, 2, 7])
 @pytest.mark.parametrize("x,D", [("bf16", 128), ("f32", 256), ("f16", 64), ("f32", 128), ("bf16", 192)])
 def test_attention_every_variant(dev, rng, monkeypatch, variant, splits, x, D):
@@ -446,6 +446,40 @@ def test_offsets_past_32_bits(dev, rng):
     one = on(dev, np.array([0, 1], np.int32))[0]
     got = ops.KvAttention(Hkv, Hkv, D, dev)(q.to(dev), cache, t[0], one, t[2])
     check_attention(got, None, q.double().numpy(), small, np.array([[0, 1]]), np.array([0, 1]), ctx, D ** -0.5, True, 0, "f32")
+    ops.kv_status()
+
+
+@pytest.mark.parametrize("n,splits", [(1, None), (1, 256), (33, 256)])
+def test_attention_over_half_a_billion_keys(dev, rng, monkeypatch, n, splits):
+    """2^29 + 100 keys in 256 splits (steps times splits pass 32 bits), held in five pages that the table repeats, a quarter
+    of the context each and one at its end; their values have different means. A lane adds 2^29 / 32 / 256 steps of 8 weights,
+    each to half a unit in the last place of their sum: 2^19 2^-24 = 2^-5 of it; an output sums as many steps, at most four
+    roundings of 2^-23 to a step: 2^18 2^-23 = 2^-5 again. 2^-4 covers both."""
+    if splits:
+        monkeypatch.setenv("VYBDQ_KV_SPLITS", str(splits))
+    D, page = 64, 256
+    ctx = 2 ** 29 + 100
+    W = -(-ctx // page)
+    want = random_cache(rng, 5, 1, page, D)
+    want.k_scale[:] = 2.0 ** -9
+    want.v[:] = kvcache.e4m3_encode(rng.standard_normal(want.v.shape) * 40 + np.array([-200, -100, 100, 200, 0])[:, None, None, None, None])
+    want.v_scale[:] = 2.0 ** -7
+    table = (np.arange(W, dtype=np.int64) * 4 // W).astype(np.int32)
+    table[-1] = 4
+    cache = device_cache(dev, want)
+    q = torch.from_numpy(rng.standard_normal((n, 1, D)).astype(np.float32))
+    got, stats = ops.KvAttention(1, 1, D, dev)(q.to(dev), cache, *on(dev, table[None], np.array([0, n], np.int32), np.array([ctx], np.int32)),
+                                               causal=False, lse=True, max_new=n, max_ctx=ctx)
+    times = np.bincount(table[:-1], minlength=5).astype(np.float64)[:, None] * np.ones(page)
+    times[4, :100] += 1
+    k, v = (kvcache.e4m3_decode(x).astype(np.float64) for x in (want.k[:, 0], want.v[:, 0]))
+    v = v.transpose(0, 1, 3, 2).reshape(5, page, D) * want.v_scale[:, 0, None, None]
+    s = np.einsum("nd,pkd->npk", q[:, 0].double().numpy(), k) * want.k_scale[:, 0, None] * D ** -0.5
+    w = np.exp(s - s.max()) * times
+    l = w.sum((1, 2))
+    o = np.einsum("npk,pkd->nd", w, v) / l[:, None]
+    assert np.abs(stats[:, 0].double().cpu().numpy() - np.log(l) - s.max()).max() < 2.0 ** -4
+    assert np.abs(got[:, 0].double().cpu().numpy() - o).max() < 2.0 ** -4 * np.abs(v).max()
     ops.kv_status()
 
 

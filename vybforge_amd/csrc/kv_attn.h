@@ -108,13 +108,9 @@ __device__ __forceinline__ void store_n(void *p, bool bf16, int64_t i, const flo
   }
 }
 
-// Variants. 0, 1: k_kv_attn_keys, 16 or 32 query rows to a workgroup; 3, 4: k_kv_attn_rows, 64 or 128.
-constexpr int kKvVariants = 5;
-constexpr int kv_variant_rows(int variant) { return variant == 0 ? 16 : variant == 1 ? 32 : variant == 4 ? 128 : 64; }
-// workgroups of a variant on a CU (registers, LDS)
-constexpr int kv_variant_per_cu(int variant, int64_t D) {
-  return variant < 3 ? (D <= 128 ? 2 : 1) : variant == 4 ? 2 : D <= 128 ? 4 : D == 192 ? 3 : 2;
-}
+// Variants. 0, 1: k_kv_attn_keys, 16 or 32 query rows to a workgroup; 2, 3: k_kv_attn_rows, 64 or 128.
+constexpr int kKvVariants = 4;
+constexpr int kv_variant_rows(int variant) { return variant == 0 ? 16 : variant == 1 ? 32 : variant == 2 ? 64 : 128; }
 
 constexpr float kKvRef = 12.0f;    // a row's reference is 2^-12 of its largest weight when it is taken
 constexpr float kKvMove = 15.0f;   // and is taken anew once a weight would pass 2^15
@@ -168,6 +164,12 @@ __device__ __forceinline__ void kv_tile_keys(const KvAttnArgs &a, int R, KvTile 
   t.steps = k1 > t.k0 ? (k1 - t.k0 + 31) >> 5 : 0;
   t.free0 = a.window ? t.p0 + i_hi - a.window + 1 : 0;
   t.free1 = a.causal ? t.p0 + i_lo + 1 : t.ctx;
+}
+
+// The first step of split i of S. (No product of steps and splits: 2^25 steps in 256 splits pass 32 bits.)
+__device__ __forceinline__ int kv_split(int steps, int i, int S) {
+  const int rest = steps % S;
+  return steps / S * i + (i < rest ? i : rest);
 }
 
 // The 16 query rows r .. r + 15 as operands of S^T = K Q^T, one row per column: lane (col, g4) holds dims
@@ -422,8 +424,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_kv_attn_keys(const Kv
     const bool whole = S == 1 || t.r0 > 0;
     if (whole && split > 0) return;
     kv_tile_keys(a, R, t);
-    const int t0 = whole ? 0 : t.steps * split / S;
-    const int t1 = whole ? t.steps : t.steps * (split + 1) / S;
+    const int t0 = whole ? 0 : kv_split(t.steps, split, S), t1 = whole ? t.steps : kv_split(t.steps, split + 1, S);
 
     // pages of a step's two blocks; a block behind the sequence's end takes the last page (its keys are masked)
     auto page_of = [&](int st, int n) {
@@ -585,7 +586,7 @@ __global__ void __launch_bounds__(64 * NW, NCT > 1 || D == 256 || (TWO && D == 1
   KvTile t;
   if (!kv_tile_unit(a, R, gridDim.x / Hkv - 1 - blockIdx.x / Hkv, t)) return;
   kv_tile_keys(a, R, t);
-  const int t0 = t.steps * split / S, t1 = t.steps * (split + 1) / S;
+  const int t0 = kv_split(t.steps, split, S), t1 = kv_split(t.steps, split + 1, S);
   const int last_page = t.ctx > 0 ? (t.ctx - 1) >> ps : 0;
   const uint32_t koff = col * D + 16 * g4, voff = 4 * (g4 * D + 4 * col);
 

@@ -1,6 +1,7 @@
 // vybdq_kv_attn: checks, the choice of variant and key split, and the dispatch (kernel: kv_attn.h).
 #include "kv_attn.h"
 
+#include <cmath>
 #include <cstdlib>
 #include <string>
 
@@ -14,70 +15,91 @@ constexpr int64_t kKvPartRows = 131072;  // rows of split results that a workspa
 constexpr int64_t kKvArrivalBytes = 16384;
 
 struct KvShape {
-  int64_t D, Hkv, G, T, B, new_rows, steps;  // new_rows: most rows of a sequence; steps: of 32 keys, at most
+  int64_t D, Hkv, G, T, B, new_rows, tokens;  // new_rows, tokens: most rows and most keys of a sequence
   bool two, causal;
-  int64_t part_rows;  // rows of split results that the workspace holds
+  int64_t window, part_rows;  // part_rows: rows of split results that the workspace holds
 };
 struct KvPlan {
   int variant;
   int64_t units, splits;
+  double time;
 };
 
-// Key splits of a variant. Times in us as measured (MI355X):
+// How many splits fit the workspace. (k_kv_attn_keys counts arrivals there too.)
+static int64_t kv_held(const KvShape &s, int variant, int64_t wgs) {
+  if (variant < 2 && wgs * 4 > kKvArrivalBytes) return 1;
+  const int64_t held = s.part_rows / kv_variant_rows(variant) / wgs;
+  return held < 1 ? 1 : held < 256 ? held : 256;
+}
+
+// The plan of a variant: the number of key splits that takes the least time by these figures, in us as measured (MI355X).
 // - k_kv_attn_keys: a workgroup takes a step of 32 keys in (0.08 + 0.0011 D) WR us when it is not held up by the others
 //   (one sequence of 131072 keys, 8 heads of 128: 8 splits 108 us, 16 splits 60, 32 splits 47 = 5.8 TB/s), together they
-//   take 1 / 5.5 TB/s, not quite hiding one under the other, and the last one joins its tile's splits in about 0.02 D / 128 us a row and split (192 splits: 67 us).
-//   48 sequences of 2 k to 8 k keys: 1 split 117 us, 2 113, 4 105, 8 109.
-// - k_kv_attn_rows: rounds of workgroups, each about 6 steps of its own besides its keys, and a launch to join them.
-static int64_t kv_splits(const KvShape &s, int variant, int64_t wgs) {
-  const int64_t R = kv_variant_rows(variant), held = s.part_rows / R / wgs;
-  const int64_t slots = device_cu_count() * kv_variant_per_cu(variant, s.D);
-  if (const char *e = tuning_env("VYBDQ_KV_SPLITS")) return atoi(e) < 1 || held < 1 ? 1 : atoi(e) < held ? atoi(e) : held;
-  int64_t S = 1;
-  double best = 1e30;
+//   take 1 / 5.5 TB/s, not quite hiding one under the other, and the last one joins its tile's splits in about 0.02 D / 128
+//   us a row and split (192 splits: 67 us). 48 sequences of 2 k to 8 k keys: 1 split 117 us, 2 113, 4 105, 8 109.
+// - k_kv_attn_rows: a step of 32 keys takes 0.24 + 0.0028 D us alone on a CU and no less than 0.04 + 0.0023 D for each
+//   workgroup of a CU that runs one; two terms 1.22 and 1.39 times that, 128 rows 1.22 and 1.68 times. A workgroup's rows
+//   and results cost about 6 steps. Joining takes 4 us and the partial results' way to memory and back. (512 tokens
+//   behind 7680, 32 / 8 heads, D = 128 in 64 rows: 1 split 150 us, 2 114, 4 100, 8 107. Over 200 measured times of D = 64
+//   to 256 the figures are off by 10 % rms, and the number that they choose costs at most 13 % more than the best.)
+static KvPlan kv_plan_variant(const KvShape &s, int variant) {
+  const int64_t R = kv_variant_rows(variant), cus = device_cu_count();
+  const int64_t units = variant < 2 ? s.B : s.T * s.G / R + s.B, held = kv_held(s, variant, units * s.Hkv);
+  // workgroups that have keys: sequences of equal length
+  const int64_t even = (s.T + s.B - 1) / s.B * s.G;
+  const int64_t wgs = (variant < 2 ? s.B : s.B * ((even + R - 1) / R)) * s.Hkv;
+  int64_t keys = s.tokens;
+  if (s.window && s.window + R / s.G < keys) keys = s.window + R / s.G;
+  const int64_t steps = (keys + 31) / 32;
   const int64_t rows = s.new_rows * s.G < R ? s.new_rows * s.G : R;
-  const double read = static_cast<double>(wgs) * s.steps * 64 * s.D / 5.5e6;
-  for (int64_t n = 1; n <= 256 && (n == 1 || (n <= held && 4 * n <= s.steps)); ++n) {
-    const double rounds = static_cast<double>((wgs * n + slots - 1) / slots);
-    double time;
-    if (variant < 3) {
-      const double alone = rounds * s.steps / n * (0.08 + 0.0011 * s.D) * (R / 16);
-      time = (alone > read ? alone : read) + 0.3 * alone + (n > 1 ? 0.5 + 0.02 * n * rows * s.D / 128 : 0);
-    } else {
-      time = rounds * (static_cast<double>(s.steps) / n + 6) + (n > 1 ? 6 : 0);
+  const double alone = variant < 2 ? (0.08 + 0.0011 * s.D) * (R / 16)
+                                   : (0.24 + 0.0028 * s.D) * (s.two ? 1.22 : 1.0) * (R == 128 ? 1.22 : 1.0);
+  const double share = (0.04 + 0.0023 * s.D) * (s.two ? 1.39 : 1.0) * (R == 128 ? 1.68 : 1.0);
+  // of the most keys, how many a workgroup sees on average
+  const double seen = !s.causal || s.window ? 1.0 : s.new_rows < keys ? 1.0 - 0.5 * s.new_rows / keys : 0.5;
+  auto time_of = [&](int64_t n) {
+    const double mine = static_cast<double>(steps) / n;
+    if (variant < 2) {
+      const int64_t slots = cus * (s.D <= 128 ? 2 : 1);
+      const double own = alone * mine * ((wgs * n + slots - 1) / slots), read = static_cast<double>(wgs) * steps * 64 * s.D / 5.5e6;
+      return (own > read ? own : read) + 0.3 * own + (n > 1 ? 0.5 + 0.02 * n * rows * s.D / 128 : 0);
     }
-    if (time < best) {
-      best = time;
-      S = n;
+    const double one = (mine + 6) * alone, all = (mine * seen + 6) * share * ((wgs * n + cus - 1) / cus);
+    return sqrt(sqrt(one * one * one * one + all * all * all * all)) + (n > 1 ? 4 + 1.2e-6 * wgs * n * R * (s.D + 2) : 0);
+  };
+  KvPlan p{variant, units, 1, 0};
+  if (const char *e = tuning_env("VYBDQ_KV_SPLITS")) {
+    p.splits = atoi(e) < 1 ? 1 : atoi(e) < held ? atoi(e) : held;
+    return p;
+  }
+  p.time = time_of(1);
+  for (int64_t n = 2; n <= held && 4 * n <= steps; ++n) {
+    const double time = time_of(n);
+    if (time < p.time) {
+      p.time = time;
+      p.splits = n;
     }
   }
-  return S;
+  return p;
 }
 
 // Variant by the rows that share keys. Up to 32 (a decode step, drafted tokens): k_kv_attn_keys, whose waves need not
 // wait for each other (16 sequences of 8 tokens, 4 heads a key head, 6000 keys: D = 128 46 us against 53 with
 // k_kv_attn_rows, D = 256 98 against 123); more: k_kv_attn_rows, whose waves share the conversion (16 tokens: 34 us against
 // 68). Its tiles of 128 rows need half the cache reads, those of 64 keep more waves and even out better: 128 rows only
-// where D = 128 leaves room for their registers and they still fill the chip (512 tokens behind 3584, 4 sequences: 158 us
-// against 183; a prompt of 2048: 67 against 60, of 4096: 182 against 184).
+// where D = 128 leaves room for their registers and the figures above give them the lesser time (512 tokens behind 7680: 92
+// us against 100; a prompt of 2048: 64 against 57).
 static KvPlan kv_plan(const KvShape &s) {
   const int64_t rows = s.new_rows * s.G;
-  int variant = rows <= 16 ? 0 : rows <= 32 ? 1 : 3;
-  bool given = false;
+  const bool wide = s.D == 128 && !s.two;
   if (const char *e = tuning_env("VYBDQ_KV_VARIANT")) {
-    variant = atoi(e) < 0 || atoi(e) >= kKvVariants ? variant : atoi(e);
-    given = true;
+    const int v = atoi(e);
+    if (v >= 0 && v < (wide ? kKvVariants : kKvVariants - 1)) return kv_plan_variant(s, v);
   }
-  auto make = [&](int v) {
-    const int64_t units = v < 2 ? s.B : s.T * s.G / kv_variant_rows(v) + s.B, wgs = units * s.Hkv;
-    return KvPlan{v, units, wgs * 4 <= kKvArrivalBytes ? kv_splits(s, v, wgs) : 1};
-  };
-  if (s.D == 128 && !s.two && (given ? variant == 4 : variant == 3)) {
-    const KvPlan p = make(4);
-    const double seen = s.causal ? 1.0 - 0.5 * s.new_rows / (32.0 * s.steps) : 1.0;
-    if (given || p.units * s.Hkv * p.splits * seen >= 0.75 * device_cu_count() * kv_variant_per_cu(4, s.D)) return p;
-  }
-  return make(variant == 4 ? 3 : variant);
+  const KvPlan p = kv_plan_variant(s, rows <= 16 ? 0 : rows <= 32 ? 1 : 2);
+  if (p.variant < 2 || !wide) return p;
+  const KvPlan q = kv_plan_variant(s, 3);
+  return q.time < p.time ? q : p;
 }
 
 }  // namespace vybdq
@@ -120,7 +142,7 @@ extern "C" int vybdq_kv_attn(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs, i
   const bool two = x_dt == VYBDQ_F32;
   const int64_t cap = W * page, tokens = max_ctx >= 1 && max_ctx < cap ? max_ctx : cap;
   const int64_t most = max_new >= 1 && max_new < T ? max_new : T;
-  const KvShape shape{D, Hkv, G, T, B, most, (tokens + 31) / 32, two, causal != 0,
+  const KvShape shape{D, Hkv, G, T, B, most, tokens, two, causal != 0, window,
                       ws && ws_bytes > kKvArrivalBytes ? (ws_bytes - kKvArrivalBytes) / ((D + 2) * 4) : 0};
   KvPlan plan = kv_plan(shape);
   VYBDQ_REQUIRE(plan.units * Hkv < (int64_t(1) << 31), VYBDQ_ERR_SHAPE, "too many rows in one call");

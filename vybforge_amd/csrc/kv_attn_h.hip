@@ -14,7 +14,7 @@ template <int D>
 static void launch(int variant, const KvAttnArgs &a, dim3 grid, hipStream_t s) {
   if (variant == 0) hipLaunchKernelGGL((k_kv_attn_keys<D, 1, false>), grid, dim3(256), 0, s, a);
   else if (variant == 1) hipLaunchKernelGGL((k_kv_attn_keys<D, 2, false>), grid, dim3(256), 0, s, a);
-  else if (variant == 3) launch_rows<D, 1>(a, grid, s);
+  else if (variant == 2) launch_rows<D, 1>(a, grid, s);
   else if constexpr (D == 128) launch_rows<D, 2>(a, grid, s);
 }
 
