@@ -336,8 +336,76 @@ struct KvSink {
     }
   }
 
-  // All S splits' results of the tile, joined in split order by the last workgroup to arrive. The partials are stored
-  // through the XCD's L2 and have completed before the arrival is counted; they are read by device-coherent loads.
+  static __device__ __forceinline__ f2 load_through(const float *p) {
+    return __builtin_bit_cast(f2, __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  }
+
+  // Items it, it + step, .. (N of them, those before `items`) of a tile's rows from S splits' results at `all`: item i is 4 dims
+  // of a row. Joined in split order, with N W splits' loads to a round trip. THROUGH: read past the caches, 8 bytes at a time.
+  template <int N, int W, bool THROUGH>
+  __device__ __forceinline__ void finish_joined(const float *all, int S, int it, int step, int items) const {
+    constexpr int64_t kSize = static_cast<int64_t>(R) * (D + 2);
+    int r[N], d[N];
+    float mr[N], lr[N], x[N][4];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = it + i * step < items ? it + i * step : it;
+      r[i] = at / (D / 4);
+      d[i] = at % (D / 4) * 4;
+      mr[i] = kKvNone;
+      lr[i] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[i][e] = 0.f;
+    }
+#pragma unroll 1
+    for (int w0 = 0; w0 < S; w0 += W) {
+      f2 ml[N][W];
+      f4 v[N][W];
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float *pw = all + (w0 + w < S ? w0 + w : S - 1) * kSize;
+          const float *pv = pw + 2 * R + r[i] * D + d[i];
+          if constexpr (THROUGH) {
+            ml[i][w] = load_through(pw + 2 * r[i]);
+            const f2 lo = load_through(pv), hi = load_through(pv + 2);
+            v[i][w] = f4{lo.x, lo.y, hi.x, hi.y};
+          } else {
+            ml[i][w] = reinterpret_cast<const f2 *>(pw)[r[i]];
+            v[i][w] = *reinterpret_cast<const f4 *>(pv);
+          }
+        }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float now = mr[i];
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+          if (w0 + w < S) now = fmaxf(now, ml[i][w].x);
+        const float f0 = __builtin_amdgcn_exp2f(mr[i] - now);
+        mr[i] = now;
+        lr[i] *= f0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][e] *= f0;
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+          if (w0 + w < S) {
+            const float f = __builtin_amdgcn_exp2f(ml[i][w].x - now);
+            lr[i] = __builtin_fmaf(f, ml[i][w].y, lr[i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[i][e] = __builtin_fmaf(f, v[i][w][e], x[i][e]);
+          }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (it + i * step < items) finish<4>(r[i], mr[i], lr[i], d[i], x[i]);
+  }
+
+  // All S splits' results of the tile, joined by the last workgroup to arrive. They are stored through the XCD's L2 and
+  // have completed before the arrival is counted. Few are read past the caches; for many, what the caches hold of them is
+  // dropped first, 1 us that 16-byte reads make good (5 splits, 30 rows of 256 dims: 44.0 us against 46.0 past the caches, 12
+  // of 256 33.2 in both, 12 of 128 19.6 past the caches against 20.1, 6 of 128 18.0 against 19.1).
   __device__ __forceinline__ void join(int S, bool &is_last) const {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -349,45 +417,15 @@ struct KvSink {
     }
     __syncthreads();
     if (!is_last) return;
-    constexpr int64_t kSize = static_cast<int64_t>(R) * (D + 2);
-    const float *all = a.part + blockIdx.x * S * kSize;
-    const int n_rows = t.rows - t.r0 < R ? t.rows - t.r0 : R;
-    for (int it = threadIdx.x; it < n_rows * (D / 4); it += blockDim.x) {
-      const int r = it / (D / 4), d = it % (D / 4) * 4;
-      float mr = kKvNone, lr = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int w0 = 0; w0 < S; w0 += 8) {  // 24 independent loads to a round trip
-        uint64_t ml[8], v[8][2];
-#pragma unroll
-        for (int w = 0; w < 8; ++w) {
-          const float *pw = all + (w0 + w < S ? w0 + w : S - 1) * kSize;
-          ml[w] = __hip_atomic_load(reinterpret_cast<const uint64_t *>(pw) + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            v[w][e] = __hip_atomic_load(reinterpret_cast<const uint64_t *>(pw + 2 * R + r * D + d) + e, __ATOMIC_RELAXED,
-                                        __HIP_MEMORY_SCOPE_AGENT);
-        }
-        float now = mr;
-#pragma unroll
-        for (int w = 0; w < 8; ++w)
-          if (w0 + w < S) now = fmaxf(now, __uint_as_float(static_cast<uint32_t>(ml[w])));
-        const float f0 = __builtin_amdgcn_exp2f(mr - now);
-        lr *= f0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] *= f0;
-        mr = now;
-#pragma unroll
-        for (int w = 0; w < 8; ++w)
-          if (w0 + w < S) {
-            const float f = __builtin_amdgcn_exp2f(__uint_as_float(static_cast<uint32_t>(ml[w])) - now);
-            lr = __builtin_fmaf(f, __uint_as_float(static_cast<uint32_t>(ml[w] >> 32)), lr);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              x[2 * e] = __builtin_fmaf(f, __uint_as_float(static_cast<uint32_t>(v[w][e])), x[2 * e]);
-              x[2 * e + 1] = __builtin_fmaf(f, __uint_as_float(static_cast<uint32_t>(v[w][e] >> 32)), x[2 * e + 1]);
-            }
-          }
-      }
-      finish<4>(r, mr, lr, d, x);
+    const float *all = a.part + static_cast<int64_t>(blockIdx.x) * S * (R * (D + 2));
+    const int n_rows = t.rows - t.r0 < R ? t.rows - t.r0 : R, items = n_rows * (D / 4);
+    if (items <= 512) {
+#pragma unroll 1
+      for (int it = threadIdx.x; it < items; it += 256) finish_joined<1, 8, true>(all, S, it, 256, items);
+    } else {
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+#pragma unroll 1
+      for (int it = threadIdx.x; it < items; it += 1024) finish_joined<4, 4, false>(all, S, it, 256, items);
     }
   }
 };
@@ -545,6 +583,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_kv_attn_keys(const Kv
       ml_w[wave][1][col] = l[0];
     }
     __syncthreads();
+#pragma unroll 1
     for (int it = threadIdx.x; it < R * (D / 4); it += 256) {
       const int r = it / (D / 4), d = it % (D / 4) * 4, r16 = r & 15, w0 = r >> 4;
       float mr = kKvNone, lr = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
@@ -748,45 +787,13 @@ __global__ void __launch_bounds__(64 * NW, NCT > 1 || D == 256 || (TWO && D == 1
 // time. In the same launch, as k_kv_attn_keys does it, one workgroup would read all S R (D + 2) floats alone.
 template <int D, int R, bool TWO>
 __global__ void __launch_bounds__(256) k_kv_attn_join(const KvAttnArgs a, int S) {
-  constexpr int64_t kSize = static_cast<int64_t>(R) * (D + 2);
   const int Hkv = a.c.Hkv, h = blockIdx.x % Hkv;
   KvTile t;
   if (!kv_tile_unit(a, R, gridDim.x / Hkv - 1 - blockIdx.x / Hkv, t)) return;
-  const float *all = a.part + blockIdx.x * S * kSize;
+  const float *all = a.part + static_cast<int64_t>(blockIdx.x) * S * (R * (D + 2));
   const KvSink<D, R, TWO, false> sink{a, t, h, true, nullptr};
-  for (int it = threadIdx.x; it < 8 * (D / 4); it += 256) {
-    const int r = blockIdx.y * 8 + it / (D / 4), d = it % (D / 4) * 4;
-    if (t.r0 + r >= t.rows) return;
-    float mr = kKvNone, lr = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int w0 = 0; w0 < S; w0 += 4) {  // 8 independent loads to a round trip
-      f2 ml[4];
-      f4 v[4];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float *pw = all + (w0 + w < S ? w0 + w : S - 1) * kSize;
-        ml[w] = reinterpret_cast<const f2 *>(pw)[r];
-        v[w] = *reinterpret_cast<const f4 *>(pw + 2 * R + r * D + d);
-      }
-      float now = mr;
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        if (w0 + w < S) now = fmaxf(now, ml[w].x);
-      const float f0 = __builtin_amdgcn_exp2f(mr - now);
-      mr = now;
-      lr *= f0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] *= f0;
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        if (w0 + w < S) {
-          const float f = __builtin_amdgcn_exp2f(ml[w].x - now);
-          lr = __builtin_fmaf(f, ml[w].y, lr);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(f, v[w][e], x[e]);
-        }
-    }
-    sink.template finish<4>(r, mr, lr, d, x);
-  }
+  const int r0 = blockIdx.y * 8, left = t.rows - t.r0 - r0, items = (left < 8 ? left : 8) * (D / 4);
+  for (int it = threadIdx.x; it < items; it += 256) sink.template finish_joined<1, 4, false>(all, S, r0 * (D / 4) + it, 256, r0 * (D / 4) + items);
 }
 
 }  // namespace vybdq

@@ -35,8 +35,8 @@ static int64_t kv_held(const KvShape &s, int variant, int64_t wgs) {
 // The plan of a variant: the number of key splits that takes the least time by these figures, in us as measured (MI355X).
 // - k_kv_attn_keys: a workgroup takes a step of 32 keys in (0.08 + 0.0011 D) WR us when it is not held up by the others
 //   (one sequence of 131072 keys, 8 heads of 128: 8 splits 108 us, 16 splits 60, 32 splits 47 = 5.8 TB/s), together they
-//   take 1 / 5.5 TB/s, not quite hiding one under the other, and the last one joins its tile's splits in about 0.02 D / 128
-//   us a row and split (192 splits: 67 us). 48 sequences of 2 k to 8 k keys: 1 split 117 us, 2 113, 4 105, 8 109.
+//   take 1 / 5.5 TB/s, not quite hiding one under the other, and the last one joins its tile's splits at about 1 us a
+//   round trip (192 splits of 4 rows: 67 us against 47). 48 sequences of 2 k to 8 k keys: 1 split 117 us, 2 113, 4 105, 8 109.
 // - k_kv_attn_rows: a step of 32 keys takes 0.24 + 0.0028 D us alone on a CU and no less than 0.04 + 0.0023 D for each
 //   workgroup of a CU that runs one; two terms 1.22 and 1.39 times that, 128 rows 1.22 and 1.68 times. A workgroup's rows
 //   and results cost about 6 steps. Joining takes 4 us and the partial results' way to memory and back. (512 tokens
@@ -57,12 +57,16 @@ static KvPlan kv_plan_variant(const KvShape &s, int variant) {
   const double share = (0.04 + 0.0023 * s.D) * (s.two ? 1.39 : 1.0) * (R == 128 ? 1.68 : 1.0);
   // of the most keys, how many a workgroup sees on average
   const double seen = !s.causal || s.window ? 1.0 : s.new_rows < keys ? 1.0 - 0.5 * s.new_rows / keys : 0.5;
+  const int64_t items = rows * (s.D / 4);
+  auto join = [&](int64_t n) {  // round trips of the last workgroup
+    return items <= 512 ? 1 + 0.7 * ((n + 7) / 8) * ((items + 255) / 256) : 4 + 1.0 * ((n + 3) / 4) * ((items + 1023) / 1024);
+  };
   auto time_of = [&](int64_t n) {
     const double mine = static_cast<double>(steps) / n;
     if (variant < 2) {
       const int64_t slots = cus * (s.D <= 128 ? 2 : 1);
       const double own = alone * mine * ((wgs * n + slots - 1) / slots), read = static_cast<double>(wgs) * steps * 64 * s.D / 5.5e6;
-      return (own > read ? own : read) + 0.3 * own + (n > 1 ? 0.5 + 0.02 * n * rows * s.D / 128 : 0);
+      return (own > read ? own : read) + 0.3 * own + (n > 1 ? join(n) : 0);
     }
     const double one = (mine + 6) * alone, all = (mine * seen + 6) * share * ((wgs * n + cus - 1) / cus);
     return sqrt(sqrt(one * one * one * one + all * all * all * all)) + (n > 1 ? 4 + 1.2e-6 * wgs * n * R * (s.D + 2) : 0);
