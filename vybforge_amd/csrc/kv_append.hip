@@ -16,7 +16,12 @@
 // A thread reads 16 dims of a token's k (both halves of its pairs) and 4 dims of four slots of v and keeps them in registers
 // until the page's largest magnitude is known (512 threads: all of a page of 64 tokens of 128 dims); of a larger page the
 // rest is read again (from L2). Query heads are rotated by workgroups of their own (gridDim.y), which need not wait for a page's
-// magnitude.
+// magnitude; a thread rotates up to four heads of its group by the angles that it has read (one head each: 39.9 us
+// against 36.5 below).
+//
+// Bound by memory when there is much of it, MI355X: five prompts of 1 to 1638 tokens, 32 / 8 heads of 128, bf16, 127 MB:
+// 36.5 us, 3.5 TB/s; 16 of 256 in float32, 85 MB: 20.9 us, 4.1 TB/s (a large copy runs at 4.7). A decode step is bound by
+// the launch: 7 us on the GPU for one sequence as for 128.
 #include "kv.h"
 
 #include <mutex>
@@ -59,29 +64,37 @@ struct KvAppendArgs {
   int32_t per_seq;  // 1: workgroup (b, head) takes every page of sequence b; 0: one page per workgroup
 };
 
+// 8 elements as they lie in memory, and as float32
 template <int DT>
-__device__ __forceinline__ void load_n(const void *p, int64_t i, float (&x)[8]) {
-  if constexpr (DT == VYBDQ_F32) {
-    const f4 *s = reinterpret_cast<const f4 *>(static_cast<const float *>(p) + i);
-    const f4 a = s[0], b = s[1];
+struct KvEight {
+  u4 w[DT == VYBDQ_F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void *p, int64_t i) {
+    const u4 *s = reinterpret_cast<const u4 *>(static_cast<const uint8_t *>(p) + i * (DT == VYBDQ_F32 ? 4 : 2));
+    w[0] = s[0];
+    if constexpr (DT == VYBDQ_F32) w[1] = s[1];
+  }
+  __device__ __forceinline__ void unpack(float (&x)[8]) const {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      x[j] = a[j];
-      x[4 + j] = b[j];
-    }
-  } else if constexpr (DT == VYBDQ_F16) {
-    const h8 a = *reinterpret_cast<const h8 *>(static_cast<const _Float16 *>(p) + i);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = static_cast<float>(a[j]);
-  } else {
-    const u4 a = *reinterpret_cast<const u4 *>(static_cast<const uint16_t *>(p) + i);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t w = a[j];
-      x[2 * j] = __uint_as_float(w << 16);
-      x[2 * j + 1] = __uint_as_float(w & 0xffff0000u);
+      if constexpr (DT == VYBDQ_F32) {
+        x[j] = __uint_as_float(w[0][j]);
+        x[4 + j] = __uint_as_float(w[1][j]);
+      } else if constexpr (DT == VYBDQ_F16) {
+        x[2 * j] = half_bits_to_f32(w[0][j] & 0xffffu);
+        x[2 * j + 1] = half_bits_to_f32(w[0][j] >> 16);
+      } else {
+        x[2 * j] = __uint_as_float(w[0][j] << 16);
+        x[2 * j + 1] = __uint_as_float(w[0][j] & 0xffff0000u);
+      }
     }
   }
+};
+
+template <int DT>
+__device__ __forceinline__ void load_n(const void *p, int64_t i, float (&x)[8]) {
+  KvEight<DT> r;
+  r.load(p, i);
+  r.unpack(x);
 }
 
 template <int DT>
@@ -105,6 +118,10 @@ __device__ __forceinline__ void load_n(const void *p, int64_t i, float (&x)[4]) 
   }
 }
 
+// query heads that a thread rotates by the same angles at most: 64 bytes of cos and sin go with 32 of a bf16 head's piece (of a
+// float32 head's 64: two heads 20.8 us where four take 23.3)
+constexpr int kv_turn_heads(int dt) { return dt == VYBDQ_F32 ? 2 : 4; }
+
 // Piece i of a row's D / 16: 16 dims that hold both members of their pairs, 8 from dim lo and 8 from dim hi.
 struct KvPiece {
   int lo, hi;
@@ -115,30 +132,29 @@ __device__ __forceinline__ KvPiece kv_piece(const KvAppendArgs &a, int i) {
   return {16 * i, 16 * i + 8};  // (pairs of neighbours, or dims behind R)
 }
 
-// Piece i of the row at element `at`, rotated to position pos.
-template <int DT>
-__device__ __forceinline__ void rotated16(const KvAppendArgs &a, const void *p, int64_t at, int i, int pos, float (&x)[2][8]) {
-#pragma clang fp contract(off)
-  const KvPiece d = kv_piece(a, i);
-  load_n<DT>(p, at + d.lo, x[0]);
-  load_n<DT>(p, at + d.hi, x[1]);
-  if (16 * i >= a.R) return;
-  const int64_t row = static_cast<int64_t>(pos) * (a.R >> 1) + 8 * i;
-  float c[8], s[8];
+// cos and sin of piece i's pairs at position pos.
+__device__ __forceinline__ void kv_turn(const KvAppendArgs &a, int i, int pos, float (&c)[8], float (&s)[8]) {
+  const int64_t row = 16 * i < a.R ? static_cast<int64_t>(pos) * (a.R >> 1) + 8 * i : 0;
+  if (a.R == 0) return;
   load_n<VYBDQ_F32>(a.cosv, row, c);
   load_n<VYBDQ_F32>(a.sinv, row, s);
-  auto turn = [](float &u, float &w, float cj, float sj) {
-    const float uc = u * cj, ws = w * sj, wc = w * cj, us = u * sj;
-    u = uc - ws;
-    w = wc + us;
-  };
-  if (a.inter) {
+}
+
+// Piece i of a row, rotated.
+__device__ __forceinline__ void rotate16(const KvAppendArgs &a, int i, const float (&c)[8], const float (&s)[8], float (&x)[2][8]) {
+#pragma clang fp contract(off)
+  if (16 * i >= a.R) return;
+  // (by selects: two branches would be merged into one that indexes x by a variable, in scratch memory)
+  float u[8], v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) turn(x[j >> 2][2 * (j & 3)], x[j >> 2][2 * (j & 3) + 1], c[j], s[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) turn(x[0][j], x[1][j], c[j], s[j]);
+  for (int j = 0; j < 8; ++j) {
+    const float p = a.inter ? x[j >> 2][2 * (j & 3)] : x[0][j], q = a.inter ? x[j >> 2][2 * (j & 3) + 1] : x[1][j];
+    const float pc = p * c[j], qs = q * s[j], qc = q * c[j], ps = p * s[j];
+    u[j] = pc - qs;
+    v[j] = qc + ps;
   }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e >> 3][e & 7] = a.inter ? (e & 1 ? v[e >> 1] : u[e >> 1]) : e < 8 ? u[e & 7] : v[e & 7];
 }
 
 template <int DT>
@@ -228,27 +244,47 @@ __global__ void __launch_bounds__(512, 4) k_kv_append(const KvAppendArgs a) {
   }
   const int p0 = sq.ctx - sq.n;  // position of the first row
   const int last = (sq.ctx - 1) >> a.c.ps;
+  if (blockIdx.y > 0) {  // query heads
+    for (int64_t i = (p0 >> a.c.ps) + j; i <= last; ++i) {
+      const int base = static_cast<int>(i) << a.c.ps, lo = p0 > base ? p0 : base;
+      const int nt = (sq.ctx - base < P ? sq.ctx - base : P) - (lo - base);
+      const int64_t row0 = sq.s0 + (lo - p0);
+      constexpr int kHeads = kv_turn_heads(DT);
+      const int chunks = (a.G + kHeads - 1) / kHeads, heads = (a.G + chunks - 1) / chunks, per_token = chunks * D16;
+      for (int it = (blockIdx.y - 1) * nthr + tid; it < nt * per_token; it += (gridDim.y - 1) * nthr) {
+        const int t = it / per_token, r = it % per_token, d = r % D16, g0 = r / D16 * heads;
+        const KvPiece p = kv_piece(a, d);
+        const int64_t from = (row0 + t) * a.ldq + (h * a.G + g0) * D, to = ((row0 + t) * Hkv * a.G + h * a.G + g0) * D;
+        float c[8], s[8];
+        kv_turn(a, d, lo + t, c, s);
+        KvEight<DT> raw[kHeads][2];
+#pragma unroll
+        for (int g = 0; g < kHeads; ++g) {
+          const int64_t at = from + (g < heads && g0 + g < a.G ? g : 0) * D;
+          raw[g][0].load(a.q, at + p.lo);
+          raw[g][1].load(a.q, at + p.hi);
+        }
+#pragma unroll
+        for (int g = 0; g < kHeads; ++g) {
+          if (g < heads && g0 + g < a.G) {
+            float x[2][8];
+            raw[g][0].unpack(x[0]);
+            raw[g][1].unpack(x[1]);
+            rotate16(a, d, c, s, x);
+            store8<DT>(a.q_out, to + g * D + p.lo, x[0]);
+            store8<DT>(a.q_out, to + g * D + p.hi, x[1]);
+          }
+        }
+      }
+      if (!a.per_seq) break;
+    }
+    return;
+  }
   for (int64_t i = (p0 >> a.c.ps) + j; i <= last; ++i) {
     const int base = static_cast<int>(i) << a.c.ps;
     const int lo = p0 > base ? p0 : base, hi = sq.ctx < base + P ? sq.ctx : base + P;
     const int keep = lo - base, nt = hi - lo;
     const int64_t row0 = sq.s0 + (lo - p0);
-
-    if (blockIdx.y > 0) {  // query heads
-      const int per_token = a.G * D16;
-      for (int it = (blockIdx.y - 1) * nthr + tid; it < nt * per_token; it += (gridDim.y - 1) * nthr) {
-        const int t = it / per_token, r = it % per_token;
-        const int hq = h * a.G + r / D16, d = r % D16;
-        float x[2][8];
-        rotated16<DT>(a, a.q, (row0 + t) * a.ldq + static_cast<int64_t>(hq) * D, d, lo + t, x);
-        const int64_t at = ((row0 + t) * Hkv * a.G + hq) * D;
-        const KvPiece p = kv_piece(a, d);
-        store8<DT>(a.q_out, at + p.lo, x[0]);
-        store8<DT>(a.q_out, at + p.hi, x[1]);
-      }
-      if (!a.per_seq) break;
-      continue;
-    }
 
     const int pg = a.b.table[static_cast<int64_t>(b) * a.b.W + i];
     const bool valid = pg >= 0 && pg < a.c.n_pages;
@@ -268,7 +304,14 @@ __global__ void __launch_bounds__(512, 4) k_kv_append(const KvAppendArgs a) {
       const int nk = nt * D16, g0 = keep >> 2, nv = (((keep + nt + 3) >> 2) - g0) * D4;
       auto load_k = [&](int it, float (&x)[2][8]) {
         const int t = it / D16;
-        rotated16<DT>(a, a.k, (row0 + t) * a.ldk + h * D, it % D16, lo + t, x);
+        const KvPiece p = kv_piece(a, it % D16);
+        const int64_t at = (row0 + t) * a.ldk + h * D;
+        load_n<DT>(a.k, at + p.lo, x[0]);
+        load_n<DT>(a.k, at + p.hi, x[1]);
+        if (16 * (it % D16) >= a.R) return;
+        float c[8], s[8];
+        kv_turn(a, it % D16, lo + t, c, s);
+        rotate16(a, it % D16, c, s, x);
       };
       auto load_v = [&](int it, float (&x)[4][4]) {  // slots 4 g .., dims d ..; slots that are not new: zero
         const int t0 = 4 * (g0 + it / D4) - keep, d = it % D4 * 4;
@@ -467,10 +510,10 @@ extern "C" int vybdq_kv_append(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs,
   const int rc = kv_status_address(a.b.status);
   if (rc) return rc;
   // threads: a page's pieces of 16 dims (a decode step's 8 to 16: one wave, so that all workgroups of a batch are resident);
-  // query heads: about four pieces to a thread
+  // query heads: one turn of a piece to a thread
   const int64_t rows = max_new >= 1 && max_new < page ? max_new : T < page ? T : page;
   const int threads = rows * (D / 16) <= 64 ? 64 : rows * (D / 16) <= 256 ? 256 : 512;
-  const int64_t q_wgs = q ? (rows * a.G * (D / 16) + 4 * threads - 1) / (4 * threads) : 0;
+  const int64_t q_wgs = q ? (rows * ((a.G + kv_turn_heads(x_dt) - 1) / kv_turn_heads(x_dt)) * (D / 16) + threads - 1) / threads : 0;
   const dim3 grid(static_cast<unsigned>(units * Hkv), static_cast<unsigned>(1 + (q_wgs < 64 ? q_wgs : 64)));
   hipStream_t s = as_stream(stream);
   VYBDQ_DISPATCH_IN(x_dt, DT, launch_append<DT>(static_cast<int>(D), a, grid, threads, s));
