@@ -563,7 +563,8 @@ int vybdq_quant_q8_act(uint64_t X, uint64_t Xq, uint64_t Xs, int64_t M, int64_t 
    values (|y| <= 448 * 2^e, e in [-60, 60]); code = y / scale to nearest, ties to even. Rows that begin inside a page keep
    its earlier tokens: e then does not shrink, and where it grows their codes are rounded anew to the larger scale.
    Slots behind the last row stay as they are. A token with an infinity or NaN in a head's rotated k or its v is stored
-   so that exactly the attention rows that see it are NaN. K, V, cos, sin, q_out and every row 16-byte aligned. */
+   so that exactly the attention rows that see it are NaN. K, V, cos, sin, q_out and every row 16-byte aligned; q_out may be
+   q (ldq = Hq D). (T / page + 2 B) Hkv must be below 2^23. */
 int vybdq_kv_append(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs, int64_t n_pages, int64_t Hkv, int64_t D, int64_t page,
                     uint64_t k, uint64_t v, uint64_t q, uint64_t q_out, int x_dt, int64_t ldk, int64_t ldv, int64_t ldq,
                     int64_t Hq, uint64_t cos, uint64_t sin, int64_t R, int64_t n_pos, int interleaved, uint64_t table,
@@ -579,7 +580,8 @@ int64_t vybdq_kv_attn_workspace_size(int64_t D);
    operands are fp16 (codes exactly; q scaled by a power of two per row; float32 q and its weights in two fp16 terms).
    ws: 256-byte aligned, of vybdq_kv_attn_workspace_size(D) bytes, zero-filled once before the first call (arrival
    counters that every completed call leaves at zero); a smaller one splits less, 0 not at all. Calls that share a
-   workspace must not overlap. One launch. */
+   workspace must not overlap. out may be q (ldq = Hq D). One launch, and one to join the results where more than 32 rows of a
+   head's sequence split their keys. (T Hq / (64 Hkv) + B) Hkv must be below 2^24. */
 int vybdq_kv_attn(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs, int64_t n_pages, int64_t Hkv, int64_t D, int64_t page,
                   uint64_t q, int x_dt, int64_t ldq, int64_t Hq, uint64_t out, uint64_t lse, uint64_t table, int64_t W,
                   uint64_t q_start, uint64_t ctx, int64_t T, int64_t B, int64_t max_new, int64_t max_ctx, double scale,

@@ -545,6 +545,96 @@ def test_graphs_of_a_decode_loop(dev, rng):
     ops.kv_status()
 
 
+@pytest.mark.parametrize("Hq,n", [(2, 90), (4, 12)])
+def test_graph_of_a_chunk(dev, rng, Hq, n):
+    """A chunk's attention with its keys split (a launch for the join at 90 rows a head), captured and replayed at other
+    lengths, with eager calls of the same workspace between the replays."""
+    table, start, ctx, n_pages = tables(rng, [(n, 3000), (1, 900)], 64)
+    cache = device_cache(dev, random_cache(rng, n_pages, 1, 64, 64))
+    attend, t = ops.KvAttention(Hq, 1, 64, dev), on(dev, table, start, ctx)
+    q = torch.zeros(n + 1, Hq, 64, device=dev, dtype=torch.float16)
+    args = dict(max_new=n, max_ctx=3000, lse=True)
+    attend(q, cache, *t, **args)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, lse = attend(q, cache, *t, **args)
+    for i in range(6):
+        q.copy_(torch.randn(q.shape, device=dev))
+        t[2].copy_(torch.tensor([3000 - 411 * i, 900 - 170 * i], dtype=torch.int32))
+        g.replay()
+        eager, eager_lse = attend(q, cache, *t, **args)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager) and torch.equal(lse, eager_lse), i
+    ops.kv_status()
+
+
+def test_two_streams_at_once(dev, rng):
+    """Two batches in one cache on two streams, each with a workspace of its own; their contexts share pages."""
+    D, page = 128, 64
+    table, _, _, n_pages = tables(rng, [(0, 4000), (0, 4000)], page)
+    table[1, :40] = table[0, :40]
+    cache = device_cache(dev, random_cache(rng, n_pages, 2, page, D))
+    start, ctx = on(dev, np.array([0, 3], np.int32), np.array([3999], np.int32))
+    batches = [on(dev, table[b:b + 1])[0] for b in range(2)]
+    attends = [ops.KvAttention(4, 2, D, dev) for _ in range(2)]
+    q = [torch.randn(3, 4, D, device=dev) for _ in range(2)]
+    k, v = (torch.randn(3, 2, D, device=dev) for _ in range(2))
+    step = lambda b: (ops.kv_append(cache, k, v, batches[b], start, ctx), attends[b](q[b], cache, batches[b], start, ctx))[1]
+    alone = [step(b).clone() for b in range(2)]
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for b in range(2):
+            with torch.cuda.stream(sides[b]):
+                got.append(step(b))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(alone, got))
+    ops.kv_status()
+
+
+@pytest.mark.parametrize("x", ["bf16", "f32"])
+def test_rows_behind_the_last_sequence_stay(dev, rng, x):
+    """A padded batch: rows past q_start[B], and sequences without rows, leave outputs and cache as they were."""
+    D, page = 64, 16
+    lens = [(3, 20), (0, 0), (40, 40), (0, 7)]
+    table, start, ctx, n_pages = tables(rng, lens, page)
+    want = random_cache(rng, n_pages, 1, page, D)
+    cache, t = device_cache(dev, want), on(dev, table, start, ctx)
+    T = 50
+    q, k, v = (torch.randn(T, h, D, device=dev).to(DT[x]) for h in (2, 1, 1))
+    q_out, out = (torch.full((T, 2, D), 7.0, device=dev, dtype=DT[x]) for _ in range(2))
+    attend = ops.KvAttention(2, 1, D, dev)
+    for max_new in (None, 1, 40):
+        ops.kv_append(cache, k, v, *t, q=q, q_out=q_out, max_new=max_new)
+        attend(q, cache, *t, out=out, max_new=max_new)
+        assert (q_out[43:] == 7.0).all() and (out[43:] == 7.0).all()
+        assert torch.equal(q_out[:43], q[:43])
+    f = lambda a: a.float().cpu().numpy()
+    for _ in range(3):
+        oracle_append(want, f(k), f(v), None, table, start, ctx, None, None, False)
+    same_cache(cache, want)
+    check_attention(out[:43], None, q[:43].double().cpu().numpy(), want, table, start, ctx, D ** -0.5, True, 0, x)
+    ops.kv_status()
+
+
+@pytest.mark.parametrize("n,Hq", [(1, 4), (5, 6), (100, 2)])
+def test_outputs_in_place(dev, rng, n, Hq):
+    """q_out and out may be q."""
+    D, page = 64, 64
+    table, start, ctx, n_pages = tables(rng, [(n, 2000), (n, 300)], page)
+    cache, t = device_cache(dev, random_cache(rng, n_pages, 2, page, D)), on(dev, table, start, ctx)
+    cos, sin = on(dev, *angles(2000, D))
+    q, k, v = (torch.randn(2 * n, h, D, device=dev).bfloat16() for h in (Hq, 2, 2))
+    attend, args = ops.KvAttention(Hq, 2, D, dev), dict(max_new=n, max_ctx=2000)
+    turned = ops.kv_append(cache, k, v, *t, q=q, cos=cos, sin=sin)
+    want = attend(turned, cache, *t, **args)
+    assert ops.kv_append(cache, k, v, *t, q=q, cos=cos, sin=sin, q_out=q) is q and torch.equal(q, turned)
+    assert attend(q, cache, *t, out=q, **args) is q and torch.equal(q, want)
+    ops.kv_status()
+
+
 def test_attention_block_of_a_decoding_host(dev, rng):
     """A prompt, then decoded tokens, of one attention block as a host runs it: RMSNorm, fused q|k|v GEMV on packed q4_0
     weights, append, attention, output projection with the residual. Every stage against float64 on that stage's own inputs."""

@@ -30,6 +30,7 @@ BOTH = [
     (dict(R=24), _lib.ERR_SHAPE, "R must"), (dict(R=80), _lib.ERR_SHAPE, "R must"), (dict(cos=0), _lib.ERR_ARG, "cos and sin"),
     (dict(n_pos=0), _lib.ERR_ARG, "cos and sin"), (dict(q_out=0), _lib.ERR_ARG, "q_out"), (dict(ldv=120), _lib.ERR_SHAPE, "stride"),
     (dict(v=20), _lib.ERR_ALIGN, "16-byte"), (dict(sin=20), _lib.ERR_ALIGN, "16-byte"),
+    (dict(B=2 ** 20 - 1, Hkv=8, Hq=8), _lib.ERR_SHAPE, "2\\^23"), (dict(T=2 ** 26, page=16, Hkv=2), _lib.ERR_SHAPE, "2\\^23"),
 ])
 def test_append_refuses(change, code, text):
     assert _lib.lib.vybdq_kv_append(*(APPEND | change).values()) == code
@@ -38,6 +39,7 @@ def test_append_refuses(change, code, text):
 
 @pytest.mark.parametrize("change,code,text", BOTH + [
     (dict(window=-1), _lib.ERR_SHAPE, "window"), (dict(window=2 ** 30), _lib.ERR_SHAPE, "window"), (dict(out=0), _lib.ERR_ARG, "null"),
+    (dict(B=2 ** 20 - 1, Hkv=32, Hq=32), _lib.ERR_SHAPE, "2\\^24"), (dict(T=2 ** 28, Hkv=4, Hq=4), _lib.ERR_SHAPE, "2\\^24"),
     (dict(out=20), _lib.ERR_ALIGN, "16-byte"), (dict(lse=6), _lib.ERR_ALIGN, "4-byte"), (dict(ws=128), _lib.ERR_ALIGN, "256-byte"),
 ])
 def test_attention_refuses(change, code, text):

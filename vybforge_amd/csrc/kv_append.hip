@@ -19,9 +19,10 @@
 // magnitude; a thread rotates up to four heads of its group by the angles that it has read (one head each: 39.9 us
 // against 36.5 below).
 //
-// Bound by memory when there is much of it, MI355X: five prompts of 1 to 1638 tokens, 32 / 8 heads of 128, bf16, 127 MB:
-// 36.5 us, 3.5 TB/s; 16 of 256 in float32, 85 MB: 20.9 us, 4.1 TB/s (a large copy runs at 4.7). A decode step is bound by
-// the launch: 7 us on the GPU for one sequence as for 128.
+// Bound by memory when there is much of it, MI355X: five prompts of up to 1638 tokens, 32 / 8 heads of 128, bf16, 127 MB:
+// 36.5 us, 3.5 TB/s; seven of up to 301 tokens, 24 / 4 heads of 256, float32, 85 MB: 20.9 us, 4.1 TB/s (a large copy runs
+// at 4.7). A decode step takes 6 us on the GPU for one sequence and 7 for 128, about 2 of them the launch; asking for k and v
+// before the page is known, or for the old codes of a group of slots before the page's magnitude is, changed neither.
 #include "kv.h"
 
 #include <mutex>
@@ -472,6 +473,8 @@ extern "C" int vybdq_kv_append(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs,
   VYBDQ_REQUIRE(W >= 1 && W * page < (int64_t(1) << 31), VYBDQ_ERR_SHAPE, "W must be at least 1 and W * page below 2^31");
   VYBDQ_REQUIRE(R >= 0 && R <= D && R % 16 == 0, VYBDQ_ERR_SHAPE, "R must be a multiple of 16 in 0 .. D");
   VYBDQ_REQUIRE(!q || (Hq >= Hkv && Hq % Hkv == 0 && Hq <= 16384), VYBDQ_ERR_SHAPE, "Hq must be a multiple of Hkv");
+  // (a grid holds less than 2^32 threads along x)
+  VYBDQ_REQUIRE((T / page + 2 * B) * Hkv < (int64_t(1) << 23), VYBDQ_ERR_SHAPE, "(T / page + 2 B) Hkv must be below 2^23");
   if (T == 0 || B == 0) return VYBDQ_OK;
   VYBDQ_REQUIRE(K && V && Ks && Vs && k && v && table && q_start && ctx, VYBDQ_ERR_ARG, "null pointer");
   VYBDQ_REQUIRE(!q || q_out, VYBDQ_ERR_ARG, "q needs q_out");
@@ -506,7 +509,6 @@ extern "C" int vybdq_kv_append(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs,
   a.inter = interleaved != 0;
   a.per_seq = max_new == 1;
   const int64_t units = a.per_seq ? B : (T >> ps) + 2 * B;
-  VYBDQ_REQUIRE(units * Hkv < (int64_t(1) << 31), VYBDQ_ERR_SHAPE, "too many pages in one call");
   const int rc = kv_status_address(a.b.status);
   if (rc) return rc;
   // threads: a page's pieces of 16 dims (a decode step's 8 to 16: one wave, so that all workgroups of a batch are resident);

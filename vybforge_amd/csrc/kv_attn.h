@@ -16,10 +16,19 @@
 // 2^-26 of the row's largest). For float32 queries both are split into two fp16 terms (22 bits).
 //
 // A wave owns 16 NCT query rows (row = token * G + head of the group; the G query heads of a key head read the
-// same keys, so they share its tiles). WT waves of a workgroup take turns over the keys (32 at a time) and are
-// joined through LDS; WR waves own different rows. With few rows the keys are split over workgroups too (gridDim.y):
-// each stores its (m, l, acc), and the last one to arrive joins them in split order, so results do not depend
-// on the order of arrival.
+// same keys, so they share its tiles) and takes 32 keys at a step. Few rows: k_kv_attn_keys, whose waves take turns over the
+// keys; more: k_kv_attn_rows, whose waves own rows each and share the keys. Where the rows alone leave the chip idle the keys
+// are split over workgroups too (gridDim.y): each stores its (m, l, acc), and they are joined in split order, so results do
+// not depend on the order of arrival.
+//
+// What bounds them, MI355X (a large copy runs at 4.7 TB/s, a large fp16 product at 1089 TFLOP/s): 48 sequences of 2 to 8 k
+// tokens, one row each, 32 / 8 heads of 128: 105 us, 4.9 TB/s of codes; 4 of up to 131072: 143 us, 5.1 TB/s. A prompt of 4096
+// tokens: 173 us, 793 TFLOP/s; 513 tokens behind 32 k: 345 us, 791 TFLOP/s. Of the prompt's 173 us the matrix instructions
+// (18 cycles each on a SIMD with four waves) are 64, the LDS reads that feed them 30 (128 rows) to 60 (64 rows) beside them;
+// without loads and conversion it took 141 us, without exponentials 169. With heads of 64 a step of 16 rows is 140 cycles
+// of matrix instructions and some 250 of vector instructions, most of them the softmax: 457 TFLOP/s with a window of 4096.
+// 32x32x16 instructions in the same scheme were no faster (prompt 177 to 188 us, heads of 64 83 to 97 against 87), nor were
+// two tiles of 16 rows of heads of 64 to a wave (93 against 87).
 #pragma once
 
 #include "kv.h"
@@ -611,11 +620,9 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_kv_attn_keys(const Kv
 // used, and its codes were asked for one step earlier still. The pages and scales of 128 blocks of 16 keys at a time
 // go through LDS as well (scalar loads would be waited for with every wait for LDS data).
 // The last units first: with a causal mask they have the most keys.
-template <int D, int NCT, int NW, bool TWO>
-__global__ void __launch_bounds__(64 * NW, NCT > 1 || D == 256 || (TWO && D == 192) ? 2 : TWO || D == 192 ? 3 : 4) k_kv_attn_rows(const KvAttnArgs a) {
-  constexpr int C = D / 64, R = 16 * NCT * NW, NQ = TWO ? 2 : 1;
-  // 64 dims of a block of 16 keys are a unit: the step's 2 C units of K, then 2 C of V, are dealt to the waves in turn
-  constexpr int kMine = (4 * C + NW - 1) / NW;
+template <int D, int NCT, bool TWO>
+__global__ void __launch_bounds__(256, NCT > 1 || D == 256 || (TWO && D == 192) ? 2 : TWO || D == 192 ? 3 : 4) k_kv_attn_rows(const KvAttnArgs a) {
+  constexpr int C = D / 64, R = 64 * NCT, NQ = TWO ? 2 : 1;
   __shared__ h8 tile[2][8 * C][64];  // K of block n: 2 (n C + c) + y; V: 4 C + 4 c + d, its first four values of block 0
   __shared__ u4 meta[2][128];        // a block's page, K scale, V exponent e and 2^-e
   const int lane = threadIdx.x & 63, col = lane & 15, g4 = lane >> 4;
@@ -632,7 +639,7 @@ __global__ void __launch_bounds__(64 * NW, NCT > 1 || D == 256 || (TWO && D == 1
   // Blocks 128 batch .. of this split. A block behind the sequence's end takes the last page (its keys are masked); one
   // outside the cache reads page 0 with a NaN scale.
   auto ask = [&](int batch) {
-    for (int i = threadIdx.x; i < 128; i += 64 * NW) {
+    for (int i = threadIdx.x; i < 128; i += 256) {
       const int at = ((t.k0 >> 4) + 2 * t0 + 128 * batch + i) >> (ps - 4);
       const int pg = t.table[at < last_page ? at : last_page];
       const bool bad = static_cast<uint32_t>(pg) >= static_cast<uint32_t>(a.c.n_pages);
@@ -644,24 +651,22 @@ __global__ void __launch_bounds__(64 * NW, NCT > 1 || D == 256 || (TWO && D == 1
     }
   };
   auto block_meta = [&](int st, int n) -> const u4 & { return meta[(st - t0) >> 6 & 1][(2 * (st - t0) + n) & 127]; };
-  // this wave's unit i: is it one, is it K's (known at compile time for all but a mixed turn), which block and dims
-  auto unit = [&](int i) { return wave + i * NW; };
-  auto mine = [&](int i) { return 4 * C % NW == 0 || unit(i) < 4 * C; };
-  auto is_k = [&](int i) { return (i + 1) * NW <= 2 * C || (i * NW < 2 * C && unit(i) < 2 * C); };
+  // 64 dims of a block of 16 keys are a unit: the step's 2 C units of K, then 2 C of V, are dealt to the four waves in turn.
+  // This wave's unit i: is it K's (known at compile time for all but a mixed turn), which block and dims.
+  auto unit = [&](int i) { return wave + 4 * i; };
+  auto is_k = [&](int i) { return 4 * (i + 1) <= 2 * C || (4 * i < 2 * C && unit(i) < 2 * C); };
   auto block_of = [&](int i) { return (is_k(i) ? unit(i) : unit(i) - 2 * C) / C; };
   auto dims_of = [&](int i) { return unit(i) % C; };
-  u2 coming[kMine];  // page and K scale of the blocks that are fetched next
-  u4 code[kMine];
-  uint32_t ks[kMine];
+  u2 coming[C];  // page and K scale of the blocks that are fetched next
+  u4 code[C];
+  uint32_t ks[C];
   auto peek = [&](int st) {
 #pragma unroll
-    for (int i = 0; i < kMine; ++i)
-      if (mine(i)) coming[i] = *reinterpret_cast<const u2 *>(&block_meta(st, block_of(i)));
+    for (int i = 0; i < C; ++i) coming[i] = *reinterpret_cast<const u2 *>(&block_meta(st, block_of(i)));
   };
   auto fetch = [&](int st) {
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      if (!mine(i)) continue;
+    for (int i = 0; i < C; ++i) {
       const int pg = __builtin_amdgcn_readfirstlane(coming[i].x);
       ks[i] = __builtin_amdgcn_readfirstlane(coming[i].y);
       const int64_t at = (((static_cast<int64_t>(pg) * Hkv + h) << ps) + ((t.k0 + 32 * st + 16 * block_of(i)) & in_page)) * D;
@@ -673,8 +678,7 @@ __global__ void __launch_bounds__(64 * NW, NCT > 1 || D == 256 || (TWO && D == 1
   auto write = [&](int st) {
     const int buf = st & 1, tok = t.k0 + 32 * st;
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      if (!mine(i)) continue;
+    for (int i = 0; i < C; ++i) {
       if (is_k(i)) {
         tile[buf][2 * unit(i)][lane] = kv_dec8(code[i].x, code[i].y);
         tile[buf][2 * unit(i) + 1][lane] = kv_dec8(code[i].z, code[i].w);

@@ -132,6 +132,8 @@ extern "C" int vybdq_kv_attn(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs, i
   VYBDQ_REQUIRE(T * Hq < (int64_t(1) << 31), VYBDQ_ERR_SHAPE, "T * Hq must be below 2^31");
   VYBDQ_REQUIRE(W >= 1 && W * page < (int64_t(1) << 30), VYBDQ_ERR_SHAPE, "W must be at least 1 and W * page below 2^30");
   VYBDQ_REQUIRE(window >= 0 && window < (int64_t(1) << 30), VYBDQ_ERR_SHAPE, "window must be in 0 .. 2^30 - 1");
+  // (a grid holds less than 2^32 threads along x)
+  VYBDQ_REQUIRE((T * (Hq / Hkv) / 64 + B) * Hkv < (int64_t(1) << 24), VYBDQ_ERR_SHAPE, "(T Hq / (64 Hkv) + B) Hkv must be below 2^24");
   if (T == 0 || B == 0) return VYBDQ_OK;
   VYBDQ_REQUIRE(K && V && Ks && Vs && q && out && table && q_start && ctx, VYBDQ_ERR_ARG, "null pointer");
   VYBDQ_REQUIRE(ldq >= Hq * D, VYBDQ_ERR_SHAPE, "a row stride is smaller than a row");
@@ -149,7 +151,6 @@ extern "C" int vybdq_kv_attn(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs, i
   const KvShape shape{D, Hkv, G, T, B, most, tokens, two, causal != 0, window,
                       ws && ws_bytes > kKvArrivalBytes ? (ws_bytes - kKvArrivalBytes) / ((D + 2) * 4) : 0};
   KvPlan plan = kv_plan(shape);
-  VYBDQ_REQUIRE(plan.units * Hkv < (int64_t(1) << 31), VYBDQ_ERR_SHAPE, "too many rows in one call");
   KvAttnArgs a{};
   const int rc = kv_status_address(a.b.status);
   if (rc) return rc;

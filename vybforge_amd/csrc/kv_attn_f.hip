@@ -5,7 +5,7 @@ namespace vybdq {
 
 template <int D, int NCT>
 static void launch_rows(const KvAttnArgs &a, dim3 grid, hipStream_t s) {
-  hipLaunchKernelGGL((k_kv_attn_rows<D, NCT, 4, true>), grid, dim3(256), 0, s, a);
+  hipLaunchKernelGGL((k_kv_attn_rows<D, NCT, true>), grid, dim3(256), 0, s, a);
   if (grid.y > 1)
     hipLaunchKernelGGL((k_kv_attn_join<D, 64 * NCT, true>), dim3(grid.x, 8 * NCT), dim3(256), 0, s, a, static_cast<int>(grid.y));
 }
