@@ -74,6 +74,7 @@ static KvPlan kv_plan_variant(const KvShape &s, int variant) {
   KvPlan p{variant, units, 1, 0};
   if (const char *e = tuning_env("VYBDQ_KV_SPLITS")) {
     p.splits = atoi(e) < 1 ? 1 : atoi(e) < held ? atoi(e) : held;
+    p.time = time_of(p.splits);
     return p;
   }
   p.time = time_of(1);
