@@ -551,7 +551,8 @@ int vybdq_quant_q8_act(uint64_t X, uint64_t Xq, uint64_t Xs, int64_t M, int64_t 
    ctx[b] tokens (int32 [B]); table int32 [B][W] names the page of its tokens i page .. i page + page - 1. The pages
    that a call appends to must differ between sequences; pages that are only read may be shared.
    max_new and max_ctx are the caller's bounds on a sequence's rows and tokens (0: unknown). They choose the launch
-   shape; results are right for any value, but for vybdq_kv_attn's last bits (the split of the keys).
+   shape; results are right for any value, but for vybdq_kv_attn's last bits (the split of the keys, which the lengths of the
+   whole batch take part in).
    What the device finds wrong with the tables is skipped, or NaN in the outputs concerned, and reported by the next
    vybdq_kv_status(); nothing outside the cache and the outputs is read or written whatever they hold.
 

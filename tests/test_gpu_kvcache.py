@@ -293,7 +293,7 @@ def test_attention_split_keys(dev, rng, x, n):
 
 
 @pytest.mark.parametrize("variant", [0, 1, 2, 3])
-@pytest.mark.parametrize("splits", [1, 2, 7])
+@pytest.mark.parametrize("splits", [1, 2, 7, -2, -7])
 @pytest.mark.parametrize("x,D", [("bf16", 128), ("f32", 256), ("f16", 64), ("f32", 128), ("bf16", 192)])
 def test_attention_every_variant(dev, rng, monkeypatch, variant, splits, x, D):
     """Kernel variants and key splits other than the chosen ones, on odd lengths, with and without a window; more keys than
@@ -446,6 +446,51 @@ def test_offsets_past_32_bits(dev, rng):
     one = on(dev, np.array([0, 1], np.int32))[0]
     got = ops.KvAttention(Hkv, Hkv, D, dev)(q.to(dev), cache, t[0], one, t[2])
     check_attention(got, None, q.double().numpy(), small, np.array([[0, 1]]), np.array([0, 1]), ctx, D ** -0.5, True, 0, "f32")
+    ops.kv_status()
+
+
+@pytest.mark.parametrize("splits", [-2, -3, -40])
+@pytest.mark.parametrize("B", [2, 64, 65, 200])
+def test_attention_splits_by_length(dev, rng, monkeypatch, B, splits):
+    """Splits that go with the sequences' lengths: one long and many short, all empty but one, all alike, no rows at all."""
+    monkeypatch.setenv("VYBDQ_KV_VARIANT", "0")
+    monkeypatch.setenv("VYBDQ_KV_SPLITS", str(splits))
+    attend = ops.KvAttention(2, 1, 64, dev)
+    for lens in ([(1, int(c)) for c in rng.integers(1, 400, B - 1)] + [(2, 3000)],
+                 [(0, 0)] * (B - 2) + [(1, 2000), (0, 50)],
+                 [(1, 130)] * B,
+                 [(0, 0)] * B):
+        for _ in range(2):
+            run_attention(dev, rng, lens, 2, 1, 64, 16, "f16", window=0 if B < 65 else 1000, attend=attend)
+    run_attention(dev, rng, [(1, 0), (1, 1)] * (B // 2), 2, 1, 64, 16, "f16", attend=attend)
+
+
+def test_attention_splits_by_length_with_bad_tables(dev, rng, monkeypatch):
+    """A sequence whose rows, length or pages are wrong among good ones; a good call of the same workspace afterwards."""
+    monkeypatch.setenv("VYBDQ_KV_SPLITS", "-5")
+    D, page = 64, 16
+    lens = [(1, 600), (1, 20), (1, 300)]
+    table, start, ctx, n_pages = tables(rng, lens, page)
+    cache = device_cache(dev, random_cache(rng, n_pages, 1, page, D))
+    attend, q = ops.KvAttention(2, 1, D, dev), torch.randn(3, 2, D, device=dev)
+    good = attend(q, cache, *on(dev, table, start, ctx))
+    for change in ((0, 2 ** 31 - 1), (0, -2 ** 31), (2, 2 ** 30), (1, -1)):
+        c = ctx.copy()
+        c[change[0]] = change[1]
+        out = attend(q, cache, *on(dev, table, start, c))
+        torch.cuda.synchronize()
+        for b in range(3):
+            assert b == change[0] or (out[b] - good[b]).abs().max() < 1e-5, (change, b)
+        if change[1] > 0:
+            with pytest.raises(_lib.VybdqError, match="ctx"):
+                ops.kv_status()
+        assert torch.equal(attend(q, cache, *on(dev, table, start, ctx)), good)
+    s = start.copy()
+    s[2] = 40
+    attend(q, cache, *on(dev, table, s, ctx))
+    with pytest.raises(_lib.VybdqError, match="q_start"):
+        ops.kv_status()
+    assert torch.equal(attend(q, cache, *on(dev, table, start, ctx)), good)
     ops.kv_status()
 
 

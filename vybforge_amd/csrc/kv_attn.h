@@ -18,11 +18,11 @@
 // A wave owns 16 NCT query rows (row = token * G + head of the group; the G query heads of a key head read the
 // same keys, so they share its tiles) and takes 32 keys at a step. Few rows: k_kv_attn_keys, whose waves take turns over the
 // keys; more: k_kv_attn_rows, whose waves own rows each and share the keys. Where the rows alone leave the chip idle the keys
-// are split over workgroups too (gridDim.y): each stores its (m, l, acc), and they are joined in split order, so results do
+// are split over workgroups too: each stores its (m, l, acc), and they are joined in split order, so results do
 // not depend on the order of arrival.
 //
 // What bounds them, MI355X (a large copy runs at 4.7 TB/s, a large fp16 product at 1089 TFLOP/s): 48 sequences of 2 to 8 k
-// tokens, one row each, 32 / 8 heads of 128: 105 us, 4.9 TB/s of codes; 4 of up to 131072: 143 us, 5.1 TB/s. A prompt of 4096
+// tokens, one row each, 32 / 8 heads of 128: 102 us, 5.1 TB/s of codes; 4 of up to 131072: 132 us, 5.5 TB/s. A prompt of 4096
 // tokens: 173 us, 793 TFLOP/s; 513 tokens behind 32 k: 345 us, 791 TFLOP/s. Of the prompt's 173 us the matrix instructions
 // (18 cycles each on a SIMD with four waves) are 64, the LDS reads that feed them 30 (128 rows) to 60 (64 rows) beside them;
 // without loads and conversion it took 141 us, without exponentials 169. With heads of 64 a step of 16 rows is 140 cycles
@@ -32,6 +32,8 @@
 #pragma once
 
 #include "kv.h"
+
+#include <type_traits>
 
 namespace vybdq {
 
@@ -47,6 +49,8 @@ struct KvAttnArgs {
   int32_t G, dt;       // dt: F32, F16 or BF16 of q and out
   int32_t causal, window;
   float scale2;        // scale * log2(e)
+  int32_t splits;      // k_kv_attn_keys: workgroups of a sequence and head, on average
+  int32_t by_length;   // and whether a sequence's number of them goes with its length
 };
 
 // Four e4m3 codes as fp16 (exact).
@@ -179,6 +183,89 @@ __device__ __forceinline__ void kv_tile_keys(const KvAttnArgs &a, int R, KvTile 
 __device__ __forceinline__ int kv_split(int steps, int i, int S) {
   const int rest = steps % S;
   return steps / S * i + (i < rest ? i : rest);
+}
+
+// The sum over this lane and those below it.
+template <class T>
+__device__ __forceinline__ T lane_scan(T v) {
+  auto from = [&](auto ctrl, auto rows) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  v += from(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});  // row_shr 1, 2, 4, 8: rows of 16
+  v += from(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  v += from(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  v += from(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  v += from(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row_bcast 15: into rows 1 and 3
+  v += from(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // row_bcast 31: into rows 2 and 3
+  return v;
+}
+
+// Which sequence and part of its keys unit u of k_kv_attn_keys takes. There are B a.splits units for each head. By length, a
+// sequence has a number of them that goes with its own keys (those of its first tile, in steps of 32), so that sequences of
+// unequal lengths end together: the largest share, of four tried, whose parts fit in the units. Every workgroup finds the same
+// numbers. That costs 1 us at its start, and the longest sequence's join takes longer.
+struct KvPart {
+  int b, split, S;
+};
+__device__ __forceinline__ KvPart kv_part(const KvAttnArgs &a, int R, int u) {
+  const int B = a.b.B, S = a.splits;
+  if (!a.by_length) return {u / S, u % S, S};
+  const int lane = threadIdx.x & 63, each = (B + 63) >> 6, lo = lane * each, hi = lo + each < B ? lo + each : B;
+  auto steps = [&](int b) {
+    const int s0 = a.b.q_start[b], s1 = a.b.q_start[b + 1], ctx = a.b.ctx[b];
+    if (s0 < 0 || s0 >= s1 || s1 > a.b.T || ctx <= 0 || ctx > (a.b.W << a.c.ps)) return 0.f;
+    KvTile t;
+    t.rows = (s1 - s0) * a.G;
+    t.r0 = 0;
+    t.ctx = ctx;
+    t.p0 = ctx - (s1 - s0);
+    kv_tile_keys(a, R, t);
+    return static_cast<float>(t.steps);
+  };
+  auto parts = [](float steps, float share) {
+    const int n = static_cast<int>(ceilf(steps * share));
+    return n > 1 ? n : 1;
+  };
+  const float first = lo < hi ? steps(lo) : 0.f;  // (B <= 64: all that a lane has)
+  float total = first;
+  for (int b = lo + 1; b < hi; ++b) total += steps(b);
+  total = lane_scan(total);
+  total = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(total), 63));
+  // parts per step: units / total, and less, down to what fits whatever is rounded up: sum of ceil(x) < sum of x + B
+  float share[4];
+  int sum[4], upto[4];
+  const float inv = total > 0.f ? B / total : 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    share[k] = fminf((S - k * (1.f / 3)) * inv, 0.25f);
+    sum[k] = lo < hi ? parts(first, share[k]) : 0;
+  }
+  for (int b = lo + 1; b < hi; ++b) {
+    const float x = steps(b);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum[k] += parts(x, share[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) upto[k] = lane_scan(sum[k]);
+  float chosen = 0.f;  // (one part each, should rounding ever leave none that fits)
+  int mine = hi > lo ? hi - lo : 0, last = hi > lo ? hi : B;
+#pragma unroll
+  for (int k = 3; k >= 0; --k)
+    if (__builtin_amdgcn_readlane(upto[k], 63) <= B * S) {
+      chosen = share[k];
+      mine = sum[k];
+      last = upto[k];
+    }
+  const int owner = __popcll(__ballot(last <= u));  // the lane whose sequences hold unit u
+  KvPart p{-1, u - (last - mine), 1};
+  for (int b = lo; b < hi && p.b < 0; ++b) {
+    p.S = parts(b == lo ? first : steps(b), chosen);
+    if (p.split < p.S) p.b = b;
+    else p.split -= p.S;
+  }
+  if (owner >= 64) return {-1, 0, 1};
+  return {__builtin_amdgcn_readlane(p.b, owner), __builtin_amdgcn_readlane(p.split, owner), __builtin_amdgcn_readlane(p.S, owner)};
 }
 
 // The 16 query rows r .. r + 15 as operands of S^T = K Q^T, one row per column: lane (col, g4) holds dims
@@ -349,11 +436,10 @@ struct KvSink {
     return __builtin_bit_cast(f2, __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
   }
 
-  // Items it, it + step, .. (N of them, those before `items`) of a tile's rows from S splits' results at `all`: item i is 4 dims
+  // Items it, it + step, .. (N of them, those before `items`) of a tile's rows from S splits' results at `all`, `stride` floats apart: item i is 4 dims
   // of a row. Joined in split order, with N W splits' loads to a round trip. THROUGH: read past the caches, 8 bytes at a time.
   template <int N, int W, bool THROUGH>
-  __device__ __forceinline__ void finish_joined(const float *all, int S, int it, int step, int items) const {
-    constexpr int64_t kSize = static_cast<int64_t>(R) * (D + 2);
+  __device__ __forceinline__ void finish_joined(const float *all, int64_t stride, int S, int it, int step, int items) const {
     int r[N], d[N];
     float mr[N], lr[N], x[N][4];
 #pragma unroll
@@ -374,7 +460,7 @@ struct KvSink {
       for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          const float *pw = all + (w0 + w < S ? w0 + w : S - 1) * kSize;
+          const float *pw = all + (w0 + w < S ? w0 + w : S - 1) * stride;
           const float *pv = pw + 2 * R + r[i] * D + d[i];
           if constexpr (THROUGH) {
             ml[i][w] = load_through(pw + 2 * r[i]);
@@ -415,26 +501,26 @@ struct KvSink {
   // have completed before the arrival is counted. Few are read past the caches; for many, what the caches hold of them is
   // dropped first, 1 us that 16-byte reads make good (5 splits, 30 rows of 256 dims: 44.0 us against 46.0 past the caches, 12
   // of 256 33.2 in both, 12 of 128 19.6 past the caches against 20.1, 6 of 128 18.0 against 19.1).
-  __device__ __forceinline__ void join(int S, bool &is_last) const {
+  __device__ __forceinline__ void join(uint32_t *count, int split, int S, bool &is_last) const {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) {
-      uint32_t *count = a.arrivals + blockIdx.x;
       const uint32_t old = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       is_last = old == static_cast<uint32_t>(S - 1);
       if (is_last) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
     if (!is_last) return;
-    const float *all = a.part + static_cast<int64_t>(blockIdx.x) * S * (R * (D + 2));
+    const int64_t stride = static_cast<int64_t>(a.c.Hkv) * (R * (D + 2));
+    const float *all = part - split * stride;
     const int n_rows = t.rows - t.r0 < R ? t.rows - t.r0 : R, items = n_rows * (D / 4);
     if (items <= 512) {
 #pragma unroll 1
-      for (int it = threadIdx.x; it < items; it += 256) finish_joined<1, 8, true>(all, S, it, 256, items);
+      for (int it = threadIdx.x; it < items; it += 256) finish_joined<1, 8, true>(all, stride, S, it, 256, items);
     } else {
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
 #pragma unroll 1
-      for (int it = threadIdx.x; it < items; it += 1024) finish_joined<4, 4, false>(all, S, it, 256, items);
+      for (int it = threadIdx.x; it < items; it += 1024) finish_joined<4, 4, false>(all, stride, S, it, 256, items);
     }
   }
 };
@@ -459,10 +545,11 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_kv_attn_keys(const Kv
   __shared__ bool is_last;
   const int lane = threadIdx.x & 63, col = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave % WR, wt = wave / WR;
-  const int Hkv = a.c.Hkv, h = blockIdx.x % Hkv, b = blockIdx.x / Hkv, S = gridDim.y, split = blockIdx.y;
-  const int ps = a.c.ps, in_page = (1 << ps) - 1;
+  const int Hkv = a.c.Hkv, h = blockIdx.x % Hkv, ps = a.c.ps, in_page = (1 << ps) - 1;
+  const KvPart part = kv_part(a, R, blockIdx.x / Hkv);
+  const int split = part.split, S = part.S;
   KvTile t;
-  if (!kv_tile_seq(a, b, t)) return;
+  if (part.b < 0 || !kv_tile_seq(a, part.b, t)) return;
   const uint32_t koff = col * D + 16 * g4, voff = 4 * (g4 * D + 4 * col);
   const int last_page = t.ctx > 0 ? (t.ctx - 1) >> ps : 0;
 
@@ -578,7 +665,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_kv_attn_keys(const Kv
     }
 
     // the waves' results, joined through LDS
-    const KvSink<D, R, TWO, true> sink{a, t, h, whole, a.part + (static_cast<int64_t>(blockIdx.x) * S + split) * (R * (D + 2))};
+    const KvSink<D, R, TWO, true> sink{a, t, h, whole, a.part + static_cast<int64_t>(blockIdx.x) * (R * (D + 2))};
     l[0] = col_sum(l[0]);
     if (t.r0 > 0) __syncthreads();
 #pragma unroll
@@ -608,7 +695,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_kv_attn_keys(const Kv
       }
       sink.template put<4>(r, mr, lr, d, x);
     }
-    if (!whole) sink.join(S, is_last);
+    if (!whole) sink.join(a.arrivals + part.b * Hkv + h, split, S, is_last);
   }
 }
 
@@ -797,7 +884,7 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(const KvAttnArgs a, int S)
   const float *all = a.part + static_cast<int64_t>(blockIdx.x) * S * (R * (D + 2));
   const KvSink<D, R, TWO, false> sink{a, t, h, true, nullptr};
   const int r0 = blockIdx.y * 8, left = t.rows - t.r0 - r0, items = (left < 8 ? left : 8) * (D / 4);
-  for (int it = threadIdx.x; it < items; it += 256) sink.template finish_joined<1, 4, false>(all, S, r0 * (D / 4) + it, 256, r0 * (D / 4) + items);
+  for (int it = threadIdx.x; it < items; it += 256) sink.template finish_joined<1, 4, false>(all, R * (D + 2), S, r0 * (D / 4) + it, 256, r0 * (D / 4) + items);
 }
 
 }  // namespace vybdq

@@ -23,6 +23,7 @@ struct KvPlan {
   int variant;
   int64_t units, splits;
   double time;
+  bool by_length;  // k_kv_attn_keys: more splits for longer sequences
 };
 
 // How many splits fit the workspace. (k_kv_attn_keys counts arrivals there too.)
@@ -71,10 +72,12 @@ static KvPlan kv_plan_variant(const KvShape &s, int variant) {
     const double one = (mine + 6) * alone, all = (mine * seen + 6) * share * ((wgs * n + cus - 1) / cus);
     return sqrt(sqrt(one * one * one * one + all * all * all * all)) + (n > 1 ? 4 + 1.2e-6 * wgs * n * R * (s.D + 2) : 0);
   };
-  KvPlan p{variant, units, 1, 0};
+  KvPlan p{variant, units, 1, 0, false};
   if (const char *e = tuning_env("VYBDQ_KV_SPLITS")) {
-    p.splits = atoi(e) < 1 ? 1 : atoi(e) < held ? atoi(e) : held;
+    const int64_t n = atoi(e) < 0 ? -atoi(e) : atoi(e);
+    p.splits = n < 1 ? 1 : n < held ? n : held;
     p.time = time_of(p.splits);
+    p.by_length = atoi(e) < 0 && variant < 2 && s.B > 1 && p.splits > 1;
     return p;
   }
   p.time = time_of(1);
@@ -85,6 +88,10 @@ static KvPlan kv_plan_variant(const KvShape &s, int variant) {
       p.splits = n;
     }
   }
+  // By length where the call is long enough to gain by it. Sequences of one to the full length, us with and without: 12 of
+  // 6000 tokens, 4 heads of 128: 16.2, 15.1; of 256, 2 rows: 26.9, 27.6, 5 rows 38.1, 42.0; 48 of 8192, 8 heads of 128: 101.3,
+  // 104.4; 4 of 131072: 131, 142. (All of full length: 34.6, 33.0 and 55.2, 54.3.)
+  p.by_length = variant < 2 && s.B > 1 && p.splits > 1 && p.time >= 25;
   return p;
 }
 
@@ -171,7 +178,10 @@ extern "C" int vybdq_kv_attn(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs, i
   a.causal = causal != 0;
   a.window = static_cast<int32_t>(window);
   a.scale2 = static_cast<float>(scale * 1.4426950408889634);
-  const dim3 grid(static_cast<unsigned>(plan.units * Hkv), static_cast<unsigned>(plan.splits));
+  a.splits = static_cast<int32_t>(plan.splits);
+  a.by_length = plan.by_length;
+  const dim3 grid(static_cast<unsigned>(plan.units * Hkv * (plan.variant < 2 ? plan.splits : 1)),
+                  static_cast<unsigned>(plan.variant < 2 ? 1 : plan.splits));
   if (two) kv_attn_launch_f(static_cast<int>(D), plan.variant, a, grid, as_stream(stream));
   else kv_attn_launch_h(static_cast<int>(D), plan.variant, a, grid, as_stream(stream));
   return check_launch("vybdq_kv_attn");

@@ -622,7 +622,7 @@ def _kv_rows(x, shape, cache, what):
     if x.shape != shape:
         raise ValueError(f"{what} must be {list(shape)}")
     row, head, one = x.stride()
-    if one != 1 or (head != shape[2] and shape[1] != 1):
+    if (one != 1 or (head != shape[2] and shape[1] != 1)) and shape[0]:
         raise ValueError(f"{what}: the heads of a row must be consecutive")
     if x.get_device() != cache.index:
         raise ValueError(f"{what} must be on the cache's device")
