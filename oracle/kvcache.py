@@ -94,7 +94,7 @@ class Cache:
 
 def attention(q, k, v, p0, ctx, scale, causal=True, window=0):
     """q [n, D] at positions p0 ..., k, v [ctx, D], all float64: out [n, D], lse [n], and for a bound on a computation's
-    error sum_j p_j |v_j| [n, D] and max_j scale sum_d |q_d k_jd| [n]."""
+    error sum_j p_j |v_j| [n, D] and max_j |scale| sum_d |q_d k_jd| [n]."""
     pos, j = p0 + np.arange(len(q))[:, None], np.arange(ctx)[None, :]
     seen = np.ones((len(q), ctx), bool)
     if causal:
@@ -116,5 +116,5 @@ def attention(q, k, v, p0, ctx, scale, causal=True, window=0):
         lse[i] = m + np.log(p.sum())
         p /= p.sum()
         out[i], weight[i] = p @ v[at], p @ np.abs(v[at])
-        reach[i] = (np.abs(k[at]) @ np.abs(q[i])).max() * scale
+        reach[i] = (np.abs(k[at]) @ np.abs(q[i])).max() * abs(scale)
     return out, lse, weight, reach

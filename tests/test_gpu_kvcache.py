@@ -311,6 +311,11 @@ def test_attention_query_magnitudes(dev, rng, x, q_scale):
     run_attention(dev, rng, [(1, 90), (20, 64)], 2, 1, 64, 16, x, q_scale=q_scale)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
+def test_attention_scales(dev, rng, scale):
+    run_attention(dev, rng, [(1, 90), (40, 64)], 2, 1, 64, 16, "f32", scale=scale)
+
+
 def test_attention_page_scales_far_apart(dev, rng):
     """Pages whose value scales differ by 2^70, the ones with small values with nearly all the weight."""
     D, page = 64, 16

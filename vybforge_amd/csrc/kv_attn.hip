@@ -26,6 +26,11 @@ struct KvPlan {
   bool by_length;  // k_kv_attn_keys: more splits for longer sequences
 };
 
+// The most keys that a tile of R rows reads.
+static int64_t kv_keys(const KvShape &s, int64_t R) {
+  return s.window && s.window + R / s.G < s.tokens ? s.window + R / s.G : s.tokens;
+}
+
 // How many splits fit the workspace. (k_kv_attn_keys counts arrivals there too.)
 static int64_t kv_held(const KvShape &s, int variant, int64_t wgs) {
   if (variant < 2 && wgs * 4 > kKvArrivalBytes) return 1;
@@ -35,9 +40,9 @@ static int64_t kv_held(const KvShape &s, int variant, int64_t wgs) {
 
 // The plan of a variant: the number of key splits that takes the least time by these figures, in us as measured (MI355X).
 // - k_kv_attn_keys: a workgroup takes a step of 32 keys in (0.08 + 0.0011 D) WR us when it is not held up by the others
-//   (one sequence of 131072 keys, 8 heads of 128: 8 splits 108 us, 16 splits 60, 32 splits 47 = 5.8 TB/s), together they
+//   (one sequence of 131072 keys, 8 heads of 128: 8 splits 83 us, 16 splits 48, 32 splits 46 = 5.9 TB/s), together they
 //   take 1 / 5.5 TB/s, not quite hiding one under the other, and the last one joins its tile's splits at about 1 us a
-//   round trip (192 splits of 4 rows: 67 us against 47). 48 sequences of 2 k to 8 k keys: 1 split 117 us, 2 113, 4 105, 8 109.
+//   round trip (192 splits of 4 rows: 71 us against 46). 48 sequences of 2 k to 8 k keys: 1 split 114 us, 2 110, 4 105, 8 109.
 // - k_kv_attn_rows: a step of 32 keys takes 0.24 + 0.0028 D us alone on a CU and no less than 0.04 + 0.0023 D for each
 //   workgroup of a CU that runs one; two terms 1.22 and 1.39 times that, 128 rows 1.22 and 1.68 times. A workgroup's rows
 //   and results cost about 6 steps. Joining takes 4 us and the partial results' way to memory and back. (512 tokens
@@ -49,9 +54,7 @@ static KvPlan kv_plan_variant(const KvShape &s, int variant) {
   // workgroups that have keys: sequences of equal length
   const int64_t even = (s.T + s.B - 1) / s.B * s.G;
   const int64_t wgs = (variant < 2 ? s.B : s.B * ((even + R - 1) / R)) * s.Hkv;
-  int64_t keys = s.tokens;
-  if (s.window && s.window + R / s.G < keys) keys = s.window + R / s.G;
-  const int64_t steps = (keys + 31) / 32;
+  const int64_t keys = kv_keys(s, R), steps = (keys + 31) / 32;
   const int64_t rows = s.new_rows * s.G < R ? s.new_rows * s.G : R;
   const double alone = variant < 2 ? (0.08 + 0.0011 * s.D) * (R / 16)
                                    : (0.24 + 0.0028 * s.D) * (s.two ? 1.22 : 1.0) * (R == 128 ? 1.22 : 1.0);
@@ -81,7 +84,7 @@ static KvPlan kv_plan_variant(const KvShape &s, int variant) {
     return p;
   }
   p.time = time_of(1);
-  for (int64_t n = 2; n <= held && 4 * n <= steps; ++n) {
+  for (int64_t n = 2; n <= held && 4 * n <= steps; n += 1 + n / 16) {  // (some 60 numbers at most: this is host time)
     const double time = time_of(n);
     if (time < p.time) {
       p.time = time;
@@ -95,12 +98,14 @@ static KvPlan kv_plan_variant(const KvShape &s, int variant) {
   return p;
 }
 
-// Variant by the rows that share keys. Up to 32 (a decode step, drafted tokens): k_kv_attn_keys, whose waves need not
-// wait for each other (16 sequences of 8 tokens, 4 heads a key head, 6000 keys: D = 128 46 us against 53 with
-// k_kv_attn_rows, D = 256 98 against 123); more: k_kv_attn_rows, whose waves share the conversion (16 tokens: 34 us against
-// 68). Its tiles of 128 rows need half the cache reads, those of 64 keep more waves and even out better: 128 rows only
-// where D = 128 leaves room for their registers and the figures above give them the lesser time (512 tokens behind 7680: 92
-// us against 100; a prompt of 2048: 64 against 57).
+// Variant by the rows that share keys. Up to 16 (a decode step): k_kv_attn_keys, whose waves need not wait for each other. 17
+// to 32 (drafted tokens): the same, but for few sequences of many keys, whose last workgroups would be long in joining
+// 32 rows; k_kv_attn_rows joins them in a launch of its own (8 rows of 4 heads, 8 key heads of 128, bf16, us of the one and
+// the other: 1 sequence of 300 keys 9.9, 11.9, of 2000 15.3, 12.3, of 12000 25.6, 19.2; 3 of 2000 20.0, 15.5, of 12000 31.8,
+// 34.0; 8 of 2000 20.7, 19.9, of 12000 43.7, 49.9; 20 of 12000 112, 130). More: k_kv_attn_rows, whose waves share the
+// conversion (16 sequences of 6000 keys, 64 rows: 78 us against 147). Its tiles of 128 rows need half the cache reads, those
+// of 64 keep more waves and even out better: 128 rows only where D = 128 leaves room for their registers and the figures
+// above give them the lesser time (512 tokens behind 7680: 93 us against 103; a prompt of 2048: 64 against 57).
 static KvPlan kv_plan(const KvShape &s) {
   const int64_t rows = s.new_rows * s.G;
   const bool wide = s.D == 128 && !s.two;
@@ -108,8 +113,11 @@ static KvPlan kv_plan(const KvShape &s) {
     const int v = atoi(e);
     if (v >= 0 && v < (wide ? kKvVariants : kKvVariants - 1)) return kv_plan_variant(s, v);
   }
-  const KvPlan p = kv_plan_variant(s, rows <= 16 ? 0 : rows <= 32 ? 1 : 2);
-  if (p.variant < 2 || !wide) return p;
+  const int64_t steps = (kv_keys(s, 32) + 31) / 32;
+  if (rows <= 16) return kv_plan_variant(s, 0);
+  if (rows <= 32 && (steps < 60 || s.B * s.Hkv * steps > 3500)) return kv_plan_variant(s, 1);
+  const KvPlan p = kv_plan_variant(s, 2);
+  if (!wide) return p;
   const KvPlan q = kv_plan_variant(s, 3);
   return q.time < p.time ? q : p;
 }
