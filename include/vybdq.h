@@ -546,10 +546,10 @@ int vybdq_quant_q8_act(uint64_t X, uint64_t Xq, uint64_t Xs, int64_t M, int64_t 
    each of Hkv heads of D = 64, 128, 192 or 256 dims; codes are e4m3 (OCP, no infinities):
      K  [n_pages][Hkv][page][D]         V  [n_pages][Hkv][page / 4][D][4] (slot s, dim d at [s / 4][d][s % 4])
      Ks, Vs float32 [n_pages][Hkv]      powers of two; value = code * scale
-   The batch, read on the device (calls can be captured; the tables may change between replays): sequence b < B has
-   rows q_start[b] .. q_start[b + 1] - 1 (int32 [B + 1], rising, within 0 .. T) of k, v and q; they are the last of its
-   ctx[b] tokens (int32 [B]); table int32 [B][W] names the page of its tokens i page .. i page + page - 1. The pages
-   that a call appends to must differ between sequences; pages that are only read may be shared.
+   The batch, read on the device (calls can be captured; the tables may change between replays, not during a call):
+   sequence b < B has rows q_start[b] .. q_start[b + 1] - 1 (int32 [B + 1], rising, within 0 .. T) of k, v and q; they are
+   the last of its ctx[b] tokens (int32 [B]); table int32 [B][W] names the page of its tokens i page .. i page + page - 1.
+   The pages that a call appends to must differ between sequences; pages that are only read may be shared.
    max_new and max_ctx are the caller's bounds on a sequence's rows and tokens (0: unknown). They choose the launch
    shape; results are right for any value, but for vybdq_kv_attn's last bits (the split of the keys, which the lengths of the
    whole batch take part in).
@@ -581,8 +581,8 @@ int64_t vybdq_kv_attn_workspace_size(int64_t D);
    operands are fp16 (codes exactly; q scaled by a power of two per row; float32 q and its weights in two fp16 terms).
    ws: 256-byte aligned, of vybdq_kv_attn_workspace_size(D) bytes, zero-filled once before the first call (arrival
    counters that every completed call leaves at zero); a smaller one splits less, 0 not at all. Calls that share a
-   workspace must not overlap. out may be q (ldq = Hq D). One launch, and one to join the results where more than 32 rows of a
-   head's sequence split their keys. (T Hq / (64 Hkv) + B) Hkv must be below 2^24. */
+   workspace must not overlap. out may be q (ldq = Hq D). One launch, or a second to join the results where more than 16
+   rows of a head's sequence split their keys. (T Hq / (64 Hkv) + B) Hkv must be below 2^24. */
 int vybdq_kv_attn(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs, int64_t n_pages, int64_t Hkv, int64_t D, int64_t page,
                   uint64_t q, int x_dt, int64_t ldq, int64_t Hq, uint64_t out, uint64_t lse, uint64_t table, int64_t W,
                   uint64_t q_start, uint64_t ctx, int64_t T, int64_t B, int64_t max_new, int64_t max_ctx, double scale,

@@ -201,71 +201,46 @@ __device__ __forceinline__ T lane_scan(T v) {
   return v;
 }
 
-// Which sequence and part of its keys unit u of k_kv_attn_keys takes. There are B a.splits units for each head. By length, a
-// sequence has a number of them that goes with its own keys (those of its first tile, in steps of 32), so that sequences of
-// unequal lengths end together: the largest share, of four tried, whose parts fit in the units. Every workgroup finds the same
-// numbers. That costs 1 us at its start, and the longest sequence's join takes longer.
+// Which sequence and part of its keys unit u of k_kv_attn_keys takes. There are B a.splits units for each head. By length (B up
+// to 64, a lane each), a sequence has a number of them that goes with its own keys (those of its first tile, in steps of 32),
+// so that sequences of unequal lengths end together: the largest share, of four tried, whose parts fit in the units. Every
+// workgroup finds the same numbers. That costs 1 us at its start, and the longest sequence's join takes longer.
 struct KvPart {
   int b, split, S;
 };
 __device__ __forceinline__ KvPart kv_part(const KvAttnArgs &a, int R, int u) {
   const int B = a.b.B, S = a.splits;
   if (!a.by_length) return {u / S, u % S, S};
-  const int lane = threadIdx.x & 63, each = (B + 63) >> 6, lo = lane * each, hi = lo + each < B ? lo + each : B;
-  auto steps = [&](int b) {
+  const int b = threadIdx.x & 63;
+  float steps = 0.f;
+  if (b < B) {
     const int s0 = a.b.q_start[b], s1 = a.b.q_start[b + 1], ctx = a.b.ctx[b];
-    if (s0 < 0 || s0 >= s1 || s1 > a.b.T || ctx <= 0 || ctx > (a.b.W << a.c.ps)) return 0.f;
-    KvTile t;
-    t.rows = (s1 - s0) * a.G;
-    t.r0 = 0;
-    t.ctx = ctx;
-    t.p0 = ctx - (s1 - s0);
-    kv_tile_keys(a, R, t);
-    return static_cast<float>(t.steps);
-  };
-  auto parts = [](float steps, float share) {
-    const int n = static_cast<int>(ceilf(steps * share));
-    return n > 1 ? n : 1;
-  };
-  const float first = lo < hi ? steps(lo) : 0.f;  // (B <= 64: all that a lane has)
-  float total = first;
-  for (int b = lo + 1; b < hi; ++b) total += steps(b);
-  total = lane_scan(total);
-  total = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(total), 63));
-  // parts per step: units / total, and less, down to what fits whatever is rounded up: sum of ceil(x) < sum of x + B
-  float share[4];
-  int sum[4], upto[4];
-  const float inv = total > 0.f ? B / total : 0.f;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    share[k] = fminf((S - k * (1.f / 3)) * inv, 0.25f);
-    sum[k] = lo < hi ? parts(first, share[k]) : 0;
-  }
-  for (int b = lo + 1; b < hi; ++b) {
-    const float x = steps(b);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) sum[k] += parts(x, share[k]);
-  }
-#pragma unroll
-  for (int k = 0; k < 4; ++k) upto[k] = lane_scan(sum[k]);
-  float chosen = 0.f;  // (one part each, should rounding ever leave none that fits)
-  int mine = hi > lo ? hi - lo : 0, last = hi > lo ? hi : B;
-#pragma unroll
-  for (int k = 3; k >= 0; --k)
-    if (__builtin_amdgcn_readlane(upto[k], 63) <= B * S) {
-      chosen = share[k];
-      mine = sum[k];
-      last = upto[k];
+    if (s0 >= 0 && s0 < s1 && s1 <= a.b.T && ctx > 0 && ctx <= (a.b.W << a.c.ps)) {
+      KvTile t;
+      t.rows = (s1 - s0) * a.G;
+      t.r0 = 0;
+      t.ctx = ctx;
+      t.p0 = ctx - (s1 - s0);
+      kv_tile_keys(a, R, t);
+      steps = static_cast<float>(t.steps);
     }
-  const int owner = __popcll(__ballot(last <= u));  // the lane whose sequences hold unit u
-  KvPart p{-1, u - (last - mine), 1};
-  for (int b = lo; b < hi && p.b < 0; ++b) {
-    p.S = parts(b == lo ? first : steps(b), chosen);
-    if (p.split < p.S) p.b = b;
-    else p.split -= p.S;
   }
-  if (owner >= 64) return {-1, 0, 1};
-  return {__builtin_amdgcn_readlane(p.b, owner), __builtin_amdgcn_readlane(p.split, owner), __builtin_amdgcn_readlane(p.S, owner)};
+  const float total = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lane_scan(steps)), 63));
+  // parts per step: units / total, and less, down to what fits whatever is rounded up: sum of ceil(x) < sum of x + B
+  const float inv = total > 0.f ? B / total : 0.f;
+  int mine = b < B ? 1 : 0, upto = b < B ? b + 1 : B;  // (one part each, should rounding ever leave none that fits)
+#pragma unroll
+  for (int k = 3; k >= 0; --k) {
+    const int n = static_cast<int>(ceilf(steps * fminf((S - k * (1.f / 3)) * inv, 0.25f)));
+    const int parts = b < B ? (n > 1 ? n : 1) : 0, sum = lane_scan(parts);
+    if (__builtin_amdgcn_readlane(sum, 63) <= B * S) {
+      mine = parts;
+      upto = sum;
+    }
+  }
+  const int owner = __popcll(__ballot(upto <= u));
+  if (owner >= 64) return {-1, 0, 1};  // (a unit that no sequence has)
+  return {owner, u - __builtin_amdgcn_readlane(upto - mine, owner), __builtin_amdgcn_readlane(mine, owner)};
 }
 
 // The 16 query rows r .. r + 15 as operands of S^T = K Q^T, one row per column: lane (col, g4) holds dims

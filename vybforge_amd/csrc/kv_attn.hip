@@ -80,7 +80,7 @@ static KvPlan kv_plan_variant(const KvShape &s, int variant) {
     const int64_t n = atoi(e) < 0 ? -atoi(e) : atoi(e);
     p.splits = n < 1 ? 1 : n < held ? n : held;
     p.time = time_of(p.splits);
-    p.by_length = atoi(e) < 0 && variant < 2 && s.B > 1 && p.splits > 1;
+    p.by_length = atoi(e) < 0 && variant < 2 && s.B > 1 && s.B <= 64 && p.splits > 1;
     return p;
   }
   p.time = time_of(1);
@@ -91,10 +91,11 @@ static KvPlan kv_plan_variant(const KvShape &s, int variant) {
       p.splits = n;
     }
   }
-  // By length where the call is long enough to gain by it. Sequences of one to the full length, us with and without: 12 of
-  // 6000 tokens, 4 heads of 128: 16.2, 15.1; of 256, 2 rows: 26.9, 27.6, 5 rows 38.1, 42.0; 48 of 8192, 8 heads of 128: 101.3,
-  // 104.4; 4 of 131072: 131, 142. (All of full length: 34.6, 33.0 and 55.2, 54.3.)
-  p.by_length = variant < 2 && s.B > 1 && p.splits > 1 && p.time >= 25;
+  // By length where the call is long enough to gain by it (more than 64 sequences are many workgroups already). Sequences of
+  // one to the full length, us with and without: 12 of 6000 tokens, 4 heads of 128: 16.2, 15.1; of 256, 2 rows: 26.9, 27.6, 5
+  // rows 38.1, 42.0; 48 of 8192, 8 heads of 128: 101.3, 104.4; 4 of 131072: 131, 142. (All of full length: 34.6, 33.0 and
+  // 55.2, 54.3.)
+  p.by_length = variant < 2 && s.B > 1 && s.B <= 64 && p.splits > 1 && p.time >= 25;
   return p;
 }
 
