@@ -13,7 +13,7 @@
 // cache straight into operand registers (16-byte loads, one e4m3 -> fp16 conversion per two codes; every e4m3
 // value is an fp16 value). Rounded to fp16: the query row, scaled by the power of two that brings its largest
 // value into [2^14, 2^15) (exact for fp16 and bf16 values within 2^-38 of the largest), and w (11 bits down to
-// 2^-26 of the row's largest). For float32 queries both are split into two fp16 terms (22 bits).
+// 2^-22 of the row's largest). For float32 queries both are split into two fp16 terms (22 bits).
 //
 // A wave owns 16 NCT query rows (row = token * G + head of the group; the G query heads of a key head read the
 // same keys, so they share its tiles) and takes 32 keys at a step. Few rows: k_kv_attn_keys, whose waves take turns over the
@@ -125,8 +125,15 @@ __device__ __forceinline__ void store_n(void *p, bool bf16, int64_t i, const flo
 constexpr int kKvVariants = 4;
 constexpr int kv_variant_rows(int variant) { return variant == 0 ? 16 : variant == 1 ? 32 : variant == 2 ? 64 : 128; }
 
-constexpr float kKvRef = 12.0f;    // a row's reference is 2^-12 of its largest weight when it is taken
-constexpr float kKvMove = 15.0f;   // and is taken anew once a weight would pass 2^15
+// A row's reference is 2^-8 of its largest weight, or up to twice that, when it is taken, and is taken anew once a weight would
+// pass 2^15: weights as fp16 operands then hold all their bits down to 2^-22 of the largest and vanish below 2^-33. It is a
+// whole number, so that it adds to a V scale's exponent without rounding, and no larger, because exponents from 8 on are
+// rounded to 2^-21. With two terms (float32 queries) the reference is the largest weight, and the 2^12 that two terms
+// need are a product behind the exponential: 22 bits down to 2^-15 of the largest, below that 2^-37 of it. (lse, relative, of
+// 4 keys and float32 queries: 1.9e-7, with the 2^12 in the exponent 4.7e-7; of 34 keys and bf16 ones with 2^12: 2.3e-7.)
+constexpr float kv_ref(bool two) { return two ? 0.0f : 8.0f; }
+constexpr float kv_move(bool two) { return two ? 3.0f : 15.0f; }
+constexpr float kv_lift(bool two) { return two ? 4096.0f : 1.0f; }
 constexpr float kKvNone = -1e30f;  // the reference of a row that has seen nothing (finite: no inf - inf)
 #define KV_NEG_INF (-__builtin_inff())
 
@@ -329,7 +336,7 @@ __device__ __forceinline__ void kv_weights(const f4 (&s)[NCT][2], const KvRows<C
     for (int e = 1; e < 8; ++e) top[ct] = fmaxf(top[ct], t[ct][e]);
     any = fmaxf(any, top[ct]);
   }
-  if (__ballot(any > kKvMove)) {
+  if (__ballot(any > kv_move(TWO))) {
 #pragma unroll
     for (int ct = 0; ct < NCT; ++ct) {
       // the largest exponent itself, not its difference to the old reference (which may be kKvNone)
@@ -339,7 +346,7 @@ __device__ __forceinline__ void kv_weights(const f4 (&s)[NCT][2], const KvRows<C
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           big = fmaxf(big, t[ct][4 * n + e] == KV_NEG_INF ? KV_NEG_INF : __builtin_fmaf(s[ct][n][e], q[ct].qc * ks[n], ev[n]));
-      const float now = fmaxf(m[ct], col_max(big) - kKvRef);
+      const float now = fmaxf(m[ct], ceilf(col_max(big)) - kv_ref(TWO));
       const float f = __builtin_amdgcn_exp2f(m[ct] - now);
       m[ct] = now;
       l[ct] *= f;
@@ -354,8 +361,9 @@ __device__ __forceinline__ void kv_weights(const f4 (&s)[NCT][2], const KvRows<C
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float w = __builtin_amdgcn_exp2f(t[ct][4 * n + e]);
+        float w = __builtin_amdgcn_exp2f(t[ct][4 * n + e]);
         l[ct] = __builtin_fmaf(w, iv[n], l[ct]);  // not of the rounded weight: lse is a float32 result
+        w *= kv_lift(TWO);
         const _Float16 f = static_cast<_Float16>(w);
         p[ct][0][4 * n + e] = f;
         if constexpr (TWO) p[ct][1][4 * n + e] = static_cast<_Float16>(w - static_cast<float>(f));
@@ -378,12 +386,17 @@ struct KvSink {
     const int rr = t.r0 + r;
     if (rr >= t.rows) return;
     const int64_t at = (t.sq.s0 + rr / a.G) * (static_cast<int64_t>(a.c.Hkv) * a.G) + h * a.G + rr % a.G;
-    const float f = lr == 0.f ? 0.f : 1.0f / lr;
+    const float f = lr == 0.f ? 0.f : (1.0f / kv_lift(TWO)) / lr;
     float y[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) y[e] = x[e] * f;
     store_n<TWO, N>(a.out, a.dt == VYBDQ_BF16, at * D + d, y);
-    if (a.lse && d == 0) a.lse[at] = lr == 0.f ? KV_NEG_INF : (mr + __builtin_amdgcn_logf(lr)) * 0.6931471805599453f;
+    if (a.lse && d == 0) {  // ln 2 (m + log2 l), the logarithm of a number near one, ln 2 as a float32 and the rest of it
+      constexpr double kLn2 = 0.6931471805599453;
+      constexpr float hi = static_cast<float>(kLn2), lo = static_cast<float>(kLn2 - hi), r = kv_ref(TWO);
+      const float at_max = mr + r, rest = __builtin_amdgcn_logf(lr * (TWO ? 1.0f : 1.0f / 256));
+      a.lse[at] = lr == 0.f ? KV_NEG_INF : __builtin_fmaf(at_max, hi, __builtin_fmaf(rest, hi, at_max * lo));
+    }
   }
   template <int N>
   __device__ __forceinline__ void put(int r, float mr, float lr, int d, const float (&x)[N]) const {
