@@ -23,12 +23,12 @@
 //
 // What bounds them, MI355X (a large copy runs at 4.7 TB/s, a large fp16 product at 1089 TFLOP/s): 48 sequences of 2 to 8 k
 // tokens, one row each, 32 / 8 heads of 128: 102 us, 5.1 TB/s of codes; 4 of up to 131072: 132 us, 5.5 TB/s. A prompt of 4096
-// tokens: 173 us, 793 TFLOP/s; 513 tokens behind 32 k: 345 us, 791 TFLOP/s. Of the prompt's 173 us the matrix instructions
-// (18 cycles each on a SIMD with four waves) are 64, the LDS reads that feed them 30 (128 rows) to 60 (64 rows) beside them;
-// without loads and conversion it took 141 us, without exponentials 169. With heads of 64 a step of 16 rows is 130 cycles
-// of matrix instructions and some 310 of vector instructions, two thirds of them the softmax: 457 TFLOP/s with a window of 4096.
-// 32x32x16 instructions in the same scheme were no faster (prompt 177 to 188 us, heads of 64 83 to 97 against 87), nor were
-// two tiles of 16 rows of heads of 64 to a wave (93 against 87).
+// tokens: 170 us, 807 TFLOP/s; 513 tokens behind 32 k: 344 us, 795 TFLOP/s. Of the prompt's time the matrix instructions
+// (18 cycles each on a SIMD with four waves) are 64 us, the LDS reads that feed them 30 (128 rows) to 60 (64 rows) beside
+// them; when it took 180, it took 141 without loads and conversion and 169 without exponentials. With heads of 64 a step
+// of 16 rows is 130 cycles of matrix instructions and some 310 of vector instructions, two thirds of them the softmax: 457
+// TFLOP/s with a window of 4096. 32x32x16 instructions in the same scheme were no faster (prompt 177 to 188 us, heads of
+// 64 83 to 97 against 87), nor were two tiles of 16 rows of heads of 64 to a wave (93 against 87).
 #pragma once
 
 #include "kv.h"
