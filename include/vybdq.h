@@ -579,6 +579,8 @@ int64_t vybdq_kv_attn_workspace_size(int64_t D);
    j > p_i - window if window > 0. A row that sees nothing is 0, with lse -infinity. lse (float32 [T][Hq], or 0): the natural
    log of the sum of exp(scale q . k). q, out: x_dt, q's row stride ldq. Softmax and sums are float32 in one pass;
    operands are fp16 (codes exactly; q scaled by a power of two per row; float32 q and its weights in two fp16 terms).
+   V scales within one row's context may lie 2^100 apart: a key whose V scale is 2^d below the largest that counts is lost
+   once its weight is below 2^(d - 126) of the row's largest.
    ws: 256-byte aligned, of vybdq_kv_attn_workspace_size(D) bytes, zero-filled once before the first call (arrival
    counters that every completed call leaves at zero); a smaller one splits less, 0 not at all. Calls that share a
    workspace must not overlap. out may be q (ldq = Hq D). One launch, or a second to join the results where more than 16
