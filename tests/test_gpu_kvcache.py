@@ -550,6 +550,22 @@ def test_other_stream(dev, rng):
     assert torch.equal(here, there)
 
 
+def test_workspace_made_behind_other_work_is_ready_on_another_stream(dev, rng):
+    table, start, ctx, n_pages = tables(rng, [(1, 4000)], 64)
+    cache, t = device_cache(dev, random_cache(rng, n_pages, 1, 64, 64)), on(dev, table, start, ctx)
+    q = torch.randn(1, 4, 64, device=dev)
+    want = ops.KvAttention(4, 1, 64, dev)(q, cache, *t).clone()
+    side, a = torch.cuda.Stream(), torch.randn(4096, 4096, device=dev)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        a = a @ a * 1e-3
+    attend = ops.KvAttention(4, 1, 64, dev)
+    with torch.cuda.stream(side):
+        got = attend(q, cache, *t)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
 def test_graphs_of_a_decode_loop(dev, rng):
     """Append and attention captured for two batch sizes over one cache and one workspace; the tables move on between
     replays, eager calls run between them, and every replay equals the eager result."""

@@ -716,6 +716,8 @@ class KvAttention:
         self.ws_bytes = _lib.lib.vybdq_kv_attn_workspace_size(head_dim)
         # zero-filled once: the arrival counters at its start must be zero (each call leaves them so)
         self.ws = torch.zeros(self.ws_bytes + 256, dtype=torch.uint8, device=device)
+        if self.ws.is_cuda and not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(self.ws.device).synchronize()  # the first call may be on another stream
         self.ws_ptr, self.index = (self.ws.data_ptr() + 255) // 256 * 256, self.ws.get_device()
 
     def __call__(self, q, cache, page_table, q_start, ctx, scale=None, causal=True, window=0, max_new=None,
