@@ -580,7 +580,9 @@ int64_t vybdq_kv_attn_workspace_size(int64_t D);
    log of the sum of exp(scale q . k). q, out: x_dt, q's row stride ldq. Softmax and sums are float32 in one pass;
    operands are fp16 (codes exactly; q scaled by a power of two per row; float32 q and its weights in two fp16 terms).
    V scales within one row's context may lie 2^100 apart: a key whose V scale is 2^d below the largest that counts is lost
-   once its weight is below 2^(d - 126) of the row's largest.
+   once its weight is below 2^(d - 126) of the row's largest. Scores may be as large as float32 holds
+   (times log2 e; past that they give NaN or nothing). In a row with scores past 2900000 (2^22 ln 2) either way, and in up
+   to 31 rows beside it, V scales may lie 2^22 apart (2^15 for float32 q) before weights lose bits.
    ws: 256-byte aligned, of vybdq_kv_attn_workspace_size(D) bytes, zero-filled once before the first call (arrival
    counters that every completed call leaves at zero); a smaller one splits less, 0 not at all. Calls that share a
    workspace must not overlap. out may be q (ldq = Hq D). One launch, or a second to join the results where more than 16

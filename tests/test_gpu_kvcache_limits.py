@@ -1,0 +1,177 @@
+"""Attention over the 8-bit cache at the ends of its ranges: scores past the whole numbers that float32 tells apart, and
+below every reference; sliding windows behind which pages are gone; batches larger than one lane or one counter each."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import kvcache
+from vybforge_amd import ops
+
+from test_gpu_kvcache import DT, check_attention, device_cache, on, random_cache, tables, tolerance
+
+pytestmark = pytest.mark.gpu
+
+VARIANTS = [(0, "bf16", 64), (0, "f32", 256), (1, "f16", 128), (1, "f32", 64), (2, "f16", 64), (2, "f32", 128), (2, "bf16", 192),
+            (2, "f32", 256), (3, "bf16", 128), (3, "f16", 128)]
+LENS = [(1, 700), (70, 203), (0, 50), (33, 33), (5, 90), (3, 2)]
+
+
+def force(monkeypatch, variant, splits):
+    monkeypatch.setenv("VYBDQ_KV_VARIANT", str(variant))
+    monkeypatch.setenv("VYBDQ_KV_SPLITS", str(splits))
+
+
+def score_error(reach, D, x):
+    """tolerance()'s bound on a score's error, in nats."""
+    return reach * ((D + 8) * 2.0 ** -24 + (2.0 ** -22 if x == "f32" else 0)) + (64 + 1.5 * reach) * 2.0 ** -24 + 2.0 ** -22
+
+
+def check_large(got, stats, q, want, table, start, ctx, scale, window, x):
+    """Rows whose scores stay below 2^18 by tolerance(). Of the others, whose scores are only known to more than one nat: the
+    output lies among the values that the row sees, lse at the largest score; and where the largest score leads the next by
+    more than both may be off and 40 nats (the weights of 3000 keys together below 2^-46), the output is that key's value,
+    up to the rounding of its weight (2^-11, of two terms 2^-21), of their quotient and of the output. How many were led."""
+    T, Hq, D = q.shape
+    G, led, large = Hq // want.k.shape[1], 0, 0
+    got, stats = got.double().cpu().numpy(), stats.double().cpu().numpy()
+    half, wr = torch.finfo(DT[x]).eps / 2, 2.0 ** -21 if x == "f32" else 2.0 ** -11
+    for b in range(len(ctx)):
+        n = int(start[b + 1] - start[b])
+        heads = [want.values(table[b], ctx[b], h) for h in range(Hq // G)]
+        for hq in range(Hq):
+            k, v = heads[hq // G]
+            r = slice(start[b], start[b + 1])
+            o, z, weight, reach = kvcache.attention(q[r, hq], k, v, ctx[b] - n, ctx[b], scale, True, window)
+            to, tz = tolerance(o, np.where(np.isfinite(z), z, 0), weight, reach, D, ctx[b], x)
+            for i in range(n):
+                y, s, pos = got[start[b] + i, hq], stats[start[b] + i, hq], ctx[b] - n + i
+                seen = np.arange(max(0, pos - window + 1) if window else 0, pos + 1)
+                if not len(seen):
+                    assert (y == 0).all() and np.isneginf(s), (b, hq, i)
+                    continue
+                if reach[i] < 2.0 ** 18:
+                    assert (np.abs(y - o[i]) <= to[i]).all() and abs(s - z[i]) <= tz[i], (b, hq, i)
+                    continue
+                large += 1
+                ds = score_error(reach[i], D, x)
+                t, vs = (k[seen] @ q[start[b] + i, hq]) * scale, v[seen]
+                assert abs(s - z[i]) <= ds + 2.0 ** -22 * abs(z[i]), (b, hq, i, s, z[i])
+                room = (half + wr + (2 * len(seen) + 128) * 2.0 ** -23) * (1 + half) * np.abs(vs).max(0)
+                assert (y <= vs.max(0) + room).all() and (y >= vs.min(0) - room).all(), (b, hq, i, y)
+                order = np.argsort(t)
+                if len(t) > 1 and t[order[-1]] - t[order[-2]] <= 2 * ds + 40:
+                    continue
+                led += 1
+                top = vs[order[-1]]
+                assert (np.abs(y - top) <= (half + wr + 2.0 ** -21) * (1 + half) * np.abs(top)).all(), (b, hq, i)
+    return led, large
+
+
+def run_large(dev, rng, lens, Hq, Hkv, D, page, x, size, sign=1, window=0, mixed=False):
+    """Scores of about `size` nats, all negative with sign < 0; mixed: rows of sizes of their own, and pages whose keys are
+    small, so that a row's scores jump from small to large and back."""
+    table, start, ctx, n_pages = tables(rng, lens, page)
+    want = random_cache(rng, n_pages, Hkv, page, D)
+    want.k_scale[:] = 2.0 ** rng.integers(-1, 2, want.k_scale.shape)
+    if mixed:
+        want.k_scale *= 2.0 ** rng.choice([0, -30], want.k_scale.shape)
+    if sign < 0:
+        want.k &= 0x7f
+    q = rng.standard_normal((int(start[-1]), Hq, D)) * (2.0 ** rng.integers(-30, 1, (int(start[-1]), Hq, 1)) if mixed else 1)
+    q = torch.from_numpy((-np.abs(q) if sign < 0 else q).astype(np.float32)).to(DT[x])
+    scale = size / (80 * D ** 0.5)
+    got, stats = ops.KvAttention(Hq, Hkv, D, dev)(q.to(dev), device_cache(dev, want), *on(dev, table, start, ctx), scale=scale,
+                                                  window=window, lse=True)
+    ops.kv_status()
+    return check_large(got, stats, q.double().numpy(), want, table, start, ctx, scale, window, x)
+
+
+@pytest.mark.parametrize("size", [1e8, 1e9, 1e12, 1e33])
+@pytest.mark.parametrize("variant,x,D", VARIANTS)
+def test_large_scores(dev, rng, monkeypatch, variant, x, D, size):
+    for splits in (1, 3):
+        force(monkeypatch, variant, splits)
+        led, large = run_large(dev, rng, LENS, 2, 1, D, 16, x, size)
+        assert large > 100 and led > 0.9 * large
+
+
+@pytest.mark.parametrize("size", [1e9, 1e35])
+@pytest.mark.parametrize("variant,x,D", VARIANTS)
+def test_rows_whose_scores_are_all_far_below_zero(dev, rng, monkeypatch, variant, x, D, size):
+    """They have weights that sum to one like any others, and a finite lse."""
+    for splits in (1, 3):
+        force(monkeypatch, variant, splits)
+        led, large = run_large(dev, rng, LENS, 2, 2, D, 32, x, size, sign=-1)
+        assert large > 100 and led > 0.9 * large
+
+
+@pytest.mark.parametrize("variant,x,D", VARIANTS)
+def test_large_and_small_scores_side_by_side(dev, rng, monkeypatch, variant, x, D):
+    """Rows of all sizes in one wave, over pages of small and of large keys."""
+    for splits, window in ((1, 0), (3, 0), (2, 40)):
+        force(monkeypatch, variant, splits)
+        led, large = run_large(dev, rng, LENS, 3, 1, D, 16, x, 1e9, window=window, mixed=True)
+        assert large > 50 and led > 0.5 * large
+
+
+@pytest.mark.parametrize("x", ["f16", "f32"])
+@pytest.mark.parametrize("n", [1, 6, 80])
+def test_large_queries_and_keys(dev, rng, x, n):
+    """Entries of some thousands in q and K at the usual scale, by the plan's own choice of kernel and splits."""
+    D, page, Hq = 128, 64, 4
+    table, start, ctx, n_pages = tables(rng, [(n, 2000), (n, 100)], page)
+    want = random_cache(rng, n_pages, 1, page, D)
+    want.k_scale[:] = 2.0 ** 6
+    q = torch.from_numpy((rng.standard_normal((2 * n, Hq, D)) * 3000).astype(np.float32)).to(DT[x])
+    got, stats = ops.KvAttention(Hq, 1, D, dev)(q.to(dev), device_cache(dev, want), *on(dev, table, start, ctx), lse=True, max_new=n)
+    led, large = check_large(got, stats, q.double().numpy(), want, table, start, ctx, D ** -0.5, 0, x)
+    assert large == 2 * n * Hq and led > 0.9 * large
+
+
+@pytest.mark.parametrize("size", [1.0, 1e9, -1e9, -1e32])
+@pytest.mark.parametrize("variant,x,D", VARIANTS)
+def test_equal_scores_have_equal_weights(dev, rng, monkeypatch, variant, x, D, size):
+    """All keys alike, over pages with scales of their own (the same values by other codes): every row is the mean of the
+    values that it sees, whatever the scores' size, with lse the score and the logarithm of their number."""
+    page, lens = 16, LENS[:-1]
+    table, start, ctx, n_pages = tables(rng, lens, page)
+    want = random_cache(rng, n_pages, 1, page, D)
+    key, shift = rng.choice([8.0, 9.0, 12.0, 15.0, 30.0], D), rng.integers(-3, 4, n_pages)
+    want.k[:] = kvcache.e4m3_encode(key * 2.0 ** -shift[:, None, None, None])
+    want.k_scale[:] = 2.0 ** (shift[:, None] - 3.0)
+    scale = size / (1.5 * D)
+    q = torch.from_numpy(np.abs(rng.standard_normal((int(start[-1]), 2, D))).astype(np.float32)).to(DT[x])
+    for splits in (1, 5):
+        force(monkeypatch, variant, splits)
+        got, stats = ops.KvAttention(2, 1, D, dev)(q.to(dev), device_cache(dev, want), *on(dev, table, start, ctx), scale=scale, lse=True)
+        got, stats = got.double().cpu().numpy(), stats.double().cpu().numpy()
+        for b, (n, c) in enumerate(lens):
+            k, v = want.values(table[b], c, 0)
+            for i in range(n):
+                seen = c - n + i + 1
+                for h in range(2):
+                    qr = q[start[b] + i, h].double().numpy()
+                    z, reach = qr @ k[0] * scale + np.log(seen), abs(qr @ k[0] * scale)
+                    mean, weight = v[:seen].mean(0), np.abs(v[:seen]).mean(0)
+                    rel = (2.0 ** -21 if x == "f32" else 2.0 ** -11) + (2 * c + 128) * 2.0 ** -23 + 2.0 ** -20
+                    half = torch.finfo(DT[x]).eps / 2
+                    at = start[b] + i, h
+                    assert (np.abs(got[at] - mean) <= half * np.abs(mean) + rel * (1 + half) * weight).all(), (b, i, h)
+                    assert abs(stats[at] - z) <= score_error(reach, D, x) + (c + 64) * 2.0 ** -23 + 2.0 ** -22 * (1 + abs(z)), (b, i, h)
+    ops.kv_status()
+
+
+def test_large_scores_and_value_scales_far_apart(dev, rng, monkeypatch):
+    """The page of the leading key has values 2^12 below the largest page's."""
+    for variant, x, D in VARIANTS:
+        force(monkeypatch, variant, 2)
+        table, start, ctx, n_pages = tables(rng, [(2, 200)], 16)
+        want = random_cache(rng, n_pages, 1, 16, D)
+        want.k_scale[:] = 1.0
+        want.v_scale[:, 0] = 2.0 ** rng.choice([-12, -6, 0], n_pages)
+        q = torch.from_numpy(rng.standard_normal((2, 4, D)).astype(np.float32)).to(DT[x])
+        scale = 1e9 / (80 * D ** 0.5)
+        got, stats = ops.KvAttention(4, 1, D, dev)(q.to(dev), device_cache(dev, want), *on(dev, table, start, ctx), scale=scale, lse=True)
+        led, large = check_large(got, stats, q.double().numpy(), want, table, start, ctx, scale, 0, x)
+        assert led >= 7 and large == 8

@@ -5,7 +5,7 @@
 //   w_ij = 2^(t_ij - m_i), acc_i = sum_j w_ij v_j, l_i = sum_j w_ij 2^-ev, o_i = acc_i / l_i
 // with v_j, k_j the bare codes: the K scale is one factor per 16 keys in the exponent's fma, and the V scale rides
 // in the exponent too, so no code is ever multiplied by its scale. m_i is a running reference that follows the
-// largest t: w stays within 2^15, whatever the pages' scales are. One pass over the keys.
+// largest t: w stays within 2^15, whatever the pages' scales are (references from 2^22 on: kKvFar below). One pass over the keys.
 //
 // Matrix instructions (16x16x32 fp16, float32 sums) on transposed products, so that nothing is ever moved between
 // lanes: S^T = K Q^T puts 4 consecutive keys of one query row in a lane, and that is already the layout in which
@@ -134,8 +134,20 @@ constexpr int kv_variant_rows(int variant) { return variant == 0 ? 16 : variant 
 constexpr float kv_ref(bool two) { return two ? 0.0f : 8.0f; }
 constexpr float kv_move(bool two) { return two ? 3.0f : 15.0f; }
 constexpr float kv_lift(bool two) { return two ? 4096.0f : 1.0f; }
-constexpr float kKvNone = -1e30f;  // the reference of a row that has seen nothing (finite: no inf - inf)
+constexpr float kKvNone = -3.402823466e38f;  // the reference of a row that has seen nothing: the lowest finite (no inf - inf)
 #define KV_NEG_INF (-__builtin_inff())
+
+// From references of 2^22 on (scores times log2 e) float32 no longer holds a score and a V scale's exponent side by side, nor
+// what is left of a product beside its rounded self: t - m, rounded other than m was, could leave a weight at 2^64 or at nothing.
+// A wave one of whose rows gets there keeps the two apart from then on: weight 2^((p - m) + (ev - scale)), with p the product
+// rounded to float32, m the largest p of the row, and scale, one number for the wave, 2^-8 of the largest V scale so far (two
+// terms: that scale). Equal products then have equal weights of whatever size they are, and none is above 2^8. The price is that
+// V scales count against each other over a whole wave: weights of pages 2^22 (two terms: 2^15) below the largest lose bits.
+constexpr float kKvFar = 4194304.0f;
+struct KvFar {
+  float limit;  // kv_move(), or NaN in a wave that is there: every step then takes the branch that moves references
+  float scale;
+};
 
 // What the kernels only read, through the constant address space: uniform reads become scalar loads.
 template <class T>
@@ -298,14 +310,27 @@ __device__ __forceinline__ void kv_load_rows(const KvAttnArgs &a, const KvTile &
     }
 }
 
+__device__ __forceinline__ float kv_uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
+
 // Weights of one tile of scores. s[ct][n]: the products of 2 blocks of 16 keys with the rows of column tile ct; ks, ev, iv: the
-// blocks' K scale, V exponent and 2^-ev. Updates m, l and acc, returns the weights as operands of O^T = V^T P^T.
+// blocks' K scale, V exponent and 2^-ev. Updates m, far, l and acc, returns the weights as operands of O^T = V^T P^T.
 template <int NCT, int C, bool TWO>
 __device__ __forceinline__ void kv_weights(const f4 (&s)[NCT][2], const KvRows<C, TWO> (&q)[NCT], const float (&ks)[2],
-                                           const float (&ev)[2], const float (&iv)[2], int tok, bool masked, float (&m)[NCT],
-                                           float (&l)[NCT], f4 (&acc)[NCT][4 * C], h8 (&p)[NCT][TWO ? 2 : 1]) {
+                                           const float (&ev)[2], const float (&iv)[2], int tok, bool masked, KvFar &far,
+                                           float (&m)[NCT], float (&l)[NCT], f4 (&acc)[NCT][4 * C], h8 (&p)[NCT][TWO ? 2 : 1]) {
   const int g4 = (threadIdx.x & 63) >> 4;
   float t[NCT][8];
+  auto hide = [&]() {
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = tok + 16 * n + 4 * g4 + e;
+          t[ct][4 * n + e] = key >= q[ct].lo && key < q[ct].hi ? t[ct][4 * n + e] : KV_NEG_INF;
+        }
+  };
   auto exponents = [&]() {  // t - m
 #pragma unroll
     for (int ct = 0; ct < NCT; ++ct)
@@ -315,17 +340,7 @@ __device__ __forceinline__ void kv_weights(const f4 (&s)[NCT][2], const KvRows<C
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[ct][4 * n + e] = __builtin_fmaf(s[ct][n][e], ck, add);
       }
-    if (masked) {
-#pragma unroll
-      for (int ct = 0; ct < NCT; ++ct)
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int key = tok + 16 * n + 4 * g4 + e;
-            t[ct][4 * n + e] = key >= q[ct].lo && key < q[ct].hi ? t[ct][4 * n + e] : KV_NEG_INF;
-          }
-    }
+    if (masked) hide();
   };
   exponents();
   float top[NCT], any = KV_NEG_INF;
@@ -336,24 +351,71 @@ __device__ __forceinline__ void kv_weights(const f4 (&s)[NCT][2], const KvRows<C
     for (int e = 1; e < 8; ++e) top[ct] = fmaxf(top[ct], t[ct][e]);
     any = fmaxf(any, top[ct]);
   }
-  if (__ballot(any > kv_move(TWO))) {
+  // (told to be rare: laid out as likely ones, the two branches cost a prompt 3 %)
+  if (__builtin_expect(__ballot(!(any <= far.limit)) != 0, 0)) {
+    if (__builtin_expect(far.limit == kv_move(TWO), 1)) {
+      float now[NCT];
+      bool beyond = false;
 #pragma unroll
-    for (int ct = 0; ct < NCT; ++ct) {
-      // the largest exponent itself, not its difference to the old reference (which may be kKvNone)
-      float big = KV_NEG_INF;
+      for (int ct = 0; ct < NCT; ++ct) {
+        // the largest exponent itself, not its difference to the old reference (which may be kKvNone)
+        float big = KV_NEG_INF;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          big = fmaxf(big, t[ct][4 * n + e] == KV_NEG_INF ? KV_NEG_INF : __builtin_fmaf(s[ct][n][e], q[ct].qc * ks[n], ev[n]));
-      const float now = fmaxf(m[ct], ceilf(col_max(big)) - kv_ref(TWO));
-      const float f = __builtin_amdgcn_exp2f(m[ct] - now);
-      m[ct] = now;
-      l[ct] *= f;
+          for (int e = 0; e < 4; ++e)
+            big = fmaxf(big, t[ct][4 * n + e] == KV_NEG_INF ? KV_NEG_INF : __builtin_fmaf(s[ct][n][e], q[ct].qc * ks[n], ev[n]));
+        now[ct] = fmaxf(m[ct], ceilf(col_max(big)) - kv_ref(TWO));
+        beyond |= fabsf(now[ct]) >= kKvFar && now[ct] != kKvNone;
+      }
+      if (__ballot(beyond)) {
+        far = {__builtin_nanf(""), kv_uniform(fmaxf(ev[0], ev[1]) - kv_ref(TWO))};
 #pragma unroll
-      for (int d = 0; d < 4 * C; ++d) acc[ct][d] *= f;
+        for (int ct = 0; ct < NCT; ++ct) m[ct] -= far.scale;
+      } else {
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct) {
+          const float f = __builtin_amdgcn_exp2f(m[ct] - now[ct]);
+          m[ct] = now[ct];
+          l[ct] *= f;
+#pragma unroll
+          for (int d = 0; d < 4 * C; ++d) acc[ct][d] *= f;
+        }
+        exponents();
+      }
     }
-    exponents();
+    if (far.limit != kv_move(TWO)) {
+#pragma clang fp contract(off)
+      const float scale = kv_uniform(fmaxf(far.scale, fmaxf(ev[0], ev[1]) - kv_ref(TWO)));
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float ck = q[ct].qc * ks[n];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t[ct][4 * n + e] = s[ct][n][e] * ck;
+        }
+      if (masked) hide();
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) {
+        float big = t[ct][0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) big = fmaxf(big, t[ct][e]);
+        big = col_max(big);
+        // (whole numbers where they can be, as elsewhere: p - m is then rounded once)
+        const float now = fmaxf(m[ct], fabsf(big) < kKvFar ? ceilf(big) : big);
+        const float f = __builtin_amdgcn_exp2f((m[ct] - now) + (far.scale - scale));
+        m[ct] = now;
+        l[ct] *= f;
+#pragma unroll
+        for (int d = 0; d < 4 * C; ++d) acc[ct][d] *= f;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t[ct][4 * n + e] = (t[ct][4 * n + e] - now) + (ev[n] - scale);
+      }
+      far.scale = scale;
+    }
   }
 #pragma unroll
   for (int ct = 0; ct < NCT; ++ct)
@@ -368,6 +430,21 @@ __device__ __forceinline__ void kv_weights(const f4 (&s)[NCT][2], const KvRows<C
         p[ct][0][4 * n + e] = f;
         if constexpr (TWO) p[ct][1][4 * n + e] = static_cast<_Float16>(w - static_cast<float>(f));
       }
+}
+
+// A wave's sums as every other's: m alone their reference. It stays the row's p where that is far, so that equal products are
+// joined with equal weights.
+template <int NCT, int C, bool TWO>
+__device__ __forceinline__ void kv_settle(const KvFar &far, float (&m)[NCT], float (&l)[NCT], f4 (&acc)[NCT][4 * C]) {
+  if (far.limit == kv_move(TWO)) return;
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    const float r = fabsf(m[ct]) < kKvFar ? kv_ref(TWO) : 0.f, f = __builtin_amdgcn_exp2f(far.scale + r);
+    m[ct] -= r;
+    l[ct] *= f;
+#pragma unroll
+    for (int d = 0; d < 4 * C; ++d) acc[ct][d] *= f;
+  }
 }
 
 // Where a tile's results go: the output, or the workspace as one of S partial results. COHERENT: partials that another
@@ -583,6 +660,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_kv_attn_keys(const Kv
     }
 
     KvRows<C, TWO> q[1];
+    KvFar far = {kv_move(TWO), 0.f};
     float m[1] = {kKvNone}, l[1] = {t.past ? __builtin_nanf("") : 0.f};
     f4 acc[1][4 * C];
     kv_load_rows<C, TWO>(a, t, t.r0 + 16 * wr, h, q[0]);
@@ -626,7 +704,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_kv_attn_keys(const Kv
         }
       }
       h8 p[1][NQ];
-      kv_weights<1, C, TWO>(s, q, ks, ev, iv, tok, tok < t.free0 || tok + 32 > t.free1, m, l, acc, p);
+      kv_weights<1, C, TWO>(s, q, ks, ev, iv, tok, tok < t.free0 || tok + 32 > t.free1, far, m, l, acc, p);
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -655,6 +733,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) k_kv_attn_keys(const Kv
 
     // the waves' results, joined through LDS
     const KvSink<D, R, TWO, true> sink{a, t, h, whole, a.part + static_cast<int64_t>(blockIdx.x) * (R * (D + 2))};
+    kv_settle<1, C, TWO>(far, m, l, acc);
     l[0] = col_sum(l[0]);
     if (t.r0 > 0) __syncthreads();
 #pragma unroll
@@ -785,6 +864,7 @@ __global__ void __launch_bounds__(256, NCT > 1 || D == 256 || (TWO && D == 192) 
     fetch(t0);
   }
   KvRows<C, TWO> q[NCT];
+  KvFar far = {kv_move(TWO), 0.f};
   float m[NCT], l[NCT];
   f4 acc[NCT][4 * C];
 #pragma unroll
@@ -835,7 +915,7 @@ __global__ void __launch_bounds__(256, NCT > 1 || D == 256 || (TWO && D == 192) 
 #pragma unroll
     for (int d = 0; d < 2 * C; ++d) vf[d] = tile[buf][4 * C + d][lane];
     h8 p[NCT][NQ];
-    kv_weights<NCT, C, TWO>(s, q, sk, ev, iv, tok, tok < t.free0 || tok + 32 > t.free1, m, l, acc, p);
+    kv_weights<NCT, C, TWO>(s, q, sk, ev, iv, tok, tok < t.free0 || tok + 32 > t.free1, far, m, l, acc, p);
 #pragma unroll
     for (int d = 0; d < 4 * C; ++d) {
 #pragma unroll
@@ -848,6 +928,7 @@ __global__ void __launch_bounds__(256, NCT > 1 || D == 256 || (TWO && D == 192) 
   }
 
   const KvSink<D, R, TWO, false> sink{a, t, h, S == 1, a.part + (static_cast<int64_t>(blockIdx.x) * S + split) * (R * (D + 2))};
+  kv_settle<NCT, C, TWO>(far, m, l, acc);
 #pragma unroll
   for (int ct = 0; ct < NCT; ++ct) {
     l[ct] = col_sum(l[ct]);
