@@ -576,7 +576,8 @@ int64_t vybdq_kv_attn_workspace_size(int64_t D);
 
 /* out [T][Hq][D] = softmax over the keys j that row i of its sequence sees of (scale q_i . k_j), times v_j; query head h
    reads key head h / (Hq / Hkv). With p_i = ctx - rows + i the row's position, it sees j < ctx, j <= p_i if causal, and
-   j > p_i - window if window > 0. A row that sees nothing is 0, with lse -infinity. lse (float32 [T][Hq], or 0): the natural
+   j > p_i - window if window > 0. Pages behind the window of a sequence's first row are not read, nor their table entries: a
+   host may have given them away. A row that sees nothing is 0, with lse -infinity. lse (float32 [T][Hq], or 0): the natural
    log of the sum of exp(scale q . k). q, out: x_dt, q's row stride ldq. Softmax and sums are float32 in one pass;
    operands are fp16 (codes exactly; q scaled by a power of two per row; float32 q and its weights in two fp16 terms).
    V scales within one row's context may lie 2^100 apart: a key whose V scale is 2^d below the largest that counts is lost

@@ -175,3 +175,25 @@ def test_large_scores_and_value_scales_far_apart(dev, rng, monkeypatch):
         got, stats = ops.KvAttention(4, 1, D, dev)(q.to(dev), device_cache(dev, want), *on(dev, table, start, ctx), scale=scale, lse=True)
         led, large = check_large(got, stats, q.double().numpy(), want, table, start, ctx, scale, 0, x)
         assert led >= 7 and large == 8
+
+
+@pytest.mark.parametrize("gone", ["outside", "reused"])
+@pytest.mark.parametrize("variant,x,D", VARIANTS)
+def test_pages_behind_the_window_are_not_looked_at(dev, rng, monkeypatch, variant, x, D, gone):
+    """A host that frees them leaves entries that name no page, or a page with NaN codes and scales."""
+    for page, window, splits in ((16, 5, 1), (16, 40, 2), (16, 65, 1), (32, 40, 2), (64, 33, 1)):
+        force(monkeypatch, variant, splits)
+        lens = [(n, c) for n in (1, 3, 40) for c in (120, 129, 150, 160, 185)]
+        table, start, ctx, n_pages = tables(rng, lens, page)
+        want = random_cache(rng, n_pages + 1, 1, page, D)
+        want.k[n_pages], want.v[n_pages], want.k_scale[n_pages], want.v_scale[n_pages] = 0x7f, 0x7f, np.nan, np.nan
+        left = table.copy()
+        for b, (n, c) in enumerate(lens):
+            first = max(0, c - n - window + 1) // page  # the page of the first key that the first row sees
+            left[b, :first] = -1 - b if gone == "outside" else n_pages
+        q = torch.from_numpy(rng.standard_normal((int(start[-1]), 2, D)).astype(np.float32)).to(DT[x])
+        for causal in (True, False):
+            got, stats = ops.KvAttention(2, 1, D, dev)(q.to(dev), device_cache(dev, want), *on(dev, left, start, ctx), causal=causal,
+                                                       window=window, lse=True)
+            check_attention(got, stats, q.double().numpy(), want, table, start, ctx, D ** -0.5, causal, window, x)
+            ops.kv_status()

@@ -192,7 +192,7 @@ __device__ __forceinline__ void kv_tile_keys(const KvAttnArgs &a, int R, KvTile 
   int k1 = a.causal ? t.p0 + i_hi + 1 : t.ctx;
   k1 = k1 > 0 ? k1 : 0;
   const int first = a.window ? t.p0 + i_lo - a.window + 1 : 0;
-  t.k0 = (first > 0 ? first : 0) & ~31;
+  t.k0 = (first > 0 ? first : 0) & ~15;  // (whole blocks of 16: the pages before them may be gone)
   t.steps = k1 > t.k0 ? (k1 - t.k0 + 31) >> 5 : 0;
   t.free0 = a.window ? t.p0 + i_hi - a.window + 1 : 0;
   t.free1 = a.causal ? t.p0 + i_lo + 1 : t.ctx;
