@@ -197,3 +197,22 @@ def test_pages_behind_the_window_are_not_looked_at(dev, rng, monkeypatch, varian
                                                        window=window, lse=True)
             check_attention(got, stats, q.double().numpy(), want, table, start, ctx, D ** -0.5, causal, window, x)
             ops.kv_status()
+
+
+@pytest.mark.parametrize("variant,x,D", VARIANTS)
+def test_a_tile_is_not_touched_by_rows_of_another(dev, rng, monkeypatch, variant, x, D):
+    """The places of a sequence's last tile that hold no row do not take part: its rows have the same bits whatever the first
+    row holds (which another workgroup may be writing, with the output in place of q), however large its scores are."""
+    force(monkeypatch, variant, 1)
+    table, start, ctx, n_pages = tables(rng, [(133, 300)], 16)
+    want = random_cache(rng, n_pages, 1, 16, D)
+    cache, t = device_cache(dev, want), on(dev, table, start, ctx)
+    attend = ops.KvAttention(1, 1, D, dev)
+    q = torch.from_numpy(rng.standard_normal((133, 1, D)).astype(np.float32)).to(DT[x]).to(dev)
+    got, stats = attend(q, cache, *t, lse=True)
+    for first in (30.0, 1000.0, 0.0):
+        q[0] = q[0].sign() * first
+        again, again_stats = attend(q, cache, *t, lse=True)
+        assert torch.equal(again[128:], got[128:]) and torch.equal(again_stats[128:], stats[128:]), first
+        here = q.clone()
+        assert torch.equal(attend(here, cache, *t, out=here), again)

@@ -278,7 +278,8 @@ __device__ __forceinline__ void kv_load_rows(const KvAttnArgs &a, const KvTile &
   const int lane = threadIdx.x & 63, g4 = lane >> 4;
   r += lane & 15;
   const bool have = r < t.rows;
-  const int rr = have ? r : 0;  // rows past the last: the first one's values, not stored
+  // (places past the last row: its values, not stored; a row of this tile, which no other workgroup writes where out is q)
+  const int rr = have ? r : t.rows - 1;
   const int i = rr / a.G, hq = h * a.G + rr % a.G;
   q.hi = !have ? 0 : a.causal ? t.p0 + i + 1 : t.ctx;
   q.lo = a.window ? t.p0 + i - a.window + 1 : 0;
