@@ -216,3 +216,16 @@ def test_a_tile_is_not_touched_by_rows_of_another(dev, rng, monkeypatch, variant
         assert torch.equal(again[128:], got[128:]) and torch.equal(again_stats[128:], stats[128:]), first
         here = q.clone()
         assert torch.equal(attend(here, cache, *t, out=here), again)
+
+
+def test_attention_object_is_refused_in_a_capture(dev):
+    a = torch.ones(4, device=dev)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        b = a + 1
+        with pytest.raises(RuntimeError, match="before a capture"):
+            ops.KvAttention(2, 1, 64, dev)
+    for _ in range(2):
+        g.replay()
+    torch.cuda.synchronize()
+    assert (b == 2).all()

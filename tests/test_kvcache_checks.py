@@ -100,3 +100,12 @@ def test_attention_object_checks():
     for args in ((4, 3, 64), (0, 1, 64), (4, 2, 100)):
         with pytest.raises(ValueError):
             ops.KvAttention(*args, device="cpu")
+
+
+def test_attention_object_is_not_made_in_a_capture(monkeypatch):
+    """Its workspace would be cleared by replays only, and an eager call before the first one would count on what was there."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before a capture"):
+        ops.KvAttention(4, 2, 64, device="cuda")
+    with pytest.raises(RuntimeError, match="before a capture"):
+        ops.KvAttention(4, 2, 64, device=torch.device("cuda", 0))

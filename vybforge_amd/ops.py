@@ -707,16 +707,18 @@ def kv_append(cache, k, v, page_table, q_start, ctx, q=None, cos=None, sin=None,
 
 class KvAttention:
     """Attention over a KvCache (vybdq_kv_attn), with its workspace. Calls of one object must not overlap (one stream, or
-    streams that wait for each other; so for the replays of graphs that captured them)."""
+    streams that wait for each other; so for the replays of graphs that captured them). Made outside of captures."""
 
     def __init__(self, n_heads, n_kv_heads, head_dim, device="cuda"):
         _need(head_dim in KV_HEAD_DIMS, f"head_dim must be one of {KV_HEAD_DIMS}")
         _need(n_kv_heads >= 1 and n_heads >= 1 and n_heads % n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads")
+        if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("KvAttention must be made before a capture (only replays would clear its workspace)")
         self.Hq, self.Hkv, self.D, self.scale = n_heads, n_kv_heads, head_dim, head_dim ** -0.5
         self.ws_bytes = _lib.lib.vybdq_kv_attn_workspace_size(head_dim)
         # zero-filled once: the arrival counters at its start must be zero (each call leaves them so)
         self.ws = torch.zeros(self.ws_bytes + 256, dtype=torch.uint8, device=device)
-        if self.ws.is_cuda and not torch.cuda.is_current_stream_capturing():
+        if self.ws.is_cuda:
             torch.cuda.current_stream(self.ws.device).synchronize()  # the first call may be on another stream
         self.ws_ptr, self.index = (self.ws.data_ptr() + 255) // 256 * 256, self.ws.get_device()
 
