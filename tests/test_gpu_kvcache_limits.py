@@ -8,7 +8,7 @@ import torch
 from oracle import kvcache
 from vybforge_amd import ops
 
-from test_gpu_kvcache import DT, check_attention, device_cache, on, random_cache, tables, tolerance
+from test_gpu_kvcache import DT, check_attention, device_cache, on, random_cache, same_cache, tables, tolerance
 
 pytestmark = pytest.mark.gpu
 
@@ -229,3 +229,24 @@ def test_attention_object_is_refused_in_a_capture(dev):
         g.replay()
     torch.cuda.synchronize()
     assert (b == 2).all()
+
+
+def test_append_at_a_position_past_two_to_the_thirty(dev, rng):
+    """The last angles of tables of 2^30 + 16 rows (32 GiB each, of which one row is written and read)."""
+    D, page, R, pos = 64, 256, 16, 2 ** 30 + 7
+    cos, sin = (torch.empty(2 ** 30 + 16, R // 2, device=dev) for _ in range(2))
+    angle = torch.from_numpy(rng.uniform(0, 6, R // 2).astype(np.float32))
+    cos[pos], sin[pos] = angle.cos().to(dev), angle.sin().to(dev)
+    want = random_cache(rng, 2, 1, page, D)
+    cache = device_cache(dev, want)
+    table = torch.ones(1, pos // page + 1, dtype=torch.int32, device=dev)
+    k, v = (rng.standard_normal((1, 1, D)).astype(np.float32) for _ in range(2))
+    got = ops.kv_append(cache, *on(dev, k, v), table, *on(dev, np.array([0, 1], np.int32), np.array([pos + 1], np.int32)),
+                        q=on(dev, k)[0], cos=cos, sin=sin)
+    ops.kv_status()
+    turned = kvcache.rotate(k[0], 0, angle.cos().numpy()[None], angle.sin().numpy()[None], False)
+    np.testing.assert_array_equal(got[0].cpu().numpy(), turned)
+    want.append(turned[None], v, np.array([1]), pos % page + 1)
+    same_cache(cache, want)
+    del cos, sin
+    torch.cuda.empty_cache()

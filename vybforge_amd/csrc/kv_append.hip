@@ -505,7 +505,7 @@ extern "C" int vybdq_kv_append(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs,
   a.ldq = ldq;
   a.G = q ? static_cast<int32_t>(Hq / Hkv) : 0;
   a.R = static_cast<int32_t>(R);
-  a.n_pos = static_cast<int32_t>(n_pos < (int64_t(1) << 30) ? n_pos : (int64_t(1) << 30));
+  a.n_pos = static_cast<int32_t>(n_pos < INT32_MAX ? n_pos : INT32_MAX);
   a.inter = interleaved != 0;
   a.per_seq = max_new == 1;
   const int64_t units = a.per_seq ? B : (T >> ps) + 2 * B;
