@@ -250,3 +250,102 @@ def test_append_at_a_position_past_two_to_the_thirty(dev, rng):
     same_cache(cache, want)
     del cos, sin
     torch.cuda.empty_cache()
+
+
+# ---- batches and splits that other tests do not reach ------------------------------------------------
+
+@pytest.mark.parametrize("splits", [1, 2, 7])
+@pytest.mark.parametrize("variant,x,D", VARIANTS)
+def test_every_kernel_by_name(dev, rng, monkeypatch, variant, x, D, splits):
+    """Each kernel where it exists (128 rows a workgroup: fp16 and bf16 queries, D = 128), past a batch of 64 steps."""
+    force(monkeypatch, variant, splits)
+    lens = [(1, 2300), (140, 333), (0, 50), (33, 33), (5, 90)]
+    for Hq, Hkv, page, window, causal in ((3, 1, 16, 0, True), (4, 2, 64, 77, False)):
+        table, start, ctx, n_pages = tables(rng, lens, page)
+        want = random_cache(rng, n_pages, Hkv, page, D)
+        q = torch.from_numpy(rng.standard_normal((int(start[-1]), Hq, D)).astype(np.float32)).to(DT[x])
+        got, stats = ops.KvAttention(Hq, Hkv, D, dev)(q.to(dev), device_cache(dev, want), *on(dev, table, start, ctx), window=window,
+                                                      causal=causal, lse=True)
+        check_attention(got, stats, q.double().numpy(), want, table, start, ctx, D ** -0.5, causal, window, x)
+    ops.kv_status()
+
+
+def test_chosen_splits_by_length(dev, rng):
+    """A call long enough that the plan itself gives longer sequences more splits: eager, and captured and replayed at other
+    lengths; every replay equals the eager result, which is checked once."""
+    D, page, n, Hq, Hkv = 256, 16, 5, 24, 4
+    lens = [(n, int(c)) for c in np.linspace(6000, 300, 12)]
+    table, start, ctx, n_pages = tables(rng, lens, page)
+    want = random_cache(rng, n_pages, Hkv, page, D)
+    cache, t = device_cache(dev, want), on(dev, table, start, ctx)
+    attend, args = ops.KvAttention(Hq, Hkv, D, dev), dict(max_new=n, max_ctx=6000, lse=True)
+    q = torch.from_numpy(rng.standard_normal((12 * n, Hq, D)).astype(np.float32))
+    qd = q.to(dev)
+    first, first_stats = (a.clone() for a in attend(qd, cache, *t, **args))
+    for h in (0, 11, 23):  # (all heads would take the oracle a while)
+        k_of, part = h // (Hq // Hkv), kvcache.Cache(want.k[:, [h // 6]], want.v[:, [h // 6]], want.k_scale[:, [h // 6]], want.v_scale[:, [h // 6]])
+        check_attention(first[:, h:h + 1], first_stats[:, h:h + 1], q[:, h:h + 1].double().numpy(), part, table, start, ctx, D ** -0.5,
+                        True, 0, "f32")
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        out, stats = attend(qd, cache, *t, **args)
+    for i in range(5):
+        t[2].copy_(torch.from_numpy(np.roll(ctx, i) - 13 * i))
+        t[0].copy_(torch.from_numpy(np.roll(table, i, 0)))
+        g.replay()
+        eager, eager_stats = attend(qd, cache, *t, **args)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager) and torch.equal(stats, eager_stats), i
+        if i == 0:
+            assert torch.equal(out, first) and torch.equal(stats, first_stats)
+    ops.kv_status()
+
+
+@pytest.mark.parametrize("B,Hkv,max_new", [(5000, 1, 1), (700, 8, 1), (700, 8, None), (70000, 1, None)])
+def test_thousands_of_sequences(dev, rng, B, Hkv, max_new):
+    """First tokens of more sequences than a wave has lanes twice over, and of more (sequence, head) pairs than the workspace
+    counts arrivals for: attention returns what append stored, with the score as lse."""
+    D, G = 64, 2
+    q, k, v = (torch.randn(B, h, D, device=dev) for h in (G * Hkv, Hkv, Hkv))
+    cache = ops.KvCache.empty(B, Hkv, D, 16, dev)
+    cache.k.view(torch.uint8).fill_(0x7f)
+    cache.v.view(torch.uint8).fill_(0x7f)
+    table = torch.randperm(B, device=dev).to(torch.int32)[:, None].contiguous()
+    start, ctx = torch.arange(B + 1, dtype=torch.int32, device=dev), torch.ones(B, dtype=torch.int32, device=dev)
+    ops.kv_append(cache, k, v, table, start, ctx, max_new=max_new)
+    out, lse = ops.KvAttention(G * Hkv, Hkv, D, dev)(q, cache, table, start, ctx, lse=True, max_new=max_new, max_ctx=4000)
+    at = table[:, 0].long()
+    kept = cache.k.view(torch.uint8)[at, :, 0].view(torch.float8_e4m3fn).double() * cache.k_scale[at, :, None].double()
+    vals = cache.v.view(torch.uint8)[at, :, 0, :, 0].contiguous().view(torch.float8_e4m3fn).double() * cache.v_scale[at, :, None].double()
+    assert ((kept - k.double()).abs() <= 2.0 ** -4 * k.double().abs() + cache.k_scale[at, :, None] * 2.0 ** -10).all()
+    assert ((vals - v.double()).abs() <= 2.0 ** -4 * v.double().abs() + cache.v_scale[at, :, None] * 2.0 ** -10).all()
+    each = lambda t: t.repeat_interleave(G, 1)
+    score, reach = ((f(q.double()) * f(each(kept))).sum(-1) * D ** -0.5 for f in (lambda t: t, torch.abs))
+    assert ((out.double() - each(vals)).abs() <= (2.0 ** -21 + 2.0 ** -22) * each(vals).abs()).all()
+    assert ((lse.double() - score).abs() <= reach * (D + 8) * 2.0 ** -24 + reach * 2.0 ** -21 + 64 * 2.0 ** -24 + 2.0 ** -21).all()
+    ops.kv_status()
+
+
+@pytest.mark.parametrize("variant,x,D", [v for v in VARIANTS if v[0] >= 2])
+def test_chunks_of_many_sequences(dev, rng, monkeypatch, variant, x, D):
+    """More sequences than a wave has lanes, of many rows each, some of none."""
+    force(monkeypatch, variant, 2)
+    lens = [(int(n), int(n + c)) for n, c in zip(rng.integers(0, 40, 150), rng.integers(0, 60, 150))]
+    table, start, ctx, n_pages = tables(rng, lens, 16)
+    want = random_cache(rng, n_pages, 1, 16, D)
+    q = torch.from_numpy(rng.standard_normal((int(start[-1]), 1, D)).astype(np.float32)).to(DT[x])
+    got, stats = ops.KvAttention(1, 1, D, dev)(q.to(dev), device_cache(dev, want), *on(dev, table, start, ctx), lse=True)
+    check_attention(got, stats, q.double().numpy(), want, table, start, ctx, D ** -0.5, True, 0, x)
+    ops.kv_status()
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(1024, 1024), (2048, 1), (999, 3)])
+def test_many_heads(dev, rng, Hq, Hkv):
+    D, page, lens = 64, 16, [(1, 40), (2, 3)]
+    table, start, ctx, n_pages = tables(rng, lens, page)
+    want = random_cache(rng, n_pages, Hkv, page, D)
+    q = torch.from_numpy(rng.standard_normal((3, Hq, D)).astype(np.float32)).to(torch.bfloat16)
+    got, stats = ops.KvAttention(Hq, Hkv, D, dev)(q.to(dev), device_cache(dev, want), *on(dev, table, start, ctx), lse=True)
+    check_attention(got, stats, q.double().numpy(), want, table, start, ctx, D ** -0.5, True, 0, "bf16")
+    ops.kv_status()
