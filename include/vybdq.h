@@ -585,8 +585,9 @@ int64_t vybdq_kv_attn_workspace_size(int64_t D);
    (times log2 e; past that they give NaN or nothing). In a row with scores past 2900000 (2^22 ln 2) either way, and in up
    to 31 rows beside it, V scales may lie 2^22 apart (2^15 for float32 q) before weights lose bits.
    ws: 256-byte aligned, of vybdq_kv_attn_workspace_size(D) bytes, zero-filled once before the first call (arrival
-   counters that every completed call leaves at zero); a smaller one splits less, 0 not at all. Calls that share a
-   workspace must not overlap. out may be q (ldq = Hq D). One launch, or a second to join the results where more than 16
+   counters that every completed call leaves at zero); a smaller one splits less, 0 not at all. A split sums at most 2^24
+   keys (max_ctx, W * page and window bound them): a call that would need more is refused. Calls that share a workspace
+   must not overlap. out may be q (ldq = Hq D). One launch, or a second to join the results where more than 16
    rows of a head's sequence split their keys. (T Hq / (64 Hkv) + B) Hkv must be below 2^24. */
 int vybdq_kv_attn(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs, int64_t n_pages, int64_t Hkv, int64_t D, int64_t page,
                   uint64_t q, int x_dt, int64_t ldq, int64_t Hq, uint64_t out, uint64_t lse, uint64_t table, int64_t W,

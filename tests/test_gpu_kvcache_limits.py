@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import kvcache
-from vybforge_amd import ops
+from vybforge_amd import _lib, ops
 
 from test_gpu_kvcache import DT, check_attention, device_cache, on, random_cache, same_cache, tables, tolerance
 
@@ -300,6 +300,41 @@ def test_chosen_splits_by_length(dev, rng):
         if i == 0:
             assert torch.equal(out, first) and torch.equal(stats, first_stats)
     ops.kv_status()
+
+
+@pytest.mark.parametrize("variant,n", [(0, 1), (1, 1), (2, 33)])
+@pytest.mark.parametrize("splits", [None, 40, 256])
+def test_every_key_of_half_a_billion_counts_once(dev, monkeypatch, variant, n, splits):
+    """2^29 + 100 keys of equal scores and values of one: all weights are the same power of two, so that a lane's sums (at most
+    2^24 keys, four to an addition) are exact whole numbers of it, and the joined ones are rounded 300 times at most: a split
+    of 256 that is lost, doubled or short of one key in 2^10 of its own would show."""
+    D, page, ctx = 64, 256, 2 ** 29 + 100
+    monkeypatch.setenv("VYBDQ_KV_VARIANT", str(variant))
+    if splits:
+        monkeypatch.setenv("VYBDQ_KV_SPLITS", str(splits))
+    attend, cache, batch = half_a_billion(dev, n, D, page, ctx)
+    got, stats = attend(torch.zeros(n, 1, D, device=dev), cache, *batch, causal=False, lse=True, max_new=n, max_ctx=ctx)
+    assert np.abs(stats.double().cpu().numpy() - np.log(ctx)).max() < 300 * 2.0 ** -23 / 16
+    assert np.abs(got.double().cpu().numpy() - 1).max() < 300 * 2.0 ** -23
+    ops.kv_status()
+
+
+def half_a_billion(dev, n, D, page, ctx):
+    codes = lambda *s: torch.full(s, 0x38, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)  # (ones)
+    cache = ops.KvCache(codes(1, 1, page, D), codes(1, 1, page // 4, D, 4), *(torch.ones(1, 1, device=dev) for _ in range(2)))
+    table = torch.zeros(1, -(-ctx // page), dtype=torch.int32, device=dev)
+    return ops.KvAttention(1, 1, D, dev), cache, (table, *on(dev, np.array([0, n], np.int32), np.array([ctx], np.int32)))
+
+
+@pytest.mark.parametrize("variant", [0, 1, 2])
+@pytest.mark.parametrize("splits", [1, 5, 32])
+def test_more_keys_to_a_split_than_float32_sums_are_refused(dev, monkeypatch, variant, splits):
+    force(monkeypatch, variant, splits)
+    attend, cache, batch = half_a_billion(dev, 1, 64, 256, 2 ** 29 + 100)
+    with pytest.raises(_lib.VybdqError, match="2\\^24"):
+        attend(torch.zeros(1, 1, 64, device=dev), cache, *batch, causal=False, max_new=1)
+    got, stats = attend(torch.zeros(1, 1, 64, device=dev), cache, *batch, max_new=1, window=1000, lse=True)
+    assert (got == 1).all() and abs(stats.item() - np.log(1000)) < 2.0 ** -20
 
 
 @pytest.mark.parametrize("B,Hkv,max_new", [(5000, 1, 1), (700, 8, 1), (700, 8, None), (70000, 1, None)])

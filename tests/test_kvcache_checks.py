@@ -47,6 +47,14 @@ def test_attention_refuses(change, code, text):
     assert re.search(text, _lib.last_error())
 
 
+@pytest.mark.parametrize("change", [dict(), dict(ws=0, ws_bytes=0, max_ctx=2 ** 24 + 1), dict(window=2 ** 25), dict(x_dt=1, T=100),
+                                    dict(Hq=64, Hkv=2, ldq=4096)])
+def test_attention_refuses_more_keys_than_a_split_can_sum(change):
+    """No workspace to split 2^29 keys, or a bound on them, in."""
+    assert _lib.lib.vybdq_kv_attn(*(ATTN | dict(W=2 ** 25) | change).values()) == _lib.ERR_SHAPE
+    assert "2^24" in _lib.last_error()
+
+
 def test_nothing_to_do_is_no_launch():
     assert _lib.lib.vybdq_kv_append(*(APPEND | dict(T=0)).values()) == _lib.OK
     assert _lib.lib.vybdq_kv_append(*(APPEND | dict(B=0)).values()) == _lib.OK

@@ -421,16 +421,20 @@ __device__ __forceinline__ void kv_weights(const f4 (&s)[NCT][2], const KvRows<C
 #pragma unroll
   for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < 2; ++n) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_exp2f(t[ct][4 * n + e]);
+      // not of the rounded weights: lse is a float32 result
+      l[ct] = __builtin_fmaf((w[0] + w[1]) + (w[2] + w[3]), iv[n], l[ct]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float w = __builtin_amdgcn_exp2f(t[ct][4 * n + e]);
-        l[ct] = __builtin_fmaf(w, iv[n], l[ct]);  // not of the rounded weight: lse is a float32 result
-        w *= kv_lift(TWO);
-        const _Float16 f = static_cast<_Float16>(w);
+        const float x = w[e] * kv_lift(TWO);
+        const _Float16 f = static_cast<_Float16>(x);
         p[ct][0][4 * n + e] = f;
-        if constexpr (TWO) p[ct][1][4 * n + e] = static_cast<_Float16>(w - static_cast<float>(f));
+        if constexpr (TWO) p[ct][1][4 * n + e] = static_cast<_Float16>(x - static_cast<float>(f));
       }
+    }
 }
 
 // A wave's sums as every other's: m alone their reference. It stays the row's p where that is far, so that equal products are

@@ -13,6 +13,10 @@ void kv_attn_launch_f(int D, int variant, const KvAttnArgs &a, dim3 grid, hipStr
 
 constexpr int64_t kKvPartRows = 131072;  // rows of split results that a workspace holds
 constexpr int64_t kKvArrivalBytes = 16384;
+// Keys to a split at most. A lane adds a split's weights four at a time, a matrix instruction's sum those of 32: 2^20 and 2^19
+// float32 additions here. Of equal weights each is rounded alike, by up to 2^-24 of the sum so far: 2^-5 of one of them at the
+// end. (From 2^24 additions on nothing is added any more: 2^29 keys in one split gave half their sum.)
+constexpr int64_t kKvSplitKeys = int64_t(1) << 24;
 
 struct KvShape {
   int64_t D, Hkv, G, T, B, new_rows, tokens;  // new_rows, tokens: most rows and most keys of a sequence
@@ -75,7 +79,8 @@ static KvPlan kv_plan_variant(const KvShape &s, int variant) {
     const double one = (mine + 6) * alone, all = (mine * seen + 6) * share * ((wgs * n + cus - 1) / cus);
     return sqrt(sqrt(one * one * one * one + all * all * all * all)) + (n > 1 ? 4 + 1.2e-6 * wgs * n * R * (s.D + 2) : 0);
   };
-  KvPlan p{variant, units, 1, 0, false};
+  const int64_t least = (keys + kKvSplitKeys - 1) / kKvSplitKeys;
+  KvPlan p{variant, units, least < held ? least : held, 0, false};
   if (const char *e = tuning_env("VYBDQ_KV_SPLITS")) {
     const int64_t n = atoi(e) < 0 ? -atoi(e) : atoi(e);
     p.splits = n < 1 ? 1 : n < held ? n : held;
@@ -83,8 +88,8 @@ static KvPlan kv_plan_variant(const KvShape &s, int variant) {
     p.by_length = atoi(e) < 0 && variant < 2 && s.B > 1 && s.B <= 64 && p.splits > 1;
     return p;
   }
-  p.time = time_of(1);
-  for (int64_t n = 2; n <= held && 4 * n <= steps; n += 1 + n / 16) {  // (some 60 numbers at most: this is host time)
+  p.time = time_of(p.splits);
+  for (int64_t n = p.splits + 1; n <= held && 4 * n <= steps; n += 1 + n / 16) {  // (some 60 numbers at most: this is host time)
     const double time = time_of(n);
     if (time < p.time) {
       p.time = time;
@@ -167,7 +172,9 @@ extern "C" int vybdq_kv_attn(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs, i
   const int64_t most = max_new >= 1 && max_new < T ? max_new : T;
   const KvShape shape{D, Hkv, G, T, B, most, tokens, two, causal != 0, window,
                       ws && ws_bytes > kKvArrivalBytes ? (ws_bytes - kKvArrivalBytes) / ((D + 2) * 4) : 0};
-  KvPlan plan = kv_plan(shape);
+  const KvPlan plan = kv_plan(shape);
+  VYBDQ_REQUIRE(kv_keys(shape, kv_variant_rows(plan.variant)) <= plan.splits * kKvSplitKeys, VYBDQ_ERR_SHAPE,
+                "more than 2^24 keys of a row to a split (of max_ctx, or of W * page): the workspace is too small to split them");
   KvAttnArgs a{};
   const int rc = kv_status_address(a.b.status);
   if (rc) return rc;
