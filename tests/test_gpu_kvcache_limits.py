@@ -1,6 +1,9 @@
 """Attention over the 8-bit cache at the ends of its ranges: scores past the whole numbers that float32 tells apart, and
 below every reference; sliding windows behind which pages are gone; batches larger than one lane or one counter each."""
 
+import concurrent.futures
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -383,4 +386,27 @@ def test_many_heads(dev, rng, Hq, Hkv):
     q = torch.from_numpy(rng.standard_normal((3, Hq, D)).astype(np.float32)).to(torch.bfloat16)
     got, stats = ops.KvAttention(Hq, Hkv, D, dev)(q.to(dev), device_cache(dev, want), *on(dev, table, start, ctx), lse=True)
     check_attention(got, stats, q.double().numpy(), want, table, start, ctx, D ** -0.5, True, 0, "bf16")
+    ops.kv_status()
+
+
+def test_an_error_is_reported_once_whoever_asks(dev):
+    """Four threads ask at once after a bad batch: one of them is told."""
+    cache = ops.KvCache.empty(2, 1, 64, 16, dev)
+    k = torch.zeros(1, 1, 64, device=dev)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)
+    table, start, ctx, together = i32(7)[None], i32(0, 1), i32(1), threading.Barrier(4)
+
+    def ask(_):
+        together.wait()
+        try:
+            ops.kv_status()
+        except _lib.VybdqError as e:
+            return str(e)
+
+    with concurrent.futures.ThreadPoolExecutor(4) as pool:
+        for i in range(40):
+            ops.kv_append(cache, k, k, table, start, ctx)
+            torch.cuda.synchronize()
+            told = [e for e in pool.map(ask, range(4)) if e]
+            assert len(told) == 1 and "page of the table" in told[0], (i, told)
     ops.kv_status()

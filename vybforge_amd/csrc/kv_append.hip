@@ -54,6 +54,9 @@ int kv_status_address(uint32_t *&ptr) {
   return VYBDQ_OK;
 }
 
+// What was reported so far, taken and cleared in one step: a call that another thread has launched meanwhile may report more.
+__global__ void k_kv_status_take(uint32_t *status) { status[1] = __hip_atomic_exchange(status, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
 struct KvAppendArgs {
   KvCacheArgs c;
   KvBatchArgs b;
@@ -528,10 +531,11 @@ extern "C" int vybdq_kv_status(void) {
   if (rc) return rc;
   uint32_t v = 0;
   hipError_t e = hipDeviceSynchronize();
-  if (e == hipSuccess) e = hipMemcpy(&v, st, 4, hipMemcpyDeviceToHost);
-  if (e == hipSuccess && v) {
-    const uint32_t zero = 0;
-    e = hipMemcpy(st, &zero, 4, hipMemcpyHostToDevice);
+  if (e == hipSuccess) {
+    std::lock_guard<std::mutex> lock(g_kv_mu);  // (the word that k_kv_status_take leaves is this call's until it is read)
+    hipLaunchKernelGGL(k_kv_status_take, dim3(1), dim3(1), 0, nullptr, st);
+    e = hipGetLastError();
+    if (e == hipSuccess) e = hipMemcpy(&v, st + 1, 4, hipMemcpyDeviceToHost);
   }
   if (e != hipSuccess) return set_error(VYBDQ_ERR_HIP, std::string("vybdq_kv_status: ") + hipGetErrorString(e));
   if (v & kKvBadRows) return set_error(VYBDQ_ERR_SHAPE, "q_start was not a rising sequence within the rows");
