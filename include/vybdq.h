@@ -549,7 +549,8 @@ int vybdq_quant_q8_act(uint64_t X, uint64_t Xq, uint64_t Xs, int64_t M, int64_t 
    The batch, read on the device (calls can be captured; the tables may change between replays, not during a call):
    sequence b < B has rows q_start[b] .. q_start[b + 1] - 1 (int32 [B + 1], rising, within 0 .. T) of k, v and q; they are
    the last of its ctx[b] tokens (int32 [B]); table int32 [B][W] names the page of its tokens i page .. i page + page - 1.
-   The pages that a call appends to must differ between sequences; pages that are only read may be shared.
+   The pages that a call appends to must all be different ones, within a sequence and between sequences; pages that are only
+   read may be shared.
    max_new and max_ctx are the caller's bounds on a sequence's rows and tokens (0: unknown). They choose the launch
    shape; results are right for any value, but for vybdq_kv_attn's last bits (the split of the keys, which the lengths of the
    whole batch take part in).
@@ -561,7 +562,7 @@ int vybdq_quant_q8_act(uint64_t X, uint64_t Xq, uint64_t Xs, int64_t M, int64_t 
    consecutive: slices of one q|k|v projection's output). Rotation of the first R dims (R % 16 == 0, 0: none) by
    cos, sin float32 [n_pos][R / 2], row = the token's position: pairs (i, i + R / 2), or (2 i, 2 i + 1) with
    interleaved; float32, each product and sum rounded once. A page's scale is 2^e with the least e that holds its
-   values (|y| <= 448 * 2^e, e in [-60, 60]); code = y / scale to nearest, ties to even. Rows that begin inside a page keep
+   values (|y| <= 448 * 2^e, e in [-60, 60]; larger ones are held to 448 * 2^60); code = y / scale to nearest, ties to even. Rows that begin inside a page keep
    its earlier tokens: e then does not shrink, and where it grows their codes are rounded anew to the larger scale.
    Slots behind the last row stay as they are. A token with an infinity or NaN in a head's rotated k or its v is stored
    so that exactly the attention rows that see it are NaN. K, V, cos, sin, q_out and every row 16-byte aligned; q_out may be
@@ -571,7 +572,8 @@ int vybdq_kv_append(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs, int64_t n_
                     int64_t Hq, uint64_t cos, uint64_t sin, int64_t R, int64_t n_pos, int interleaved, uint64_t table,
                     int64_t W, uint64_t q_start, uint64_t ctx, int64_t T, int64_t B, int64_t max_new, uint64_t stream);
 
-/* Workspace bytes that vybdq_kv_attn splits keys in, for any batch at this D; -1 for an unsupported D. */
+/* Workspace bytes that vybdq_kv_attn splits keys in, for any batch at this D (131072 rows of D + 2 floats: 34.6 MB at D = 64,
+   68.2 at 128, 101.7 at 192, 135.3 at 256); -1 for an unsupported D. */
 int64_t vybdq_kv_attn_workspace_size(int64_t D);
 
 /* out [T][Hq][D] = softmax over the keys j that row i of its sequence sees of (scale q_i . k_j), times v_j; query head h

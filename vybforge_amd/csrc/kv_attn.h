@@ -12,8 +12,8 @@
 // O^T = V^T P^T wants P^T, the order of the 32 keys within an instruction being free. K and V codes go from the
 // cache straight into operand registers (16-byte loads, one e4m3 -> fp16 conversion per two codes; every e4m3
 // value is an fp16 value). Rounded to fp16: the query row, scaled by the power of two that brings its largest
-// value into [2^14, 2^15) (exact for fp16 and bf16 values within 2^-38 of the largest), and w (11 bits down to
-// 2^-22 of the row's largest). For float32 queries both are split into two fp16 terms (22 bits).
+// value into [2^14, 2^15) (exact for fp16 values, and for bf16 ones down to 2^-31 of the largest; below that off by 2^-39 of it
+// at most), and w (11 bits down to 2^-22 of the row's largest). For float32 queries both are split into two fp16 terms (22 bits).
 //
 // A wave owns 16 NCT query rows (row = token * G + head of the group; the G query heads of a key head read the
 // same keys, so they share its tiles) and takes 32 keys at a step. Few rows: k_kv_attn_keys, whose waves take turns over the
@@ -22,11 +22,11 @@
 // not depend on the order of arrival.
 //
 // What bounds them, MI355X (a large copy runs at 4.7 TB/s, a large fp16 product at 1089 TFLOP/s): 48 sequences of 2 to 8 k
-// tokens, one row each, 32 / 8 heads of 128: 102 us, 5.1 TB/s of codes; 4 of up to 131072: 132 us, 5.5 TB/s. A prompt of 4096
-// tokens: 170 us, 807 TFLOP/s; 513 tokens behind 32 k: 344 us, 795 TFLOP/s. Of the prompt's time the matrix instructions
+// tokens, one row each, 32 / 8 heads of 128: 101 us, 5.1 TB/s of codes; 4 of up to 131072: 132 us, 5.5 TB/s. A prompt of 4096
+// tokens: 165 us, 831 TFLOP/s; 513 tokens behind 32 k: 331 us, 825 TFLOP/s. Of the prompt's time the matrix instructions
 // (18 cycles each on a SIMD with four waves) are 64 us, the LDS reads that feed them 30 (128 rows) to 60 (64 rows) beside
 // them; when it took 180, it took 141 without loads and conversion and 169 without exponentials. With heads of 64 a step
-// of 16 rows is 130 cycles of matrix instructions and some 310 of vector instructions, two thirds of them the softmax: 457
+// of 16 rows is 130 cycles of matrix instructions and some 310 of vector instructions, two thirds of them the softmax: 464
 // TFLOP/s with a window of 4096. 32x32x16 instructions in the same scheme were no faster (prompt 177 to 188 us, heads of
 // 64 83 to 97 against 87), nor were two tiles of 16 rows of heads of 64 to a wave (93 against 87).
 #pragma once

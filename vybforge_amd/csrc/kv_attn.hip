@@ -108,7 +108,8 @@ static KvPlan kv_plan_variant(const KvShape &s, int variant) {
 // to 32 (drafted tokens): the same, but for few sequences of many keys, whose last workgroups would be long in joining
 // 32 rows; k_kv_attn_rows joins them in a launch of its own (8 rows of 4 heads, 8 key heads of 128, bf16, us of the one and
 // the other: 1 sequence of 300 keys 9.9, 11.9, of 2000 15.3, 12.3, of 12000 25.6, 19.2; 3 of 2000 20.0, 15.5, of 12000 31.8,
-// 34.0; 8 of 2000 20.7, 19.9, of 12000 43.7, 49.9; 20 of 12000 112, 130). More: k_kv_attn_rows, whose waves share the
+// 34.0; 8 of 2000 20.7, 19.9, of 12000 43.7, 49.9; 20 of 12000 112, 130: the rule takes the slower one at 8 of 2000, by 4 %, and
+// stands on these eight for other head sizes and float32 queries too). More: k_kv_attn_rows, whose waves share the
 // conversion (16 sequences of 6000 keys, 64 rows: 78 us against 147). Its tiles of 128 rows need half the cache reads, those
 // of 64 keep more waves and even out better: 128 rows only where D = 128 leaves room for their registers and the figures
 // above give them the lesser time (512 tokens behind 7680: 93 us against 103; a prompt of 2048: 64 against 57).

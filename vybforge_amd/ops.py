@@ -706,8 +706,9 @@ def kv_append(cache, k, v, page_table, q_start, ctx, q=None, cos=None, sin=None,
 
 
 class KvAttention:
-    """Attention over a KvCache (vybdq_kv_attn), with its workspace. Calls of one object must not overlap (one stream, or
-    streams that wait for each other; so for the replays of graphs that captured them). Made outside of captures."""
+    """Attention over a KvCache (vybdq_kv_attn), with its workspace (68 MB of device memory at a head_dim of 128, in proportion
+    for others). Calls of one object must not overlap (one stream, or streams that wait for each other; so for the replays of
+    graphs that captured them). Made outside of captures."""
 
     def __init__(self, n_heads, n_kv_heads, head_dim, device="cuda"):
         _need(head_dim in KV_HEAD_DIMS, f"head_dim must be one of {KV_HEAD_DIMS}")
