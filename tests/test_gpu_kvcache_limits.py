@@ -410,3 +410,25 @@ def test_an_error_is_reported_once_whoever_asks(dev):
             told = [e for e in pool.map(ask, range(4)) if e]
             assert len(told) == 1 and "page of the table" in told[0], (i, told)
     ops.kv_status()
+
+
+@pytest.mark.parametrize("n", [1, 20, 70])
+def test_small_workspaces(dev, rng, n):
+    """None, no room behind the counters, room for a few rows of splits: fewer splits, the same results to their rounding; what
+    lies behind the given bytes stays."""
+    D, page, Hq, Hkv = 64, 64, 4, 2
+    table, start, ctx, n_pages = tables(rng, [(n, 5000), (n, 900)], page)
+    want = random_cache(rng, n_pages, Hkv, page, D)
+    cache, t = device_cache(dev, want), on(dev, table, start, ctx)
+    q = torch.from_numpy(rng.standard_normal((2 * n, Hq, D)).astype(np.float32))
+    attend, counters = ops.KvAttention(Hq, Hkv, D, dev), 16384
+    whole = attend.ws_bytes
+    for room in (-counters, 0, 1000, 200000, 3000000, whole - counters):
+        attend.ws_bytes = counters + room
+        attend.ws.zero_()
+        end = attend.ws_ptr - attend.ws.data_ptr() + attend.ws_bytes
+        attend.ws[end:] = 0x5a
+        got, stats = attend(q.to(dev), cache, *t, max_new=n, max_ctx=5000, lse=True)
+        check_attention(got, stats, q.double().numpy(), want, table, start, ctx, D ** -0.5, True, 0, "f32")
+        assert (attend.ws[end:] == 0x5a).all() and (attend.ws[attend.ws_ptr - attend.ws.data_ptr():][:max(0, min(counters, counters + room))] == 0).all()
+    ops.kv_status()
