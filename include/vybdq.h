@@ -562,8 +562,9 @@ int vybdq_quant_q8_act(uint64_t X, uint64_t Xq, uint64_t Xs, int64_t M, int64_t 
    consecutive: slices of one q|k|v projection's output). Rotation of the first R dims (R % 16 == 0, 0: none) by
    cos, sin float32 [n_pos][R / 2], row = the token's position: pairs (i, i + R / 2), or (2 i, 2 i + 1) with
    interleaved; float32, each product and sum rounded once. A page's scale is 2^e with the least e that holds its
-   values (|y| <= 448 * 2^e, e in [-60, 60]; larger ones are held to 448 * 2^60); code = y / scale to nearest, ties to even. Rows that begin inside a page keep
-   its earlier tokens: e then does not shrink, and where it grows their codes are rounded anew to the larger scale.
+   values (|y| <= 448 * 2^e, e in [-60, 60]; larger ones are held to 448 * 2^60); code = y / scale to nearest, ties to
+   even. Rows that begin inside a page keep its earlier tokens: e then does not shrink, and where it grows their codes are
+   rounded anew to the larger scale.
    Slots behind the last row stay as they are. A token with an infinity or NaN in a head's rotated k or its v is stored
    so that exactly the attention rows that see it are NaN. K, V, cos, sin, q_out and every row 16-byte aligned; q_out may be
    q (ldq = Hq D). (T / page + 2 B) Hkv must be below 2^23. */
@@ -583,9 +584,9 @@ int64_t vybdq_kv_attn_workspace_size(int64_t D);
    log of the sum of exp(scale q . k). q, out: x_dt, q's row stride ldq. Softmax and sums are float32 in one pass;
    operands are fp16 (codes exactly; q scaled by a power of two per row; float32 q and its weights in two fp16 terms).
    V scales within one row's context may lie 2^100 apart: a key whose V scale is 2^d below the largest that counts is lost
-   once its weight is below 2^(d - 126) of the row's largest. Scores may be as large as float32 holds
-   (times log2 e; past that they give NaN or nothing). In a row with scores past 2900000 (2^22 ln 2) either way, and in up
-   to 31 rows beside it, V scales may lie 2^22 apart (2^15 for float32 q) before weights lose bits.
+   once its weight is below 2^(d - 126) of the row's largest. Scores may be as large as float32 holds (times
+   log2 e; past that they give NaN or nothing). In a row with scores past 2900000 (2^22 ln 2) either way, and in up to 31
+   rows beside it, V scales may lie 2^22 apart (2^15 for float32 q) before weights lose bits.
    ws: 256-byte aligned, of vybdq_kv_attn_workspace_size(D) bytes, zero-filled once before the first call (arrival
    counters that every completed call leaves at zero); a smaller one splits less, 0 not at all. A split sums at most 2^24
    keys (max_ctx, W * page and window bound them): a call that would need more is refused. Calls that share a workspace

@@ -55,7 +55,9 @@ int kv_status_address(uint32_t *&ptr) {
 }
 
 // What was reported so far, taken and cleared in one step: a call that another thread has launched meanwhile may report more.
-__global__ void k_kv_status_take(uint32_t *status) { status[1] = __hip_atomic_exchange(status, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__global__ void k_kv_status_take(uint32_t *status) {
+  status[1] = __hip_atomic_exchange(status, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 
 struct KvAppendArgs {
   KvCacheArgs c;
