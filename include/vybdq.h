@@ -601,6 +601,61 @@ int vybdq_kv_attn(uint64_t K, uint64_t V, uint64_t Ks, uint64_t Vs, int64_t n_pa
    positions) in vybdq_kv_append or vybdq_kv_attn since the previous call on this device, and clears it. */
 int vybdq_kv_status(void);
 
+/* ---- 8-bit floating-point weights: quantizer, product, router with groups, MoE layer ---------- */
+
+/* A matrix W [N][K] is e4m3 codes (OCP, no infinities) W uint8 [N][K] with scales Ws float32 [ceil(N / 128)][ceil(K / 128)], one
+   for each block of 128 x 128 (weight = code * scale; the layout of checkpoints in that form). Activations X [M][K] are codes
+   Xq uint8 [M][K] with scales Xs float32 [M][ceil(K / 128)], one for each row and 128 columns. K is a multiple of 16 (the last
+   block may be short), N and M are anything.
+
+   vybdq_quant_fp8: X (x_dt F32, F16 or BF16, row stride ldx in elements) to Xq, Xs. Scale = 2^e with the least e in -100 .. 120
+   for which every |x| of the block is at most 448 * 2^e, code = e4m3(x / scale) to nearest, ties to even (one rounding: the
+   division is exact). A block with an infinity or NaN has the scale NaN. Rows of X and Xq 16-byte aligned;
+   M ceil(K / 128) below 2^28. */
+int vybdq_quant_fp8(uint64_t X, int x_dt, int64_t ldx, uint64_t Xq, uint64_t Xs, int64_t M, int64_t K, uint64_t stream);
+
+/* Y [M][N] (y_dt F32, F16, BF16 or F64; row stride ldy, 0 = N) = RS + sum over blocks b of Xs[m][b] Ws[n / 128][b] times the
+   sum of Xq W over the block's k; RS: as Y (its row stride too) or 0. Scales may be any float32. Products are exact, sums
+   over a block and over blocks are float32; for F16 and BF16 outputs a block's sum comes from the e4m3 matrix
+   instruction, which aligns its 128 products to the largest (1.4e-5 of the sum's rms for normal data, 3e-4 of the largest
+   product at most). W and Xq 16-byte aligned. ceil(M / 128) ceil(N / 128) below 2^22, M and N below 2^24. */
+int vybdq_gemm_fp8(uint64_t W, uint64_t Ws, uint64_t Xq, uint64_t Xs, uint64_t Y, int64_t M, int64_t N, int64_t K, int y_dt,
+                   int64_t ldy, uint64_t RS, uint64_t stream);
+
+/* vybdq_quant_fp8 and vybdq_gemm_fp8 in one call: X x_dt, row stride ldx. ws: 256-byte aligned, of
+   vybdq_linear_fp8_workspace_size(M, N, K) bytes (-1: unsupported), any contents; the size covers every smaller M. Calls that
+   share a workspace must not overlap. */
+int64_t vybdq_linear_fp8_workspace_size(int64_t M, int64_t N, int64_t K);
+int vybdq_linear_fp8(uint64_t W, uint64_t Ws, uint64_t X, int x_dt, int64_t ldx, uint64_t Y, int64_t M, int64_t N, int64_t K,
+                     int y_dt, int64_t ldy, uint64_t RS, uint64_t ws, int64_t ws_bytes, uint64_t stream);
+
+/* Router: score = sigmoid(logit), or softmax over the E logits (softmax = 1); choice = score + bias (bias float32 [E] or 0: it
+   only selects). With groups > 1 (a divisor of E, at most 64) expert e belongs to group e / (E / groups), a group's value is
+   the sum of its group_top (1 or 2) best choices, and only the top_groups best groups take part. idx_out int32 [T][topk]: the
+   best choices, descending; w_out float32 [T][topk] = score, over (their sum + 1e-20) with renorm = 1, times scale. Ties go
+   to the lower id. float64 throughout, rounded once; without a bias choices compare as their logits do. A NaN comes below every number.
+   vybdq_moe_route is the case softmax = 0, renorm = 1, groups = 1. E up to 1024, topk up to 64 and within
+   top_groups * E / groups. */
+int vybdq_moe_route_groups(uint64_t logits, int logits_dt, uint64_t bias, uint64_t idx_out, uint64_t w_out, int64_t T, int64_t E,
+                           int64_t topk, double scale, int softmax, int renorm, int64_t groups, int64_t top_groups,
+                           int64_t group_top, uint64_t stream);
+
+/* Workspace bytes for vybdq_moe_forward_fp8 with T or fewer tokens, or -1 for an unsupported shape. */
+int64_t vybdq_moe_fp8_workspace_size(int64_t T, int64_t H, int64_t I, int64_t E, int64_t topk);
+
+/* out [T][H] (F32, F16 or BF16) = sum over s of w[t, s] FFN_idx[t, s](x[t]) + FFN_shared(x[t]), routed as vybdq_moe_route_groups
+   does, FFN(x) = a Wd with a = silu(min(x Wg, limit)) * clamp(x Wu, -limit, limit) (limit > 0, infinity: none). x and a are
+   quantized as vybdq_quant_fp8 does (a from its float32 values); everything else is float32. Experts: gate, up e4m3
+   [E][I][H], down [E][H][I] with scales [E][I / 128][H / 128] and [E][H / 128][I / 128]; the shared expert (weight 1) one such
+   matrix each, or all six 0. H and I multiples of 128. idx_out, w_out (optional) receive the routing. x, out and codes 16-byte
+   aligned. ws: 256-byte aligned, vybdq_moe_fp8_workspace_size bytes, any contents; calls that share one must not overlap. */
+int vybdq_moe_forward_fp8(uint64_t x, int x_dt, uint64_t logits, int logits_dt, uint64_t bias, uint64_t gate, uint64_t gate_s,
+                          uint64_t up, uint64_t up_s, uint64_t down, uint64_t down_s, uint64_t sh_gate, uint64_t sh_gate_s,
+                          uint64_t sh_up, uint64_t sh_up_s, uint64_t sh_down, uint64_t sh_down_s, uint64_t out, int out_dt,
+                          uint64_t idx_out, uint64_t w_out, int64_t T, int64_t H, int64_t I, int64_t E, int64_t topk,
+                          double scale, double limit, int softmax, int renorm, int64_t groups, int64_t top_groups,
+                          int64_t group_top, uint64_t ws, int64_t ws_bytes, uint64_t stream);
+
 #ifdef __cplusplus
 }
 #endif

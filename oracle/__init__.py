@@ -35,6 +35,8 @@ repository root):
                             native/kernels/layer.vyb:989-1066,1551-1590, vmath.vyb:7-40
   kvcache  the paged 8-bit key/value cache: append with rotation, attention (this library's own
            format, include/vybdq.h; no counterpart in the reference)
+  fp8      e4m3 matrices with block scales: quantizer, product, router with groups, MoE layer (no
+           counterpart in the reference)
 
 Pinning (what checks each function, all under tests/):
   q4_0 decode      the reference's frozen GGUF fixture block (interleaved order) and

@@ -1,0 +1,94 @@
+"""e4m3 matrices with a scale for each block of 128 x 128 in numpy: the quantizer of activations bit for bit, the product, the
+router with groups and the mixture-of-experts layer in float64.
+
+Layout and semantics are those of include/vybdq.h (vybdq_quant_fp8, vybdq_gemm_fp8, vybdq_moe_route_groups,
+vybdq_moe_forward_fp8).
+"""
+
+import numpy as np
+
+from oracle.kvcache import e4m3_decode, e4m3_encode
+
+E_MIN, E_MAX = -100, 120
+
+
+def blocks(n):
+    return -(-n // 128)
+
+
+def quant(x):
+    """codes uint8 [M, K], scales float32 [M, ceil(K / 128)] of x [M, K]."""
+    x = np.asarray(x, np.float64)
+    M, K = x.shape
+    codes, scales = np.zeros((M, K), np.uint8), np.empty((M, blocks(K)), np.float32)
+    for b in range(blocks(K)):
+        part = x[:, 128 * b:128 * (b + 1)]
+        ok = np.isfinite(part).all(1)
+        f, e = np.frexp(np.where(ok, np.abs(np.where(np.isfinite(part), part, 0)).max(1), 0.0))
+        e = np.where(f == 0, E_MIN, np.where(f <= 0.875, e - 9, e - 8)).clip(E_MIN, E_MAX)
+        scales[:, b] = np.where(ok, 2.0 ** e, np.nan)
+        codes[ok, 128 * b:128 * (b + 1)] = e4m3_encode(part[ok] / 2.0 ** e[ok, None])
+    return codes, scales
+
+
+def activations(codes, scales):
+    """float64 values of activations."""
+    return e4m3_decode(codes) * np.repeat(scales.astype(np.float64), 128, 1)[:, :codes.shape[1]]
+
+
+def weights(codes, scales):
+    """float64 values of a matrix."""
+    N, K = codes.shape
+    s = np.repeat(np.repeat(scales.astype(np.float64), 128, 0)[:N], 128, 1)[:, :K]
+    return e4m3_decode(codes) * s
+
+
+def route(logits, topk, bias=None, scale=2.5, softmax=False, renorm=True, groups=1, top_groups=1, group_top=2):
+    """idx int64 [T, topk], w float64 [T, topk]; ties to the lower id, NaN below every number."""
+    l = np.asarray(logits, np.float64)
+    T, E = l.shape
+    idx, w = np.zeros((T, topk), np.int64), np.zeros((T, topk))
+    with np.errstate(all="ignore"):
+        for t in range(T):
+            if softmax:
+                top = np.max(l[t])
+                p = np.exp(l[t] - (0.0 if top == -np.inf else top))
+                score = p / p.sum() if p.sum() != 0 else np.zeros(E)
+            else:
+                score = 1.0 / (1.0 + np.exp(-l[t]))
+            choice = score + np.asarray(bias, np.float64) if bias is not None else score
+            order = choice if bias is not None else l[t]  # both scores rise with the logit
+
+            def ranked(values, ids):  # descending, NaN last, ties to the lower id
+                return sorted(ids, key=lambda i: (1, 0.0, i) if np.isnan(values[i]) else (0, -values[i], i))
+
+            ids = list(range(E))
+            if groups > 1:
+                S, value = E // groups, np.empty(groups)
+                for g in range(groups):
+                    best = ranked(order, range(g * S, (g + 1) * S))[:group_top]
+                    value[g] = order[best[0]] if group_top == 1 else sum(choice[i] for i in best)
+                keep = ranked(value, range(groups))[:top_groups]
+                ids = [i for i in ids if i // S in keep]
+            idx[t] = ranked(order, ids)[:topk]
+            s = score[idx[t]]
+            w[t] = s / (s.sum() + 1e-20) * scale if renorm else s * scale
+    return idx, w
+
+
+def ffn(x, gate, up, down, limit):
+    """x float64 [M, H] (quantized values); (codes, scales) of the three matrices."""
+    g, u = x @ weights(*gate).T, x @ weights(*up).T
+    g, u = np.minimum(g, limit), np.clip(u, -limit, limit)
+    a = g / (1.0 + np.exp(-g)) * u
+    return activations(*quant(a)) @ weights(*down).T
+
+
+def moe(x, idx, w, gate, up, down, shared=None, limit=10.0):
+    """out float64 [T, H] of the layer for the routing idx, w; gate, up, down: (codes, scales) with a leading E."""
+    xq = activations(*quant(x))
+    out = ffn(xq, *shared, limit) if shared else np.zeros_like(xq)
+    for e in np.unique(idx):
+        t, s = np.nonzero(idx == e)
+        out[t] += w[t, s][:, None] * ffn(xq[t], *[(c[e], d[e]) for c, d in (gate, up, down)], limit)
+    return out

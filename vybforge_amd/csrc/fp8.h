@@ -1,0 +1,65 @@
+// 8-bit floating-point matrices: e4m3 codes with a float32 scale for each block of 128 x 128 weights, and for each row
+// and 128 columns of activations. What the quantizer (fp8_quant.hip), the products (fp8_mm.h) and the experts
+// (moe_fp8.hip) share.
+//
+//   weight W[n, k] = code * Ws[n / 128][k / 128]      activation X[m, k] = code * Xs[m][k / 128]
+//   Xs = 2^e with the least e in [-100, 120] for which every |x| of the block is at most 448 * 2^e (448: the largest e4m3);
+//   code = e4m3(x * 2^-e), ties to even: the product with a power of two is exact, so a code is x rounded once. A block that
+//   holds an infinity or NaN has the scale NaN (and zero codes): exactly the rows of the product that it takes part in are NaN.
+#pragma once
+
+#include "common.h"
+
+#include <type_traits>
+
+namespace vybdq {
+
+constexpr int kFp8ExpMin = -100, kFp8ExpMax = 120;
+constexpr float kFp8Max = 448.0f;
+
+typedef int i8v __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ float fp8_exp2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+// The exponent of a block whose largest |x| has the bits `u` (finite): 448 = 1.75 * 2^8.
+__device__ __forceinline__ int fp8_exponent(uint32_t u) {
+  const int x = static_cast<int>(u >> 23) - 127, e = (u & 0x7fffffu) <= 0x600000u ? x - 8 : x - 7;
+  return e < kFp8ExpMin ? kFp8ExpMin : (e > kFp8ExpMax ? kFp8ExpMax : e);
+}
+
+// A block's scale and the factor of its codes from the bits of its largest |x|.
+__device__ __forceinline__ float fp8_scale(uint32_t amax, float &inv) {
+  if (amax >= 0x7f800000u) {
+    inv = 0.f;
+    return __uint_as_float(0x7fc00000u);
+  }
+  const int e = fp8_exponent(amax);
+  inv = fp8_exp2(-e);
+  return fp8_exp2(e);
+}
+
+// Four values times a power of two as e4m3 codes, rounded to nearest even and held to +-448 (zeros where
+// inv = 0: the block holds an infinity or NaN).
+__device__ __forceinline__ uint32_t fp8_codes4(float a, float b, float c, float d, float inv) {
+  auto cl = [&](float x) { return inv == 0.f ? 0.f : __builtin_amdgcn_fmed3f(x * inv, -kFp8Max, kFp8Max); };
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(cl(a), cl(b), 0, false);
+  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(cl(c), cl(d), lo, true));
+}
+
+// Largest 32-bit value over the 16 lanes of a row, in every lane (DPP, on the VALU).
+__device__ __forceinline__ uint32_t row16_max_u32(uint32_t v) {
+  auto step = [&](auto ctrl) {
+    const uint32_t o = static_cast<uint32_t>(
+        __builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(ctrl)::value, 0xf, 0xf, false));
+    v = o > v ? o : v;
+  };
+  step(std::integral_constant<int, DPP_QUAD_XOR1>{});
+  step(std::integral_constant<int, DPP_QUAD_XOR2>{});
+  step(std::integral_constant<int, DPP_HALF_MIRROR>{});
+  step(std::integral_constant<int, DPP_ROW_MIRROR>{});
+  return v;
+}
+
+int fp8_quant_rows(const void *X, int x_dt, int64_t M, int64_t K, int64_t ldx, uint8_t *Xq, float *Xs, hipStream_t s);
+
+}  // namespace vybdq

@@ -1,0 +1,177 @@
+// Mixture-of-experts layer over e4m3 experts with block scales (fp8.h), gfx950.
+//
+//   router (route_groups.h) -> idx, w;  x -> codes and scales per token and 128 columns
+//   expert e: a = silu(min(x Wg_e, L)) * clamp(x Wu_e, -L, L) in float32, then codes and scales per row and 128 columns
+//             e_out = a Wd_e
+//   out[t] = sum over s of w[t, s] e_out[idx[t, s]](t) + shared(x[t]), float32, rounded once to out_dt
+//
+// On the stream, no host synchronisation: quantizer, router, bucketing (rows by expert and the list of their m-tiles; the
+// shared expert's rows and tiles are one more expert's), gate and up of all rows with the activation and its quantizer as
+// epilogue (k_fp8_mm<.., FP8_GATE_UP>: float32 gate and up never leave registers), down (FP8_DOWN), the weighted sum.
+#include "fp8_mm.h"
+#include "route_groups.h"
+
+namespace vybdq {
+
+int moe_bucket(const int *idx, int64_t T, int64_t E, int64_t topk, int BMr, bool shared, int *pos, int *row_map, int4 *tiles,
+               int *ntiles, hipStream_t s);
+int64_t moe_tiles_bound(int64_t T, int64_t E, int64_t k, int64_t rows);
+
+// out[t][h] = sum over s of w[t, s] rows[pos[t, s]][h] + shared[t][h] in slot order; four columns to a thread.
+template <int ODT>
+__global__ void __launch_bounds__(256) k_moe_fp8_sum(const float *__restrict__ rows, const float *__restrict__ shared,
+                                                     const int *__restrict__ pos, const float *__restrict__ w, int64_t T,
+                                                     int topk, int64_t H, void *__restrict__ out) {
+  const int64_t i = 4 * (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x);
+  if (i >= T * H) return;
+  const int64_t t = i / H, h = i - t * H;
+  f4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < topk; ++s) {
+    const f4 v = *reinterpret_cast<const f4 *>(rows + static_cast<int64_t>(pos[t * topk + s]) * H + h);
+    const float ws = w[t * topk + s];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] = fmaf(ws, v[j], acc[j]);
+  }
+  if (shared) acc += *reinterpret_cast<const f4 *>(shared + i);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) store_elem<ODT>(out, nullptr, i + j, acc[j]);
+}
+
+struct MoeFp8Ws {
+  int *idx, *pos, *row_map, *ntiles;
+  int4 *tiles;
+  float *w, *xs, *as, *rows;
+  uint8_t *xq, *aq;
+  int64_t bytes;
+};
+
+static MoeFp8Ws moe_fp8_layout(char *base, int64_t T, int64_t H, int64_t I, int64_t E, int64_t k) {
+  MoeFp8Ws m{};
+  int64_t off = 0;
+  auto take = [&](int64_t n) {
+    char *p = base ? base + off : nullptr;
+    off += (n + 255) / 256 * 256;
+    return p;
+  };
+  const int64_t R = T * k + T;  // rows, the shared expert's among them
+  m.idx = reinterpret_cast<int *>(take(4 * T * k));
+  m.w = reinterpret_cast<float *>(take(4 * T * k));
+  m.pos = reinterpret_cast<int *>(take(4 * T * k));
+  m.row_map = reinterpret_cast<int *>(take(4 * R));
+  m.tiles = reinterpret_cast<int4 *>(take(16 * moe_tiles_bound(T, E, k, 16)));
+  m.ntiles = reinterpret_cast<int *>(take(4));
+  m.xq = reinterpret_cast<uint8_t *>(take(T * H));
+  m.xs = reinterpret_cast<float *>(take(4 * T * (H / 128)));
+  m.aq = reinterpret_cast<uint8_t *>(take(R * I));
+  m.as = reinterpret_cast<float *>(take(4 * R * (I / 128)));
+  m.rows = reinterpret_cast<float *>(take(4 * R * H));
+  m.bytes = off;
+  return m;
+}
+
+static bool moe_fp8_shape(int64_t T, int64_t H, int64_t I, int64_t E, int64_t k) {
+  return T >= 0 && T < (1 << 20) && H >= 128 && H % 128 == 0 && H <= 65536 && I >= 128 && I % 128 == 0 && I <= 65536 && E >= 1 &&
+         E <= 1024 && k >= 1 && k <= E && k <= 64 && T * k < (1 << 22) &&
+         moe_tiles_bound(T, E, k, 16) * ((H > I ? H : I) / 128) < (int64_t(1) << 22);  // (workgroups of a launch)
+}
+
+template <int MODE, bool HALF>
+static int moe_fp8_mm(int BM, Fp8MmArgs &a, int64_t tiles, hipStream_t s) {
+  a.n_tiles = MODE == FP8_GATE_UP ? a.N / 128 : (a.N + 255) / 256;
+  const int64_t units = tiles * a.n_tiles;
+  if (BM == 16) return fp8_mm_launch<1, 2, 1, 8, 4, MODE, HALF>(a, units, s);
+  if (BM == 64) return fp8_mm_launch<4, 4, 1, 4, 3, MODE, HALF>(a, units, s);
+  return fp8_mm_launch<4, 4, 2, 4, 3, MODE, HALF>(a, units, s);
+}
+
+}  // namespace vybdq
+
+using namespace vybdq;
+
+extern "C" int64_t vybdq_moe_fp8_workspace_size(int64_t T, int64_t H, int64_t I, int64_t E, int64_t topk) {
+  return moe_fp8_shape(T, H, I, E, topk) ? moe_fp8_layout(nullptr, T, H, I, E, topk).bytes : -1;
+}
+
+extern "C" int vybdq_moe_forward_fp8(uint64_t x, int x_dt, uint64_t logits, int logits_dt, uint64_t bias, uint64_t gate,
+                                     uint64_t gate_s, uint64_t up, uint64_t up_s, uint64_t down, uint64_t down_s,
+                                     uint64_t sh_gate, uint64_t sh_gate_s, uint64_t sh_up, uint64_t sh_up_s, uint64_t sh_down,
+                                     uint64_t sh_down_s, uint64_t out, int out_dt, uint64_t idx_out, uint64_t w_out, int64_t T,
+                                     int64_t H, int64_t I, int64_t E, int64_t topk, double scale, double limit, int softmax,
+                                     int renorm, int64_t groups, int64_t top_groups, int64_t group_top, uint64_t ws,
+                                     int64_t ws_bytes, uint64_t stream) {
+  VYBDQ_REQUIRE(dt_valid_in(x_dt), VYBDQ_ERR_ARG, "x_dt must be F32, F16 or BF16");
+  VYBDQ_REQUIRE(dt_valid_in(out_dt), VYBDQ_ERR_ARG, "out_dt must be F32, F16 or BF16");
+  VYBDQ_REQUIRE(moe_fp8_shape(T, H, I, E, topk), VYBDQ_ERR_SHAPE,
+                "H and I must be multiples of 128 up to 65536, E up to 1024, topk up to 64, and not too many tokens");
+  const bool shared = sh_gate != 0;
+  VYBDQ_REQUIRE(shared == (sh_gate_s != 0) && shared == (sh_up != 0) && shared == (sh_up_s != 0) && shared == (sh_down != 0) &&
+                    shared == (sh_down_s != 0),
+                VYBDQ_ERR_ARG, "shared expert: give all three matrices with their scales or none");
+  MoeFp8Ws m = moe_fp8_layout(reinterpret_cast<char *>(ws), T, H, I, E, topk);
+  RouteArgs r;
+  int rc = route_groups_args(__func__, r, logits, logits_dt, bias, idx_out ? idx_out : (ws ? reinterpret_cast<uint64_t>(m.idx) : 0),
+                             w_out ? w_out : (ws ? reinterpret_cast<uint64_t>(m.w) : 0), ws || (idx_out && w_out) ? T : 0, E, topk,
+                             scale, softmax, renorm, groups, top_groups, group_top);
+  if (rc || T == 0) return rc;
+  VYBDQ_REQUIRE(x && logits && gate && gate_s && up && up_s && down && down_s && out, VYBDQ_ERR_ARG, "null input or output");
+  VYBDQ_REQUIRE(limit > 0, VYBDQ_ERR_ARG, "limit must be positive");
+  VYBDQ_REQUIRE((x | gate | up | down | sh_gate | sh_up | sh_down | out) % 16 == 0 &&
+                    (gate_s | up_s | down_s | sh_gate_s | sh_up_s | sh_down_s) % 4 == 0,
+                VYBDQ_ERR_ALIGN, "x, out and codes must be 16-byte aligned, scales 4-byte");
+  VYBDQ_REQUIRE(ws && ws % 256 == 0 && ws_bytes >= m.bytes, VYBDQ_ERR_WORKSPACE,
+                "workspace must be 256-byte aligned and of vybdq_moe_fp8_workspace_size bytes");
+  hipStream_t s = as_stream(stream);
+  rc = fp8_quant_rows(reinterpret_cast<const void *>(x), x_dt, T, H, H, m.xq, m.xs, s);
+  if (rc) return rc;
+  rc = route_groups_launch(r, s);
+  if (rc) return rc;
+  const int64_t n = T * topk, hit = E < n ? E : n;
+  const int BM = n <= 8 * hit ? 16 : n <= 64 * hit ? 64 : 128;
+  rc = moe_bucket(r.idx, T, E, topk, BM, shared, m.pos, m.row_map, m.tiles, m.ntiles, s);
+  if (rc) return rc;
+  const int64_t tiles = moe_tiles_bound(T, E, topk, BM);
+  Fp8MmArgs g{};
+  g.X = m.xq;
+  g.Xs = m.xs;
+  g.W = reinterpret_cast<const uint8_t *>(gate);
+  g.Ws = reinterpret_cast<const float *>(gate_s);
+  g.W2 = reinterpret_cast<const uint8_t *>(up);
+  g.W2s = reinterpret_cast<const float *>(up_s);
+  g.Ss = reinterpret_cast<const uint8_t *>(sh_gate);
+  g.Sss = reinterpret_cast<const float *>(sh_gate_s);
+  g.S2 = reinterpret_cast<const uint8_t *>(sh_up);
+  g.S2s = reinterpret_cast<const float *>(sh_up_s);
+  g.N = static_cast<int>(I);
+  g.K = static_cast<int>(H);
+  g.KB = static_cast<int>(H / 128);
+  g.w_stride = I * H;
+  g.ws_stride = (I / 128) * (H / 128);
+  g.tiles = m.tiles;
+  g.ntiles = m.ntiles;
+  g.row_map = m.row_map;
+  g.H = m.aq;
+  g.Hs = m.as;
+  g.limit = static_cast<float>(limit);
+  rc = moe_fp8_mm<FP8_GATE_UP, true>(BM, g, tiles, s);
+  if (rc) return rc;
+  Fp8MmArgs d = g;
+  d.X = m.aq;
+  d.Xs = m.as;
+  d.W = reinterpret_cast<const uint8_t *>(down);
+  d.Ws = reinterpret_cast<const float *>(down_s);
+  d.Ss = reinterpret_cast<const uint8_t *>(sh_down);
+  d.Sss = reinterpret_cast<const float *>(sh_down_s);
+  d.N = static_cast<int>(H);
+  d.K = static_cast<int>(I);
+  d.KB = static_cast<int>(I / 128);
+  d.row_map = nullptr;
+  d.Y = m.rows;
+  d.ldy = H;
+  rc = out_dt == VYBDQ_F32 ? moe_fp8_mm<FP8_DOWN, true>(BM, d, tiles, s) : moe_fp8_mm<FP8_DOWN, false>(BM, d, tiles, s);
+  if (rc) return rc;
+  const float *sh = shared ? m.rows + n * H : nullptr;
+  const unsigned grid = static_cast<unsigned>((T * H / 4 + 255) / 256);
+  VYBDQ_DISPATCH_IN(out_dt, ODT, hipLaunchKernelGGL((k_moe_fp8_sum<ODT>), dim3(grid), dim3(256), 0, s, m.rows, sh, m.pos, r.w, T,
+                                                    static_cast<int>(topk), H, reinterpret_cast<void *>(out)));
+  return check_launch("moe sum");
+}

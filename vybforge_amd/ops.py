@@ -448,11 +448,24 @@ def router_logits(X, W, y_dtype=torch.float64):
     return Y
 
 
-def moe_route(logits, topk, bias=None, scale=2.5):
+SCORES = ("sigmoid", "softmax")
+
+
+def moe_route(logits, topk, bias=None, scale=2.5, score="sigmoid", renorm=True, groups=1, top_groups=1, group_top=2):
+    """idx int32 [T, topk], w float32 [T, topk]: the best choices (score + bias) of every token and their scores.
+
+    score: "sigmoid" or "softmax" of the logits [T, E]; renorm: weights over their sum; groups: only the experts of the
+    top_groups groups with the best sum of group_top (1 or 2) choices (vybdq_moe_route_groups; the default arguments are
+    vybdq_moe_route)."""
     T, E = logits.shape
     _need(bias is None or (bias.numel() == E and bias.dtype == torch.float32), "bias must be float32 [E]")
+    _need(score in SCORES, f"score must be one of {SCORES}")
     idx = torch.empty((T, topk), dtype=torch.int32, device=logits.device)
     w = torch.empty((T, topk), dtype=torch.float32, device=logits.device)
+    if groups != 1 or top_groups != 1 or score != "sigmoid" or not renorm:
+        call("vybdq_moe_route_groups", _ptr(logits), _dt(logits.dtype), _ptr(bias), _ptr(idx), _ptr(w), T, E, topk,
+             float(scale), score == "softmax", renorm, groups, top_groups, group_top, _stream())
+        return idx, w
     call("vybdq_moe_route", _ptr(logits), _dt(logits.dtype), _ptr(bias), _ptr(idx), _ptr(w), T, E, topk,
          float(scale), _stream())
     return idx, w
@@ -756,3 +769,186 @@ def kv_status():
     """Synchronise, and raise if a batch's tables were wrong in kv_append or KvAttention since the last call
     (vybdq_kv_status)."""
     call("vybdq_kv_status")
+
+
+# ---- 8-bit floating-point weights ----------------------------------------------------------------
+
+E4M3 = torch.float8_e4m3fn
+
+
+def _blocks(n):
+    return -(-n // 128)
+
+
+def _fp8_device(t, device, what):
+    if t.device != device:
+        raise ValueError(f"{what} must be on {device}")
+
+
+def _fp8_stream(index):
+    now = torch._C._cuda_getDevice()
+    if now != index:
+        raise ValueError(f"the weights are on device {index}, the current device is {now}")
+    return torch._C._cuda_getCurrentRawStream(now)
+
+
+def _fp8_matrix(W, Ws, lead, what):
+    """Checks codes lead + [N, K] and scales lead + [ceil(N / 128), ceil(K / 128)]; returns N, K."""
+    _need(W.dim() == len(lead) + 2 and tuple(W.shape[:-2]) == lead, f"{what} must be {list(lead)} + [N, K]")
+    N, K = W.shape[-2:]
+    _need(W.dtype == E4M3, f"{what}: codes must be float8_e4m3fn")
+    _need(K >= 16 and K % 16 == 0 and N >= 1, f"{what}: K must be a positive multiple of 16")
+    _need(tuple(Ws.shape) == lead + (_blocks(N), _blocks(K)) and Ws.dtype == torch.float32,
+          f"{what}: scales must be float32 {list(lead + (_blocks(N), _blocks(K)))}")
+    _need(W.is_contiguous() and Ws.is_contiguous(), f"{what}: codes and scales must be contiguous")
+    _need(W.device == Ws.device, f"{what}: codes and scales must be on one device")
+    return N, K
+
+
+def _fp8_rows(X, K):
+    """Address, rows and row stride of X [M, K] (or [K]) whose rows may be slices of a wider matrix."""
+    if X.dim() == 1:
+        X = X[None]
+    if X.dim() != 2 or X.shape[1] != K:
+        raise ValueError(f"X must be [M, {K}]")
+    if not X.is_cuda:
+        raise ValueError("tensor must be on the GPU")
+    M = X.shape[0]
+    if X.stride(1) != 1 and M and K > 1:
+        raise ValueError("the elements of a row of X must be consecutive")
+    return X.data_ptr(), M, X.stride(0) if M > 1 else K
+
+
+def quant_fp8(X, out=None):
+    """X [M, K] (or [K]) to e4m3 codes [M, K] and float32 scales [M, ceil(K / 128)] (vybdq_quant_fp8): a power of two for each
+    row and 128 columns. out: preallocated (codes, scales)."""
+    K = X.shape[-1]
+    p, M, ldx = _fp8_rows(X, K)
+    if out is None:
+        q = torch.empty((M, K), dtype=E4M3, device=X.device)
+        d = torch.empty((M, _blocks(K)), dtype=torch.float32, device=X.device)
+    else:
+        q, d = out
+        _need(q.dtype == E4M3 and q.numel() == M * K, f"codes must be float8_e4m3fn [{M}, {K}]")
+        _need(d.dtype == torch.float32 and d.numel() == M * _blocks(K), f"scales must be float32 [{M}, {_blocks(K)}]")
+        _fp8_device(q, X.device, "codes")
+        _fp8_device(d, X.device, "scales")
+    call("vybdq_quant_fp8", p, _dt(X.dtype), ldx, _ptr(q), _ptr(d), M, K, _fp8_stream(X.get_device()))
+    return q, d
+
+
+def _fp8_out(out, M, N, y_dtype, residual, device):
+    if out is None:
+        out = torch.empty((M, N), dtype=y_dtype, device=device)
+    _check_out(out, (M, N))
+    _fp8_device(out, device, "out")
+    _check_residual(residual, out)
+    if residual is not None:
+        _fp8_device(residual, device, "residual")
+    return out
+
+
+def gemm_fp8(W, Ws, Xq, Xs, y_dtype=torch.float32, residual=None, out=None):
+    """Y [M, N] = X W^T (+ residual) of e4m3 codes Xq [M, K], W [N, K] and their scales Xs [M, ceil(K / 128)],
+    Ws [ceil(N / 128), ceil(K / 128)] (vybdq_gemm_fp8)."""
+    N, K = _fp8_matrix(W, Ws, (), "W")
+    M = Xq.shape[0]
+    _need(Xq.dim() == 2 and Xq.shape[1] == K and Xq.dtype == E4M3, f"Xq must be float8_e4m3fn [M, {K}]")
+    _need(tuple(Xs.shape) == (M, _blocks(K)) and Xs.dtype == torch.float32, f"Xs must be float32 [{M}, {_blocks(K)}]")
+    for t, what in ((Xq, "Xq"), (Xs, "Xs")):
+        _fp8_device(t, W.device, what)
+    out = _fp8_out(out, M, N, y_dtype, residual, W.device)
+    call("vybdq_gemm_fp8", _ptr(W), _ptr(Ws), _ptr(Xq), _ptr(Xs), _ptr(out), M, N, K, _dt(out.dtype), 0, _ptr(residual),
+         _fp8_stream(W.get_device()))
+    return out
+
+
+class Fp8Linear:
+    """x [M, K] -> y [M, N] through a matrix of e4m3 codes [N, K] with float32 scales [ceil(N / 128), ceil(K / 128)]: x is
+    quantized (quant_fp8) and multiplied (vybdq_linear_fp8), with the workspace for up to max_rows rows. Calls of one object
+    must not overlap (one stream, or streams that wait for each other; so for the replays of graphs that captured them)."""
+
+    def __init__(self, W, Ws, max_rows=64):
+        self.N, self.K = _fp8_matrix(W, Ws, (), "W")
+        self.W, self.Ws, self.max_rows, self.index = W, Ws, max_rows, W.get_device()
+        self.ws_bytes = _lib.lib.vybdq_linear_fp8_workspace_size(max_rows, self.N, self.K)
+        if self.ws_bytes < 0:
+            raise ValueError("unsupported shape")
+        self.ws = torch.empty(self.ws_bytes + 256, dtype=torch.uint8, device=W.device)
+        self.ws_ptr = (self.ws.data_ptr() + 255) // 256 * 256
+        self._w = (W.data_ptr(), Ws.data_ptr())
+
+    def __call__(self, X, y_dtype=torch.float32, residual=None, out=None):
+        """y [M, N] (+ residual) for X [M, K] (float32, float16 or bfloat16; rows may be slices of a wider matrix)."""
+        p, M, ldx = _fp8_rows(X, self.K)
+        if M > self.max_rows:
+            raise ValueError(f"X has {M} rows, the workspace is for {self.max_rows}")
+        if X.get_device() != self.index:
+            raise ValueError("X must be on the weights' device")
+        out = _fp8_out(out, M, self.N, y_dtype, residual, self.W.device)
+        call("vybdq_linear_fp8", *self._w, p, _dt(X.dtype), ldx, _ptr(out), M, self.N, self.K, _dt(out.dtype), 0, _ptr(residual),
+             self.ws_ptr, self.ws_bytes, _fp8_stream(self.index))
+        return out
+
+
+class MoeFp8Layer:
+    """Mixture-of-experts layer over e4m3 experts (vybdq_moe_forward_fp8).
+
+    gate, up: (codes [E, I, H], scales float32 [E, I / 128, H / 128]); down: (codes [E, H, I], scales [E, H / 128, I / 128]);
+    shared: three such pairs without the E, or None. The routing arguments are moe_route's; limit clamps gate and up
+    (math.inf: not). The workspace grows with the largest batch; calls of one object must not overlap."""
+
+    def __init__(self, gate, up, down, topk=8, shared=None, scale=2.5, limit=10.0, bias=None, score="sigmoid", renorm=True,
+                 groups=1, top_groups=1, group_top=2):
+        _need(gate[0].dim() == 3, "gate must be [E, I, H]")
+        E, I, H = gate[0].shape
+        _need(H % 128 == 0 and I % 128 == 0, "H and I must be multiples of 128")
+        for (W, Ws), shape, what in zip((gate, up, down), ((I, H), (I, H), (H, I)), ("gate", "up", "down")):
+            _need(_fp8_matrix(W, Ws, (E,), what) == shape, f"{what} must be {[E, *shape]}")
+        dev = gate[0].device
+        tensors = [t for pair in (gate, up, down) for t in pair]
+        if shared is not None:
+            for (W, Ws), shape, what in zip(shared, ((I, H), (I, H), (H, I)), ("gate", "up", "down")):
+                _need(_fp8_matrix(W, Ws, (), "shared " + what) == shape, f"shared {what} must be {list(shape)}")
+            tensors += [t for pair in shared for t in pair]
+        _need(all(t.device == dev for t in tensors), "the layer's tensors must be on one device")
+        _need(bias is None or (bias.numel() == E and bias.dtype == torch.float32 and bias.device == dev),
+              "bias must be float32 [E] on the weights' device")
+        _need(score in SCORES, f"score must be one of {SCORES}")
+        self.H, self.I, self.E, self.topk, self.index = H, I, E, topk, gate[0].get_device()
+        self.tensors, self.bias, self.device = tensors, bias, dev
+        self._w = tuple(_ptr(t) for t in tensors) + (0,) * (12 - len(tensors))
+        self._routing = (float(scale), float(limit), score == "softmax", renorm, groups, top_groups, group_top)
+        self._ws, self._ws_bytes, self._ws_t, self._captured, self._graphs = None, 0, 0, None, []
+
+    def _workspace(self, T):
+        if self._ws is None or self._ws_t < T:  # the size for T tokens covers fewer
+            n = _lib.lib.vybdq_moe_fp8_workspace_size(T, self.H, self.I, self.E, self.topk)
+            if n < 0:
+                raise ValueError("unsupported MoE shape")
+            if self._ws is not None:  # calls on this stream may still use it
+                self._ws.record_stream(torch.cuda.current_stream(self.device))
+            self._ws = torch.empty(n + 256, dtype=torch.uint8, device=self.device)
+            self._ws_bytes, self._ws_t = n, T
+        if self._captured is not self._ws and torch.cuda.is_current_stream_capturing():
+            self._captured = self._ws
+            self._graphs.append(self._ws)  # a graph's replays write to it, whatever size later calls need
+        return (self._ws.data_ptr() + 255) // 256 * 256, self._ws_bytes
+
+    def __call__(self, x, logits, out_dtype=torch.float32, out=None, routing=False):
+        """out [T, H] for x [T, H] and logits [T, E] (and the routing when routing=True)."""
+        T = x.shape[0]
+        _need(x.dim() == 2 and x.shape[1] == self.H, f"x must be [T, {self.H}]")
+        _need(logits.dim() == 2 and tuple(logits.shape) == (T, self.E), f"logits must be [T, {self.E}]")
+        for t, what in ((x, "x"), (logits, "logits")):
+            _fp8_device(t, self.device, what)
+        out = _fp8_out(out, T, self.H, out_dtype, None, self.device)
+        idx = w = None
+        if routing:
+            idx = torch.empty((T, self.topk), dtype=torch.int32, device=x.device)
+            w = torch.empty((T, self.topk), dtype=torch.float32, device=x.device)
+        ws, nb = self._workspace(T)
+        call("vybdq_moe_forward_fp8", _ptr(x), _dt(x.dtype), _ptr(logits), _dt(logits.dtype), _ptr(self.bias), *self._w, _ptr(out),
+             _dt(out.dtype), _ptr(idx), _ptr(w), T, self.H, self.I, self.E, self.topk, *self._routing, ws, nb,
+             _fp8_stream(self.index))
+        return (out, idx, w) if routing else out
