@@ -14,6 +14,11 @@ static int fp8_gemm_tiles(Fp8MmArgs &a, hipStream_t s) {
   };
   if (a.M <= 16) return fp8_mm_launch<1, 2, 1, 4, 4, FP8_DENSE, HALF>(a, units(16, 128), s);
   if (a.M <= 64) return fp8_mm_launch<4, 2, 1, 4, 3, FP8_DENSE, HALF>(a, units(64, 128), s);
+  if (a.K % 128 == 0 && a.KB >= 4 && a.M > 64) {
+    if (a.M <= 128) return fp8_pipe_launch<4, 2, 2, 4, 4, FP8_DENSE, HALF>(a, units(128, 128), s);
+    if (HALF || a.M <= 512) return fp8_pipe_launch<4, 4, 2, 4, 3, FP8_DENSE, HALF>(a, units(128, 256), s);
+    return fp8_pipe_launch<8, 4, 2, 4, 2, FP8_DENSE, false>(a, units(256, 256), s);
+  }
   if (a.M <= 512) return fp8_mm_launch<4, 4, 2, 2, 2, FP8_DENSE, HALF>(a, units(128, 128), s);
   return fp8_mm_launch<8, 4, 2, 4, 2, FP8_DENSE, HALF>(a, units(256, 256), s);
 }
@@ -29,10 +34,15 @@ static int fp8_gemm(const uint8_t *W, const float *Ws, const uint8_t *Xq, const 
   a.N = static_cast<int>(N);
   a.K = static_cast<int>(K);
   a.KB = static_cast<int>((K + 127) / 128);
+  a.xs_row = a.KB;
+  a.xs_block = 1;
+  a.x_rows = M;
   a.Y = Y;
   a.ydt = y_dt;
   a.ldy = ldy;
   a.RS = RS;
+  const int64_t es = 4 * dt_size(y_dt);
+  a.wide = N % 4 == 0 && ldy % 4 == 0 && (reinterpret_cast<uint64_t>(Y) | reinterpret_cast<uint64_t>(RS)) % es == 0;
   // float32 outputs keep float32 sums; those of 16 bits round by more than the e4m3 instruction loses
   return y_dt == VYBDQ_F32 || y_dt == VYBDQ_F64 ? fp8_gemm_tiles<true>(a, s) : fp8_gemm_tiles<false>(a, s);
 }

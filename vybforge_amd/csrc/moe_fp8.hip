@@ -71,7 +71,7 @@ static MoeFp8Ws moe_fp8_layout(char *base, int64_t T, int64_t H, int64_t I, int6
 
 static bool moe_fp8_shape(int64_t T, int64_t H, int64_t I, int64_t E, int64_t k) {
   return T >= 0 && T < (1 << 20) && H >= 128 && H % 128 == 0 && H <= 65536 && I >= 128 && I % 128 == 0 && I <= 65536 && E >= 1 &&
-         E <= 1024 && k >= 1 && k <= E && k <= 64 && T * k < (1 << 22) &&
+         E <= 1024 && k >= 1 && k <= E && k <= 64 && T * k < (1 << 22) && T * H < (int64_t(1) << 32) &&
          moe_tiles_bound(T, E, k, 16) * ((H > I ? H : I) / 128) < (int64_t(1) << 22);  // (workgroups of a launch)
 }
 
@@ -79,6 +79,7 @@ template <int MODE, bool HALF>
 static int moe_fp8_mm(int BM, Fp8MmArgs &a, int64_t tiles, hipStream_t s) {
   a.n_tiles = MODE == FP8_GATE_UP ? a.N / 128 : (a.N + 255) / 256;
   const int64_t units = tiles * a.n_tiles;
+  if (BM == 128 && a.KB >= 3) return fp8_pipe_launch<4, 4, 2, 4, 3, MODE, HALF>(a, units, s);
   if (BM == 16) return fp8_mm_launch<1, 2, 1, 8, 4, MODE, HALF>(a, units, s);
   if (BM == 64) return fp8_mm_launch<4, 4, 1, 4, 3, MODE, HALF>(a, units, s);
   return fp8_mm_launch<4, 4, 2, 4, 3, MODE, HALF>(a, units, s);
@@ -144,6 +145,9 @@ extern "C" int vybdq_moe_forward_fp8(uint64_t x, int x_dt, uint64_t logits, int 
   g.N = static_cast<int>(I);
   g.K = static_cast<int>(H);
   g.KB = static_cast<int>(H / 128);
+  g.xs_row = g.KB;
+  g.xs_block = 1;
+  g.x_rows = T;
   g.w_stride = I * H;
   g.ws_stride = (I / 128) * (H / 128);
   g.tiles = m.tiles;
@@ -164,6 +168,7 @@ extern "C" int vybdq_moe_forward_fp8(uint64_t x, int x_dt, uint64_t logits, int 
   d.N = static_cast<int>(H);
   d.K = static_cast<int>(I);
   d.KB = static_cast<int>(I / 128);
+  d.xs_row = d.KB;
   d.row_map = nullptr;
   d.Y = m.rows;
   d.ldy = H;
