@@ -618,9 +618,13 @@ int vybdq_quant_fp8(uint64_t X, int x_dt, int64_t ldx, uint64_t Xq, uint64_t Xs,
    sum of Xq W over the block's k; RS: as Y (its row stride too) or 0. Scales may be any float32. Products are exact, sums
    over a block and over blocks are float32; for F16 and BF16 outputs a block's sum comes from the e4m3 matrix
    instruction, which aligns its 128 products to the largest (1.4e-5 of the sum's rms for normal data, 3e-4 of the largest
-   product at most). W and Xq 16-byte aligned. ceil(M / 128) ceil(N / 128) below 2^22, M and N below 2^24. */
+   product at most). W and Xq 16-byte aligned. ceil(M / 128) ceil(N / 128) below 2^22, M and N below 2^24.
+   ws: 256-byte aligned, any contents, or 0; with vybdq_gemm_fp8_workspace_size(M, N, K) bytes (-1: unsupported; the size covers
+   every smaller M; at most 64 MiB) calls whose tiles do not fill the GPU split K and add float32 sums in a second launch (last
+   bits may differ from the unsplit sum); a smaller one is not used. Calls that share a workspace must not overlap. */
+int64_t vybdq_gemm_fp8_workspace_size(int64_t M, int64_t N, int64_t K);
 int vybdq_gemm_fp8(uint64_t W, uint64_t Ws, uint64_t Xq, uint64_t Xs, uint64_t Y, int64_t M, int64_t N, int64_t K, int y_dt,
-                   int64_t ldy, uint64_t RS, uint64_t stream);
+                   int64_t ldy, uint64_t RS, uint64_t ws, int64_t ws_bytes, uint64_t stream);
 
 /* vybdq_quant_fp8 and vybdq_gemm_fp8 in one call: X x_dt, row stride ldx. ws: 256-byte aligned, of
    vybdq_linear_fp8_workspace_size(M, N, K) bytes (-1: unsupported), any contents; the size covers every smaller M. Calls that

@@ -12,7 +12,7 @@ from oracle.kvcache import e4m3_decode
 from vybforge_amd import _lib, ops
 
 QUANT = dict(X=16, x_dt=0, ldx=256, Xq=16, Xs=4, M=3, K=256, stream=0)
-GEMM = dict(W=16, Ws=4, Xq=16, Xs=4, Y=4, M=3, N=5, K=256, y_dt=0, ldy=0, RS=0, stream=0)
+GEMM = dict(W=16, Ws=4, Xq=16, Xs=4, Y=4, M=3, N=5, K=256, y_dt=0, ldy=0, RS=0, ws=0, ws_bytes=0, stream=0)
 LINEAR = dict(W=16, Ws=4, X=16, x_dt=0, ldx=256, Y=4, M=3, N=5, K=256, y_dt=0, ldy=0, RS=0, ws=256, ws_bytes=1 << 20, stream=0)
 ROUTE = dict(logits=8, logits_dt=0, bias=4, idx=4, w=4, T=3, E=64, topk=4, scale=1.0, softmax=0, renorm=1, groups=8, top_groups=2,
              group_top=2, stream=0)
@@ -42,7 +42,8 @@ def test_quantizer_refuses(change, code, text):
 
 
 @pytest.mark.parametrize("change,code,text", PRODUCT + [
-    (dict(Xq=0), _lib.ERR_ARG, "null"), (dict(Xq=24), _lib.ERR_ALIGN, "Xq"), (dict(Xs=2), _lib.ERR_ALIGN, "Xs")])
+    (dict(Xq=0), _lib.ERR_ARG, "null"), (dict(Xq=24), _lib.ERR_ALIGN, "Xq"), (dict(Xs=2), _lib.ERR_ALIGN, "Xs"),
+    (dict(ws=128), _lib.ERR_WORKSPACE, "workspace"), (dict(ws_bytes=-1), _lib.ERR_WORKSPACE, "workspace")])
 def test_product_refuses(change, code, text):
     refused("vybdq_gemm_fp8", GEMM, change, code, text)
 
@@ -92,10 +93,12 @@ def test_nothing_to_do_is_no_launch():
 
 
 def test_workspace_sizes():
-    size = _lib.lib.vybdq_linear_fp8_workspace_size
+    part, size = _lib.lib.vybdq_gemm_fp8_workspace_size, _lib.lib.vybdq_linear_fp8_workspace_size
     for bad in ((-1, 16, 128), (1, 0, 128), (1, 16, 120), (1, 16, 0), (2 ** 24, 16, 128)):
-        assert size(*bad) == -1
-    for N, K in ((1, 16), (1000, 2576), (17408, 5120)):
+        assert size(*bad) == part(*bad) == -1
+    for N, K in ((1, 16), (1000, 2576), (17408, 5120), (300, 17408), (5, 1024)):
+        rest = [part(M, N, K) for M in (0, 1, 2, 5, 16, 17, 33, 64, 65, 100, 256, 257, 600, 1024, 1025, 4096)]
+        assert rest == sorted(rest) and max(rest) <= 1 << 26
         got = [size(M, N, K) for M in (0, 1, 2, 5, 16, 17, 33, 64, 65, 100, 256, 257, 600, 4096)]
         assert got == sorted(got) and got[1] >= K
     size = _lib.lib.vybdq_moe_fp8_workspace_size

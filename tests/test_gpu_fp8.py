@@ -120,7 +120,7 @@ def product_bound(xc, xs, wc, ws, y):
     return out, err + HALF[y] * (np.abs(out) + err) + (2.0 ** -25 if y == "f16" else 2.0 ** -140)
 
 
-def check_product(dev, rng, M, N, K, y, rs=False, make=matrix):
+def check_product(dev, rng, M, N, K, y, rs=False, make=matrix, split=False):
     (wc, ws), x = make(rng, N, K), rng.standard_normal((M, K)) * np.exp(rng.standard_normal((M, fp8.blocks(K)))).repeat(128, 1)[:, :K]
     xc, xs = fp8.quant(x.astype(np.float32))
     want, tol = product_bound(xc, xs, wc, ws, y)
@@ -129,7 +129,10 @@ def check_product(dev, rng, M, N, K, y, rs=False, make=matrix):
         r = torch.from_numpy(rng.standard_normal((M, N))).to(DT[y]).to(dev)
         want = want + r.double().cpu().numpy()
         tol = tol + HALF[y] * np.abs(r.double().cpu().numpy())
-    out = ops.gemm_fp8(*on(dev, (wc, ws)), *on(dev, (xc, xs)), y_dtype=DT[y], residual=r)
+    work = ops.Fp8Workspace([(M, N, K)], dev) if split else None
+    if split:
+        work.buf.fill_(0x7f)  # any contents (NaN, as float32)
+    out = ops.gemm_fp8(*on(dev, (wc, ws)), *on(dev, (xc, xs)), y_dtype=DT[y], residual=r, workspace=work)
     got = out.double().cpu().numpy()
     assert out.shape == (M, N) and (np.abs(got - want) <= tol).all(), np.abs((got - want) / tol).max()
     return out
@@ -151,6 +154,31 @@ def test_product_types_and_residuals(dev, rng, M, N, K, y):
 @pytest.mark.parametrize("M,N,K", [(1, 4000, 8192), (7, 200, 17408), (40, 300, 12288), (530, 700, 1536), (1030, 520, 640)])
 def test_product_long(dev, rng, M, N, K):
     check_product(dev, rng, M, N, K, "bf16", make=normal_matrix)
+
+
+@pytest.mark.parametrize("y", ["f32", "bf16"])
+@pytest.mark.parametrize("tile", ["64,1", "64,3", "128,1", "128,4", "256,1", "256,2"])
+@pytest.mark.parametrize("M,N,K", [(17, 1000, 2048), (64, 37, 2176), (130, 520, 2048), (300, 1300, 1152)])
+def test_product_tiles_and_splits(dev, rng, monkeypatch, M, N, K, tile, y):
+    """Every tile of the pipeline, whole and with K split, more tiles than one to a workgroup or fewer, ragged in every way."""
+    monkeypatch.setenv("VYBDQ_FP8_TILE", tile)
+    check_product(dev, rng, M, N, K, y, rs=True, make=normal_matrix, split=True)
+
+
+def test_product_many_tiles_to_a_workgroup(dev, rng):
+    """More tiles than workgroups: each goes on from tile to tile (17 x 23 tiles of 256 x 256, 64 x 33 of 64 x 256)."""
+    for M, N, K in ((4200, 5700, 512), (64, 90000, 512)):
+        (wc, ws), (xc, xs) = normal_matrix(rng, N, K), fp8.quant(rng.standard_normal((M, K)).astype(np.float32))
+        W, X = on(dev, (wc, ws)), on(dev, (xc, xs))
+        got = ops.gemm_fp8(*W, *X)
+        rows, cols = rng.choice(M, min(M, 40), replace=False), rng.choice(N, 300, replace=False)
+        want = (fp8.activations(xc[rows], xs[rows]) @ (e4m3_decode(wc[cols]) * ws[cols // 128].repeat(128, 1)[:, :K]).T)
+        # (the bound of product_bound with the largest |x w| sum: values of rms 1 over K = 512 terms)
+        np.testing.assert_allclose(got.cpu().numpy()[np.ix_(rows, cols)], want, rtol=0, atol=134 * 2.0 ** -23 * 40)
+        again = torch.empty_like(got)
+        for i in range(0, M, 1000):
+            ops.gemm_fp8(*W, X[0][i:i + 1000], X[1][i:i + 1000], out=again[i:i + 1000])
+        assert (got - again).abs().max() < 1e-4  # (tiles of other sizes sum in the same order, block by block)
 
 
 @pytest.mark.parametrize("M", [1, 16, 40, 100, 600])

@@ -119,7 +119,8 @@ SIGNATURES = {
                       _u64, _u64, _i64, _i64, _i64, _i64, ctypes.c_double, _int, _i64, _u64, _i64, _u64],
     "vybdq_kv_status": [],
     "vybdq_quant_fp8": [_u64, _int, _i64, _u64, _u64, _i64, _i64, _u64],
-    "vybdq_gemm_fp8": [_u64, _u64, _u64, _u64, _u64, _i64, _i64, _i64, _int, _i64, _u64, _u64],
+    "vybdq_gemm_fp8_workspace_size": [_i64, _i64, _i64],
+    "vybdq_gemm_fp8": [_u64, _u64, _u64, _u64, _u64, _i64, _i64, _i64, _int, _i64, _u64, _u64, _i64, _u64],
     "vybdq_linear_fp8_workspace_size": [_i64, _i64, _i64],
     "vybdq_linear_fp8": [_u64, _u64, _u64, _int, _i64, _u64, _i64, _i64, _i64, _int, _i64, _u64, _u64, _i64, _u64],
     "vybdq_moe_route_groups": [_u64, _int, _u64, _u64, _u64, _i64, _i64, _i64, ctypes.c_double, _int, _int, _i64, _i64, _i64,
@@ -132,7 +133,7 @@ _RESTYPE = {"vybdq_last_error": ctypes.c_char_p, "vybdq_chain_workspace_size": c
             "vybdq_exl3_workspace_size": ctypes.c_int64, "vybdq_moe_workspace_size": ctypes.c_int64,
             "vybdq_moe_exl3_workspace_size": ctypes.c_int64, "vybdq_kv_attn_workspace_size": ctypes.c_int64,
             "vybdq_gemm_workspace_size": ctypes.c_int64, "vybdq_gemm_q8_0_i8_workspace_size": ctypes.c_int64,
-            "vybdq_linear_fp8_workspace_size": ctypes.c_int64, "vybdq_moe_fp8_workspace_size": ctypes.c_int64,
+            "vybdq_gemm_fp8_workspace_size": ctypes.c_int64, "vybdq_linear_fp8_workspace_size": ctypes.c_int64, "vybdq_moe_fp8_workspace_size": ctypes.c_int64,
             "vybdq_gguf_kv_float": ctypes.c_double}
 for _n in ("vybdq_gguf_open", "vybdq_gguf_info", "vybdq_gguf_find_tensor", "vybdq_gguf_find_kv",
            "vybdq_gguf_tensor_name", "vybdq_gguf_tensor_field", "vybdq_gguf_kv_key", "vybdq_gguf_kv_field",

@@ -38,12 +38,12 @@ __device__ __forceinline__ float fp8_scale(uint32_t amax, float &inv) {
   return fp8_exp2(e);
 }
 
-// Four values times a power of two as e4m3 codes, rounded to nearest even and held to +-448 (zeros where
-// inv = 0: the block holds an infinity or NaN).
+// Four values of a block times the power of two that its scale divides by, as e4m3 codes, rounded to nearest even (none is
+// above 448 then). Zeros where inv = 0: the block holds an infinity or NaN.
 __device__ __forceinline__ uint32_t fp8_codes4(float a, float b, float c, float d, float inv) {
-  auto cl = [&](float x) { return inv == 0.f ? 0.f : __builtin_amdgcn_fmed3f(x * inv, -kFp8Max, kFp8Max); };
-  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(cl(a), cl(b), 0, false);
-  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(cl(c), cl(d), lo, true));
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
+  const uint32_t v = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, lo, true));
+  return inv == 0.f ? 0u : v;
 }
 
 // Largest 32-bit value over the 16 lanes of a row, in every lane (DPP, on the VALU).

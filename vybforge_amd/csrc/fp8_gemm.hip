@@ -1,30 +1,132 @@
 // The product of e4m3 matrices (fp8_mm.h) as a GEMM, and with the quantizer in front as a linear layer, gfx950.
-#include "fp8_mm.h"
+#include "fp8_rows.h"
+
+#include <cstdio>
+#include <cstdlib>
 
 namespace vybdq {
 
+// Sums of a split product: Y = RS + the splits' float32 sums in order, four elements to a thread.
+__global__ void __launch_bounds__(256) k_fp8_join(const Fp8MmArgs a, const float *__restrict__ part, int64_t stride, int splits) {
+  const int64_t i4 = 4 * (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x);
+  const int64_t n4 = (a.N + 3) / 4 * 4;
+  const int64_t row = i4 / n4;
+  const int col = static_cast<int>(i4 - row * n4);
+  if (row >= a.M) return;
+  const int left = a.N - col;
+  const float *p = part + row * a.N + col;
+  f4 v = {0.f, 0.f, 0.f, 0.f};
+  if (a.N % 4 == 0) {
+    for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const f4 *>(p + s * stride);
+  } else {
+    for (int s = 0; s < splits; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < left) v[j] += p[s * stride + j];
+  }
+  const int64_t at = row * a.ldy + col;
+  switch (a.ydt) {
+    case VYBDQ_F32: fp8_put4<VYBDQ_F32>(a, at, left, v); break;
+    case VYBDQ_F16: fp8_put4<VYBDQ_F16>(a, at, left, v); break;
+    case VYBDQ_BF16: fp8_put4<VYBDQ_BF16>(a, at, left, v); break;
+    default: fp8_put4<VYBDQ_F64>(a, at, left, v); break;
+  }
+}
+
+// ---- which kernel ---------------------------------------------------------------------------------
+
+struct Fp8Plan {
+  int BM, splits;  // pipelined tiles of BM x 256; BM = 0: the forms for any K
+};
+
+constexpr int64_t kFp8PartBytes = int64_t(64) << 20;  // most bytes of float32 sums that a split product writes
+
+// Bytes of split sums that a call of M rows may use: rises with M, so that a workspace serves every smaller batch.
+static int64_t fp8_part_bytes(int64_t M, int64_t N, int64_t K) {
+  const int64_t one = M * N * 4, most = K / 128 / 4;  // (no split of fewer than 4 blocks)
+  if (K % 128 || most < 2 || M > 1024) return 0;
+  const int64_t n = one * (most < 16 ? most : 16);
+  return n < kFp8PartBytes ? n : kFp8PartBytes;
+}
+
+static Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t K, bool half, int64_t part) {
+  const int64_t nk = K / 128, cus = device_cu_count();
+  Fp8Plan best{0, 1};
+  if (K % 128 || nk < 4) return best;
+  double best_t = 1e30;
+  for (int c = 0; c < 3; ++c) {
+    const int BM = c == 0 ? 64 : c == 1 ? 128 : 256;
+    if (half && BM == 256) continue;
+    const double step = half ? (c == 0 ? 0.9 : 1.5) : (c == 0 ? 0.75 : c == 1 ? 1.1 : 1.95), end = c == 0 ? 2.0 : c == 1 ? 3.0 : 5.0;
+    const int64_t tiles = (M + BM - 1) / BM * ((N + 255) / 256);
+    for (int64_t S = 1; S <= 16; ++S) {
+      if (S > 1 && (nk / S < 4 || S * M * N * 4 > part)) break;
+      const int64_t rounds = (tiles * S + cus - 1) / cus;
+      double t = static_cast<double>(rounds) * (static_cast<double>((nk + S - 1) / S) * step + end);
+      const double mem = static_cast<double>(N * K + M * K) / 4.9e6;
+      t = t > mem ? t : mem;
+      t += S > 1 ? 4.0 + static_cast<double>(S * M * N) * 8 / 4.5e6 : 0.0;
+      if (t < best_t) best_t = t, best = Fp8Plan{BM, static_cast<int>(S)};
+    }
+  }
+  if (const char *e = tuning_env("VYBDQ_FP8_TILE")) {  // "BM,splits"
+    int bm = 0, sp = 0;
+    if (sscanf(e, "%d,%d", &bm, &sp) == 2 && (bm == 64 || bm == 128 || (bm == 256 && !half)) && sp >= 1 && nk / sp >= 4 &&
+        (sp == 1 || sp * M * N * 4 <= part))
+      best = Fp8Plan{bm, sp};
+  }
+  return best;
+}
+
 template <bool HALF>
-static int fp8_gemm_tiles(Fp8MmArgs &a, hipStream_t s) {
+static int fp8_gemm_tiles(Fp8MmArgs &a, float *part, int64_t part_bytes, hipStream_t s) {
   auto units = [&](int BM, int BN) {
     a.m_tiles = (a.M + BM - 1) / BM;
     a.n_tiles = (a.N + BN - 1) / BN;
-    const int64_t n = static_cast<int64_t>(a.m_tiles) * a.n_tiles;
+    const int64_t n = static_cast<int64_t>(a.m_tiles) * a.n_tiles * a.splits;
     a.units = static_cast<int>(n);
     return n;
   };
-  if (a.M <= 16) return fp8_mm_launch<1, 2, 1, 4, 4, FP8_DENSE, HALF>(a, units(16, 128), s);
-  if (a.M <= 64) return fp8_mm_launch<4, 2, 1, 4, 3, FP8_DENSE, HALF>(a, units(64, 128), s);
-  if (a.K % 128 == 0 && a.KB >= 4 && a.M > 64) {
-    if (a.M <= 128) return fp8_pipe_launch<4, 2, 2, 4, 4, FP8_DENSE, HALF>(a, units(128, 128), s);
-    if (HALF || a.M <= 512) return fp8_pipe_launch<4, 4, 2, 4, 3, FP8_DENSE, HALF>(a, units(128, 256), s);
-    return fp8_pipe_launch<8, 4, 2, 4, 2, FP8_DENSE, false>(a, units(256, 256), s);
+  a.splits = 1;
+  const int64_t allowed = fp8_part_bytes(a.M, a.N, a.K);
+  if (a.M <= 16) {
+    Fp8RowsArgs r{};
+    r.m = a;
+    return fp8_rows_launch<1, 1, 8, 5, -1, HALF>(r, s);
   }
+  const Fp8Plan p = fp8_plan(a.M, a.N, a.K, HALF, part && part_bytes >= allowed ? allowed : 0);
+  if (p.BM) {
+    Fp8MmArgs t = a;
+    t.splits = p.splits;
+    if (p.splits > 1) {
+      t.Y = part;
+      t.ydt = VYBDQ_F32;
+      t.ldy = a.N;
+      t.RS = nullptr;
+      t.wide = a.N % 4 == 0;
+      t.split_stride = static_cast<int64_t>(a.M) * a.N;
+    }
+    a.splits = p.splits;
+    const int64_t n = units(p.BM, 256);
+    t.m_tiles = a.m_tiles;
+    t.n_tiles = a.n_tiles;
+    t.units = a.units;
+    int rc;
+    if (p.BM == 64) rc = fp8_pipe_launch<4, 2, 1, 8, 3, FP8_DENSE, HALF>(t, n, s);
+    else if (p.BM == 128) rc = fp8_pipe_launch<4, 4, 2, 4, 3, FP8_DENSE, HALF>(t, n, s);
+    else rc = fp8_pipe_launch<8, 4, 2, 4, 2, FP8_DENSE, false>(t, n, s);
+    if (rc || p.splits == 1) return rc;
+    const int64_t threads = static_cast<int64_t>(a.M) * ((a.N + 3) / 4);
+    hipLaunchKernelGGL(k_fp8_join, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, s, a, part, t.split_stride, p.splits);
+    return check_launch("fp8 product (join)");
+  }
+  if (a.M <= 64) return fp8_mm_launch<4, 2, 1, 4, 3, FP8_DENSE, HALF>(a, units(64, 128), s);
   if (a.M <= 512) return fp8_mm_launch<4, 4, 2, 2, 2, FP8_DENSE, HALF>(a, units(128, 128), s);
   return fp8_mm_launch<8, 4, 2, 4, 2, FP8_DENSE, HALF>(a, units(256, 256), s);
 }
 
 static int fp8_gemm(const uint8_t *W, const float *Ws, const uint8_t *Xq, const float *Xs, void *Y, int y_dt, int64_t M,
-                    int64_t N, int64_t K, int64_t ldy, const void *RS, hipStream_t s) {
+                    int64_t N, int64_t K, int64_t ldy, const void *RS, float *part, int64_t part_bytes, hipStream_t s) {
   Fp8MmArgs a{};
   a.X = Xq;
   a.Xs = Xs;
@@ -44,7 +146,7 @@ static int fp8_gemm(const uint8_t *W, const float *Ws, const uint8_t *Xq, const 
   const int64_t es = 4 * dt_size(y_dt);
   a.wide = N % 4 == 0 && ldy % 4 == 0 && (reinterpret_cast<uint64_t>(Y) | reinterpret_cast<uint64_t>(RS)) % es == 0;
   // float32 outputs keep float32 sums; those of 16 bits round by more than the e4m3 instruction loses
-  return y_dt == VYBDQ_F32 || y_dt == VYBDQ_F64 ? fp8_gemm_tiles<true>(a, s) : fp8_gemm_tiles<false>(a, s);
+  return y_dt == VYBDQ_F32 || y_dt == VYBDQ_F64 ? fp8_gemm_tiles<true>(a, part, part_bytes, s) : fp8_gemm_tiles<false>(a, part, part_bytes, s);
 }
 
 }  // namespace vybdq
@@ -70,20 +172,26 @@ static int fp8_check(const char *func, int64_t M, int64_t N, int64_t K, uint64_t
   return VYBDQ_OK;
 }
 
+extern "C" int64_t vybdq_gemm_fp8_workspace_size(int64_t M, int64_t N, int64_t K) {
+  if (M < 0 || M >= (int64_t(1) << 24) || N < 1 || N >= (int64_t(1) << 24) || K < 16 || K % 16 || K >= (int64_t(1) << 23)) return -1;
+  return align256(fp8_part_bytes(M < 1024 ? M : 1024, N, K));  // (rises with M, none above 1024)
+}
+
 extern "C" int vybdq_gemm_fp8(uint64_t W, uint64_t Ws, uint64_t Xq, uint64_t Xs, uint64_t Y, int64_t M, int64_t N, int64_t K,
-                              int y_dt, int64_t ldy, uint64_t RS, uint64_t stream) {
+                              int y_dt, int64_t ldy, uint64_t RS, uint64_t ws, int64_t ws_bytes, uint64_t stream) {
   const int rc = fp8_check(__func__, M, N, K, W, Ws, Y, y_dt, ldy, RS);
   if (rc || M == 0) return rc;
   VYBDQ_REQUIRE(Xq && Xs, VYBDQ_ERR_ARG, "null buffer");
   VYBDQ_REQUIRE(Xq % 16 == 0 && Xs % 4 == 0, VYBDQ_ERR_ALIGN, "Xq must be 16-byte and Xs 4-byte aligned");
+  VYBDQ_REQUIRE(ws % 256 == 0 && ws_bytes >= 0, VYBDQ_ERR_WORKSPACE, "workspace must be 256-byte aligned");
   return fp8_gemm(reinterpret_cast<const uint8_t *>(W), reinterpret_cast<const float *>(Ws), reinterpret_cast<const uint8_t *>(Xq),
                   reinterpret_cast<const float *>(Xs), reinterpret_cast<void *>(Y), y_dt, M, N, K, ldy,
-                  reinterpret_cast<const void *>(RS), as_stream(stream));
+                  reinterpret_cast<const void *>(RS), reinterpret_cast<float *>(ws), ws_bytes, as_stream(stream));
 }
 
 extern "C" int64_t vybdq_linear_fp8_workspace_size(int64_t M, int64_t N, int64_t K) {
-  if (M < 0 || M >= (int64_t(1) << 24) || N < 1 || N >= (int64_t(1) << 24) || K < 16 || K % 16 || K >= (int64_t(1) << 23)) return -1;
-  return align256(M * K) + align256(M * ((K + 127) / 128) * 4);
+  const int64_t part = vybdq_gemm_fp8_workspace_size(M, N, K);
+  return part < 0 ? -1 : align256(M * K) + align256(M * ((K + 127) / 128) * 4) + part;
 }
 
 extern "C" int vybdq_linear_fp8(uint64_t W, uint64_t Ws, uint64_t X, int x_dt, int64_t ldx, uint64_t Y, int64_t M, int64_t N,
@@ -99,8 +207,10 @@ extern "C" int vybdq_linear_fp8(uint64_t W, uint64_t Ws, uint64_t X, int x_dt, i
                 "workspace must be 256-byte aligned and of vybdq_linear_fp8_workspace_size bytes");
   uint8_t *xq = reinterpret_cast<uint8_t *>(ws);
   float *xs = reinterpret_cast<float *>(ws + align256(M * K));
+  const int64_t front = align256(M * K) + align256(M * ((K + 127) / 128) * 4);
   const int qc = fp8_quant_rows(reinterpret_cast<const void *>(X), x_dt, M, K, ldx, xq, xs, as_stream(stream));
   if (qc) return qc;
   return fp8_gemm(reinterpret_cast<const uint8_t *>(W), reinterpret_cast<const float *>(Ws), xq, xs, reinterpret_cast<void *>(Y),
-                  y_dt, M, N, K, ldy, reinterpret_cast<const void *>(RS), as_stream(stream));
+                  y_dt, M, N, K, ldy, reinterpret_cast<const void *>(RS), reinterpret_cast<float *>(ws + front), ws_bytes - front,
+                  as_stream(stream));
 }

@@ -23,7 +23,9 @@ struct Fp8MmArgs {
   int64_t w_stride, ws_stride;     // codes and scales from one expert to the next
   const int4 *tiles;               // {expert (-1: shared), first row, end row, m-tile of these rows}
   const int *ntiles, *row_map;     // row -> row of X (null: itself)
-  int m_tiles, n_tiles, units;
+  int m_tiles, n_tiles, units;     // DENSE: units = tiles times splits of K
+  int splits;
+  int64_t split_stride;            // elements of Y from one split's sums to the next's (float32)
   void *Y;
   int ydt;
   int64_t ldy;
@@ -123,7 +125,8 @@ __device__ __forceinline__ void fp8_put4(const Fp8MmArgs &a, int64_t at, int lef
 // What becomes of a tile's sums: acc[n][m][i] is row m0 + 16 (MF wm + m) + (lane & 15), column n0 + 16 (NF wn + n) + 4 (lane / 16) + i
 // (GATE_UP: fragments n < NF / 2 gate, the others up, of columns n0 + 8 NF wn + ..). red: LDS for WN x BM words (GATE_UP).
 template <int MF, int NF, int WM, int WN, int MODE>
-__device__ __forceinline__ void fp8_store(const Fp8MmArgs &a, f4 (&acc)[NF][MF], int m0, int m_end, int n0, uint32_t *red) {
+__device__ __forceinline__ void fp8_store(const Fp8MmArgs &a, f4 (&acc)[NF][MF], int m0, int m_end, int n0, uint32_t *red,
+                                          int split = 0) {
   constexpr int BM = 16 * MF * WM;
   constexpr bool DUAL = MODE == FP8_GATE_UP;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -195,7 +198,7 @@ __device__ __forceinline__ void fp8_store(const Fp8MmArgs &a, f4 (&acc)[NF][MF],
 #pragma unroll
       for (int m = 0; m < MF; ++m) {
         const int row = m0 + (wm * MF + m) * 16 + (lane & 15);
-        const int64_t at = static_cast<int64_t>(row) * a.ldy + n0 + 16 * wn * NF + g4;
+        const int64_t at = split * a.split_stride + static_cast<int64_t>(row) * a.ldy + n0 + 16 * wn * NF + g4;
 #pragma unroll
         for (int n = 0; n < NF; ++n) {
           const int left = row < m_end ? a.N - (n0 + 16 * (wn * NF + n) + g4) : 0;
@@ -428,7 +431,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
   auto srd_of = [](const Buf &b) { return srd_t{b.lo, b.hi, b.bytes, 0x00027000u}; };
   // the tile to compute: rows m0 .. m_end, columns n0 .., scales of this wave's rows of W
   struct Place {
-    int m0, m_end, n0;
+    int m0, m_end, n0, nk, split;  // (blocks of K of this unit)
     const float *ws, *ws2;
   };
   uint32_t off[PER];
@@ -443,13 +446,24 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
     off[i] = static_cast<uint32_t>(r) * static_cast<uint32_t>(a.K) + 16 * c;
   }
   const uint32_t s_on = __builtin_amdgcn_readfirstlane(wave < BM / 64 || wave == 0 ? ~0u : 0u);
-  // unit u: dense tiles in groups of 8 tiles of rows, columns by columns; experts' tiles in list order, columns inside
+  // unit u: splits of K outermost; dense tiles in groups of 8 tiles of rows, columns by columns; experts' tiles in list order,
+  // columns inside
   auto tile_at = [&](int u, Tile &f) {
     Place t;
     const uint8_t *W = a.W, *W2 = a.W2;
     const float *Ws = a.Ws, *W2s = a.W2s;
     int n;
+    int k0 = 0;
+    t.nk = nk;
+    t.split = 0;
     if constexpr (MODE == FP8_DENSE) {
+      const int tiles = a.m_tiles * a.n_tiles;
+      if (a.splits > 1) {
+        t.split = u / tiles;
+        u -= t.split * tiles;
+        k0 = static_cast<int>(static_cast<int64_t>(t.split) * nk / a.splits);
+        t.nk = static_cast<int>(static_cast<int64_t>(t.split + 1) * nk / a.splits) - k0;
+      }
       const int per = 8 * a.n_tiles, g = u / per, r = u - g * per, gm = min(8, a.m_tiles - 8 * g);
       n = r / gm;
       t.m0 = (8 * g + r - n * gm) * BM;
@@ -477,10 +491,10 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
     }
     t.n0 = n * (DUAL ? 128 : BN);
     const int rows = min(BM, t.m_end - t.m0), cols = min(DUAL ? 128 : BN, a.N - t.n0);
-    f.w = buf_of(W + static_cast<int64_t>(t.n0) * a.K, static_cast<int64_t>(cols) * a.K);
+    f.w = buf_of(W + static_cast<int64_t>(t.n0) * a.K + 128 * k0, static_cast<int64_t>(cols) * a.K - 128 * k0);
     if constexpr (DUAL) f.w2 = buf_of(W2 + static_cast<int64_t>(t.n0) * a.K, static_cast<int64_t>(cols) * a.K);
     const int nb = (DUAL ? t.n0 : min(t.n0 + 16 * NF * wn, a.N - 1)) >> 7;
-    t.ws = Ws + static_cast<int64_t>(nb) * nk;
+    t.ws = Ws + static_cast<int64_t>(nb) * nk + k0;
     t.ws2 = DUAL ? W2s + static_cast<int64_t>(nb) * nk : nullptr;
     const int sr = wave * 64 + lane;  // row of this lane's scale (waves past the last do not load it)
     if constexpr (GATHER) {
@@ -493,8 +507,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
       }
       f.soff = static_cast<uint32_t>(a.row_map[t.m0 + min(sr, rows - 1)]) * static_cast<uint32_t>(a.xs_row * 4);
     } else {
-      f.x = buf_of(a.X + static_cast<int64_t>(t.m0) * a.K, static_cast<int64_t>(rows) * a.K);
-      f.s = buf_of(a.Xs + t.m0 * a.xs_row, 4 * ((rows - 1) * a.xs_row + (nk - 1) * a.xs_block + 1));
+      f.x = buf_of(a.X + static_cast<int64_t>(t.m0) * a.K + 128 * k0, static_cast<int64_t>(rows) * a.K - 128 * k0);
+      f.s = buf_of(a.Xs + t.m0 * a.xs_row + k0 * a.xs_block, 4 * ((rows - 1) * a.xs_row + (nk - 1 - k0) * a.xs_block + 1));
       f.soff = static_cast<uint32_t>(sr) * static_cast<uint32_t>(a.xs_row * 4);
     }
     return t;
@@ -582,6 +596,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
     if (u + G < units) then = tile_at(u + G, next);
     const float *ws = at.ws, *ws2 = at.ws2;
     float w0 = uniform_load(ws, 0), w1 = DUAL ? uniform_load(ws2, 0) : 0.f;
+    const int nk = at.nk;
     for (int k = 0; k < nk; ++k) {
       const uint32_t sn = sb + STAGE == ST * STAGE ? 0 : sb + STAGE;
       const char *buf = smem + sb, *nbuf = smem + sn;
@@ -671,7 +686,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
     }
     add(acc[NF - 1][MF - 2], t[NF - 1], of(sp, NF - 1));
     add(acc[NF - 1][MF - 1], tb, of(sq, NF - 1));
-    fp8_store<MF, NF, WM, WN, MODE>(a, acc, at.m0, at.m_end, at.n0, reinterpret_cast<uint32_t *>(smem + ST * STAGE));
+    fp8_store<MF, NF, WM, WN, MODE>(a, acc, at.m0, at.m_end, at.n0, reinterpret_cast<uint32_t *>(smem + ST * STAGE), at.split);
     at = then;
   }
   wait_loads<0>();  // (nothing may arrive in LDS that is another workgroup's)

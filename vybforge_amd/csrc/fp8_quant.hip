@@ -2,35 +2,9 @@
 //
 // 16 lanes take a block: 8 elements each (16 bytes of a 16-bit type), the block's largest magnitude by four DPP steps over
 // the bits of |x| (an integer maximum: infinities and NaN come out on top), 8 codes a lane.
-#include "fp8.h"
+#include "fp8_load.h"
 
 namespace vybdq {
-
-template <int DT>
-__device__ __forceinline__ void fp8_load8(const void *p, int64_t i, float (&x)[8]) {
-  if constexpr (DT == VYBDQ_F32) {
-    const f4 *q = reinterpret_cast<const f4 *>(static_cast<const float *>(p) + i);
-    const f4 a = q[0], b = q[1];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x[j] = a[j];
-      x[4 + j] = b[j];
-    }
-  } else {
-    const u4 r = *reinterpret_cast<const u4 *>(static_cast<const uint16_t *>(p) + i);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t w = r[j];
-      if constexpr (DT == VYBDQ_F16) {
-        x[2 * j] = half_bits_to_f32(w & 0xffffu);
-        x[2 * j + 1] = half_bits_to_f32(w >> 16);
-      } else {
-        x[2 * j] = __uint_as_float(w << 16);
-        x[2 * j + 1] = __uint_as_float(w & 0xffff0000u);
-      }
-    }
-  }
-}
 
 template <int DT>
 __global__ void __launch_bounds__(256) k_fp8_quant(const void *__restrict__ X, uint8_t *__restrict__ Xq,
@@ -45,18 +19,9 @@ __global__ void __launch_bounds__(256) k_fp8_quant(const void *__restrict__ X, u
   for (int j = 0; j < 8; ++j) x[j] = 0.f;
   const bool in = k < K;
   if (in) fp8_load8<DT>(X, static_cast<int64_t>(m) * ldx + k, x);
-  uint32_t a = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t v = __float_as_uint(x[j]) & 0x7fffffffu;
-    a = v > a ? v : a;
-  }
-  a = row16_max_u32(a);
-  float inv;
-  const float sc = fp8_scale(a, inv);
-  if (in)
-    *reinterpret_cast<u2 *>(Xq + static_cast<int64_t>(m) * K + k) =
-        u2{fp8_codes4(x[0], x[1], x[2], x[3], inv), fp8_codes4(x[4], x[5], x[6], x[7], inv)};
+  float sc;
+  const u2 c = fp8_quant8(x, sc);
+  if (in) *reinterpret_cast<u2 *>(Xq + static_cast<int64_t>(m) * K + k) = c;
   if ((threadIdx.x & 15) == 0) Xs[u] = sc;
 }
 

@@ -848,9 +848,11 @@ def _fp8_out(out, M, N, y_dtype, residual, device):
     return out
 
 
-def gemm_fp8(W, Ws, Xq, Xs, y_dtype=torch.float32, residual=None, out=None):
+def gemm_fp8(W, Ws, Xq, Xs, y_dtype=torch.float32, residual=None, out=None, workspace=None):
     """Y [M, N] = X W^T (+ residual) of e4m3 codes Xq [M, K], W [N, K] and their scales Xs [M, ceil(K / 128)],
-    Ws [ceil(N / 128), ceil(K / 128)] (vybdq_gemm_fp8)."""
+    Ws [ceil(N / 128), ceil(K / 128)] (vybdq_gemm_fp8).
+
+    workspace: an Fp8Workspace (K split across workgroups) or None for the unsplit product."""
     N, K = _fp8_matrix(W, Ws, (), "W")
     M = Xq.shape[0]
     _need(Xq.dim() == 2 and Xq.shape[1] == K and Xq.dtype == E4M3, f"Xq must be float8_e4m3fn [M, {K}]")
@@ -858,24 +860,42 @@ def gemm_fp8(W, Ws, Xq, Xs, y_dtype=torch.float32, residual=None, out=None):
     for t, what in ((Xq, "Xq"), (Xs, "Xs")):
         _fp8_device(t, W.device, what)
     out = _fp8_out(out, M, N, y_dtype, residual, W.device)
-    call("vybdq_gemm_fp8", _ptr(W), _ptr(Ws), _ptr(Xq), _ptr(Xs), _ptr(out), M, N, K, _dt(out.dtype), 0, _ptr(residual),
+    ws, nb = (0, 0) if workspace is None else workspace.at(W.device)
+    call("vybdq_gemm_fp8", _ptr(W), _ptr(Ws), _ptr(Xq), _ptr(Xs), _ptr(out), M, N, K, _dt(out.dtype), 0, _ptr(residual), ws, nb,
          _fp8_stream(W.get_device()))
     return out
 
 
+class Fp8Workspace:
+    """256-byte aligned workspace of gemm_fp8 and Fp8Linear for the given (M, N, K) shapes and every smaller M. Several layers may
+    share one; calls that do must not overlap (one stream, or streams that wait for each other; so for the replays of graphs
+    that captured them)."""
+
+    def __init__(self, shapes, device):
+        sizes = [_lib.lib.vybdq_linear_fp8_workspace_size(M, N, K) for M, N, K in shapes]
+        if min(sizes, default=0) < 0:
+            raise ValueError("unsupported shape")
+        self.nbytes = max(sizes, default=0)
+        self.buf = torch.empty(self.nbytes + 256, dtype=torch.uint8, device=device)
+        self.ptr = (self.buf.data_ptr() + 255) // 256 * 256
+
+    def at(self, device):
+        _fp8_device(self.buf, device, "workspace")
+        return self.ptr, self.nbytes
+
+
 class Fp8Linear:
     """x [M, K] -> y [M, N] through a matrix of e4m3 codes [N, K] with float32 scales [ceil(N / 128), ceil(K / 128)]: x is
-    quantized (quant_fp8) and multiplied (vybdq_linear_fp8), with the workspace for up to max_rows rows. Calls of one object
-    must not overlap (one stream, or streams that wait for each other; so for the replays of graphs that captured them)."""
+    quantized (quant_fp8) and multiplied (vybdq_linear_fp8), with a workspace for up to max_rows rows: its own, or an
+    Fp8Workspace that holds (max_rows, N, K). Calls that use one workspace must not overlap."""
 
-    def __init__(self, W, Ws, max_rows=64):
+    def __init__(self, W, Ws, max_rows=64, workspace=None):
         self.N, self.K = _fp8_matrix(W, Ws, (), "W")
         self.W, self.Ws, self.max_rows, self.index = W, Ws, max_rows, W.get_device()
-        self.ws_bytes = _lib.lib.vybdq_linear_fp8_workspace_size(max_rows, self.N, self.K)
-        if self.ws_bytes < 0:
-            raise ValueError("unsupported shape")
-        self.ws = torch.empty(self.ws_bytes + 256, dtype=torch.uint8, device=W.device)
-        self.ws_ptr = (self.ws.data_ptr() + 255) // 256 * 256
+        own = workspace is None
+        self.workspace = Fp8Workspace([(max_rows, self.N, self.K)], W.device) if own else workspace
+        self._ws = self.workspace.at(W.device)
+        _need(self._ws[1] >= _lib.lib.vybdq_linear_fp8_workspace_size(max_rows, self.N, self.K), "the workspace is too small")
         self._w = (W.data_ptr(), Ws.data_ptr())
 
     def __call__(self, X, y_dtype=torch.float32, residual=None, out=None):
@@ -887,7 +907,7 @@ class Fp8Linear:
             raise ValueError("X must be on the weights' device")
         out = _fp8_out(out, M, self.N, y_dtype, residual, self.W.device)
         call("vybdq_linear_fp8", *self._w, p, _dt(X.dtype), ldx, _ptr(out), M, self.N, self.K, _dt(out.dtype), 0, _ptr(residual),
-             self.ws_ptr, self.ws_bytes, _fp8_stream(self.index))
+             *self._ws, _fp8_stream(self.index))
         return out
 
 
