@@ -49,23 +49,23 @@ static int64_t fp8_part_bytes(int64_t M, int64_t N, int64_t K) {
   return n < kFp8PartBytes ? n : kFp8PartBytes;
 }
 
+// Tile height and splits with the least estimate: rounds of tiles over the chip, a round its K steps and its end; split sums written,
+// read and added. Times in us fitted over 26 shapes from 16 to 2048 rows (both instructions) with every tile and up to 16 splits
+// forced: 9% off in the mean over 200 of them, the choice never more than 2% above the best of them.
 static Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t K, bool half, int64_t part) {
   const int64_t nk = K / 128, cus = device_cu_count();
   Fp8Plan best{0, 1};
   if (K % 128 || nk < 4) return best;
+  constexpr double kStep[2][3] = {{0.84, 1.0, 1.72}, {1.07, 1.65, 0}}, kEnd[3] = {2.5, 2.8, 2.9};
   double best_t = 1e30;
-  for (int c = 0; c < 3; ++c) {
-    const int BM = c == 0 ? 64 : c == 1 ? 128 : 256;
-    if (half && BM == 256) continue;
-    const double step = half ? (c == 0 ? 0.9 : 1.5) : (c == 0 ? 0.75 : c == 1 ? 1.1 : 1.95), end = c == 0 ? 2.0 : c == 1 ? 3.0 : 5.0;
+  for (int c = 0; c < (half ? 2 : 3); ++c) {
+    const int BM = 64 << c;
     const int64_t tiles = (M + BM - 1) / BM * ((N + 255) / 256);
     for (int64_t S = 1; S <= 16; ++S) {
       if (S > 1 && (nk / S < 4 || S * M * N * 4 > part)) break;
-      const int64_t rounds = (tiles * S + cus - 1) / cus;
-      double t = static_cast<double>(rounds) * (static_cast<double>((nk + S - 1) / S) * step + end);
-      const double mem = static_cast<double>(N * K + M * K) / 4.9e6;
-      t = t > mem ? t : mem;
-      t += S > 1 ? 4.0 + static_cast<double>(S * M * N) * 8 / 4.5e6 : 0.0;
+      const double rounds = static_cast<double>((tiles * S + cus - 1) / cus);
+      const double t = rounds * (static_cast<double>((nk + S - 1) / S) * kStep[half][c] + kEnd[c]) +
+                       (S > 1 ? 3.2 + static_cast<double>(S * M * N) * 8 / 4.5e6 : 0.0);
       if (t < best_t) best_t = t, best = Fp8Plan{BM, static_cast<int>(S)};
     }
   }
@@ -76,6 +76,24 @@ static Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t K, bool half, int64_t part
       best = Fp8Plan{bm, sp};
   }
   return best;
+}
+
+// Few rows of X (fp8_rows.h) or tiles. Up to 4 rows, or 16 of at most 2^25 weights, the streaming form is the faster one (measured,
+// bf16: 1 x 17408 x 5120 22.3 us against 23.8, 1 x 2560 x 9728 10.0 / 15.2, 16 x 9728 x 2560 11.5 / 13.5); beyond, every
+// workgroup's own pass over X costs more than the tiles' second launch (16 x 17408 x 5120 32.8 / 25.0, 16 x 5120 x 17408 42 / 26).
+static bool fp8_rows_take(int64_t M, int64_t N, int64_t K) { return M <= 4 || (M <= 16 && N * K <= (int64_t(1) << 25)) || (M <= 16 && K % 128); }
+
+// Whether such a call quantizes X in its workgroups, each for itself: where that is little beside its rows of W, or all
+// workgroups do it at once (measured with the quantizer's own launch: 1 x 9728 x 2560 8.3 us against 11.0, 4 x 17408 x 5120
+// 25.1 / 26.4, 16 x 1003 x 2560 8.2 / 10.3; but 16 x 9728 x 2560 17.0 / 13.5). Its codes and scales fit with two workgroups to a CU.
+static bool fp8_rows_quant(int64_t M, int64_t N, int64_t K) {
+  return (M <= 4 || N <= 4096) && M * ((K + 127) / 128) * 132 <= 56 * 1024;
+}
+
+// 16 waves from 32 blocks of K, else 8 (1 x 2560 x 9728 10.0 us against 12.0; 1 x 6144 x 2048 9.5 / 8.9).
+template <int XDT, bool HALF>
+static int fp8_rows_run(const Fp8RowsArgs &r, hipStream_t s) {
+  return r.m.KB >= 32 ? fp8_rows_launch<1, 1, 16, 3, XDT, HALF>(r, s) : fp8_rows_launch<1, 1, 8, 3, XDT, HALF>(r, s);
 }
 
 template <bool HALF>
@@ -89,10 +107,10 @@ static int fp8_gemm_tiles(Fp8MmArgs &a, float *part, int64_t part_bytes, hipStre
   };
   a.splits = 1;
   const int64_t allowed = fp8_part_bytes(a.M, a.N, a.K);
-  if (a.M <= 16) {
+  if (fp8_rows_take(a.M, a.N, a.K)) {
     Fp8RowsArgs r{};
     r.m = a;
-    return fp8_rows_launch<1, 1, 8, 5, -1, HALF>(r, s);
+    return fp8_rows_run<-1, HALF>(r, s);
   }
   const Fp8Plan p = fp8_plan(a.M, a.N, a.K, HALF, part && part_bytes >= allowed ? allowed : 0);
   if (p.BM) {
@@ -125,8 +143,8 @@ static int fp8_gemm_tiles(Fp8MmArgs &a, float *part, int64_t part_bytes, hipStre
   return fp8_mm_launch<8, 4, 2, 4, 2, FP8_DENSE, HALF>(a, units(256, 256), s);
 }
 
-static int fp8_gemm(const uint8_t *W, const float *Ws, const uint8_t *Xq, const float *Xs, void *Y, int y_dt, int64_t M,
-                    int64_t N, int64_t K, int64_t ldy, const void *RS, float *part, int64_t part_bytes, hipStream_t s) {
+static Fp8MmArgs fp8_args(const uint8_t *W, const float *Ws, const uint8_t *Xq, const float *Xs, void *Y, int y_dt, int64_t M,
+                          int64_t N, int64_t K, int64_t ldy, const void *RS) {
   Fp8MmArgs a{};
   a.X = Xq;
   a.Xs = Xs;
@@ -145,8 +163,14 @@ static int fp8_gemm(const uint8_t *W, const float *Ws, const uint8_t *Xq, const 
   a.RS = RS;
   const int64_t es = 4 * dt_size(y_dt);
   a.wide = N % 4 == 0 && ldy % 4 == 0 && (reinterpret_cast<uint64_t>(Y) | reinterpret_cast<uint64_t>(RS)) % es == 0;
-  // float32 outputs keep float32 sums; those of 16 bits round by more than the e4m3 instruction loses
-  return y_dt == VYBDQ_F32 || y_dt == VYBDQ_F64 ? fp8_gemm_tiles<true>(a, part, part_bytes, s) : fp8_gemm_tiles<false>(a, part, part_bytes, s);
+  return a;
+}
+
+// float32 outputs keep float32 sums; those of 16 bits round by more than the e4m3 instruction loses
+static bool fp8_half(int y_dt) { return y_dt == VYBDQ_F32 || y_dt == VYBDQ_F64; }
+
+static int fp8_gemm(Fp8MmArgs a, float *part, int64_t part_bytes, hipStream_t s) {
+  return fp8_half(a.ydt) ? fp8_gemm_tiles<true>(a, part, part_bytes, s) : fp8_gemm_tiles<false>(a, part, part_bytes, s);
 }
 
 }  // namespace vybdq
@@ -184,9 +208,10 @@ extern "C" int vybdq_gemm_fp8(uint64_t W, uint64_t Ws, uint64_t Xq, uint64_t Xs,
   VYBDQ_REQUIRE(Xq && Xs, VYBDQ_ERR_ARG, "null buffer");
   VYBDQ_REQUIRE(Xq % 16 == 0 && Xs % 4 == 0, VYBDQ_ERR_ALIGN, "Xq must be 16-byte and Xs 4-byte aligned");
   VYBDQ_REQUIRE(ws % 256 == 0 && ws_bytes >= 0, VYBDQ_ERR_WORKSPACE, "workspace must be 256-byte aligned");
-  return fp8_gemm(reinterpret_cast<const uint8_t *>(W), reinterpret_cast<const float *>(Ws), reinterpret_cast<const uint8_t *>(Xq),
-                  reinterpret_cast<const float *>(Xs), reinterpret_cast<void *>(Y), y_dt, M, N, K, ldy,
-                  reinterpret_cast<const void *>(RS), reinterpret_cast<float *>(ws), ws_bytes, as_stream(stream));
+  return fp8_gemm(fp8_args(reinterpret_cast<const uint8_t *>(W), reinterpret_cast<const float *>(Ws),
+                           reinterpret_cast<const uint8_t *>(Xq), reinterpret_cast<const float *>(Xs), reinterpret_cast<void *>(Y),
+                           y_dt, M, N, K, ldy, reinterpret_cast<const void *>(RS)),
+                  reinterpret_cast<float *>(ws), ws_bytes, as_stream(stream));
 }
 
 extern "C" int64_t vybdq_linear_fp8_workspace_size(int64_t M, int64_t N, int64_t K) {
@@ -208,9 +233,15 @@ extern "C" int vybdq_linear_fp8(uint64_t W, uint64_t Ws, uint64_t X, int x_dt, i
   uint8_t *xq = reinterpret_cast<uint8_t *>(ws);
   float *xs = reinterpret_cast<float *>(ws + align256(M * K));
   const int64_t front = align256(M * K) + align256(M * ((K + 127) / 128) * 4);
-  const int qc = fp8_quant_rows(reinterpret_cast<const void *>(X), x_dt, M, K, ldx, xq, xs, as_stream(stream));
+  hipStream_t s = as_stream(stream);
+  const Fp8MmArgs a = fp8_args(reinterpret_cast<const uint8_t *>(W), reinterpret_cast<const float *>(Ws), xq, xs,
+                               reinterpret_cast<void *>(Y), y_dt, M, N, K, ldy, reinterpret_cast<const void *>(RS));
+  if (fp8_rows_take(M, N, K) && fp8_rows_quant(M, N, K)) {
+    const Fp8RowsArgs r{a, reinterpret_cast<const void *>(X), ldx};
+    if (fp8_half(y_dt)) VYBDQ_DISPATCH_IN(x_dt, XDT, return (fp8_rows_run<XDT, true>(r, s)))
+    else VYBDQ_DISPATCH_IN(x_dt, XDT, return (fp8_rows_run<XDT, false>(r, s)))
+  }
+  const int qc = fp8_quant_rows(reinterpret_cast<const void *>(X), x_dt, M, K, ldx, xq, xs, s);
   if (qc) return qc;
-  return fp8_gemm(reinterpret_cast<const uint8_t *>(W), reinterpret_cast<const float *>(Ws), xq, xs, reinterpret_cast<void *>(Y),
-                  y_dt, M, N, K, ldy, reinterpret_cast<const void *>(RS), reinterpret_cast<float *>(ws + front), ws_bytes - front,
-                  as_stream(stream));
+  return fp8_gemm(a, reinterpret_cast<float *>(ws + front), ws_bytes - front, s);
 }

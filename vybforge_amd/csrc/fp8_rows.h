@@ -1,4 +1,4 @@
-// Few rows of X (up to 64) times an e4m3 matrix: W streamed once from memory into registers, gfx950.
+// Few rows of X times an e4m3 matrix: W streamed once from memory into registers, gfx950.
 //
 // A workgroup takes 16 NF rows of W and all rows of X; its NW waves deal the K blocks among themselves (wave w: blocks w, w + NW,
 // ..), so that together they read a row's bytes in order, and each sums its blocks' products in registers; the waves' sums are
