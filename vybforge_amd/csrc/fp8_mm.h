@@ -122,7 +122,7 @@ __device__ __forceinline__ void fp8_put4(const Fp8MmArgs &a, int64_t at, int lef
     if (i < left) store_elem<DT>(a.Y, a.RS, at + i, v[i]);
 }
 
-// What becomes of a tile's sums: acc[n][m][i] is row m0 + 16 (MF wm + m) + (lane & 15), column n0 + 16 (NF wn + n) + 4 (lane / 16) + i
+// What becomes of a tile's sums: acc[n][m][i] is row m0 + 16 (WM m + wm) + (lane & 15), column n0 + 16 (NF wn + n) + 4 (lane / 16) + i
 // (GATE_UP: fragments n < NF / 2 gate, the others up, of columns n0 + 8 NF wn + ..). red: LDS for WN x BM words (GATE_UP).
 template <int MF, int NF, int WM, int WN, int MODE>
 __device__ __forceinline__ void fp8_store(const Fp8MmArgs &a, f4 (&acc)[NF][MF], int m0, int m_end, int n0, uint32_t *red,
@@ -161,11 +161,11 @@ __device__ __forceinline__ void fp8_store(const Fp8MmArgs &a, f4 (&acc)[NF][MF],
     __syncthreads();
     if (lane < 16)
 #pragma unroll
-      for (int m = 0; m < MF; ++m) red[wn * BM + (wm * MF + m) * 16 + lane] = top[m];
+      for (int m = 0; m < MF; ++m) red[wn * BM + (WM * m + wm) * 16 + lane] = top[m];
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < MF; ++m) {
-      const int r = (wm * MF + m) * 16 + (lane & 15);
+      const int r = (WM * m + wm) * 16 + (lane & 15);
       uint32_t t = 0;
 #pragma unroll
       for (int w = 0; w < WN; ++w) t = red[w * BM + r] > t ? red[w * BM + r] : t;
@@ -183,7 +183,7 @@ __device__ __forceinline__ void fp8_store(const Fp8MmArgs &a, f4 (&acc)[NF][MF],
   } else if constexpr (MODE == FP8_DOWN) {
 #pragma unroll
     for (int m = 0; m < MF; ++m) {
-      const int row = m0 + (wm * MF + m) * 16 + (lane & 15);
+      const int row = m0 + (WM * m + wm) * 16 + (lane & 15);
       if (row >= m_end) continue;
       float *y = static_cast<float *>(a.Y) + static_cast<int64_t>(row) * a.ldy;
 #pragma unroll
@@ -197,7 +197,7 @@ __device__ __forceinline__ void fp8_store(const Fp8MmArgs &a, f4 (&acc)[NF][MF],
       constexpr int DT = decltype(dt)::value;
 #pragma unroll
       for (int m = 0; m < MF; ++m) {
-        const int row = m0 + (wm * MF + m) * 16 + (lane & 15);
+        const int row = m0 + (WM * m + wm) * 16 + (lane & 15);
         const int64_t at = split * a.split_stride + static_cast<int64_t>(row) * a.ldy + n0 + 16 * wn * NF + g4;
 #pragma unroll
         for (int n = 0; n < NF; ++n) {
@@ -214,6 +214,18 @@ __device__ __forceinline__ void fp8_store(const Fp8MmArgs &a, f4 (&acc)[NF][MF],
       default: rows(std::integral_constant<int, VYBDQ_F64>{}); break;
     }
   }
+}
+
+// Unit u of the experts' tiles: its tile's list entry, column tile n and row tile m. The units of one expert take its row tiles
+// side by side, columns by columns: they run at the same time on one XCD and share its W (bytes from beyond the L2 at 4096 tokens,
+// 256 experts of 6144 x 2048: gate and up 10.8 -> 6.5 GB).
+__device__ __forceinline__ int4 fp8_expert_unit(const Fp8MmArgs &a, int u, int BM, int &n, int &m) {
+  const int t = u / a.n_tiles;
+  const int4 q = a.tiles[t];
+  const int c = (q.z - q.y + BM - 1) / BM, i = u - (t - q.w) * a.n_tiles;
+  n = i / c;
+  m = i - n * c;
+  return q;
 }
 
 // Tiles of BM = 16 MF WM rows of X by BN = 16 NF WN rows of W, a K step of one block, WM x WN waves of 16 MF x 16 NF, both
@@ -243,11 +255,11 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_mm(const Fp8MmArgs a) {
     n0 = u / a.m_tiles * BN;
     m_end = a.M;
   } else {
-    const int t = u / a.n_tiles;
-    if (t >= *a.ntiles) return;
-    n0 = (u - t * a.n_tiles) * (DUAL ? 128 : BN);
-    const int4 tile = a.tiles[t];
-    m0 = tile.y + tile.w * BM;
+    if (u >= *a.ntiles * a.n_tiles) return;
+    int n, m;
+    const int4 tile = fp8_expert_unit(a, u, BM, n, m);
+    n0 = n * (DUAL ? 128 : BN);
+    m0 = tile.y + m * BM;
     m_end = tile.z;
     if (tile.x < 0) {
       W = a.Ss;
@@ -322,7 +334,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_mm(const Fp8MmArgs a) {
   const float *wsp = Ws + static_cast<int64_t>(nb) * nk, *wsp2 = DUAL ? W2s + static_cast<int64_t>(nb) * nk : nullptr;
   static_assert(DUAL || 128 % (16 * NF) == 0, "a wave's rows of W lie in one block");
   const int lo = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) * 16);  // chunk lane >> 4; the other is at lo ^ 64
-  const int xo = wm * 16 * MF * 128, wo = (BM + wn * 16 * NF) * 128, so = (BM + BN) * 128 + (wm * 16 * MF + (lane & 15)) * 4;
+  const int xo = wm * 2048, wo = (BM + wn * 16 * NF) * 128, so = (BM + BN) * 128 + (wm * 16 + (lane & 15)) * 4;
   auto frag = [&](const char *p) {
     const u4 p0 = *reinterpret_cast<const u4 *>(p + lo), p1 = *reinterpret_cast<const u4 *>(p + (lo ^ 64));
     i8v f;
@@ -353,8 +365,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_mm(const Fp8MmArgs a) {
     for (int n = 0; n < NF; ++n) wf[n] = frag(buf + wo + 2048 * n);
 #pragma unroll
     for (int m = 0; m < MF; ++m) {
-      const i8v xf = frag(buf + xo + 2048 * m);
-      const float xs = *reinterpret_cast<const float *>(buf + so + 64 * m);
+      const i8v xf = frag(buf + xo + 2048 * WM * m);
+      const float xs = *reinterpret_cast<const float *>(buf + so + 64 * WM * m);
       const float s0 = xs * w0, s1 = xs * w1;
 #pragma unroll
       for (int n = 0; n < NF; ++n) {
@@ -405,7 +417,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
   constexpr int SB = (BM + 63) / 64 * 256, STAGE = (BM + BN) * 128 + SB;
   constexpr int RL = (BM + BN) / 8, PER = RL / NW, XPER = BM / 8 / NW;  // loads of 8 rows: to a stage, to a wave, of them of X
   constexpr bool DUAL = MODE == FP8_GATE_UP, GATHER = MODE == FP8_GATE_UP;
-  static_assert(MF >= 4 && MF % 2 == 0 && RL % NW == 0 && BM / 8 % NW == 0 && BM / 64 <= NW, "tile");
+  constexpr bool ONE = HALF || MODE != FP8_DENSE;  // a fragment of X at a time, or (dense, e4m3) the last two at once
+  static_assert(MF >= 4 && MF % 2 == 0 && (!ONE || MF == 4) && RL % NW == 0 && BM / 8 % NW == 0 && BM / 64 <= NW, "tile");
   static_assert(!DUAL || (BN == 256 && NF % 2 == 0), "a tile of gate and up holds one block of 128 columns of each");
   static_assert(DUAL || 128 % (16 * NF) == 0, "a wave's rows of W lie in one block");
   static_assert(PER * (ST - 1) <= 63, "loads that vmcnt can count");
@@ -428,7 +441,10 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
                static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(q >> 32) & 0xffffu)),
                static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(bytes)))};
   };
-  auto srd_of = [](const Buf &b) { return srd_t{b.lo, b.hi, b.bytes, 0x00027000u}; };
+  auto srd_of = [](const Buf &b) {
+    return srd_t{static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(b.lo)), static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(b.hi)),
+                 static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(b.bytes)), 0x00027000u};
+  };
   // the tile to compute: rows m0 .. m_end, columns n0 .., scales of this wave's rows of W
   struct Place {
     int m0, m_end, n0, nk, split;  // (blocks of K of this unit)
@@ -446,8 +462,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
     off[i] = static_cast<uint32_t>(r) * static_cast<uint32_t>(a.K) + 16 * c;
   }
   const uint32_t s_on = __builtin_amdgcn_readfirstlane(wave < BM / 64 || wave == 0 ? ~0u : 0u);
-  // unit u: splits of K outermost; dense tiles in groups of 8 tiles of rows, columns by columns; experts' tiles in list order,
-  // columns inside
+  // unit u: splits of K outermost; dense tiles in groups of 8 tiles of rows, columns by columns; experts' tiles:
+  // fp8_expert_unit
   auto tile_at = [&](int u, Tile &f) {
     Place t;
     const uint8_t *W = a.W, *W2 = a.W2;
@@ -469,11 +485,11 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
       t.m0 = (8 * g + r - n * gm) * BM;
       t.m_end = a.M;
     } else {
-      const int e = u / a.n_tiles;
-      n = u - e * a.n_tiles;
-      const int4 q = a.tiles[e];
+      int m;
+      const int4 q = fp8_expert_unit(a, u, BM, n, m);
+      n = __builtin_amdgcn_readfirstlane(n);
       const int x = __builtin_amdgcn_readfirstlane(q.x);
-      t.m0 = __builtin_amdgcn_readfirstlane(q.y + q.w * BM);
+      t.m0 = __builtin_amdgcn_readfirstlane(q.y + m * BM);
       t.m_end = __builtin_amdgcn_readfirstlane(q.z);
       if (x < 0) {
         W = a.Ss;
@@ -530,7 +546,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
              __builtin_amdgcn_readfirstlane(s_on));
   };
   const int lo = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) * 16);
-  const int xo = wm * 16 * MF * 128, wo = (BM + wn * 16 * NF) * 128, so = (BM + BN) * 128 + (wm * 16 * MF + (lane & 15)) * 4;
+  const int xo = wm * 2048, wo = (BM + wn * 16 * NF) * 128, so = (BM + BN) * 128 + (wm * 16 + (lane & 15)) * 4;
   auto frag = [&](const char *p) {
     const u4 p0 = *reinterpret_cast<const u4 *>(p + lo), p1 = *reinterpret_cast<const u4 *>(p + (lo ^ 64));
     i8v f;
@@ -541,7 +557,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
     }
     return f;
   };
-  auto scale_of = [&](const char *p, int m) { return *reinterpret_cast<const float *>(p + so + 64 * m); };
+  auto x_of = [&](const char *p, int m) { return frag(p + xo + 2048 * WM * m); };
+  auto scale_of = [&](const char *p, int m) { return *reinterpret_cast<const float *>(p + so + 64 * WM * m); };
   auto add = [&](f4 &c, const f4 &v, float s) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) c[i] = fmaf(v[i], s, c[i]);
@@ -574,9 +591,14 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
   for (int n = 0; n < NF; ++n) wf[n] = frag(smem + wo + 2048 * n);
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    xf[m] = frag(smem + xo + 2048 * m);
+    xf[m] = x_of(smem, m);
     xs[m] = scale_of(smem, m);
   }
+  // HALF: the converted fragments, all of W (made at a step's start) and one of X (made ahead)
+  h8 wh[HALF ? NF : 1][4], xh[4];
+  if constexpr (HALF)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) xh[j] = fp8_to_h8(xf[0][2 * j], xf[0][2 * j + 1]);
   uint32_t sb = 0;  // byte offset of the current stage
   for (; u < units; u += G) {
     f4 acc[NF][MF], t[NF], tb = {0.f, 0.f, 0.f, 0.f};
@@ -597,16 +619,116 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
     const float *ws = at.ws, *ws2 = at.ws2;
     float w0 = uniform_load(ws, 0), w1 = DUAL ? uniform_load(ws2, 0) : 0.f;
     const int nk = at.nk;
-    for (int k = 0; k < nk; ++k) {
+    // step k with the first MA of MF fragments of X
+    auto step = [&](auto ma, int k) {
+      constexpr int MA = decltype(ma)::value;
       const uint32_t sn = sb + STAGE == ST * STAGE ? 0 : sb + STAGE;
       const char *buf = smem + sb, *nbuf = smem + sn;
       const int kn = k + 1 < nk ? k + 1 : k;
       const float w0n = uniform_load(ws, kn), w1n = DUAL ? uniform_load(ws2, kn) : 0.f;
       auto scales = [&](int m) { return Sc{xs[m & 3] * w0, DUAL ? xs[m & 3] * w1 : 0.f}; };
+      // the stage to load: ST steps on, from the next tile once this one's are all on their way
+      const int kk = k + ST < nk ? k + ST : k + ST - nk;
+      auto turn = [&] {
+        const bool now = k + ST == nk;
+        auto pick = [&](Buf &b, const Buf &n) {
+          b.lo = now ? n.lo : b.lo;
+          b.hi = now ? n.hi : b.hi;
+          b.bytes = now ? n.bytes : b.bytes;
+        };
+        pick(from.w, next.w);
+        if constexpr (DUAL) {
+          from.w2.lo = now ? next.w2.lo : from.w2.lo;
+          from.w2.hi = now ? next.w2.hi : from.w2.hi;
+        }
+        if constexpr (GATHER) {
+#pragma unroll
+          for (int i = 0; i < XPER; ++i) from.xoff[i] = now ? next.xoff[i] : from.xoff[i];
+          from.soff = now ? next.soff : from.soff;
+        } else {
+          pick(from.x, next.x);
+          pick(from.s, next.s);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave has read all of the stage
+        wait_loads<PER *(ST - 2)>();  // its loads of the next one have arrived (its load of scales, which some waves lack, not counted)
+        barrier();
+      };
+      if constexpr (ONE) {
+        // Fragment by fragment: while the matrix instructions of one run, the last one's products are added and (HALF: 16 cycles
+        // each, 4 to issue) the next one is converted, three vector instructions to each of them. Fragment m + 2, or the next
+        // step's, is read meanwhile; the barrier stands before the last two.
+        i8v xr[MA + 2];
+        float xv[MA + 2];
+        xr[0] = xf[0];
+        xr[1] = xf[1];
+        xv[0] = xs[0];
+        xv[1] = xs[1];
+#pragma unroll
+        for (int m = 0; m < MA; ++m) {
+          if (m == (MA > 2 ? MA - 2 : 0)) turn();
+          if (MA == 1) {  // (what was read ahead as fragment 1 is not the next step's first)
+            xr[1] = x_of(nbuf, 0);
+            xv[1] = scale_of(nbuf, 0);
+          }
+          xr[m + 2] = m + 2 < MA ? x_of(buf, m + 2) : x_of(nbuf, m + 2 - MA);
+          xv[m + 2] = m + 2 < MA ? scale_of(buf, m + 2) : scale_of(nbuf, m + 2 - MA);
+          if (HALF && m == 0)
+#pragma unroll
+            for (int n = 0; n < NF; ++n)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) wh[HALF ? n : 0][j] = fp8_to_h8(wf[n][2 * j], wf[n][2 * j + 1]);
+          const Sc s = {xv[m] * w0, DUAL ? xv[m] * w1 : 0.f};
+          if constexpr (HALF) {
+#pragma unroll
+            for (int n = 0; n < NF; ++n) {
+              add(acc[n][(m + MA - 1) % MA], t[n], of(sp, n));
+              t[n] = f4{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int n = 0; n < NF; ++n) t[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[HALF ? n : 0][j], xh[j], t[n], 0, 0, 0);
+            h8 xn[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) xn[j] = fp8_to_h8(xr[m + 1][2 * j], xr[m + 1][2 * j + 1]);
+            if (m == MA - 1)
+#pragma unroll
+              for (int n = 0; n < NF; ++n) wf[n] = frag(nbuf + wo + 2048 * n);
+#pragma unroll
+            for (int i = 0; i < 4 * NF; ++i) {
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
+              __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);  // three vector instructions
+            }
+            hold();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) xh[j] = xn[j];
+          } else {
+#pragma unroll
+            for (int n = 0; n < NF; ++n) {
+              add(acc[n][(m + MA - 1) % MA], t[n], of(sp, n));
+              t[n] = fp8_block<false>(wf[n], xr[m]);
+              if (m == MA - 1) wf[n] = frag(nbuf + wo + 2048 * n);
+              hold();
+            }
+          }
+          if (m >= MA - 2) {
+            constexpr int HP = MA > 1 ? PER / 2 : 0;
+#pragma unroll
+            for (int i = m < MA - 1 ? 0 : HP; i < (m < MA - 1 ? HP : PER); ++i) issue1(from, kk, lds0 + sb, i);
+            if (m == MA - 1) issue_s(from, kk, lds0 + sb);
+            hold();
+          }
+          sp = s;
+        }
+        xf[0] = xr[MA];
+        xf[1] = xr[MA + 1];
+        xs[0] = xv[MA];
+        xs[1] = xv[MA + 1];
+      } else {
       Sc sc = {0.f, 0.f};
 #pragma unroll
       for (int m = 0; m < MF - 2; ++m) {
-        xf[(m + 2) & 3] = frag(buf + xo + 2048 * (m + 2));
+        xf[(m + 2) & 3] = x_of(buf, m + 2);
         xs[(m + 2) & 3] = scale_of(buf, m + 2);
         const Sc s = scales(m);
 #pragma unroll
@@ -617,44 +739,21 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
             add(acc[NF - 1][MF - 2], t[NF - 1], of(sp, NF - 1));
             add(acc[NF - 1][MF - 1], tb, of(sq, NF - 1));
           }
-          t[n] = fp8_block<HALF>(wf[n], xf[m & 3]);
+          t[n] = fp8_block<false>(wf[n], xf[m & 3]);
           hold();
         }
         sc = s;
       }
       const Sc s6 = scales(MF - 2), s7 = scales(MF - 1);
-      // the stage to load: ST steps on, from the next tile once this one's are all on their way
-      const bool turn = k + ST == nk;
-      auto pick = [&](Buf &b, const Buf &n) {
-        b.lo = turn ? n.lo : b.lo;
-        b.hi = turn ? n.hi : b.hi;
-        b.bytes = turn ? n.bytes : b.bytes;
-      };
-      pick(from.w, next.w);
-      if constexpr (DUAL) {
-        from.w2.lo = turn ? next.w2.lo : from.w2.lo;
-        from.w2.hi = turn ? next.w2.hi : from.w2.hi;
-      }
-      if constexpr (GATHER) {
-#pragma unroll
-        for (int i = 0; i < XPER; ++i) from.xoff[i] = turn ? next.xoff[i] : from.xoff[i];
-        from.soff = turn ? next.soff : from.soff;
-      } else {
-        pick(from.x, next.x);
-        pick(from.s, next.s);
-      }
-      const int kk = k + ST < nk ? k + ST : k + ST - nk;
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave has read all of the stage
-      wait_loads<PER *(ST - 2)>();  // its loads of the next one have arrived (its load of scales, which some waves lack, not counted)
-      barrier();
+      turn();
 #pragma unroll
       for (int n = 0; n < NF; ++n) {
         if (n == 0) {
-          xf[MF & 3] = frag(nbuf + xo);
+          xf[MF & 3] = x_of(nbuf, 0);
           xs[MF & 3] = scale_of(nbuf, 0);
         }
         if (n == (NF > 1 ? 1 : 0)) {
-          xf[(MF + 1) & 3] = frag(nbuf + xo + 2048);
+          xf[(MF + 1) & 3] = x_of(nbuf, 1);
           xs[(MF + 1) & 3] = scale_of(nbuf, 1);
         }
         add(acc[n][MF - 3], t[n], of(sc, n));
@@ -662,8 +761,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
           add(acc[n - 1][MF - 2], t[n - 1], of(s6, n - 1));
           add(acc[n - 1][MF - 1], tb, of(s7, n - 1));
         }
-        t[n] = fp8_block<HALF>(wf[n], xf[(MF - 2) & 3]);
-        tb = fp8_block<HALF>(wf[n], xf[(MF - 1) & 3]);
+        t[n] = fp8_block<false>(wf[n], xf[(MF - 2) & 3]);
+        tb = fp8_block<false>(wf[n], xf[(MF - 1) & 3]);
         wf[n] = frag(nbuf + wo + 2048 * n);
 #pragma unroll
         for (int i = n * PER / NF; i < (n + 1) * PER / NF; ++i) issue1(from, kk, lds0 + sb, i);
@@ -680,12 +779,30 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
       }
       sp = s6;
       sq = s7;
+      }
       w0 = w0n;
       w1 = w1n;
       sb = sn;
+    };
+    auto steps = [&](auto ma) {
+      for (int k = 0; k < nk; ++k) step(ma, k);
+      if constexpr (ONE)
+#pragma unroll
+        for (int n = 0; n < NF; ++n) add(acc[n][decltype(ma)::value - 1], t[n], of(sp, n));
+    };
+    if constexpr (MODE != FP8_DENSE) {  // experts' tiles are often not full: no instructions for fragments that no row is in
+      const int rows = __builtin_amdgcn_readfirstlane(at.m_end - at.m0);
+      if (rows > 3 * 16 * WM) steps(std::integral_constant<int, 4>{});
+      else if (rows > 2 * 16 * WM) steps(std::integral_constant<int, 3>{});
+      else if (rows > 16 * WM) steps(std::integral_constant<int, 2>{});
+      else steps(std::integral_constant<int, 1>{});
+    } else {
+      steps(std::integral_constant<int, MF>{});
     }
-    add(acc[NF - 1][MF - 2], t[NF - 1], of(sp, NF - 1));
-    add(acc[NF - 1][MF - 1], tb, of(sq, NF - 1));
+    if constexpr (!ONE) {
+      add(acc[NF - 1][MF - 2], t[NF - 1], of(sp, NF - 1));
+      add(acc[NF - 1][MF - 1], tb, of(sq, NF - 1));
+    }
     fp8_store<MF, NF, WM, WN, MODE>(a, acc, at.m0, at.m_end, at.n0, reinterpret_cast<uint32_t *>(smem + ST * STAGE), at.split);
     at = then;
   }

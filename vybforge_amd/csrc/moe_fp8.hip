@@ -10,6 +10,7 @@
 // epilogue (k_fp8_mm<.., FP8_GATE_UP>: float32 gate and up never leave registers), down (FP8_DOWN), the weighted sum.
 #include "fp8_mm.h"
 #include "route_groups.h"
+#include <cstdlib>
 
 namespace vybdq {
 
@@ -79,6 +80,7 @@ template <int MODE, bool HALF>
 static int moe_fp8_mm(int BM, Fp8MmArgs &a, int64_t tiles, hipStream_t s) {
   a.n_tiles = MODE == FP8_GATE_UP ? a.N / 128 : (a.N + 255) / 256;
   const int64_t units = tiles * a.n_tiles;
+  if (BM == 64 && a.KB >= 3) return fp8_pipe_launch<4, 2, 1, 8, 3, MODE, HALF>(a, units, s);
   if (BM == 128 && a.KB >= 3) return fp8_pipe_launch<4, 4, 2, 4, 3, MODE, HALF>(a, units, s);
   if (BM == 16) return fp8_mm_launch<1, 2, 1, 8, 4, MODE, HALF>(a, units, s);
   if (BM == 64) return fp8_mm_launch<4, 4, 1, 4, 3, MODE, HALF>(a, units, s);
@@ -127,7 +129,7 @@ extern "C" int vybdq_moe_forward_fp8(uint64_t x, int x_dt, uint64_t logits, int 
   rc = route_groups_launch(r, s);
   if (rc) return rc;
   const int64_t n = T * topk, hit = E < n ? E : n;
-  const int BM = n <= 8 * hit ? 16 : n <= 64 * hit ? 64 : 128;
+  int BM = n <= 8 * hit ? 16 : n <= 64 * hit ? 64 : 128; if (const char *e = tuning_env("VYBDQ_MOE_FP8_BM")) BM = atoi(e); const char *eh = tuning_env("VYBDQ_MOE_FP8_HALF"); const bool half = !eh || eh[0] != '0';
   rc = moe_bucket(r.idx, T, E, topk, BM, shared, m.pos, m.row_map, m.tiles, m.ntiles, s);
   if (rc) return rc;
   const int64_t tiles = moe_tiles_bound(T, E, topk, BM);
@@ -156,7 +158,7 @@ extern "C" int vybdq_moe_forward_fp8(uint64_t x, int x_dt, uint64_t logits, int 
   g.H = m.aq;
   g.Hs = m.as;
   g.limit = static_cast<float>(limit);
-  rc = moe_fp8_mm<FP8_GATE_UP, true>(BM, g, tiles, s);
+  rc = half ? moe_fp8_mm<FP8_GATE_UP, true>(BM, g, tiles, s) : moe_fp8_mm<FP8_GATE_UP, false>(BM, g, tiles, s);
   if (rc) return rc;
   Fp8MmArgs d = g;
   d.X = m.aq;
