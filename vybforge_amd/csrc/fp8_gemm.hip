@@ -155,7 +155,6 @@ static Fp8MmArgs fp8_args(const uint8_t *W, const float *Ws, const uint8_t *Xq, 
   a.K = static_cast<int>(K);
   a.KB = static_cast<int>((K + 127) / 128);
   a.xs_row = a.KB;
-  a.xs_block = 1;
   a.x_rows = M;
   a.Y = Y;
   a.ydt = y_dt;

@@ -15,7 +15,7 @@ enum { FP8_DENSE = 0, FP8_GATE_UP = 1, FP8_DOWN = 2 };
 struct Fp8MmArgs {
   const uint8_t *X, *W, *W2;       // X [M][K]; W [N][K] (experts: of expert 0); W2: up (GATE_UP)
   const float *Xs, *Ws, *W2s;
-  int64_t xs_row, xs_block;        // elements from one row's scale of X to the next's, and from one block's
+  int64_t xs_row;                  // elements from one row's scales of X to the next's
   int64_t x_rows;                  // rows of X
   const uint8_t *Ss, *S2;          // the shared expert's W, W2
   const float *Sss, *S2s;
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_mm(const Fp8MmArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < SPER; ++i)
-      lds_dma4(ssrc[i] + k * a.xs_block, buf + (BM + BN) * 128 + ((wave + NW * i) * 256) % SB);
+      lds_dma4(ssrc[i] + k, buf + (BM + BN) * 128 + ((wave + NW * i) * 256) % SB);
   };
 
   f4 acc[NF][MF];
@@ -399,13 +399,13 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_mm(const Fp8MmArgs a) {
 
 typedef uint32_t srd_t __attribute__((ext_vector_type(4)));
 
-// 16 bytes a lane (4: only with `on` all ones) from buffer r to LDS: lane L's to byte address lds + 16 L (+ 4 L).
+// 16 bytes a lane from buffer r to LDS: lane L's to byte address lds + 16 L. _if: only with `on` all ones (else 0), without a branch.
 __device__ __forceinline__ void srd_dma16(const srd_t &r, uint32_t voff, uint32_t soff, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(r), "s"(soff), "s"(lds)
                : "memory", "m0");
 }
-__device__ __forceinline__ void srd_dma4(const srd_t &r, uint32_t voff, uint32_t soff, uint32_t lds, uint32_t on) {
-  asm volatile("s_mov_b32 m0, %3\n\ts_mov_b32 exec_lo, %4\n\ts_mov_b32 exec_hi, %4\n\tbuffer_load_dword %0, %1, %2 offen lds\n\t"
+__device__ __forceinline__ void srd_dma16_if(const srd_t &r, uint32_t voff, uint32_t soff, uint32_t lds, uint32_t on) {
+  asm volatile("s_mov_b32 m0, %3\n\ts_mov_b32 exec_lo, %4\n\ts_mov_b32 exec_hi, %4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds\n\t"
                "s_mov_b64 exec, -1" ::"v"(voff), "s"(r), "s"(soff), "s"(lds), "s"(on)
                : "memory", "m0");
 }
@@ -414,14 +414,14 @@ template <int MF, int NF, int WM, int WN, int ST, int MODE, bool HALF>
 __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int BM = 16 * MF * WM, BN = 16 * NF * WN, NW = WM * WN;
-  constexpr int SB = (BM + 63) / 64 * 256, STAGE = (BM + BN) * 128 + SB;
+  constexpr int STAGE = (BM + BN) * 128, SCALES = ST * STAGE, SQ = 16 * BM;  // bytes: of a stage, before the scales, of four steps' scales
   constexpr int RL = (BM + BN) / 8, PER = RL / NW, XPER = BM / 8 / NW;  // loads of 8 rows: to a stage, to a wave, of them of X
   constexpr bool DUAL = MODE == FP8_GATE_UP, GATHER = MODE == FP8_GATE_UP;
   constexpr bool ONE = HALF || MODE != FP8_DENSE;  // a fragment of X at a time, or (dense, e4m3) the last two at once
   static_assert(MF >= 4 && MF % 2 == 0 && (!ONE || MF == 4) && RL % NW == 0 && BM / 8 % NW == 0 && BM / 64 <= NW, "tile");
   static_assert(!DUAL || (BN == 256 && NF % 2 == 0), "a tile of gate and up holds one block of 128 columns of each");
   static_assert(DUAL || 128 % (16 * NF) == 0, "a wave's rows of W lie in one block");
-  static_assert(PER * (ST - 1) <= 63, "loads that vmcnt can count");
+  static_assert(ST <= 4 && PER * (ST - 1) <= 63, "loads that vmcnt can count");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int wm = wave / WN, wn = wave % WN;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)smem));
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
     }
     off[i] = static_cast<uint32_t>(r) * static_cast<uint32_t>(a.K) + 16 * c;
   }
-  const uint32_t s_on = __builtin_amdgcn_readfirstlane(wave < BM / 64 || wave == 0 ? ~0u : 0u);
+  const uint32_t s_on = __builtin_amdgcn_readfirstlane(wave < BM / 64 ? ~0u : 0u);  // waves that load scales: 64 rows each
   // unit u: splits of K outermost; dense tiles in groups of 8 tiles of rows, columns by columns; experts' tiles:
   // fp8_expert_unit
   auto tile_at = [&](int u, Tile &f) {
@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
       f.soff = static_cast<uint32_t>(a.row_map[t.m0 + min(sr, rows - 1)]) * static_cast<uint32_t>(a.xs_row * 4);
     } else {
       f.x = buf_of(a.X + static_cast<int64_t>(t.m0) * a.K + 128 * k0, static_cast<int64_t>(rows) * a.K - 128 * k0);
-      f.s = buf_of(a.Xs + t.m0 * a.xs_row + k0 * a.xs_block, 4 * ((rows - 1) * a.xs_row + (nk - 1 - k0) * a.xs_block + 1));
+      f.s = buf_of(a.Xs + t.m0 * a.xs_row + k0, 4 * ((rows - 1) * a.xs_row + nk - k0));
       f.soff = static_cast<uint32_t>(sr) * static_cast<uint32_t>(a.xs_row * 4);
     }
     return t;
@@ -541,12 +541,17 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
       srd_dma16(srd_of(t.w), off[i], 128 * k, l + 1024 * j);
     }
   };
-  auto issue_s = [&](const Tile &t, int k, uint32_t l) {
-    srd_dma4(srd_of(t.s), t.soff, static_cast<uint32_t>(k * a.xs_block * 4), l + (BM + BN) * 128 + wave * 256,
-             __builtin_amdgcn_readfirstlane(s_on));
+  // the scales of steps k .. k + 3 of a tile, at every fourth step: 16 bytes a row (single ones cost an address cycle a row and
+  // step), into the next of four places; what lies behind a tile's last step is not used
+  uint32_t place = 0;
+  auto issue_s = [&](const Tile &t, int k) {
+    const uint32_t on = (k & 3) == 0 ? s_on : 0u;
+    srd_dma16_if(srd_of(t.s), t.soff, static_cast<uint32_t>(4 * k), lds0 + SCALES + place * SQ + wave * 1024,
+                 __builtin_amdgcn_readfirstlane(on));
+    place = (place + ((k & 3) == 0 ? 1 : 0)) & 3;
   };
   const int lo = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) * 16);
-  const int xo = wm * 2048, wo = (BM + wn * 16 * NF) * 128, so = (BM + BN) * 128 + (wm * 16 + (lane & 15)) * 4;
+  const int xo = wm * 2048, wo = (BM + wn * 16 * NF) * 128, so = SCALES + (wm * 16 + (lane & 15)) * 16;
   auto frag = [&](const char *p) {
     const u4 p0 = *reinterpret_cast<const u4 *>(p + lo), p1 = *reinterpret_cast<const u4 *>(p + (lo ^ 64));
     i8v f;
@@ -558,7 +563,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
     return f;
   };
   auto x_of = [&](const char *p, int m) { return frag(p + xo + 2048 * WM * m); };
-  auto scale_of = [&](const char *p, int m) { return *reinterpret_cast<const float *>(p + so + 64 * WM * m); };
+  auto scale_of = [&](uint32_t at, int m) { return *reinterpret_cast<const float *>(smem + at + so + 256 * WM * m); };
   auto add = [&](f4 &c, const f4 &v, float s) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) c[i] = fmaf(v[i], s, c[i]);
@@ -581,7 +586,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
   for (int s = 0; s < ST; ++s) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) issue1(from, s, lds0 + s * STAGE, i);
-    issue_s(from, s, lds0 + s * STAGE);
+    issue_s(from, s);
   }
   wait_loads<PER *(ST - 1)>();
   barrier();
@@ -592,14 +597,14 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     xf[m] = x_of(smem, m);
-    xs[m] = scale_of(smem, m);
+    xs[m] = scale_of(0, m);
   }
   // HALF: the converted fragments, all of W (made at a step's start) and one of X (made ahead)
   h8 wh[HALF ? NF : 1][4], xh[4];
   if constexpr (HALF)
 #pragma unroll
     for (int j = 0; j < 4; ++j) xh[j] = fp8_to_h8(xf[0][2 * j], xf[0][2 * j + 1]);
-  uint32_t sb = 0;  // byte offset of the current stage
+  uint32_t sb = 0, cb = 0;  // byte offsets of the current stage and of its scales among them
   for (; u < units; u += G) {
     f4 acc[NF][MF], t[NF], tb = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -624,6 +629,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
       constexpr int MA = decltype(ma)::value;
       const uint32_t sn = sb + STAGE == ST * STAGE ? 0 : sb + STAGE;
       const char *buf = smem + sb, *nbuf = smem + sn;
+      const uint32_t cn = k + 1 == nk || (k & 3) == 3 ? (((cb / SQ) + 1) & 3) * SQ : cb + 4;
       const int kn = k + 1 < nk ? k + 1 : k;
       const float w0n = uniform_load(ws, kn), w1n = DUAL ? uniform_load(ws2, kn) : 0.f;
       auto scales = [&](int m) { return Sc{xs[m & 3] * w0, DUAL ? xs[m & 3] * w1 : 0.f}; };
@@ -668,56 +674,58 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
           if (m == (MA > 2 ? MA - 2 : 0)) turn();
           if (MA == 1) {  // (what was read ahead as fragment 1 is not the next step's first)
             xr[1] = x_of(nbuf, 0);
-            xv[1] = scale_of(nbuf, 0);
+            xv[1] = scale_of(cn, 0);
           }
           xr[m + 2] = m + 2 < MA ? x_of(buf, m + 2) : x_of(nbuf, m + 2 - MA);
-          xv[m + 2] = m + 2 < MA ? scale_of(buf, m + 2) : scale_of(nbuf, m + 2 - MA);
+          xv[m + 2] = m + 2 < MA ? scale_of(cb, m + 2) : scale_of(cn, m + 2 - MA);
           if (HALF && m == 0)
 #pragma unroll
             for (int n = 0; n < NF; ++n)
 #pragma unroll
               for (int j = 0; j < 4; ++j) wh[HALF ? n : 0][j] = fp8_to_h8(wf[n][2 * j], wf[n][2 * j + 1]);
           const Sc s = {xv[m] * w0, DUAL ? xv[m] * w1 : 0.f};
-          if constexpr (HALF) {
+          // the loads of the stage ST steps on, spread over what is left of the step: issued together they hold up the instructions
+          // behind them until the address unit has taken them all
+          constexpr int SUB = HALF ? 1 : NF, BY = NF / SUB;  // parts of a fragment's products, columns to a part
+          constexpr int LAST = MA > 1 ? 2 : 1, SLOTS = LAST * SUB;
+          h8 xn[HALF ? 4 : 1];
 #pragma unroll
-            for (int n = 0; n < NF; ++n) {
+          for (int p = 0; p < SUB; ++p) {
+#pragma unroll
+            for (int n = p * BY; n < (p + 1) * BY; ++n) {
               add(acc[n][(m + MA - 1) % MA], t[n], of(sp, n));
               t[n] = f4{0.f, 0.f, 0.f, 0.f};
+              if constexpr (!HALF) t[n] = fp8_block<false>(wf[n], xr[m]);
             }
+            if constexpr (HALF) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+              for (int j = 0; j < 4; ++j)
 #pragma unroll
-              for (int n = 0; n < NF; ++n) t[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[HALF ? n : 0][j], xh[j], t[n], 0, 0, 0);
-            h8 xn[4];
+                for (int n = p * BY; n < (p + 1) * BY; ++n) t[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[HALF ? n : 0][j], xh[j], t[n], 0, 0, 0);
+              if (p == SUB - 1)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) xn[j] = fp8_to_h8(xr[m + 1][2 * j], xr[m + 1][2 * j + 1]);
+                for (int j = 0; j < 4; ++j) xn[HALF ? j : 0] = fp8_to_h8(xr[m + 1][2 * j], xr[m + 1][2 * j + 1]);
+#pragma unroll
+              for (int i = 0; i < 4 * BY; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
+                __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);  // three vector instructions
+              }
+            }
             if (m == MA - 1)
 #pragma unroll
-              for (int n = 0; n < NF; ++n) wf[n] = frag(nbuf + wo + 2048 * n);
-#pragma unroll
-            for (int i = 0; i < 4 * NF; ++i) {
-              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
-              __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);  // three vector instructions
-            }
+              for (int n = p * BY; n < (p + 1) * BY; ++n) wf[n] = frag(nbuf + wo + 2048 * n);
             hold();
+            if (m >= MA - LAST) {
+              const int q = (m - (MA - LAST)) * SUB + p;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) xh[j] = xn[j];
-          } else {
-#pragma unroll
-            for (int n = 0; n < NF; ++n) {
-              add(acc[n][(m + MA - 1) % MA], t[n], of(sp, n));
-              t[n] = fp8_block<false>(wf[n], xr[m]);
-              if (m == MA - 1) wf[n] = frag(nbuf + wo + 2048 * n);
+              for (int i = q * PER / SLOTS; i < (q + 1) * PER / SLOTS; ++i) issue1(from, kk, lds0 + sb, i);
+              if (q == SLOTS - 1) issue_s(from, kk);
               hold();
             }
           }
-          if (m >= MA - 2) {
-            constexpr int HP = MA > 1 ? PER / 2 : 0;
+          if constexpr (HALF)
 #pragma unroll
-            for (int i = m < MA - 1 ? 0 : HP; i < (m < MA - 1 ? HP : PER); ++i) issue1(from, kk, lds0 + sb, i);
-            if (m == MA - 1) issue_s(from, kk, lds0 + sb);
-            hold();
-          }
+            for (int j = 0; j < 4; ++j) xh[j] = xn[j];
           sp = s;
         }
         xf[0] = xr[MA];
@@ -729,7 +737,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
 #pragma unroll
       for (int m = 0; m < MF - 2; ++m) {
         xf[(m + 2) & 3] = x_of(buf, m + 2);
-        xs[(m + 2) & 3] = scale_of(buf, m + 2);
+        xs[(m + 2) & 3] = scale_of(cb, m + 2);
         const Sc s = scales(m);
 #pragma unroll
         for (int n = 0; n < NF; ++n) {
@@ -750,11 +758,11 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
       for (int n = 0; n < NF; ++n) {
         if (n == 0) {
           xf[MF & 3] = x_of(nbuf, 0);
-          xs[MF & 3] = scale_of(nbuf, 0);
+          xs[MF & 3] = scale_of(cn, 0);
         }
         if (n == (NF > 1 ? 1 : 0)) {
           xf[(MF + 1) & 3] = x_of(nbuf, 1);
-          xs[(MF + 1) & 3] = scale_of(nbuf, 1);
+          xs[(MF + 1) & 3] = scale_of(cn, 1);
         }
         add(acc[n][MF - 3], t[n], of(sc, n));
         if (n > 0) {
@@ -766,7 +774,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
         wf[n] = frag(nbuf + wo + 2048 * n);
 #pragma unroll
         for (int i = n * PER / NF; i < (n + 1) * PER / NF; ++i) issue1(from, kk, lds0 + sb, i);
-        if (n == NF - 1) issue_s(from, kk, lds0 + sb);
+        if (n == NF - 1) issue_s(from, kk);
         hold();
       }
       if constexpr (MF % 4 != 0) {  // the ring's first places are fragments 0 and 1
@@ -783,6 +791,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
       w0 = w0n;
       w1 = w1n;
       sb = sn;
+      cb = cn;
     };
     auto steps = [&](auto ma) {
       for (int k = 0; k < nk; ++k) step(ma, k);
@@ -792,10 +801,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
     };
     if constexpr (MODE != FP8_DENSE) {  // experts' tiles are often not full: no instructions for fragments that no row is in
       const int rows = __builtin_amdgcn_readfirstlane(at.m_end - at.m0);
-      if (rows > 3 * 16 * WM) steps(std::integral_constant<int, 4>{});
-      else if (rows > 2 * 16 * WM) steps(std::integral_constant<int, 3>{});
-      else if (rows > 16 * WM) steps(std::integral_constant<int, 2>{});
-      else steps(std::integral_constant<int, 1>{});
+      if (rows > 2 * 16 * WM) steps(std::integral_constant<int, 4>{});
+      else steps(std::integral_constant<int, 2>{});
     } else {
       steps(std::integral_constant<int, MF>{});
     }
@@ -803,7 +810,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
       add(acc[NF - 1][MF - 2], t[NF - 1], of(sp, NF - 1));
       add(acc[NF - 1][MF - 1], tb, of(sq, NF - 1));
     }
-    fp8_store<MF, NF, WM, WN, MODE>(a, acc, at.m0, at.m_end, at.n0, reinterpret_cast<uint32_t *>(smem + ST * STAGE), at.split);
+    fp8_store<MF, NF, WM, WN, MODE>(a, acc, at.m0, at.m_end, at.n0, reinterpret_cast<uint32_t *>(smem + SCALES + 4 * SQ), at.split);
     at = then;
   }
   wait_loads<0>();  // (nothing may arrive in LDS that is another workgroup's)
@@ -828,7 +835,7 @@ int fp8_mm_launch(const Fp8MmArgs &a, int64_t units, hipStream_t s) {
 template <int MF, int NF, int WM, int WN, int ST, int MODE, bool HALF>
 int fp8_pipe_launch(const Fp8MmArgs &a, int64_t units, hipStream_t s) {
   constexpr int BM = 16 * MF * WM, BN = 16 * NF * WN;
-  constexpr int LDS = ST * ((BM + BN) * 128 + (BM + 63) / 64 * 256) + (MODE == FP8_GATE_UP ? 4 * WN * BM : 0);
+  constexpr int LDS = ST * (BM + BN) * 128 + 64 * BM + (MODE == FP8_GATE_UP ? 4 * WN * BM : 0);
   static_assert(LDS <= 160 * 1024, "LDS");
   static std::atomic<uint64_t> raised{0};
   static std::atomic<int64_t> resident[64];

@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(64 * NW) k_fp8_rows(const Fp8RowsArgs ra) {
           xs = xs_lds[row * nk + k];
         } else {
           xf = frag(xp[m], k);
-          xs = xsp[m][k * a.xs_block];
+          xs = xsp[m][k];
         }
 #pragma unroll
         for (int n = 0; n < NF; ++n) {

@@ -148,7 +148,6 @@ extern "C" int vybdq_moe_forward_fp8(uint64_t x, int x_dt, uint64_t logits, int 
   g.K = static_cast<int>(H);
   g.KB = static_cast<int>(H / 128);
   g.xs_row = g.KB;
-  g.xs_block = 1;
   g.x_rows = T;
   g.w_stride = I * H;
   g.ws_stride = (I / 128) * (H / 128);
