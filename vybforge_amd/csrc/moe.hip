@@ -373,15 +373,6 @@ int moe_route_bucket(const void *logits, int logits_dt, const float *bias, int64
   return check_launch("moe bucket");
 }
 
-// The bucketing alone (k_moe_bucket_tiles), of rows that a router has written to idx, with the shared expert's rows.
-int moe_bucket(const int *idx, int64_t T, int64_t E, int64_t topk, int BMr, bool shared, int *pos, int *row_map, int4 *tiles,
-               int *ntiles, hipStream_t s) {
-  hipLaunchKernelGGL(k_moe_bucket_tiles, dim3(1), dim3(256), static_cast<size_t>(2 * E) * 4, s, idx, static_cast<int>(T),
-                     static_cast<int>(topk), static_cast<int>(E), BMr, BMr, shared ? 1 : 0, pos, row_map, tiles, ntiles,
-                     static_cast<int4 *>(nullptr), static_cast<int *>(nullptr));
-  return check_launch("moe bucket");
-}
-
 // Upper bound of the row-group list of moe_route_bucket for groups of at most `rows` rows.
 int64_t moe_tiles_bound(int64_t T, int64_t E, int64_t k, int64_t rows) { return moe_max_tiles(T, E, k, rows); }
 

@@ -8,15 +8,85 @@
 // On the stream, no host synchronisation: quantizer, router, bucketing (rows by expert and the list of their m-tiles; the
 // shared expert's rows and tiles are one more expert's), gate and up of all rows with the activation and its quantizer as
 // epilogue (k_fp8_mm<.., FP8_GATE_UP>: float32 gate and up never leave registers), down (FP8_DOWN), the weighted sum.
+#include "fp8_load.h"
 #include "fp8_mm.h"
 #include "route_groups.h"
-#include <cstdlib>
 
 namespace vybdq {
 
-int moe_bucket(const int *idx, int64_t T, int64_t E, int64_t topk, int BMr, bool shared, int *pos, int *row_map, int4 *tiles,
-               int *ntiles, hipStream_t s);
 int64_t moe_tiles_bound(int64_t T, int64_t E, int64_t k, int64_t rows);
+
+// Where rows and tiles go: pos (token, slot) -> row, row -> token, the list of m-tiles.
+struct MoeFp8Lists {
+  int *pos, *row_map, *ntiles;
+  int4 *tiles;
+};
+
+// Few tokens (at most 64 rows) in one launch: workgroup 0 routes them and lists rows and tiles, the others quantize x (one token of
+// 6144 over 256 experts: 10 us against 18 of three launches).
+template <int LDT, int ENT>
+__global__ void __launch_bounds__(256) k_moe_fp8_front(const RouteArgs r, const void *__restrict__ x, int x_dt, int H,
+                                                       uint8_t *__restrict__ xq, float *__restrict__ xs, int BM, int shared,
+                                                       const MoeFp8Lists l) {
+  __shared__ int idx_lds[64];
+  if (blockIdx.x == 0) {
+    for (int t = threadIdx.x >> 6; t < r.T; t += 4) route_groups_wave<LDT, ENT>(r, t, idx_lds);
+    __syncthreads();
+    if (threadIdx.x < 64) bucket_rows_wave(idx_lds, r.T, r.topk, BM, BM, shared, l.pos, l.row_map, l.tiles, l.ntiles, nullptr, nullptr);
+    return;
+  }
+  const int64_t u = static_cast<int64_t>(blockIdx.x - 1) * 16 + (threadIdx.x >> 4);  // 16 lanes to a block of 128 (H is whole blocks)
+  if (u >= static_cast<int64_t>(r.T) * (H >> 7)) return;
+  const int64_t at = u * 128 + (threadIdx.x & 15) * 8;
+  float v[8], sc;
+  VYBDQ_DISPATCH_IN(x_dt, DT, fp8_load8<DT>(x, at, v));
+  *reinterpret_cast<u2 *>(xq + at) = fp8_quant8(v, sc);
+  if ((threadIdx.x & 15) == 0) xs[u] = sc;
+}
+
+// Many tokens, one workgroup: rows per expert, the first row and tile of each (thread e: expert e), then every (token, slot)'s row.
+// A row's place among its expert's comes from an atomic cursor: no result depends on it, each row is computed from its own token
+// alone and added through pos. 32768 rows: 21 us (70 with 256 threads).
+__global__ void __launch_bounds__(1024) k_moe_fp8_bucket(const int *__restrict__ idx, int T, int topk, int E, int BM, int shared,
+                                                         const MoeFp8Lists l) {
+  __shared__ int cnt[1024], wave_rows[16], wave_tiles[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = T * topk;
+  cnt[tid] = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += 1024) atomicAdd(&cnt[idx[i]], 1);
+  __syncthreads();
+  const int c = tid < E ? cnt[tid] : 0, mt = (c + BM - 1) / BM;
+  int r = c, t = mt;  // inclusive sums over the wave, then over the waves before
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int a = __shfl_up(r, d), b = __shfl_up(t, d);
+    r += lane >= d ? a : 0;
+    t += lane >= d ? b : 0;
+  }
+  if (lane == 63) {
+    wave_rows[wave] = r;
+    wave_tiles[wave] = t;
+  }
+  __syncthreads();
+  const int tsh = shared ? (T + BM - 1) / BM : 0;
+  int r0 = r - c, t0 = tsh + t - mt;
+  for (int w = 0; w < wave; ++w) {
+    r0 += wave_rows[w];
+    t0 += wave_tiles[w];
+  }
+  for (int m = 0; m < mt; ++m) l.tiles[t0 + m] = make_int4(tid, r0, r0 + c, m);
+  if (tid == 1023) *l.ntiles = t0 + mt;
+  cnt[tid] = r0;  // (this thread's own count was read above): the expert's cursor
+  for (int j = tid; j < tsh; j += 1024) l.tiles[j] = make_int4(-1, n, n + T, j);
+  if (shared)
+    for (int i = tid; i < T; i += 1024) l.row_map[n + i] = i;
+  __syncthreads();
+  for (int i = tid; i < n; i += 1024) {
+    const int p = atomicAdd(&cnt[idx[i]], 1);
+    l.pos[i] = p;
+    l.row_map[p] = i / topk;
+  }
+}
 
 // out[t][h] = sum over s of w[t, s] rows[pos[t, s]][h] + shared[t][h] in slot order; four columns to a thread.
 template <int ODT>
@@ -124,13 +194,29 @@ extern "C" int vybdq_moe_forward_fp8(uint64_t x, int x_dt, uint64_t logits, int 
   VYBDQ_REQUIRE(ws && ws % 256 == 0 && ws_bytes >= m.bytes, VYBDQ_ERR_WORKSPACE,
                 "workspace must be 256-byte aligned and of vybdq_moe_fp8_workspace_size bytes");
   hipStream_t s = as_stream(stream);
-  rc = fp8_quant_rows(reinterpret_cast<const void *>(x), x_dt, T, H, H, m.xq, m.xs, s);
-  if (rc) return rc;
-  rc = route_groups_launch(r, s);
-  if (rc) return rc;
+  // rows to a tile: 16 while the experts hit have 8 each in the mean, 128 from 64 on (256 experts of 6144 x 2048, 8 to a token: 48
+  // tokens 968 us with 16, 1005 with 64; 512 tokens 1575 with 64, 1739 with 128; 4096 tokens 4113 / 3909)
   const int64_t n = T * topk, hit = E < n ? E : n;
-  int BM = n <= 8 * hit ? 16 : n <= 64 * hit ? 64 : 128; if (const char *e = tuning_env("VYBDQ_MOE_FP8_BM")) BM = atoi(e); const char *eh = tuning_env("VYBDQ_MOE_FP8_HALF"); const bool half = !eh || eh[0] != '0';
-  rc = moe_bucket(r.idx, T, E, topk, BM, shared, m.pos, m.row_map, m.tiles, m.ntiles, s);
+  const int BM = n <= 8 * hit ? 16 : n <= 64 * hit ? 64 : 128;
+  const MoeFp8Lists lists{m.pos, m.row_map, m.ntiles, m.tiles};
+  if (n <= 64 && T <= 8) {
+    const dim3 grid(static_cast<unsigned>(1 + (T * (H / 128) + 15) / 16));
+#define FRONT(LDT)                                                                                                              \
+  VYBDQ_DISPATCH_ROUTE(r, hipLaunchKernelGGL((k_moe_fp8_front<LDT, ENT>), grid, dim3(256), 0, s, r, reinterpret_cast<const void *>(x), x_dt, \
+                                             static_cast<int>(H), m.xq, m.xs, BM, shared ? 1 : 0, lists))
+    if (logits_dt == VYBDQ_F64) FRONT(VYBDQ_F64)
+    else VYBDQ_DISPATCH_IN(logits_dt, LDT, FRONT(LDT))
+#undef FRONT
+    rc = check_launch("moe front");
+  } else {
+    rc = fp8_quant_rows(reinterpret_cast<const void *>(x), x_dt, T, H, H, m.xq, m.xs, s);
+    if (rc) return rc;
+    rc = route_groups_launch(r, s);
+    if (rc) return rc;
+    hipLaunchKernelGGL(k_moe_fp8_bucket, dim3(1), dim3(1024), 0, s, r.idx, static_cast<int>(T), static_cast<int>(topk), static_cast<int>(E),
+                       BM, shared ? 1 : 0, lists);
+    rc = check_launch("moe bucket");
+  }
   if (rc) return rc;
   const int64_t tiles = moe_tiles_bound(T, E, topk, BM);
   Fp8MmArgs g{};
@@ -157,7 +243,9 @@ extern "C" int vybdq_moe_forward_fp8(uint64_t x, int x_dt, uint64_t logits, int 
   g.H = m.aq;
   g.Hs = m.as;
   g.limit = static_cast<float>(limit);
-  rc = half ? moe_fp8_mm<FP8_GATE_UP, true>(BM, g, tiles, s) : moe_fp8_mm<FP8_GATE_UP, false>(BM, g, tiles, s);
+  // gate and up on fp16 instructions: what the e4m3 ones lose (1.4e-5 of a sum's rms) moves one activation in 5000 to the next
+  // code, a hundredth of the output's rms and more where it is a large one (4096 tokens: 3.9 ms, with e4m3 instructions 2.9)
+  rc = moe_fp8_mm<FP8_GATE_UP, true>(BM, g, tiles, s);
   if (rc) return rc;
   Fp8MmArgs d = g;
   d.X = m.aq;
