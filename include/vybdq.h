@@ -610,15 +610,16 @@ int vybdq_kv_status(void);
 
    vybdq_quant_fp8: X (x_dt F32, F16 or BF16, row stride ldx in elements) to Xq, Xs. Scale = 2^e with the least e in -100 .. 120
    for which every |x| of the block is at most 448 * 2^e, code = e4m3(x / scale) to nearest, ties to even (one rounding: the
-   division is exact). A block with an infinity or NaN has the scale NaN. Rows of X and Xq 16-byte aligned;
-   M ceil(K / 128) below 2^28. */
+   division is exact). A block with an infinity or NaN has the scale NaN. Rows of X and Xq 16-byte aligned; Xq and Xs must not
+   overlap X; M ceil(K / 128) below 2^28. */
 int vybdq_quant_fp8(uint64_t X, int x_dt, int64_t ldx, uint64_t Xq, uint64_t Xs, int64_t M, int64_t K, uint64_t stream);
 
 /* Y [M][N] (y_dt F32, F16, BF16 or F64; row stride ldy, 0 = N) = RS + sum over blocks b of Xs[m][b] Ws[n / 128][b] times the
    sum of Xq W over the block's k; RS: as Y (its row stride too) or 0. Scales may be any float32. Products are exact, sums
    over a block and over blocks are float32; for F16 and BF16 outputs a block's sum comes from the e4m3 matrix
    instruction, which aligns its 128 products to the largest (1.4e-5 of the sum's rms for normal data, 3e-4 of the largest
-   product at most). W and Xq 16-byte aligned. ceil(M / 128) ceil(N / 128) below 2^22, M and N below 2^24.
+   product at most). W and Xq 16-byte aligned; Y must not overlap X (RS may be Y).
+   ceil(M / 128) ceil(N / 128) below 2^22, M and N below 2^24.
    ws: 256-byte aligned, any contents, or 0; with vybdq_gemm_fp8_workspace_size(M, N, K) bytes (-1: unsupported; the size covers
    every smaller M; at most 64 MiB) calls whose tiles do not fill the GPU split K and add float32 sums in a second launch (last
    bits may differ from the unsplit sum); a smaller one is not used. Calls that share a workspace must not overlap. */
@@ -626,7 +627,7 @@ int64_t vybdq_gemm_fp8_workspace_size(int64_t M, int64_t N, int64_t K);
 int vybdq_gemm_fp8(uint64_t W, uint64_t Ws, uint64_t Xq, uint64_t Xs, uint64_t Y, int64_t M, int64_t N, int64_t K, int y_dt,
                    int64_t ldy, uint64_t RS, uint64_t ws, int64_t ws_bytes, uint64_t stream);
 
-/* vybdq_quant_fp8 and vybdq_gemm_fp8 in one call: X x_dt, row stride ldx. ws: 256-byte aligned, of
+/* vybdq_quant_fp8 and vybdq_gemm_fp8 in one call: X x_dt, row stride ldx; Y must not overlap X. ws: 256-byte aligned, of
    vybdq_linear_fp8_workspace_size(M, N, K) bytes (-1: unsupported), any contents; the size covers every smaller M. Calls that
    share a workspace must not overlap. */
 int64_t vybdq_linear_fp8_workspace_size(int64_t M, int64_t N, int64_t K);

@@ -11,9 +11,9 @@ from oracle import fp8, moe
 from oracle.kvcache import e4m3_decode
 from vybforge_amd import _lib, ops
 
-QUANT = dict(X=16, x_dt=0, ldx=256, Xq=16, Xs=4, M=3, K=256, stream=0)
-GEMM = dict(W=16, Ws=4, Xq=16, Xs=4, Y=4, M=3, N=5, K=256, y_dt=0, ldy=0, RS=0, ws=0, ws_bytes=0, stream=0)
-LINEAR = dict(W=16, Ws=4, X=16, x_dt=0, ldx=256, Y=4, M=3, N=5, K=256, y_dt=0, ldy=0, RS=0, ws=256, ws_bytes=1 << 20, stream=0)
+QUANT = dict(X=16, x_dt=0, ldx=256, Xq=1 << 44, Xs=4, M=3, K=256, stream=0)
+GEMM = dict(W=16, Ws=4, Xq=1 << 50, Xs=1 << 51, Y=4, M=3, N=5, K=256, y_dt=0, ldy=0, RS=0, ws=0, ws_bytes=0, stream=0)
+LINEAR = dict(W=16, Ws=4, X=1 << 50, x_dt=0, ldx=256, Y=4, M=3, N=5, K=256, y_dt=0, ldy=0, RS=0, ws=256, ws_bytes=1 << 20, stream=0)
 ROUTE = dict(logits=8, logits_dt=0, bias=4, idx=4, w=4, T=3, E=64, topk=4, scale=1.0, softmax=0, renorm=1, groups=8, top_groups=2,
              group_top=2, stream=0)
 MOE = dict(x=16, x_dt=0, logits=8, logits_dt=0, bias=4, gate=16, gate_s=4, up=16, up_s=4, down=16, down_s=4, sg=16, sgs=4, su=16,
@@ -36,14 +36,16 @@ def refused(name, args, change, code, text):
     (dict(M=-1), _lib.ERR_SHAPE, "M must"), (dict(M=2 ** 28), _lib.ERR_SHAPE, "2\\^28"), (dict(X=0), _lib.ERR_ARG, "null"),
     (dict(M=2 ** 27), _lib.ERR_SHAPE, "2\\^28"), (dict(Xs=0), _lib.ERR_ARG, "null"), (dict(ldx=255), _lib.ERR_SHAPE, "ldx"),
     (dict(ldx=257), _lib.ERR_ALIGN, "16-byte"), (dict(X=8), _lib.ERR_ALIGN, "16-byte"), (dict(Xq=8), _lib.ERR_ALIGN, "16-byte"),
-    (dict(Xs=2), _lib.ERR_ALIGN, "4-byte"), (dict(x_dt=1, ldx=260), _lib.ERR_ALIGN, "16-byte")])
+    (dict(Xs=2), _lib.ERR_ALIGN, "4-byte"), (dict(x_dt=1, ldx=260), _lib.ERR_ALIGN, "16-byte"),
+    (dict(Xq=16), _lib.ERR_ARG, "overlap"), (dict(X=32, Xq=16), _lib.ERR_ARG, "overlap"), (dict(Xq=16 + 2944), _lib.ERR_ARG, "overlap")])
 def test_quantizer_refuses(change, code, text):
     refused("vybdq_quant_fp8", QUANT, change, code, text)
 
 
 @pytest.mark.parametrize("change,code,text", PRODUCT + [
     (dict(Xq=0), _lib.ERR_ARG, "null"), (dict(Xq=24), _lib.ERR_ALIGN, "Xq"), (dict(Xs=2), _lib.ERR_ALIGN, "Xs"),
-    (dict(ws=128), _lib.ERR_WORKSPACE, "workspace"), (dict(ws_bytes=-1), _lib.ERR_WORKSPACE, "workspace")])
+    (dict(ws=128), _lib.ERR_WORKSPACE, "workspace"), (dict(ws_bytes=-1), _lib.ERR_WORKSPACE, "workspace"),
+    (dict(Xq=16, Y=16), _lib.ERR_ARG, "overlap"), (dict(Xs=60, Y=16), _lib.ERR_ARG, "overlap")])
 def test_product_refuses(change, code, text):
     refused("vybdq_gemm_fp8", GEMM, change, code, text)
 
@@ -52,7 +54,7 @@ def test_product_refuses(change, code, text):
     (dict(x_dt=3), _lib.ERR_ARG, "x_dt"), (dict(X=0), _lib.ERR_ARG, "null"), (dict(ldx=255), _lib.ERR_SHAPE, "ldx"),
     (dict(X=8), _lib.ERR_ALIGN, "16-byte"), (dict(ldx=257), _lib.ERR_ALIGN, "16-byte"), (dict(ws=0), _lib.ERR_WORKSPACE, "workspace"),
     (dict(ws=128), _lib.ERR_WORKSPACE, "workspace"), (dict(ws_bytes=1000), _lib.ERR_WORKSPACE, "workspace"),
-    (dict(M=2 ** 23, N=1, K=2 ** 16, ldx=2 ** 16), _lib.ERR_SHAPE, "2\\^28")])
+    (dict(M=2 ** 23, N=1, K=2 ** 16, ldx=2 ** 16), _lib.ERR_SHAPE, "2\\^28"), (dict(X=16, Y=3000), _lib.ERR_ARG, "overlap")])
 def test_linear_refuses(change, code, text):
     refused("vybdq_linear_fp8", LINEAR, change, code, text)
 

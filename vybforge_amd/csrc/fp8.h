@@ -60,6 +60,11 @@ __device__ __forceinline__ uint32_t row16_max_u32(uint32_t v) {
   return v;
 }
 
+// Whether [a, a + na) and [b, b + nb) share a byte.
+inline bool fp8_overlap(uint64_t a, int64_t na, uint64_t b, int64_t nb) {
+  return a < b + static_cast<uint64_t>(nb) && b < a + static_cast<uint64_t>(na);
+}
+
 int fp8_quant_rows(const void *X, int x_dt, int64_t M, int64_t K, int64_t ldx, uint8_t *Xq, float *Xs, hipStream_t s);
 
 }  // namespace vybdq

@@ -207,6 +207,9 @@ extern "C" int vybdq_gemm_fp8(uint64_t W, uint64_t Ws, uint64_t Xq, uint64_t Xs,
   VYBDQ_REQUIRE(Xq && Xs, VYBDQ_ERR_ARG, "null buffer");
   VYBDQ_REQUIRE(Xq % 16 == 0 && Xs % 4 == 0, VYBDQ_ERR_ALIGN, "Xq must be 16-byte and Xs 4-byte aligned");
   VYBDQ_REQUIRE(ws % 256 == 0 && ws_bytes >= 0, VYBDQ_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  const int64_t yb = ((M - 1) * ldy + N) * dt_size(y_dt);
+  VYBDQ_REQUIRE(!fp8_overlap(Y, yb, Xq, M * K) && !fp8_overlap(Y, yb, Xs, M * ((K + 127) / 128) * 4), VYBDQ_ERR_ARG,
+                "Y must not overlap X: workgroups read X while others write");
   return fp8_gemm(fp8_args(reinterpret_cast<const uint8_t *>(W), reinterpret_cast<const float *>(Ws),
                            reinterpret_cast<const uint8_t *>(Xq), reinterpret_cast<const float *>(Xs), reinterpret_cast<void *>(Y),
                            y_dt, M, N, K, ldy, reinterpret_cast<const void *>(RS)),
@@ -229,6 +232,8 @@ extern "C" int vybdq_linear_fp8(uint64_t W, uint64_t Ws, uint64_t X, int x_dt, i
   VYBDQ_REQUIRE(X % 16 == 0 && (M == 1 || ldx * dt_size(x_dt) % 16 == 0), VYBDQ_ERR_ALIGN, "rows of X must be 16-byte aligned");
   VYBDQ_REQUIRE(ws && ws % 256 == 0 && ws_bytes >= vybdq_linear_fp8_workspace_size(M, N, K), VYBDQ_ERR_WORKSPACE,
                 "workspace must be 256-byte aligned and of vybdq_linear_fp8_workspace_size bytes");
+  VYBDQ_REQUIRE(!fp8_overlap(Y, ((M - 1) * ldy + N) * dt_size(y_dt), X, ((M - 1) * (M > 1 ? ldx : K) + K) * dt_size(x_dt)), VYBDQ_ERR_ARG,
+                "Y must not overlap X: workgroups read X while others write");
   uint8_t *xq = reinterpret_cast<uint8_t *>(ws);
   float *xs = reinterpret_cast<float *>(ws + align256(M * K));
   const int64_t front = align256(M * K) + align256(M * ((K + 127) / 128) * 4);

@@ -460,11 +460,11 @@ def moe_route(logits, topk, bias=None, scale=2.5, score="sigmoid", renorm=True, 
     T, E = logits.shape
     _need(bias is None or (bias.numel() == E and bias.dtype == torch.float32), "bias must be float32 [E]")
     _need(score in SCORES, f"score must be one of {SCORES}")
-    idx = torch.empty((T, topk), dtype=torch.int32, device=logits.device)
-    w = torch.empty((T, topk), dtype=torch.float32, device=logits.device)
+    _need(bias is None or bias.device == logits.device, "bias must be on the logits' device")
+    idx, w = logits.new_empty((T, topk), dtype=torch.int32), logits.new_empty((T, topk), dtype=torch.float32)
     if groups != 1 or top_groups != 1 or score != "sigmoid" or not renorm:
-        call("vybdq_moe_route_groups", _ptr(logits), _dt(logits.dtype), _ptr(bias), _ptr(idx), _ptr(w), T, E, topk,
-             float(scale), score == "softmax", renorm, groups, top_groups, group_top, _stream())
+        call("vybdq_moe_route_groups", _ptr(logits), _dt(logits.dtype), _ptr(bias), idx.data_ptr(), w.data_ptr(), T, E, topk,
+             scale, score == "softmax", renorm, groups, top_groups, group_top, _fp8_stream(logits.get_device()))
         return idx, w
     call("vybdq_moe_route", _ptr(logits), _dt(logits.dtype), _ptr(bias), _ptr(idx), _ptr(w), T, E, topk,
          float(scale), _stream())
@@ -788,7 +788,7 @@ def _fp8_device(t, device, what):
 def _fp8_stream(index):
     now = torch._C._cuda_getDevice()
     if now != index:
-        raise ValueError(f"the weights are on device {index}, the current device is {now}")
+        raise ValueError(f"the tensors are on device {index}, the current device is {now}")
     return torch._C._cuda_getCurrentRawStream(now)
 
 
@@ -805,46 +805,51 @@ def _fp8_matrix(W, Ws, lead, what):
     return N, K
 
 
+# The checks of a decode step's calls are written out, as those of the key/value cache above.
+
 def _fp8_rows(X, K):
     """Address, rows and row stride of X [M, K] (or [K]) whose rows may be slices of a wider matrix."""
-    if X.dim() == 1:
-        X = X[None]
-    if X.dim() != 2 or X.shape[1] != K:
+    shape, stride = X.shape, X.stride()
+    if len(shape) == 1:
+        shape, stride = (1, *shape), (K, *stride)
+    if len(shape) != 2 or shape[1] != K:
         raise ValueError(f"X must be [M, {K}]")
-    if not X.is_cuda:
-        raise ValueError("tensor must be on the GPU")
-    M = X.shape[0]
-    if X.stride(1) != 1 and M and K > 1:
+    M = shape[0]
+    if stride[1] != 1 and M:
         raise ValueError("the elements of a row of X must be consecutive")
-    return X.data_ptr(), M, X.stride(0) if M > 1 else K
+    return X.data_ptr(), M, stride[0] if M > 1 else K
 
 
 def quant_fp8(X, out=None):
     """X [M, K] (or [K]) to e4m3 codes [M, K] and float32 scales [M, ceil(K / 128)] (vybdq_quant_fp8): a power of two for each
     row and 128 columns. out: preallocated (codes, scales)."""
-    K = X.shape[-1]
+    index, K = X.get_device(), X.shape[-1]
+    if index < 0:
+        raise ValueError("tensor must be on the GPU")
     p, M, ldx = _fp8_rows(X, K)
+    KB = (K + 127) // 128
     if out is None:
-        q = torch.empty((M, K), dtype=E4M3, device=X.device)
-        d = torch.empty((M, _blocks(K)), dtype=torch.float32, device=X.device)
+        q, d = X.new_empty((M, K), dtype=E4M3), X.new_empty((M, KB), dtype=torch.float32)
     else:
         q, d = out
         _need(q.dtype == E4M3 and q.numel() == M * K, f"codes must be float8_e4m3fn [{M}, {K}]")
-        _need(d.dtype == torch.float32 and d.numel() == M * _blocks(K), f"scales must be float32 [{M}, {_blocks(K)}]")
+        _need(d.dtype == torch.float32 and d.numel() == M * KB, f"scales must be float32 [{M}, {KB}]")
         _fp8_device(q, X.device, "codes")
         _fp8_device(d, X.device, "scales")
-    call("vybdq_quant_fp8", p, _dt(X.dtype), ldx, _ptr(q), _ptr(d), M, K, _fp8_stream(X.get_device()))
+        _need(q.is_contiguous() and d.is_contiguous(), "codes and scales must be contiguous")
+    call("vybdq_quant_fp8", p, _dt(X.dtype), ldx, q.data_ptr(), d.data_ptr(), M, K, _fp8_stream(index))
     return q, d
 
 
-def _fp8_out(out, M, N, y_dtype, residual, device):
+def _fp8_out(out, M, N, y_dtype, residual, like):
     if out is None:
-        out = torch.empty((M, N), dtype=y_dtype, device=device)
-    _check_out(out, (M, N))
-    _fp8_device(out, device, "out")
-    _check_residual(residual, out)
+        out = like.new_empty((M, N), dtype=y_dtype)
+    else:
+        _check_out(out, (M, N))
+        _fp8_device(out, like.device, "out")
     if residual is not None:
-        _fp8_device(residual, device, "residual")
+        _check_residual(residual, out)
+        _fp8_device(residual, like.device, "residual")
     return out
 
 
@@ -859,7 +864,7 @@ def gemm_fp8(W, Ws, Xq, Xs, y_dtype=torch.float32, residual=None, out=None, work
     _need(tuple(Xs.shape) == (M, _blocks(K)) and Xs.dtype == torch.float32, f"Xs must be float32 [{M}, {_blocks(K)}]")
     for t, what in ((Xq, "Xq"), (Xs, "Xs")):
         _fp8_device(t, W.device, what)
-    out = _fp8_out(out, M, N, y_dtype, residual, W.device)
+    out = _fp8_out(out, M, N, y_dtype, residual, W)
     ws, nb = (0, 0) if workspace is None else workspace.at(W.device)
     call("vybdq_gemm_fp8", _ptr(W), _ptr(Ws), _ptr(Xq), _ptr(Xs), _ptr(out), M, N, K, _dt(out.dtype), 0, _ptr(residual), ws, nb,
          _fp8_stream(W.get_device()))
@@ -903,9 +908,9 @@ class Fp8Linear:
         p, M, ldx = _fp8_rows(X, self.K)
         if M > self.max_rows:
             raise ValueError(f"X has {M} rows, the workspace is for {self.max_rows}")
-        if X.get_device() != self.index:
-            raise ValueError("X must be on the weights' device")
-        out = _fp8_out(out, M, self.N, y_dtype, residual, self.W.device)
+        if X.get_device() != self.index or self.index < 0:
+            raise ValueError("X must be on the weights' device, a GPU")
+        out = _fp8_out(out, M, self.N, y_dtype, residual, self.W)
         call("vybdq_linear_fp8", *self._w, p, _dt(X.dtype), ldx, _ptr(out), M, self.N, self.K, _dt(out.dtype), 0, _ptr(residual),
              *self._ws, _fp8_stream(self.index))
         return out
@@ -962,7 +967,7 @@ class MoeFp8Layer:
         _need(logits.dim() == 2 and tuple(logits.shape) == (T, self.E), f"logits must be [T, {self.E}]")
         for t, what in ((x, "x"), (logits, "logits")):
             _fp8_device(t, self.device, what)
-        out = _fp8_out(out, T, self.H, out_dtype, None, self.device)
+        out = _fp8_out(out, T, self.H, out_dtype, None, x)
         idx = w = None
         if routing:
             idx = torch.empty((T, self.topk), dtype=torch.int32, device=x.device)
