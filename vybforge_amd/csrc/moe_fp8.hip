@@ -24,13 +24,13 @@ struct MoeFp8Lists {
 
 // Few tokens (at most 64 rows) in one launch: workgroup 0 routes them and lists rows and tiles, the others quantize x (one token of
 // 6144 over 256 experts: 10 us against 18 of three launches).
-template <int LDT, int ENT>
+template <bool SOFTMAX, bool BIAS, int TOP, int ENT>
 __global__ void __launch_bounds__(256) k_moe_fp8_front(const RouteArgs r, const void *__restrict__ x, int x_dt, int H,
                                                        uint8_t *__restrict__ xq, float *__restrict__ xs, int BM, int shared,
                                                        const MoeFp8Lists l) {
   __shared__ int idx_lds[64];
   if (blockIdx.x == 0) {
-    for (int t = threadIdx.x >> 6; t < r.T; t += 4) route_groups_wave<LDT, ENT>(r, t, idx_lds);
+    for (int t = threadIdx.x >> 6; t < r.T; t += 4) route_groups_wave<SOFTMAX, BIAS, TOP, ENT>(r, t, idx_lds);
     __syncthreads();
     if (threadIdx.x < 64) bucket_rows_wave(idx_lds, r.T, r.topk, BM, BM, shared, l.pos, l.row_map, l.tiles, l.ntiles, nullptr, nullptr);
     return;
@@ -201,11 +201,10 @@ extern "C" int vybdq_moe_forward_fp8(uint64_t x, int x_dt, uint64_t logits, int 
   const MoeFp8Lists lists{m.pos, m.row_map, m.ntiles, m.tiles};
   if (n <= 64 && T <= 8) {
     const dim3 grid(static_cast<unsigned>(1 + (T * (H / 128) + 15) / 16));
-#define FRONT(LDT)                                                                                                              \
-  VYBDQ_DISPATCH_ROUTE(r, hipLaunchKernelGGL((k_moe_fp8_front<LDT, ENT>), grid, dim3(256), 0, s, r, reinterpret_cast<const void *>(x), x_dt, \
-                                             static_cast<int>(H), m.xq, m.xs, BM, shared ? 1 : 0, lists))
-    if (logits_dt == VYBDQ_F64) FRONT(VYBDQ_F64)
-    else VYBDQ_DISPATCH_IN(logits_dt, LDT, FRONT(LDT))
+#define FRONT(SM, BI, TP, ENT)                                                                                                      \
+  hipLaunchKernelGGL((k_moe_fp8_front<SM, BI, TP, ENT>), grid, dim3(256), 0, s, r, reinterpret_cast<const void *>(x), x_dt,             \
+                     static_cast<int>(H), m.xq, m.xs, BM, shared ? 1 : 0, lists)
+    VYBDQ_DISPATCH_ROUTE(r, FRONT)
 #undef FRONT
     rc = check_launch("moe front");
   } else {

@@ -25,83 +25,135 @@ struct RouteArgs {
   float *w;
 };
 
-__device__ __forceinline__ double shfl_xor_f64(double v, int d) { return __shfl_xor(v, d); }
+// exp(x) in float64, about an ulp off: x = n ln 2 + r with |r| <= ln 2 / 2 (Cody and Waite: ln 2 in two parts, so that r is
+// exact to float64), the Taylor series of r to r^13 (the rest is below 2^-57), times 2^n. No special cases but the clamp: a NaN
+// passes, below -745 the result is 0, above 710 infinity. (The library's exp and its tests of the range, at every place that
+// a template argument does not decide, made the router 2500 instructions; 16384 tokens 25 us.)
+__device__ __forceinline__ double route_exp(double x) {
+  x = x < -800.0 ? -800.0 : (x > 800.0 ? 800.0 : x);
+  const double n = __builtin_rint(x * 1.4426950408889634);
+  double r = fma(n, -0x1.62e42feep-1, x);          // the leading 32 bits of ln 2: n of them are exact
+  r = fma(n, -0x1.a39ef35793c76p-33, r);           // the rest of it
+  double p = 1.0 / 6227020800.0;
+  p = fma(p, r, 1.0 / 479001600.0);
+  p = fma(p, r, 1.0 / 39916800.0);
+  p = fma(p, r, 1.0 / 3628800.0);
+  p = fma(p, r, 1.0 / 362880.0);
+  p = fma(p, r, 1.0 / 40320.0);
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return __builtin_ldexp(p, static_cast<int>(n));
+}
 
-// The larger of two doubles, NaN below every number.
-__device__ __forceinline__ bool above(double a, double b) { return a > b || (a == a && b != b); }
+// The value of the lane that DPP control C names (every lane has one), and of lane l.
+template <int C>
+__device__ __forceinline__ double dpp_f64(double v) {
+  const uint64_t b = __double_as_longlong(v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), C, 0xf, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), C, 0xf, 0xf, false);
+  return __longlong_as_double(static_cast<long long>((static_cast<uint64_t>(hi) << 32) | lo));
+}
+__device__ __forceinline__ double lane_f64(double v, int l) {
+  const uint64_t b = __double_as_longlong(v);
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(b), l), hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), l);
+  return __longlong_as_double(static_cast<long long>((static_cast<uint64_t>(hi) << 32) | lo));
+}
 
-template <int LDT, int ENT>
+// op over the wave: the rows of 16 by DPP, then the four rows.
+template <class F>
+__device__ __forceinline__ double wave_f64(double v, F op) {
+  v = op(v, dpp_f64<DPP_QUAD_XOR1>(v));
+  v = op(v, dpp_f64<DPP_QUAD_XOR2>(v));
+  v = op(v, dpp_f64<DPP_HALF_MIRROR>(v));
+  v = op(v, dpp_f64<DPP_ROW_MIRROR>(v));
+  return op(op(lane_f64(v, 0), lane_f64(v, 16)), op(lane_f64(v, 32), lane_f64(v, 48)));
+}
+
+// TOP: 0 without groups, else the choices that a group's value sums. A NaN stands for no entry and lies below every number (as
+// fmax has it).
+template <bool SOFTMAX, bool BIAS, int TOP, int ENT>
 __device__ __forceinline__ void route_groups_wave(const RouteArgs &a, int t, int *__restrict__ idx_copy) {
-  const int lane = threadIdx.x & 63, L = 1 << a.lg;
-  const int g = lane >> a.lg, j = lane & (L - 1);
+  constexpr bool SCORES = SOFTMAX || BIAS || TOP == 2;  // every expert's score is needed, not the winners' alone
+  const int lane = threadIdx.x & 63, L = TOP ? 1 << a.lg : 64;
+  const int g = TOP ? lane >> a.lg : 0, j = lane & (L - 1), S = TOP ? a.S : a.E;
   const int64_t base = static_cast<int64_t>(t) * a.E;
-  double l[ENT];
+  auto logit = [&](int64_t i) {
+    switch (a.ldt) {
+      case VYBDQ_F64: return load_logit<VYBDQ_F64>(a.logits, i);
+      case VYBDQ_F32: return load_logit<VYBDQ_F32>(a.logits, i);
+      case VYBDQ_F16: return load_logit<VYBDQ_F16>(a.logits, i);
+      default: return load_logit<VYBDQ_BF16>(a.logits, i);
+    }
+  };
+  const double kNan = __longlong_as_double(0x7ff8000000000000ll);
+  double l[ENT], bias[ENT], score[ENT];
   uint32_t eid[ENT];
 #pragma unroll
   for (int i = 0; i < ENT; ++i) {
     const int q = j + L * i;
-    eid[i] = g < a.groups && q < a.S ? static_cast<uint32_t>(g * a.S + q) : kRouteNone;
-    l[i] = eid[i] != kRouteNone ? load_logit<LDT>(a.logits, base + eid[i]) : 0.0;
+    const bool have = (TOP == 0 || g < a.groups) && q < S;
+    eid[i] = have ? static_cast<uint32_t>(g * S + q) : kRouteNone;
+    const uint32_t at = have ? eid[i] : 0;
+    l[i] = logit(base + at);
+    bias[i] = BIAS ? static_cast<double>(a.bias[at]) : 0.0;
+    score[i] = 0.0;
   }
-  double top = 0.0, sum = 0.0;  // softmax: the largest logit (0 where all are -infinity) and the sum of exp(l - top)
-  if (a.softmax) {
-    top = -INFINITY;
+  if constexpr (SOFTMAX) {
+    // the largest logit (0 where all are -infinity; NaN if one is), exp(l - top) over their sum
+    double top = -INFINITY;
+    bool nan = false;
 #pragma unroll
-    for (int i = 0; i < ENT; ++i)
-      if (eid[i] != kRouteNone) top = l[i] > top || l[i] != l[i] ? l[i] : top;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const double o = shfl_xor_f64(top, d);
-      top = o > top || o != o ? o : top;
+    for (int i = 0; i < ENT; ++i) {
+      top = eid[i] != kRouteNone ? fmax(top, l[i]) : top;
+      nan |= eid[i] != kRouteNone && l[i] != l[i];
     }
+    top = wave_f64(top, [](double x, double y) { return fmax(x, y); });
     if (top == -INFINITY) top = 0.0;
+    if (__any(nan)) top = kNan;
+    double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < ENT; ++i)
-      if (eid[i] != kRouteNone) sum += exp(l[i] - top);
+    for (int i = 0; i < ENT; ++i) {
+      score[i] = eid[i] != kRouteNone ? route_exp(l[i] - top) : 0.0;
+      sum += score[i];
+    }
+    sum = wave_f64(sum, [](double x, double y) { return x + y; });
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum += shfl_xor_f64(sum, d);
+    for (int i = 0; i < ENT; ++i) score[i] = sum == 0.0 ? 0.0 : score[i] / sum;
+  } else if constexpr (SCORES) {
+#pragma unroll
+    for (int i = 0; i < ENT; ++i) score[i] = 1.0 / (1.0 + route_exp(-l[i]));
   }
-  auto score = [&](double x) {
-    if (!a.softmax) return 1.0 / (1.0 + exp(-x));
-    return sum == 0.0 ? 0.0 : exp(x - top) / sum;
-  };
-  const bool sums = a.groups > 1 && a.group_top == 2;  // group values need the scores themselves
   uint64_t key[ENT];
-  double b1 = -INFINITY, b2 = -INFINITY;  // this lane's best two choices (of how many: n)
-  int n = 0;
+  double b1 = kNan, b2 = kNan;  // this lane's best two choices
 #pragma unroll
   for (int i = 0; i < ENT; ++i) {
-    key[i] = 0;
-    if (eid[i] == kRouteNone) continue;
-    double c = l[i];
-    if (a.bias) c = score(c) + static_cast<double>(a.bias[eid[i]]);
-    key[i] = double_order_key(c);
-    if (a.groups > 1) {
-      if (sums && !a.bias) c = score(c);
-      if (n == 0 || above(c, b1)) {
-        b2 = n ? b1 : b2;
-        b1 = c;
-      } else if (n == 1 || above(c, b2)) {
-        b2 = c;
-      }
-      ++n;
+    const bool have = eid[i] != kRouteNone;
+    const double order = BIAS ? score[i] + bias[i] : l[i];
+    key[i] = have ? double_order_key(order) : 0;
+    if constexpr (TOP > 0) {
+      const double c = have ? (TOP == 2 && !BIAS ? score[i] : order) : kNan;
+      if (TOP == 2) b2 = fmax(b2, b1 == b1 && c == c ? fmin(b1, c) : kNan);
+      b1 = fmax(b1, c);
     }
   }
-  if (a.groups > 1) {
-    for (int d = 1; d < L; d <<= 1) {
-      const double o1 = shfl_xor_f64(b1, d), o2 = shfl_xor_f64(b2, d);
-      const int on = __shfl_xor(n, d);
-      // merge two descending pairs of which the first n and on entries (at most two) count
-      const bool mine = n > 0 && (on == 0 || !above(o1, b1));
-      const double f = mine ? b1 : o1;
-      const double x = mine ? b2 : b1, y = mine ? o1 : o2;  // candidates for the second place
-      const bool hx = mine ? n > 1 : n > 0, hy = mine ? on > 0 : on > 1;
-      b2 = hx && (!hy || !above(y, x)) ? x : y;
-      b1 = f;
-      n = n + on;
-    }
-    double value = b1;
-    if (a.group_top == 2 && n > 1) value = b1 + b2;
+  if constexpr (TOP > 0) {
+    auto merge = [&](double o1, double o2) {
+      if (TOP == 2) b2 = fmax(b1 == b1 && o1 == o1 ? fmin(b1, o1) : kNan, fmax(b2, o2));
+      b1 = fmax(b1, o1);
+    };
+    // (the lanes of a quad, then of a half row agree by then: a mirror's lane holds what lane ^ 4, ^ 8 does)
+    if (a.lg > 0) merge(dpp_f64<DPP_QUAD_XOR1>(b1), TOP == 2 ? dpp_f64<DPP_QUAD_XOR1>(b2) : 0.0);
+    if (a.lg > 1) merge(dpp_f64<DPP_QUAD_XOR2>(b1), TOP == 2 ? dpp_f64<DPP_QUAD_XOR2>(b2) : 0.0);
+    if (a.lg > 2) merge(dpp_f64<DPP_HALF_MIRROR>(b1), TOP == 2 ? dpp_f64<DPP_HALF_MIRROR>(b2) : 0.0);
+    if (a.lg > 3) merge(dpp_f64<DPP_ROW_MIRROR>(b1), TOP == 2 ? dpp_f64<DPP_ROW_MIRROR>(b2) : 0.0);
+    if (a.lg > 4) merge(__shfl_xor(b1, 16), TOP == 2 ? __shfl_xor(b2, 16) : 0.0);
+    const double value = TOP == 2 && S > 1 ? b1 + b2 : b1;
     uint64_t gk[1] = {0};
     uint32_t gi[1] = {kRouteNone};
     if (j == 0 && g < a.groups) {
@@ -120,16 +172,34 @@ __device__ __forceinline__ void route_groups_wave(const RouteArgs &a, int t, int
   }
   const uint32_t mine = route_select<ENT>(key, eid, a.topk);
   const bool slot = lane < a.topk && mine != kRouteNone;
-  const double sc = slot ? score(load_logit<LDT>(a.logits, base + mine)) : 0.0;
+  double sc = 0.0;
+  if constexpr (SCORES && ENT <= 8) {  // from the lane and entry that hold the expert
+    const int e = slot ? static_cast<int>(mine) : 0, gq = TOP ? e / S : 0, q = e - gq * S;
+    const int from = TOP ? (gq << a.lg) + (q & (L - 1)) : q & 63, at = TOP ? q >> a.lg : q >> 6;
+#pragma unroll
+    for (int i = 0; i < ENT; ++i) {
+      const double v = __shfl(score[i], from);
+      sc = at == i ? v : sc;
+    }
+    sc = slot ? sc : 0.0;
+  } else if constexpr (SOFTMAX) {
+    for (int s = 0; s < a.topk; ++s) {  // the lane that holds slot s's expert gives its score
+      const uint32_t e = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), s));
+      const int gq = TOP ? static_cast<int>(e) / S : 0, q = static_cast<int>(e) - gq * S;
+      const int from = TOP ? (gq << a.lg) + (q & (L - 1)) : q & 63, at = TOP ? q >> a.lg : q >> 6;
+      double v = 0.0;
+#pragma unroll
+      for (int i = 0; i < ENT; ++i) v = at == i ? score[i] : v;
+      v = lane_f64(v, from & 63);
+      sc = lane == s ? v : sc;
+    }
+  } else {
+    sc = slot ? 1.0 / (1.0 + route_exp(-logit(base + mine))) : 0.0;
+  }
   double den = 1.0;
   if (a.renorm) {
-    const uint64_t sb = __double_as_longlong(sc);
     double tot = 0.0;  // in slot order
-    for (int q = 0; q < a.topk; ++q) {
-      const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(sb), q);
-      const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(sb >> 32), q);
-      tot += __longlong_as_double(static_cast<long long>((static_cast<uint64_t>(hi) << 32) | lo));
-    }
+    for (int q = 0; q < a.topk; ++q) tot += lane_f64(sc, q);
     den = tot + 1e-20;
   }
   if (slot) {
@@ -140,18 +210,31 @@ __device__ __forceinline__ void route_groups_wave(const RouteArgs &a, int t, int
   }
 }
 
-// experts per lane: 4, 8, 16 or 32
+// experts per lane: 4, 8 or 32
 inline int route_groups_ent(const RouteArgs &a) {
   const int n = (a.S + (1 << a.lg) - 1) >> a.lg;
-  return n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 : 32;
+  return n <= 4 ? 4 : n <= 8 ? 8 : 32;
 }
 
-#define VYBDQ_DISPATCH_ROUTE(a, ...)                                              \
-  switch (route_groups_ent(a)) {                                                 \
-    case 4: { constexpr int ENT = 4; __VA_ARGS__; } break;                       \
-    case 8: { constexpr int ENT = 8; __VA_ARGS__; } break;                       \
-    case 16: { constexpr int ENT = 16; __VA_ARGS__; } break;                     \
-    default: { constexpr int ENT = 32; __VA_ARGS__; } break;                     \
+// Runs BODY(SOFTMAX, BIAS, TOP, ENT) with the arguments' template values.
+#define VYBDQ_ROUTE_ENT(a, BODY, SM, BI, TP)                  \
+  switch (route_groups_ent(a)) {                             \
+    case 4: BODY(SM, BI, TP, 4); break;                      \
+    case 8: BODY(SM, BI, TP, 8); break;                      \
+    default: BODY(SM, BI, TP, 32); break;                    \
+  }
+#define VYBDQ_ROUTE_TOP(a, BODY, SM, BI)                      \
+  switch ((a).groups == 1 ? 0 : (a).group_top) {             \
+    case 0: VYBDQ_ROUTE_ENT(a, BODY, SM, BI, 0) break;       \
+    case 1: VYBDQ_ROUTE_ENT(a, BODY, SM, BI, 1) break;       \
+    default: VYBDQ_ROUTE_ENT(a, BODY, SM, BI, 2) break;      \
+  }
+#define VYBDQ_DISPATCH_ROUTE(a, BODY)                         \
+  switch (((a).softmax ? 2 : 0) + ((a).bias ? 1 : 0)) {      \
+    case 0: VYBDQ_ROUTE_TOP(a, BODY, false, false) break;    \
+    case 1: VYBDQ_ROUTE_TOP(a, BODY, false, true) break;     \
+    case 2: VYBDQ_ROUTE_TOP(a, BODY, true, false) break;     \
+    default: VYBDQ_ROUTE_TOP(a, BODY, true, true) break;     \
   }
 
 // Checks the arguments and fills `a`; `func` names the entry point in errors.

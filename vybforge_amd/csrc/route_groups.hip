@@ -3,10 +3,10 @@
 
 namespace vybdq {
 
-template <int LDT, int ENT>
+template <bool SOFTMAX, bool BIAS, int TOP, int ENT>
 __global__ void __launch_bounds__(256) k_route_groups(const RouteArgs a) {
   const int t = 4 * blockIdx.x + (threadIdx.x >> 6);
-  if (t < a.T) route_groups_wave<LDT, ENT>(a, t, nullptr);
+  if (t < a.T) route_groups_wave<SOFTMAX, BIAS, TOP, ENT>(a, t, nullptr);
 }
 
 int route_groups_args(const char *func, RouteArgs &a, uint64_t logits, int logits_dt, uint64_t bias, uint64_t idx, uint64_t w,
@@ -34,11 +34,9 @@ int route_groups_args(const char *func, RouteArgs &a, uint64_t logits, int logit
 
 int route_groups_launch(const RouteArgs &a, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>((a.T + 3) / 4));
-  if (a.ldt == VYBDQ_F64) {
-    VYBDQ_DISPATCH_ROUTE(a, hipLaunchKernelGGL((k_route_groups<VYBDQ_F64, ENT>), grid, dim3(256), 0, s, a));
-  } else {
-    VYBDQ_DISPATCH_IN(a.ldt, LDT, VYBDQ_DISPATCH_ROUTE(a, hipLaunchKernelGGL((k_route_groups<LDT, ENT>), grid, dim3(256), 0, s, a)));
-  }
+#define ROUTE(SM, BI, TP, ENT) hipLaunchKernelGGL((k_route_groups<SM, BI, TP, ENT>), grid, dim3(256), 0, s, a)
+  VYBDQ_DISPATCH_ROUTE(a, ROUTE)
+#undef ROUTE
   return check_launch("moe route (groups)");
 }
 
