@@ -157,7 +157,7 @@ def test_product_long(dev, rng, M, N, K):
 
 
 @pytest.mark.parametrize("y", ["f32", "bf16"])
-@pytest.mark.parametrize("tile", ["64,1", "64,3", "128,1", "128,4", "256,1", "256,2"])
+@pytest.mark.parametrize("tile", ["64,1", "64,3", "128,1", "128,4", "192,1", "192,3", "256,1", "256,2"])
 @pytest.mark.parametrize("M,N,K", [(17, 1000, 2048), (64, 37, 2176), (130, 520, 2048), (300, 1300, 1152)])
 def test_product_tiles_and_splits(dev, rng, monkeypatch, M, N, K, tile, y):
     """Every tile of the pipeline, whole and with K split, more tiles than one to a workgroup or fewer, ragged in every way."""

@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(256) k_fp8_join(const Fp8MmArgs a, const float
 // ---- which kernel ---------------------------------------------------------------------------------
 
 struct Fp8Plan {
-  int BM, splits;  // pipelined tiles of BM x 256; BM = 0: the forms for any K
+  int BM, splits;  // pipelined tiles of BM x 256 (64, 128, 192, 256); BM = 0: the forms for any K
 };
 
 constexpr int64_t kFp8PartBytes = int64_t(64) << 20;  // most bytes of float32 sums that a split product writes
@@ -51,15 +51,16 @@ static int64_t fp8_part_bytes(int64_t M, int64_t N, int64_t K) {
 
 // Tile height and splits with the least estimate: rounds of tiles over the chip, a round its K steps and its end; split sums written,
 // read and added. Times in us fitted over 26 shapes from 16 to 2048 rows (both instructions) with every tile and up to 16 splits
-// forced: 9% off in the mean over 200 of them, the choice never more than 2% above the best of them.
+// forced: 9% off in the mean over 200 of them, the choice never more than 2% above the best of them; with the tiles of 192 rows
+// (512 x 17408 x 5120 61 us, the others 72 to 82; 2048 rows 174 / 207), 11 more shapes up to 4096 rows: at most 3%.
 static Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t K, bool half, int64_t part) {
   const int64_t nk = K / 128, cus = device_cu_count();
   Fp8Plan best{0, 1};
   if (K % 128 || nk < 4) return best;
-  constexpr double kStep[2][3] = {{0.84, 1.0, 1.72}, {1.07, 1.65, 0}}, kEnd[3] = {2.5, 2.8, 2.9};
+  constexpr double kStep[2][4] = {{0.84, 1.0, 1.25, 1.72}, {1.07, 1.65, 0, 0}}, kEnd[4] = {2.5, 2.8, 2.9, 2.9};
   double best_t = 1e30;
-  for (int c = 0; c < (half ? 2 : 3); ++c) {
-    const int BM = 64 << c;
+  for (int c = 0; c < (half ? 2 : 4); ++c) {
+    const int BM = 64 * (c + 1);
     const int64_t tiles = (M + BM - 1) / BM * ((N + 255) / 256);
     for (int64_t S = 1; S <= 16; ++S) {
       if (S > 1 && (nk / S < 4 || S * M * N * 4 > part)) break;
@@ -71,7 +72,7 @@ static Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t K, bool half, int64_t part
   }
   if (const char *e = tuning_env("VYBDQ_FP8_TILE")) {  // "BM,splits"
     int bm = 0, sp = 0;
-    if (sscanf(e, "%d,%d", &bm, &sp) == 2 && (bm == 64 || bm == 128 || (bm == 256 && !half)) && sp >= 1 && nk / sp >= 4 &&
+    if (sscanf(e, "%d,%d", &bm, &sp) == 2 && (bm == 64 || bm == 128 || ((bm == 192 || bm == 256) && !half)) && sp >= 1 && nk / sp >= 4 &&
         (sp == 1 || sp * M * N * 4 <= part))
       best = Fp8Plan{bm, sp};
   }
@@ -132,6 +133,7 @@ static int fp8_gemm_tiles(Fp8MmArgs &a, float *part, int64_t part_bytes, hipStre
     int rc;
     if (p.BM == 64) rc = fp8_pipe_launch<4, 2, 1, 8, 3, FP8_DENSE, HALF>(t, n, s);
     else if (p.BM == 128) rc = fp8_pipe_launch<4, 4, 2, 4, 3, FP8_DENSE, HALF>(t, n, s);
+    else if (p.BM == 192) rc = fp8_pipe_launch<6, 4, 2, 4, 2, FP8_DENSE, false>(t, n, s);
     else rc = fp8_pipe_launch<8, 4, 2, 4, 2, FP8_DENSE, false>(t, n, s);
     if (rc || p.splits == 1) return rc;
     const int64_t threads = static_cast<int64_t>(a.M) * ((a.N + 3) / 4);
