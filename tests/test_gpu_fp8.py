@@ -158,7 +158,7 @@ def test_product_long(dev, rng, M, N, K):
 
 @pytest.mark.parametrize("y", ["f32", "bf16"])
 @pytest.mark.parametrize("tile", ["64,1", "64,3", "128,1", "128,4", "192,1", "192,3", "256,1", "256,2"])
-@pytest.mark.parametrize("M,N,K", [(17, 1000, 2048), (64, 37, 2176), (130, 520, 2048), (300, 1300, 1152)])
+@pytest.mark.parametrize("M,N,K", [(17, 1000, 2048), (64, 37, 2176), (130, 520, 2048), (300, 1300, 1152), (33, 300, 2064), (200, 290, 1648)])
 def test_product_tiles_and_splits(dev, rng, monkeypatch, M, N, K, tile, y):
     """Every tile of the pipeline, whole and with K split, more tiles than one to a workgroup or fewer, ragged in every way."""
     monkeypatch.setenv("VYBDQ_FP8_TILE", tile)
@@ -193,6 +193,21 @@ def test_product_is_exact_where_float32_is(dev, rng, M, y):
     want = (x @ fp8.weights(wc, ws).T.astype(np.float32))
     got = ops.gemm_fp8(*on(dev, (wc, ws)), *on(dev, (xc, xs)), y_dtype=DT[y])
     assert torch.equal(got.cpu(), torch.from_numpy(want).to(DT[y]))
+
+
+@pytest.mark.parametrize("y", ["f32", "bf16"])
+@pytest.mark.parametrize("K", [1040, 1136, 2032])
+@pytest.mark.parametrize("M", [1, 16, 40, 200])
+def test_product_short_last_block_beside_nan(dev, rng, M, K, y):
+    """Rows end inside a block: what follows them in memory (the next row's first codes, all NaN) takes no part."""
+    N = 140
+    x, w = rng.integers(-3, 4, (M, K)).astype(np.float32), rng.integers(-2, 3, (N, K)).astype(np.float32)
+    wc, (xc, xs) = fp8.e4m3_encode(w), fp8.quant(x)
+    wc[1::2, :128], xc[1::2, :128] = 0x7f, 0x7f
+    got = ops.gemm_fp8(codes_to(dev, wc), torch.ones(2, fp8.blocks(K), device=dev), *on(dev, (xc, xs)), y_dtype=DT[y]).float().cpu()
+    want = torch.from_numpy(x @ w.T).to(DT[y]).float()
+    want[1::2], want[:, 1::2] = math.nan, math.nan
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
 
 
 @pytest.mark.parametrize("M", [1, 20, 130])

@@ -43,8 +43,8 @@ constexpr int64_t kFp8PartBytes = int64_t(64) << 20;  // most bytes of float32 s
 
 // Bytes of split sums that a call of M rows may use: rises with M, so that a workspace serves every smaller batch.
 static int64_t fp8_part_bytes(int64_t M, int64_t N, int64_t K) {
-  const int64_t one = M * N * 4, most = K / 128 / 4;  // (no split of fewer than 4 blocks)
-  if (K % 128 || most < 2 || M > 1024) return 0;
+  const int64_t one = M * N * 4, most = (K + 127) / 128 / 4;  // (no split of fewer than 4 blocks)
+  if (most < 2 || M > 1024) return 0;
   const int64_t n = one * (most < 16 ? most : 16);
   return n < kFp8PartBytes ? n : kFp8PartBytes;
 }
@@ -54,12 +54,13 @@ static int64_t fp8_part_bytes(int64_t M, int64_t N, int64_t K) {
 // forced: 9% off in the mean over 200 of them, the choice never more than 2% above the best of them; with the tiles of 192 rows
 // (512 x 17408 x 5120 61 us, the others 72 to 82; 2048 rows 174 / 207), 11 more shapes up to 4096 rows: at most 3%.
 static Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t K, bool half, int64_t part) {
-  const int64_t nk = K / 128, cus = device_cu_count();
+  const int64_t nk = (K + 127) / 128, cus = device_cu_count();
   Fp8Plan best{0, 1};
-  if (K % 128 || nk < 4) return best;
+  if (nk < 4) return best;
   constexpr double kStep[2][4] = {{0.84, 1.0, 1.25, 1.72}, {1.07, 1.65, 0, 0}}, kEnd[4] = {2.5, 2.8, 2.9, 2.9};
   double best_t = 1e30;
   for (int c = 0; c < (half ? 2 : 4); ++c) {
+    if (c == 2 && K % 128) continue;  // (that tile has no registers left for a short block)
     const int BM = 64 * (c + 1);
     const int64_t tiles = (M + BM - 1) / BM * ((N + 255) / 256);
     for (int64_t S = 1; S <= 16; ++S) {
@@ -72,7 +73,7 @@ static Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t K, bool half, int64_t part
   }
   if (const char *e = tuning_env("VYBDQ_FP8_TILE")) {  // "BM,splits"
     int bm = 0, sp = 0;
-    if (sscanf(e, "%d,%d", &bm, &sp) == 2 && (bm == 64 || bm == 128 || ((bm == 192 || bm == 256) && !half)) && sp >= 1 && nk / sp >= 4 &&
+    if (sscanf(e, "%d,%d", &bm, &sp) == 2 && (bm == 64 || bm == 128 || (((bm == 192 && K % 128 == 0) || bm == 256) && !half)) && sp >= 1 && nk / sp >= 4 &&
         (sp == 1 || sp * M * N * 4 <= part))
       best = Fp8Plan{bm, sp};
   }
@@ -82,7 +83,7 @@ static Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t K, bool half, int64_t part
 // Few rows of X (fp8_rows.h) or tiles. Up to 4 rows, or 16 of at most 2^25 weights, the streaming form is the faster one (measured,
 // bf16: 1 x 17408 x 5120 22.3 us against 23.8, 1 x 2560 x 9728 10.0 / 15.2, 16 x 9728 x 2560 11.5 / 13.5); beyond, every
 // workgroup's own pass over X costs more than the tiles' second launch (16 x 17408 x 5120 32.8 / 25.0, 16 x 5120 x 17408 42 / 26).
-static bool fp8_rows_take(int64_t M, int64_t N, int64_t K) { return M <= 4 || (M <= 16 && N * K <= (int64_t(1) << 25)) || (M <= 16 && K % 128); }
+static bool fp8_rows_take(int64_t M, int64_t N, int64_t K) { return M <= 4 || (M <= 16 && (N * K <= (int64_t(1) << 25) || K < 512)); }
 
 // Whether such a call quantizes X in its workgroups, each for itself: where that is little beside its rows of W, or all
 // workgroups do it at once (measured with the quantizer's own launch: 1 x 9728 x 2560 8.3 us against 11.0, 4 x 17408 x 5120
@@ -95,6 +96,17 @@ static bool fp8_rows_quant(int64_t M, int64_t N, int64_t K) {
 template <int XDT, bool HALF>
 static int fp8_rows_run(const Fp8RowsArgs &r, hipStream_t s) {
   return r.m.KB >= 32 ? fp8_rows_launch<1, 1, 16, 3, XDT, HALF>(r, s) : fp8_rows_launch<1, 1, 8, 3, XDT, HALF>(r, s);
+}
+
+template <bool HALF, bool TAIL>
+static int fp8_pipe_run(int BM, const Fp8MmArgs &t, int64_t n, hipStream_t s) {
+  if (BM == 64) return fp8_pipe_launch<4, 2, 1, 8, 3, FP8_DENSE, HALF, TAIL>(t, n, s);
+  if constexpr (!HALF) {
+    if (BM == 256) return fp8_pipe_launch<8, 4, 2, 4, 2, FP8_DENSE, false, TAIL>(t, n, s);
+    if constexpr (!TAIL)
+      if (BM == 192) return fp8_pipe_launch<6, 4, 2, 4, 2, FP8_DENSE, false>(t, n, s);
+  }
+  return fp8_pipe_launch<4, 4, 2, 4, 3, FP8_DENSE, HALF, TAIL>(t, n, s);
 }
 
 template <bool HALF>
@@ -130,11 +142,7 @@ static int fp8_gemm_tiles(Fp8MmArgs &a, float *part, int64_t part_bytes, hipStre
     t.m_tiles = a.m_tiles;
     t.n_tiles = a.n_tiles;
     t.units = a.units;
-    int rc;
-    if (p.BM == 64) rc = fp8_pipe_launch<4, 2, 1, 8, 3, FP8_DENSE, HALF>(t, n, s);
-    else if (p.BM == 128) rc = fp8_pipe_launch<4, 4, 2, 4, 3, FP8_DENSE, HALF>(t, n, s);
-    else if (p.BM == 192) rc = fp8_pipe_launch<6, 4, 2, 4, 2, FP8_DENSE, false>(t, n, s);
-    else rc = fp8_pipe_launch<8, 4, 2, 4, 2, FP8_DENSE, false>(t, n, s);
+    const int rc = a.K % 128 ? fp8_pipe_run<HALF, true>(p.BM, t, n, s) : fp8_pipe_run<HALF, false>(p.BM, t, n, s);
     if (rc || p.splits == 1) return rc;
     const int64_t threads = static_cast<int64_t>(a.M) * ((a.N + 3) / 4);
     hipLaunchKernelGGL(k_fp8_join, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, s, a, part, t.split_stride, p.splits);

@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_mm(const Fp8MmArgs a) {
 
 // ---- the same tiles as a persistent pipeline -----------------------------------------------------
 //
-// For K in whole blocks (at least ST of them) and e4m3 instructions. What the plain form above loses, per step of a 256 x 256
+// For at least ST blocks of K. What the plain form above loses, per step of a 256 x 256
 // tile (its matrix instructions take 0.85 us at the clock that they run at on real data): all waves read LDS at once behind the
 // barrier, then multiply; the address of each load is 64-bit arithmetic on the vector unit; a tile's last stores and the next
 // one's first loads overlap with nothing.
@@ -395,7 +395,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_mm(const Fp8MmArgs a) {
 //     matrix instructions of those two. A fragment of W is read for the next step once its last product has been issued.
 //   - The fma of a block product come a group later than its instruction (t, tb), in an order that scheduling barriers hold.
 //   - A workgroup takes tile after tile; the stages of the next one are on their way before the last step of this one.
-//   - Loads through buffer descriptors: one 32-bit offset a lane for all tiles, rows past the end come back as zeros.
+//   - Loads through buffer descriptors: one 32-bit offset a lane for all tiles, rows past the end and what lies behind a short
+//     last block come back as zeros.
 
 typedef uint32_t srd_t __attribute__((ext_vector_type(4)));
 
@@ -410,7 +411,7 @@ __device__ __forceinline__ void srd_dma16_if(const srd_t &r, uint32_t voff, uint
                : "memory", "m0");
 }
 
-template <int MF, int NF, int WM, int WN, int ST, int MODE, bool HALF>
+template <int MF, int NF, int WM, int WN, int ST, int MODE, bool HALF, bool TAIL = false>
 __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int BM = 16 * MF * WM, BN = 16 * NF * WN, NW = WM * WN;
@@ -418,6 +419,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
   constexpr int RL = (BM + BN) / 8, PER = RL / NW, XPER = BM / 8 / NW;  // loads of 8 rows: to a stage, to a wave, of them of X
   constexpr bool DUAL = MODE == FP8_GATE_UP, GATHER = MODE == FP8_GATE_UP;
   constexpr bool ONE = HALF || MODE != FP8_DENSE;  // a fragment of X at a time, or (dense, e4m3) the last two at once
+  static_assert(!TAIL || MODE == FP8_DENSE, "short blocks");
   static_assert(MF >= 4 && MF % 2 == 0 && (!ONE || MF == 4) && RL % NW == 0 && BM / 8 % NW == 0 && BM / 64 <= NW, "tile");
   static_assert(!DUAL || (BN == 256 && NF % 2 == 0), "a tile of gate and up holds one block of 128 columns of each");
   static_assert(DUAL || 128 % (16 * NF) == 0, "a wave's rows of W lie in one block");
@@ -434,6 +436,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
   struct Tile {  // where the loads of a tile come from (wave-uniform, but for the gathered rows' offsets)
     Buf x, w, w2, s;
     uint32_t xoff[GATHER ? XPER : 1], soff;
+    int last;  // TAIL: the step whose block is short
   };
   auto buf_of = [](const void *p, int64_t bytes) {
     const uint64_t q = reinterpret_cast<uint64_t>(p);
@@ -507,6 +510,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
     }
     t.n0 = n * (DUAL ? 128 : BN);
     const int rows = min(BM, t.m_end - t.m0), cols = min(DUAL ? 128 : BN, a.N - t.n0);
+    f.last = TAIL ? nk - 1 - k0 : 0;
     f.w = buf_of(W + static_cast<int64_t>(t.n0) * a.K + 128 * k0, static_cast<int64_t>(cols) * a.K - 128 * k0);
     if constexpr (DUAL) f.w2 = buf_of(W2 + static_cast<int64_t>(t.n0) * a.K, static_cast<int64_t>(cols) * a.K);
     const int nb = (DUAL ? t.n0 : min(t.n0 + 16 * NF * wn, a.N - 1)) >> 7;
@@ -530,15 +534,18 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
     return t;
   };
   // load i of stage k of a tile, into the stage at LDS byte l
+  // (chunks behind the end of a short block: offsets past the buffer, which read as zeros)
+  const uint32_t behind = TAIL && 16 * ((lane & 7) ^ (lane >> 3)) >= (a.K & 127) ? 0x80000000u : 0u;
   auto issue1 = [&](const Tile &t, int k, uint32_t l, int i) {
     const int j = wave + NW * i;
+    const uint32_t at = TAIL ? off[i] + (k == t.last ? behind : 0u) : off[i];
     if (i < XPER) {  // (known where the loop over i is unrolled: no branch)
-      srd_dma16(srd_of(t.x), GATHER ? t.xoff[i < XPER ? i : 0] : off[i], 128 * k, l + 1024 * j);
+      srd_dma16(srd_of(t.x), GATHER ? t.xoff[i < XPER ? i : 0] : at, 128 * k, l + 1024 * j);
     } else if constexpr (DUAL) {
       const bool up = (8 * j - BM) % (16 * NF) >= 8 * NF;
-      srd_dma16(srd_of(Buf{up ? t.w2.lo : t.w.lo, up ? t.w2.hi : t.w.hi, t.w.bytes}), off[i], 128 * k, l + 1024 * j);
+      srd_dma16(srd_of(Buf{up ? t.w2.lo : t.w.lo, up ? t.w2.hi : t.w.hi, t.w.bytes}), at, 128 * k, l + 1024 * j);
     } else {
-      srd_dma16(srd_of(t.w), off[i], 128 * k, l + 1024 * j);
+      srd_dma16(srd_of(t.w), at, 128 * k, l + 1024 * j);
     }
   };
   // the scales of steps k .. k + 3 of a tile, at every fourth step: 16 bytes a row (single ones cost an address cycle a row and
@@ -654,6 +661,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
         } else {
           pick(from.x, next.x);
           pick(from.s, next.s);
+          if constexpr (TAIL) from.last = now ? next.last : from.last;
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave has read all of the stage
         wait_loads<PER *(ST - 2)>();  // its loads of the next one have arrived (its load of scales, which some waves lack, not counted)
@@ -817,7 +825,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
 }
 
 // Launch of one instantiation over `units` workgroups (below 2^22).
-template <int MF, int NF, int WM, int WN, int ST, int MODE, bool HALF>
+template <int MF, int NF, int WM, int WN, int ST, int MODE, bool HALF, bool TAIL = false>
 int fp8_mm_launch(const Fp8MmArgs &a, int64_t units, hipStream_t s) {
   constexpr int BM = 16 * MF * WM, BN = 16 * NF * WN, LDS = ST * ((BM + BN) * 128 + (BM + 63) / 64 * 256);
   static_assert(LDS <= 160 * 1024, "LDS");
@@ -832,14 +840,14 @@ int fp8_mm_launch(const Fp8MmArgs &a, int64_t units, hipStream_t s) {
 }
 
 // The pipeline: as many workgroups as the device holds at once, at most `units`.
-template <int MF, int NF, int WM, int WN, int ST, int MODE, bool HALF>
+template <int MF, int NF, int WM, int WN, int ST, int MODE, bool HALF, bool TAIL = false>
 int fp8_pipe_launch(const Fp8MmArgs &a, int64_t units, hipStream_t s) {
   constexpr int BM = 16 * MF * WM, BN = 16 * NF * WN;
   constexpr int LDS = ST * (BM + BN) * 128 + 64 * BM + (MODE == FP8_GATE_UP ? 4 * WN * BM : 0);
   static_assert(LDS <= 160 * 1024, "LDS");
   static std::atomic<uint64_t> raised{0};
   static std::atomic<int64_t> resident[64];
-  auto *fn = &k_fp8_pipe<MF, NF, WM, WN, ST, MODE, HALF>;
+  auto *fn = &k_fp8_pipe<MF, NF, WM, WN, ST, MODE, HALF, TAIL>;
   int rc = ensure_lds_limit(reinterpret_cast<const void *>(fn), LDS, raised, "fp8 product"), per_cu = 1;
   if (!rc) rc = resident_per_cu(reinterpret_cast<const void *>(fn), 64 * WM * WN, LDS, resident, per_cu, "fp8 product");
   if (rc) return rc;
