@@ -617,8 +617,8 @@ int vybdq_quant_fp8(uint64_t X, int x_dt, int64_t ldx, uint64_t Xq, uint64_t Xs,
 /* Y [M][N] (y_dt F32, F16, BF16 or F64; row stride ldy, 0 = N) = RS + sum over blocks b of Xs[m][b] Ws[n / 128][b] times the
    sum of Xq W over the block's k; RS: as Y (its row stride too) or 0. Scales may be any float32. Products are exact, sums
    over a block and over blocks are float32; for F16 and BF16 outputs a block's sum comes from the e4m3 matrix
-   instruction, which aligns its 128 products to the largest (1.4e-5 of the sum's rms for normal data, 3e-4 of the largest
-   product at most). W and Xq 16-byte aligned; Y must not overlap X (RS may be Y).
+   instruction, which aligns its 128 products to the largest (1.4e-5 of the sum's rms for normal data, and within 2^-10 of the largest
+   product). W and Xq 16-byte aligned; Y must not overlap X (RS may be Y).
    ceil(M / 128) ceil(N / 128) below 2^22, M and N below 2^24.
    ws: 256-byte aligned, any contents, or 0; with vybdq_gemm_fp8_workspace_size(M, N, K) bytes (-1: unsupported; the size covers
    every smaller M; at most 64 MiB) calls whose tiles do not fill the GPU split K and add float32 sums in a second launch (last

@@ -217,8 +217,8 @@ __device__ __forceinline__ void fp8_store(const Fp8MmArgs &a, f4 (&acc)[NF][MF],
 }
 
 // Unit u of the experts' tiles: its tile's list entry, column tile n and row tile m. The units of one expert take its row tiles
-// side by side, columns by columns: they run at the same time on one XCD and share its W (bytes from beyond the L2 at 4096 tokens,
-// 256 experts of 6144 x 2048: gate and up 10.8 -> 6.5 GB).
+// side by side, columns by columns: they run at the same time on one XCD and share its W (4096 tokens over 256 experts of
+// 6144 x 2048: the layer 4.07 ms with the tiles in list order, 3.9 so).
 __device__ __forceinline__ int4 fp8_expert_unit(const Fp8MmArgs &a, int u, int BM, int &n, int &m) {
   const int t = u / a.n_tiles;
   const int4 q = a.tiles[t];
