@@ -195,7 +195,8 @@ extern "C" int vybdq_moe_forward_fp8(uint64_t x, int x_dt, uint64_t logits, int 
                 "workspace must be 256-byte aligned and of vybdq_moe_fp8_workspace_size bytes");
   hipStream_t s = as_stream(stream);
   // rows to a tile: 16 while the experts hit have 8 each in the mean, 128 from 64 on (256 experts of 6144 x 2048, 8 to a token: 48
-  // tokens 968 us with 16, 1005 with 64; 512 tokens 1575 with 64, 1739 with 128; 4096 tokens 4113 / 3909)
+  // tokens 968 us with 16, 1005 with 64; 512 tokens 1575 with 64, 1739 with 128; 2048 tokens 2560 / 2665; 2800 tokens 3070 / 2985;
+  // 4096 tokens 4113 / 3909, with 192 rows 4150)
   const int64_t n = T * topk, hit = E < n ? E : n;
   const int BM = n <= 8 * hit ? 16 : n <= 64 * hit ? 64 : 128;
   const MoeFp8Lists lists{m.pos, m.row_map, m.ntiles, m.tiles};
