@@ -352,6 +352,17 @@ def test_route_types_with_ties(dev, rng, dt):
         check_route(dev, logits, 9, np.zeros(96), dt=dt, score=score, groups=12, top_groups=5)
 
 
+@pytest.mark.parametrize("E,groups,top,k", [(300, 1, 1, 64), (512, 1, 1, 9), (400, 2, 1, 40), (1000, 4, 2, 64), (600, 1, 1, 20)])
+def test_route_ties_among_a_lanes_entries(dev, rng, E, groups, top, k):
+    # (5 to 8 entries to a lane, then more: equal values in one lane, in several, and NaN, which come last)
+    logits = rng.integers(-1, 2, (20, E)).astype(np.float64)
+    logits[10:, ::2] = -np.inf
+    check_route(dev, logits, k, dt=torch.bfloat16, score="softmax", groups=groups, top_groups=top, group_top=1)
+    logits[15:, 1::3] = np.nan
+    check_route(dev, logits, k, dt=torch.float16, groups=groups, top_groups=top, group_top=1)
+    check_route(dev, logits[:15], k, np.zeros(E), dt=torch.float32, groups=groups, top_groups=top)
+
+
 def test_route_masked_and_saturated(dev, rng):
     logits = rng.standard_normal((12, 64)).astype(np.float32)
     logits[0] = -np.inf                     # nothing left: weights 0

@@ -741,60 +741,60 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
         xs[0] = xv[MA];
         xs[1] = xv[MA + 1];
       } else {
-      Sc sc = {0.f, 0.f};
+        Sc sc = {0.f, 0.f};
 #pragma unroll
-      for (int m = 0; m < MF - 2; ++m) {
-        xf[(m + 2) & 3] = x_of(buf, m + 2);
-        xs[(m + 2) & 3] = scale_of(cb, m + 2);
-        const Sc s = scales(m);
+        for (int m = 0; m < MF - 2; ++m) {
+          xf[(m + 2) & 3] = x_of(buf, m + 2);
+          xs[(m + 2) & 3] = scale_of(cb, m + 2);
+          const Sc s = scales(m);
+#pragma unroll
+          for (int n = 0; n < NF; ++n) {
+            if (m > 0) {
+              add(acc[n][m - 1], t[n], of(sc, n));
+            } else if (n == 0) {
+              add(acc[NF - 1][MF - 2], t[NF - 1], of(sp, NF - 1));
+              add(acc[NF - 1][MF - 1], tb, of(sq, NF - 1));
+            }
+            t[n] = fp8_block<false>(wf[n], xf[m & 3]);
+            hold();
+          }
+          sc = s;
+        }
+        const Sc s6 = scales(MF - 2), s7 = scales(MF - 1);
+        turn();
 #pragma unroll
         for (int n = 0; n < NF; ++n) {
-          if (m > 0) {
-            add(acc[n][m - 1], t[n], of(sc, n));
-          } else if (n == 0) {
-            add(acc[NF - 1][MF - 2], t[NF - 1], of(sp, NF - 1));
-            add(acc[NF - 1][MF - 1], tb, of(sq, NF - 1));
+          if (n == 0) {
+            xf[MF & 3] = x_of(nbuf, 0);
+            xs[MF & 3] = scale_of(cn, 0);
           }
-          t[n] = fp8_block<false>(wf[n], xf[m & 3]);
+          if (n == (NF > 1 ? 1 : 0)) {
+            xf[(MF + 1) & 3] = x_of(nbuf, 1);
+            xs[(MF + 1) & 3] = scale_of(cn, 1);
+          }
+          add(acc[n][MF - 3], t[n], of(sc, n));
+          if (n > 0) {
+            add(acc[n - 1][MF - 2], t[n - 1], of(s6, n - 1));
+            add(acc[n - 1][MF - 1], tb, of(s7, n - 1));
+          }
+          t[n] = fp8_block<false>(wf[n], xf[(MF - 2) & 3]);
+          tb = fp8_block<false>(wf[n], xf[(MF - 1) & 3]);
+          wf[n] = frag(nbuf + wo + 2048 * n);
+#pragma unroll
+          for (int i = n * PER / NF; i < (n + 1) * PER / NF; ++i) issue1(from, kk, lds0 + sb, i);
+          if (n == NF - 1) issue_s(from, kk);
           hold();
         }
-        sc = s;
-      }
-      const Sc s6 = scales(MF - 2), s7 = scales(MF - 1);
-      turn();
-#pragma unroll
-      for (int n = 0; n < NF; ++n) {
-        if (n == 0) {
-          xf[MF & 3] = x_of(nbuf, 0);
-          xs[MF & 3] = scale_of(cn, 0);
+        if constexpr (MF % 4 != 0) {  // the ring's first places are fragments 0 and 1
+          const i8v x0 = xf[MF & 3], x1 = xf[(MF + 1) & 3];
+          const float f0 = xs[MF & 3], f1 = xs[(MF + 1) & 3];
+          xf[0] = x0;
+          xf[1] = x1;
+          xs[0] = f0;
+          xs[1] = f1;
         }
-        if (n == (NF > 1 ? 1 : 0)) {
-          xf[(MF + 1) & 3] = x_of(nbuf, 1);
-          xs[(MF + 1) & 3] = scale_of(cn, 1);
-        }
-        add(acc[n][MF - 3], t[n], of(sc, n));
-        if (n > 0) {
-          add(acc[n - 1][MF - 2], t[n - 1], of(s6, n - 1));
-          add(acc[n - 1][MF - 1], tb, of(s7, n - 1));
-        }
-        t[n] = fp8_block<false>(wf[n], xf[(MF - 2) & 3]);
-        tb = fp8_block<false>(wf[n], xf[(MF - 1) & 3]);
-        wf[n] = frag(nbuf + wo + 2048 * n);
-#pragma unroll
-        for (int i = n * PER / NF; i < (n + 1) * PER / NF; ++i) issue1(from, kk, lds0 + sb, i);
-        if (n == NF - 1) issue_s(from, kk);
-        hold();
-      }
-      if constexpr (MF % 4 != 0) {  // the ring's first places are fragments 0 and 1
-        const i8v x0 = xf[MF & 3], x1 = xf[(MF + 1) & 3];
-        const float f0 = xs[MF & 3], f1 = xs[(MF + 1) & 3];
-        xf[0] = x0;
-        xf[1] = x1;
-        xs[0] = f0;
-        xs[1] = f1;
-      }
-      sp = s6;
-      sq = s7;
+        sp = s6;
+        sq = s7;
       }
       w0 = w0n;
       w1 = w1n;
