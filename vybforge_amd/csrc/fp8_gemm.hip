@@ -52,7 +52,8 @@ static int64_t fp8_part_bytes(int64_t M, int64_t N, int64_t K) {
 // Tile height and splits with the least estimate: rounds of tiles over the chip, a round its K steps and its end; split sums written,
 // read and added. Times in us fitted over 26 shapes from 16 to 2048 rows (both instructions) with every tile and up to 16 splits
 // forced: 9% off in the mean over 200 of them, the choice never more than 2% above the best of them; with the tiles of 192 rows
-// (512 x 17408 x 5120 61 us, the others 72 to 82; 2048 rows 174 / 207), 11 more shapes up to 4096 rows: at most 3%.
+// (512 x 17408 x 5120 62 us, the others 68 to 81; 2048 rows 176 / 207), 11 more shapes up to 4096 rows: at most 5% (4096 x 9728 x 2560
+// 131 us, 124 with 128 rows). A K that ends inside a block: 512 x 17408 x 5136 84 us with the same estimate.
 static Fp8Plan fp8_plan(int64_t M, int64_t N, int64_t K, bool half, int64_t part) {
   const int64_t nk = (K + 127) / 128, cus = device_cu_count();
   Fp8Plan best{0, 1};
