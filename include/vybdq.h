@@ -610,15 +610,16 @@ int vybdq_kv_status(void);
 
    vybdq_quant_fp8: X (x_dt F32, F16 or BF16, row stride ldx in elements) to Xq, Xs. Scale = 2^e with the least e in -100 .. 120
    for which every |x| of the block is at most 448 * 2^e, code = e4m3(x / scale) to nearest, ties to even (one rounding: the
-   division is exact). A block with an infinity or NaN has the scale NaN. Rows of X and Xq 16-byte aligned; Xq and Xs must not
-   overlap X; M ceil(K / 128) below 2^28. */
+   division is exact). A block with an infinity or NaN has the scale NaN. Rows of X and Xq 16-byte aligned; X, Xq and Xs must not
+   overlap (here and below: share a byte; neighbouring columns of one wider matrix do not); M ceil(K / 128) below 2^28. */
 int vybdq_quant_fp8(uint64_t X, int x_dt, int64_t ldx, uint64_t Xq, uint64_t Xs, int64_t M, int64_t K, uint64_t stream);
 
 /* Y [M][N] (y_dt F32, F16, BF16 or F64; row stride ldy, 0 = N) = RS + sum over blocks b of Xs[m][b] Ws[n / 128][b] times the
    sum of Xq W over the block's k; RS: as Y (its row stride too) or 0. Scales may be any float32. Products are exact, sums
    over a block and over blocks are float32; for F16 and BF16 outputs a block's sum comes from the e4m3 matrix
    instruction, which aligns its 128 products to the largest (1.4e-5 of the sum's rms for normal data, and within 2^-10 of the largest
-   product). W and Xq 16-byte aligned; Y must not overlap X (RS may be Y).
+   product). W and Xq 16-byte aligned; Y must not overlap X, W, Ws or RS (RS may be Y itself), nor the part of ws that is used
+   any of these.
    ceil(M / 128) ceil(N / 128) below 2^22, M and N below 2^24.
    ws: 256-byte aligned, any contents, or 0; with vybdq_gemm_fp8_workspace_size(M, N, K) bytes (-1: unsupported; the size covers
    every smaller M; at most 64 MiB) calls whose tiles do not fill the GPU split K and add float32 sums in a second launch (last
@@ -627,8 +628,8 @@ int64_t vybdq_gemm_fp8_workspace_size(int64_t M, int64_t N, int64_t K);
 int vybdq_gemm_fp8(uint64_t W, uint64_t Ws, uint64_t Xq, uint64_t Xs, uint64_t Y, int64_t M, int64_t N, int64_t K, int y_dt,
                    int64_t ldy, uint64_t RS, uint64_t ws, int64_t ws_bytes, uint64_t stream);
 
-/* vybdq_quant_fp8 and vybdq_gemm_fp8 in one call: X x_dt, row stride ldx; Y must not overlap X. ws: 256-byte aligned, of
-   vybdq_linear_fp8_workspace_size(M, N, K) bytes (-1: unsupported), any contents; the size covers every smaller M. Calls that
+/* vybdq_quant_fp8 and vybdq_gemm_fp8 in one call: X x_dt, row stride ldx; what must not overlap there must not here. ws: 256-byte
+   aligned, of vybdq_linear_fp8_workspace_size(M, N, K) bytes (-1: unsupported), any contents; the size covers every smaller M. Calls that
    share a workspace must not overlap. */
 int64_t vybdq_linear_fp8_workspace_size(int64_t M, int64_t N, int64_t K);
 int vybdq_linear_fp8(uint64_t W, uint64_t Ws, uint64_t X, int x_dt, int64_t ldx, uint64_t Y, int64_t M, int64_t N, int64_t K,
@@ -640,7 +641,7 @@ int vybdq_linear_fp8(uint64_t W, uint64_t Ws, uint64_t X, int x_dt, int64_t ldx,
    best choices, descending; w_out float32 [T][topk] = score, over (their sum + 1e-20) with renorm = 1, times scale. Ties go
    to the lower id. float64 throughout, rounded once; without a bias choices compare as their logits do. A NaN comes below every number.
    vybdq_moe_route is the case softmax = 0, renorm = 1, groups = 1. E up to 1024, topk up to 64 and within
-   top_groups * E / groups. */
+   top_groups * E / groups. idx_out and w_out must not overlap each other, the logits or the bias. */
 int vybdq_moe_route_groups(uint64_t logits, int logits_dt, uint64_t bias, uint64_t idx_out, uint64_t w_out, int64_t T, int64_t E,
                            int64_t topk, double scale, int softmax, int renorm, int64_t groups, int64_t top_groups,
                            int64_t group_top, uint64_t stream);
@@ -653,7 +654,8 @@ int64_t vybdq_moe_fp8_workspace_size(int64_t T, int64_t H, int64_t I, int64_t E,
    quantized as vybdq_quant_fp8 does (a from its float32 values); everything else is float32. Experts: gate, up e4m3
    [E][I][H], down [E][H][I] with scales [E][I / 128][H / 128] and [E][H / 128][I / 128]; the shared expert (weight 1) one such
    matrix each, or all six 0. H and I multiples of 128. idx_out, w_out (optional) receive the routing. x, out and codes 16-byte
-   aligned. ws: 256-byte aligned, vybdq_moe_fp8_workspace_size bytes, any contents; calls that share one must not overlap. */
+   aligned. out may lie over x and the logits; idx_out, w_out and ws must not overlap each other, out or an input. ws: 256-byte
+   aligned, vybdq_moe_fp8_workspace_size bytes, any contents; calls that share one must not overlap. */
 int vybdq_moe_forward_fp8(uint64_t x, int x_dt, uint64_t logits, int logits_dt, uint64_t bias, uint64_t gate, uint64_t gate_s,
                           uint64_t up, uint64_t up_s, uint64_t down, uint64_t down_s, uint64_t sh_gate, uint64_t sh_gate_s,
                           uint64_t sh_up, uint64_t sh_up_s, uint64_t sh_down, uint64_t sh_down_s, uint64_t out, int out_dt,

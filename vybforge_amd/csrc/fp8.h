@@ -10,7 +10,9 @@
 
 #include "common.h"
 
+#include <initializer_list>
 #include <type_traits>
+#include <utility>
 
 namespace vybdq {
 
@@ -60,9 +62,35 @@ __device__ __forceinline__ uint32_t row16_max_u32(uint32_t v) {
   return v;
 }
 
-// Whether [a, a + na) and [b, b + nb) share a byte.
-inline bool fp8_overlap(uint64_t a, int64_t na, uint64_t b, int64_t nb) {
-  return a < b + static_cast<uint64_t>(nb) && b < a + static_cast<uint64_t>(na);
+// Rows of `width` bytes every `pitch` bytes from `at` on (width <= pitch).
+struct Fp8Span {
+  uint64_t at;
+  int64_t rows, width, pitch;
+};
+inline Fp8Span fp8_bytes(uint64_t at, int64_t n) { return {at, 1, n, n}; }
+
+// Whether two buffers share a byte: exact, so that neighbouring columns of one wider matrix pass.
+inline bool fp8_overlap(Fp8Span a, Fp8Span b) {
+  for (Fp8Span *s : {&a, &b})
+    if (s->rows == 1 || s->pitch == s->width) *s = fp8_bytes(s->at, s->rows * s->width);
+  auto size = [](const Fp8Span &s) { return s.width > 0 ? static_cast<uint64_t>((s.rows - 1) * s.pitch + s.width) : 0; };
+  if (!a.at || !b.at || size(a) == 0 || size(b) == 0) return false;  // (0: not given)
+  if (a.at >= b.at + size(b) || b.at >= a.at + size(a)) return false;
+  if (a.rows == 1) std::swap(a, b);
+  // one row of b: whether the first row of a that ends behind its start begins before its end
+  auto row = [&](uint64_t at) {
+    const int64_t d = static_cast<int64_t>(at - a.at), i = d < a.width ? 0 : (d - a.width) / a.pitch + 1;
+    return i < a.rows && i * a.pitch < d + b.width;
+  };
+  if (b.rows == 1) return row(b.at);
+  if (a.pitch == b.pitch) {  // b's row j begins d bytes into row j + q of a's pitch
+    if (a.at > b.at) std::swap(a, b);
+    const int64_t q = static_cast<int64_t>(b.at - a.at) / a.pitch, d = static_cast<int64_t>(b.at - a.at) % a.pitch;
+    return (q < a.rows && d < a.width) || (q + 1 < a.rows && d + b.width > a.pitch);
+  }
+  for (int64_t j = 0; j < b.rows; ++j)
+    if (row(b.at + static_cast<uint64_t>(j * b.pitch))) return true;
+  return false;
 }
 
 int fp8_quant_rows(const void *X, int x_dt, int64_t M, int64_t K, int64_t ldx, uint8_t *Xq, float *Xs, hipStream_t s);

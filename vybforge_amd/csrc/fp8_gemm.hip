@@ -206,6 +206,24 @@ static int fp8_check(const char *func, int64_t M, int64_t N, int64_t K, uint64_t
   return VYBDQ_OK;
 }
 
+// Y and the workspace are written while workgroups still read everything else; RS may be Y itself, whose elements are read by the
+// thread that writes them.
+static int fp8_check_overlap(const char *func, int64_t M, int64_t N, int64_t K, uint64_t W, uint64_t Ws, uint64_t Y, int y_dt,
+                             int64_t ldy, uint64_t RS, const Fp8Span &ws, std::initializer_list<Fp8Span> x) {
+  auto bad = [&](const char *msg) { return set_error(VYBDQ_ERR_ARG, std::string(func) + ": " + msg); };
+  const Fp8Span y{Y, M, N * dt_size(y_dt), ldy * dt_size(y_dt)}, rs{RS, M, y.width, y.pitch};
+  const Fp8Span w = fp8_bytes(W, N * K), s = fp8_bytes(Ws, (N + 127) / 128 * ((K + 127) / 128) * 4);
+  for (const Fp8Span &in : x) {
+    if (fp8_overlap(y, in)) return bad("Y must not overlap X: workgroups read X while others write");
+    if (fp8_overlap(ws, in)) return bad("the workspace must not overlap X");
+  }
+  if (fp8_overlap(y, w) || fp8_overlap(y, s)) return bad("Y must not overlap W or Ws");
+  if (RS != Y && fp8_overlap(y, rs)) return bad("RS must be Y or not overlap it");
+  if (fp8_overlap(ws, w) || fp8_overlap(ws, s) || fp8_overlap(ws, y) || fp8_overlap(ws, rs))
+    return bad("the workspace must not overlap W, Ws, Y or RS");
+  return VYBDQ_OK;
+}
+
 extern "C" int64_t vybdq_gemm_fp8_workspace_size(int64_t M, int64_t N, int64_t K) {
   if (M < 0 || M >= (int64_t(1) << 24) || N < 1 || N >= (int64_t(1) << 24) || K < 16 || K % 16 || K >= (int64_t(1) << 23)) return -1;
   return align256(fp8_part_bytes(M < 1024 ? M : 1024, N, K));  // (rises with M, none above 1024)
@@ -218,9 +236,10 @@ extern "C" int vybdq_gemm_fp8(uint64_t W, uint64_t Ws, uint64_t Xq, uint64_t Xs,
   VYBDQ_REQUIRE(Xq && Xs, VYBDQ_ERR_ARG, "null buffer");
   VYBDQ_REQUIRE(Xq % 16 == 0 && Xs % 4 == 0, VYBDQ_ERR_ALIGN, "Xq must be 16-byte and Xs 4-byte aligned");
   VYBDQ_REQUIRE(ws % 256 == 0 && ws_bytes >= 0, VYBDQ_ERR_WORKSPACE, "workspace must be 256-byte aligned");
-  const int64_t yb = ((M - 1) * ldy + N) * dt_size(y_dt);
-  VYBDQ_REQUIRE(!fp8_overlap(Y, yb, Xq, M * K) && !fp8_overlap(Y, yb, Xs, M * ((K + 127) / 128) * 4), VYBDQ_ERR_ARG,
-                "Y must not overlap X: workgroups read X while others write");
+  const int64_t part = fp8_part_bytes(M, N, K), used = ws && ws_bytes >= part ? part : 0;
+  const int orc = fp8_check_overlap(__func__, M, N, K, W, Ws, Y, y_dt, ldy, RS, fp8_bytes(ws, used),
+                                    {fp8_bytes(Xq, M * K), fp8_bytes(Xs, M * ((K + 127) / 128) * 4)});
+  if (orc) return orc;
   return fp8_gemm(fp8_args(reinterpret_cast<const uint8_t *>(W), reinterpret_cast<const float *>(Ws),
                            reinterpret_cast<const uint8_t *>(Xq), reinterpret_cast<const float *>(Xs), reinterpret_cast<void *>(Y),
                            y_dt, M, N, K, ldy, reinterpret_cast<const void *>(RS)),
@@ -243,8 +262,9 @@ extern "C" int vybdq_linear_fp8(uint64_t W, uint64_t Ws, uint64_t X, int x_dt, i
   VYBDQ_REQUIRE(X % 16 == 0 && (M == 1 || ldx * dt_size(x_dt) % 16 == 0), VYBDQ_ERR_ALIGN, "rows of X must be 16-byte aligned");
   VYBDQ_REQUIRE(ws && ws % 256 == 0 && ws_bytes >= vybdq_linear_fp8_workspace_size(M, N, K), VYBDQ_ERR_WORKSPACE,
                 "workspace must be 256-byte aligned and of vybdq_linear_fp8_workspace_size bytes");
-  VYBDQ_REQUIRE(!fp8_overlap(Y, ((M - 1) * ldy + N) * dt_size(y_dt), X, ((M - 1) * (M > 1 ? ldx : K) + K) * dt_size(x_dt)), VYBDQ_ERR_ARG,
-                "Y must not overlap X: workgroups read X while others write");
+  const int orc = fp8_check_overlap(__func__, M, N, K, W, Ws, Y, y_dt, ldy, RS, fp8_bytes(ws, vybdq_linear_fp8_workspace_size(M, N, K)),
+                                    {Fp8Span{X, M, K * dt_size(x_dt), ldx * dt_size(x_dt)}});
+  if (orc) return orc;
   uint8_t *xq = reinterpret_cast<uint8_t *>(ws);
   float *xs = reinterpret_cast<float *>(ws + align256(M * K));
   const int64_t front = align256(M * K) + align256(M * ((K + 127) / 128) * 4);

@@ -52,7 +52,8 @@ extern "C" int vybdq_quant_fp8(uint64_t X, int x_dt, int64_t ldx, uint64_t Xq, u
   VYBDQ_REQUIRE(M == 1 || ldx >= K, VYBDQ_ERR_SHAPE, "ldx is smaller than a row");
   VYBDQ_REQUIRE((X | Xq) % 16 == 0 && (M == 1 || ldx * dt_size(x_dt) % 16 == 0) && Xs % 4 == 0, VYBDQ_ERR_ALIGN,
                 "rows of X and Xq must be 16-byte aligned, Xs 4-byte");
-  VYBDQ_REQUIRE(!fp8_overlap(X, ((M - 1) * (M > 1 ? ldx : K) + K) * dt_size(x_dt), Xq, M * K), VYBDQ_ERR_ARG, "Xq must not overlap X");
+  const Fp8Span x{X, M, K * dt_size(x_dt), ldx * dt_size(x_dt)}, xq = fp8_bytes(Xq, M * K), xs = fp8_bytes(Xs, M * ((K + 127) / 128) * 4);
+  VYBDQ_REQUIRE(!fp8_overlap(x, xq) && !fp8_overlap(x, xs) && !fp8_overlap(xq, xs), VYBDQ_ERR_ARG, "X, Xq and Xs must not overlap");
   return fp8_quant_rows(reinterpret_cast<const void *>(X), x_dt, M, K, ldx, reinterpret_cast<uint8_t *>(Xq),
                         reinterpret_cast<float *>(Xs), as_stream(stream));
 }

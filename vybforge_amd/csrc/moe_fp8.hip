@@ -193,6 +193,24 @@ extern "C" int vybdq_moe_forward_fp8(uint64_t x, int x_dt, uint64_t logits, int 
                 VYBDQ_ERR_ALIGN, "x, out and codes must be 16-byte aligned, scales 4-byte");
   VYBDQ_REQUIRE(ws && ws % 256 == 0 && ws_bytes >= m.bytes, VYBDQ_ERR_WORKSPACE,
                 "workspace must be 256-byte aligned and of vybdq_moe_fp8_workspace_size bytes");
+  {
+    // (x and logits have been read when out is written, so it may lie over them)
+    const int64_t wb = I * H, sb = (I / 128) * (H / 128) * 4;
+    Fp8Span in[15] = {fp8_bytes(x, T * H * dt_size(x_dt)), fp8_bytes(logits, T * E * dt_size(logits_dt)),
+                      fp8_bytes(bias, 4 * E)};
+    int n_in = 3;
+    for (const uint64_t p : {gate, up, down}) in[n_in++] = fp8_bytes(p, E * wb);
+    for (const uint64_t p : {gate_s, up_s, down_s}) in[n_in++] = fp8_bytes(p, E * sb);
+    for (const uint64_t p : {sh_gate, sh_up, sh_down}) in[n_in++] = fp8_bytes(p, wb);
+    for (const uint64_t p : {sh_gate_s, sh_up_s, sh_down_s}) in[n_in++] = fp8_bytes(p, sb);
+    const Fp8Span o = fp8_bytes(out, T * H * dt_size(out_dt)), i = fp8_bytes(idx_out, 4 * T * topk), w = fp8_bytes(w_out, 4 * T * topk);
+    const Fp8Span work = fp8_bytes(ws, m.bytes);
+    bool alias = fp8_overlap(i, w);
+    for (const Fp8Span &r : {o, i, w}) alias = alias || fp8_overlap(work, r);
+    for (const Fp8Span &r : {i, w}) alias = alias || fp8_overlap(o, r);
+    for (const Fp8Span &r : in) alias = alias || fp8_overlap(work, r) || fp8_overlap(i, r) || fp8_overlap(w, r);
+    VYBDQ_REQUIRE(!alias, VYBDQ_ERR_ARG, "idx_out, w_out and the workspace must not overlap each other, out or an input");
+  }
   hipStream_t s = as_stream(stream);
   // rows to a tile: 16 while the experts hit have 8 each in the mean, 128 from 64 on (256 experts of 6144 x 2048, 8 to a token: 48
   // tokens 968 us with 16, 1005 with 64; 512 tokens 1575 with 64, 1739 with 128; 2048 tokens 2560 / 2665; 2800 tokens 3070 / 2985;

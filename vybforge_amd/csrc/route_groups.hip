@@ -1,4 +1,5 @@
 // The router of route_groups.h by itself: four tokens to a workgroup, one to a wave.
+#include "fp8.h"
 #include "route_groups.h"
 
 namespace vybdq {
@@ -51,5 +52,10 @@ extern "C" int vybdq_moe_route_groups(uint64_t logits, int logits_dt, uint64_t b
   const int rc = route_groups_args(__func__, a, logits, logits_dt, bias, idx_out, w_out, T, E, topk, scale, softmax, renorm,
                                    groups, top_groups, group_top);
   if (rc || T == 0) return rc;
+  const Fp8Span in[2] = {fp8_bytes(logits, T * E * dt_size(logits_dt)), fp8_bytes(bias, 4 * E)};
+  const Fp8Span i = fp8_bytes(idx_out, 4 * T * topk), w = fp8_bytes(w_out, 4 * T * topk);
+  bool alias = fp8_overlap(i, w);
+  for (const Fp8Span &r : in) alias = alias || fp8_overlap(r, i) || fp8_overlap(r, w);
+  VYBDQ_REQUIRE(!alias, VYBDQ_ERR_ARG, "idx_out and w_out must not overlap each other, the logits or the bias");
   return route_groups_launch(a, as_stream(stream));
 }
