@@ -615,10 +615,11 @@ int vybdq_kv_status(void);
 int vybdq_quant_fp8(uint64_t X, int x_dt, int64_t ldx, uint64_t Xq, uint64_t Xs, int64_t M, int64_t K, uint64_t stream);
 
 /* Y [M][N] (y_dt F32, F16, BF16 or F64; row stride ldy, 0 = N) = RS + sum over blocks b of Xs[m][b] Ws[n / 128][b] times the
-   sum of Xq W over the block's k; RS: as Y (its row stride too) or 0. Scales may be any float32. Products are exact, sums
-   over a block and over blocks are float32; for F16 and BF16 outputs a block's sum comes from the e4m3 matrix
-   instruction, which aligns its 128 products to the largest (1.4e-5 of the sum's rms for normal data, and within 2^-10 of the largest
-   product). W and Xq 16-byte aligned; Y must not overlap X, W, Ws or RS (RS may be Y itself), nor the part of ws that is used
+   sum of Xq W over the block's k; RS: as Y (its row stride too) or 0. Products of codes are exact, sums over a block and over blocks
+   are float32. Scales are any float32 whose products Xs Ws float32 holds: it rounds them once, and one past its range makes the
+   outputs infinite or NaN. For F16 and BF16 outputs a block's sum comes from the e4m3 matrix instruction, which cuts the products of
+   every eight neighbouring k below 2^-13 of the largest of the eight, a subnormal code counted as 2^-6: 1.4e-5 of the sum's rms for
+   normal data, at most 2^-10 of the sum of the products' magnitudes so counted. (An F32 output has no such loss.) W and Xq 16-byte aligned; Y must not overlap X, W, Ws or RS (RS may be Y itself), nor the part of ws that is used
    any of these.
    ceil(M / 128) ceil(N / 128) below 2^22, M and N below 2^24.
    ws: 256-byte aligned, any contents, or 0; with vybdq_gemm_fp8_workspace_size(M, N, K) bytes (-1: unsupported; the size covers
@@ -651,7 +652,8 @@ int64_t vybdq_moe_fp8_workspace_size(int64_t T, int64_t H, int64_t I, int64_t E,
 
 /* out [T][H] (F32, F16 or BF16) = sum over s of w[t, s] FFN_idx[t, s](x[t]) + FFN_shared(x[t]), routed as vybdq_moe_route_groups
    does, FFN(x) = a Wd with a = silu(min(x Wg, limit)) * clamp(x Wu, -limit, limit) (limit > 0, infinity: none). x and a are
-   quantized as vybdq_quant_fp8 does (a from its float32 values); everything else is float32. Experts: gate, up e4m3
+   quantized as vybdq_quant_fp8 does (a from its float32 values); everything else is float32, but that under an F16 or BF16 out the
+   sums of a Wd drop what those of vybdq_gemm_fp8 do. Experts: gate, up e4m3
    [E][I][H], down [E][H][I] with scales [E][I / 128][H / 128] and [E][H / 128][I / 128]; the shared expert (weight 1) one such
    matrix each, or all six 0. H and I multiples of 128. idx_out, w_out (optional) receive the routing. x, out and codes 16-byte
    aligned. out may lie over x and the logits; idx_out, w_out and ws must not overlap each other, out or an input. ws: 256-byte

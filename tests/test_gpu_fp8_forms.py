@@ -1,16 +1,20 @@
 """8-bit floating-point weights on the GPU, form by form, on data whose result is known to the last bit or bounded by arithmetic: what
-may lie beside what."""
+may lie beside what, and what the e4m3 instruction drops."""
 
 import numpy as np
 import pytest
 import torch
 
 from oracle import fp8
+from oracle.kvcache import e4m3_decode
+from tests.e4m3_cases import hard_codes
 from vybforge_amd import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
 E4M3 = torch.float8_e4m3fn
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "f64": torch.float64}
+HALF = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8, "f64": 2.0 ** -24}  # half a step of the last rounding, relative
 
 
 def stream():
@@ -84,3 +88,37 @@ def test_layer_output_over_its_input(dev, rng):
         x, logits = torch.randn(T, H, device=dev), torch.randn(T, E, device=dev)
         want, v = layer(x, logits), x.clone()
         assert layer(v, logits, out=v) is v and torch.equal(v, want)
+
+
+# ---- the e4m3 instruction ---------------------------------------------------------------------------
+
+# (rows, K, forced tile): few rows, the tiles for short K, every tile of the pipeline with whole and short last blocks
+FORMS = [(1, 640, None), (12, 1040, None), (40, 384, None), (100, 400, None), (520, 256, None), (40, 640, "64,1"), (40, 528, "64,1"),
+         (60, 1152, "64,2"), (130, 640, "128,1"), (130, 528, "128,1"), (200, 640, "192,1"), (270, 640, "256,1"), (270, 528, "256,1")]
+
+
+@pytest.mark.parametrize("kind", ["large", "subnormal", "spread", "normal"])
+@pytest.mark.parametrize("y", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("M,K,tile", FORMS)
+def test_what_the_instruction_drops(dev, rng, monkeypatch, M, K, tile, y, kind):
+    """16-bit outputs are the instruction's sums to float32, so within the bound of what it drops; float32 outputs drop nothing. What
+    float32 adds: each of a block's 128 products and of the KB blocks rounds, or is cut, by 2^-23 of the partial sums at most, with
+    two for the scales' products (as everywhere here); the codes' scales are 1, and float16 is kept off its border by 2^-12."""
+    if tile:
+        monkeypatch.setenv("VYBDQ_FP8_TILE", tile)
+    N, KB = 300, fp8.blocks(K)
+    some = np.unique(np.r_[0, M - 1, rng.integers(0, M, 10)])  # (the oracle's rows)
+    xc, wc = hard_codes(rng, M, N, K, kind)
+    f = np.float32(2.0 ** -12)
+    work = ops.Fp8Workspace([(M, N, K)], dev)
+    got = ops.gemm_fp8(torch.from_numpy(wc).to(dev).view(E4M3), torch.full((fp8.blocks(N), KB), float(f), device=dev),
+                       torch.from_numpy(xc).to(dev).view(E4M3), torch.ones(M, KB, device=dev), y_dtype=DT[y], workspace=work)
+    got, xs = got.double().cpu().numpy()[some], xc[some]
+    X, W = e4m3_decode(xs), e4m3_decode(wc)
+    exact, size = f * (X @ W.T), f * (np.abs(X) @ np.abs(W).T)
+    want = exact if y == "f32" else f * fp8.e4m3_instruction(xs, wc).sum(-1)
+    tol = (130 + KB) * 2.0 ** -23 * size
+    last = lambda v, t: HALF[y] * (np.abs(v) + t) + (2.0 ** -25 if y == "f16" else 0)
+    assert (np.abs(got - want) <= tol + last(want, tol)).all(), np.abs(got - want).max()
+    tol += 0 if y == "f32" else f * fp8.e4m3_loss(xs, wc)
+    assert (np.abs(got - exact) <= tol + last(exact, tol)).all()

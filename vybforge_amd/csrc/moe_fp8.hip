@@ -279,6 +279,7 @@ extern "C" int vybdq_moe_forward_fp8(uint64_t x, int x_dt, uint64_t logits, int 
   d.row_map = nullptr;
   d.Y = m.rows;
   d.ldy = H;
+  // (down's sums are not quantized again: a 16-bit out takes the e4m3 instruction as a 16-bit Y of the product does)
   rc = out_dt == VYBDQ_F32 ? moe_fp8_mm<FP8_DOWN, true>(BM, d, tiles, s) : moe_fp8_mm<FP8_DOWN, false>(BM, d, tiles, s);
   if (rc) return rc;
   const float *sh = shared ? m.rows + n * H : nullptr;
