@@ -17,7 +17,6 @@
 namespace vybdq {
 
 constexpr int kFp8ExpMin = -100, kFp8ExpMax = 120;
-constexpr float kFp8Max = 448.0f;
 
 typedef int i8v __attribute__((ext_vector_type(8)));
 

@@ -96,7 +96,7 @@ static bool fp8_rows_quant(int64_t M, int64_t N, int64_t K) {
 // 16 waves from 32 blocks of K, else 8 (1 x 2560 x 9728 10.0 us against 12.0; 1 x 6144 x 2048 9.5 / 8.9).
 template <int XDT, bool HALF>
 static int fp8_rows_run(const Fp8RowsArgs &r, hipStream_t s) {
-  return r.m.KB >= 32 ? fp8_rows_launch<1, 1, 16, 3, XDT, HALF>(r, s) : fp8_rows_launch<1, 1, 8, 3, XDT, HALF>(r, s);
+  return r.m.KB >= 32 ? fp8_rows_launch<16, 3, XDT, HALF>(r, s) : fp8_rows_launch<8, 3, XDT, HALF>(r, s);
 }
 
 template <bool HALF, bool TAIL>

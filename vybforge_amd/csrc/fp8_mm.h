@@ -634,7 +634,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
     const float *ws = at.ws, *ws2 = at.ws2;
     float w0 = uniform_load(ws, 0), w1 = DUAL ? uniform_load(ws2, 0) : 0.f;
     const int nk = at.nk;
-    // step k with the first MA of MF fragments of X
+    // step k with the first MA of MF fragments of X (all, or 2)
     auto step = [&](auto ma, int k) {
       constexpr int MA = decltype(ma)::value;
       const uint32_t sn = sb + STAGE == ST * STAGE ? 0 : sb + STAGE;
@@ -682,11 +682,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
         xv[1] = xs[1];
 #pragma unroll
         for (int m = 0; m < MA; ++m) {
-          if (m == (MA > 2 ? MA - 2 : 0)) turn();
-          if (MA == 1) {  // (what was read ahead as fragment 1 is not the next step's first)
-            xr[1] = x_of(nbuf, 0);
-            xv[1] = scale_of(cn, 0);
-          }
+          if (m == MA - 2) turn();
           xr[m + 2] = m + 2 < MA ? x_of(buf, m + 2) : x_of(nbuf, m + 2 - MA);
           xv[m + 2] = m + 2 < MA ? scale_of(cb, m + 2) : scale_of(cn, m + 2 - MA);
           if (HALF && m == 0)
@@ -698,7 +694,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
           // the loads of the stage ST steps on, spread over what is left of the step: issued together they hold up the instructions
           // behind them until the address unit has taken them all
           constexpr int SUB = HALF ? 1 : NF, BY = NF / SUB;  // parts of a fragment's products, columns to a part
-          constexpr int LAST = MA > 1 ? 2 : 1, SLOTS = LAST * SUB;
+          constexpr int SLOTS = 2 * SUB;
           h8 xn[HALF ? 4 : 1];
 #pragma unroll
           for (int p = 0; p < SUB; ++p) {
@@ -726,8 +722,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
 #pragma unroll
               for (int n = p * BY; n < (p + 1) * BY; ++n) wf[n] = frag(nbuf + wo + 2048 * n);
             hold();
-            if (m >= MA - LAST) {
-              const int q = (m - (MA - LAST)) * SUB + p;
+            if (m >= MA - 2) {
+              const int q = (m - (MA - 2)) * SUB + p;
 #pragma unroll
               for (int i = q * PER / SLOTS; i < (q + 1) * PER / SLOTS; ++i) issue1(from, kk, lds0 + sb, i);
               if (q == SLOTS - 1) issue_s(from, kk);
@@ -771,7 +767,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
             xf[MF & 3] = x_of(nbuf, 0);
             xs[MF & 3] = scale_of(cn, 0);
           }
-          if (n == (NF > 1 ? 1 : 0)) {
+          if (n == 1) {
             xf[(MF + 1) & 3] = x_of(nbuf, 1);
             xs[(MF + 1) & 3] = scale_of(cn, 1);
           }
@@ -828,7 +824,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_fp8_pipe(const Fp8MmArgs a) {
 }
 
 // Launch of one instantiation over `units` workgroups (below 2^22).
-template <int MF, int NF, int WM, int WN, int ST, int MODE, bool HALF, bool TAIL = false>
+template <int MF, int NF, int WM, int WN, int ST, int MODE, bool HALF>
 int fp8_mm_launch(const Fp8MmArgs &a, int64_t units, hipStream_t s) {
   constexpr int BM = 16 * MF * WM, BN = 16 * NF * WN, LDS = ST * ((BM + BN) * 128 + (BM + 63) / 64 * 256);
   static_assert(LDS <= 160 * 1024, "LDS");

@@ -1,8 +1,8 @@
 // Few rows of X times an e4m3 matrix: W streamed once from memory into registers, gfx950.
 //
-// A workgroup takes 16 NF rows of W and all rows of X; its NW waves deal the K blocks among themselves (wave w: blocks w, w + NW,
+// A workgroup takes 16 rows of W and all rows of X (up to 16); its NW waves deal the K blocks among themselves (wave w: blocks w, w + NW,
 // ..), so that together they read a row's bytes in order, and each sums its blocks' products in registers; the waves' sums are
-// added through LDS in wave order. A wave asks for D blocks of W at once and has no wait but for them: D 16 NF 128 bytes
+// added through LDS in wave order. A wave asks for D blocks of W at once and has no wait but for them: D 16 128 bytes
 // in flight to a wave.
 //   LDSX: X comes as x_dt and is quantized (fp8.h) by every workgroup for itself into LDS, while its first loads of W are on their
 //     way; otherwise X is codes and scales in memory, read like W (from L2).
@@ -17,10 +17,10 @@ namespace vybdq {
 // One row's 16-byte chunk q of LDS codes: blocks of 128 bytes, the chunks of a block at chunk ^ (row & 7).
 __device__ __forceinline__ int rows_chunk(int row, int q, int KB) { return (row * KB + (q >> 3)) * 128 + (((q & 7) ^ (row & 7)) * 16); }
 
-// Quantize rows 0 .. M - 1 of X (row r at X + src(r) ldx elements) into LDS: codes (rows_chunk) and scales [M][KB]. Chunks
+// Quantize rows 0 .. M - 1 of X (row r at X + r ldx elements) into LDS: codes (rows_chunk) and scales [M][KB]. Chunks
 // past K are zeros. All threads of the workgroup; no barrier.
-template <int DT, class F>
-__device__ __forceinline__ void rows_quant(const void *X, int64_t ldx, int M, int K, int KB, char *codes, float *scales, F src) {
+template <int DT>
+__device__ __forceinline__ void rows_quant(const void *X, int64_t ldx, int M, int K, int KB, char *codes, float *scales) {
   const int sub = threadIdx.x & 15, step = blockDim.x >> 4;  // 16 lanes to a block of 128
   const int n = M * KB;
   for (int u = threadIdx.x >> 4; u < n; u += step) {
@@ -28,7 +28,7 @@ __device__ __forceinline__ void rows_quant(const void *X, int64_t ldx, int M, in
     float x[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = 0.f;
-    if (k < K) fp8_load8<DT>(X, static_cast<int64_t>(src(r)) * ldx + k, x);
+    if (k < K) fp8_load8<DT>(X, static_cast<int64_t>(r) * ldx + k, x);
     float sc;
     const u2 c = fp8_quant8(x, sc);
     *reinterpret_cast<u2 *>(codes + rows_chunk(r, b * 8 + (sub >> 1), KB) + 8 * (sub & 1)) = c;
@@ -42,37 +42,25 @@ struct Fp8RowsArgs {
   int64_t ldx;
 };
 
-template <int MF, int NF, int NW, int D, int XDT, bool HALF>
+template <int NW, int D, int XDT, bool HALF>
 __global__ void __launch_bounds__(64 * NW) k_fp8_rows(const Fp8RowsArgs ra) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr bool LDSX = XDT >= 0;
-  static_assert(NF * MF <= NW && (!LDSX || MF == 1), "shape");
   const Fp8MmArgs &a = ra.m;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int g = lane >> 4, r16 = lane & 15;
-  const int nk = a.KB, n0 = blockIdx.x * 16 * NF;
+  const int nk = a.KB, n0 = blockIdx.x * 16;
   const int tail = a.K & 127;
   // LDS: the waves' sums, then (LDSX) scales and codes of X
   f4 *red = reinterpret_cast<f4 *>(smem);
-  float *xs_lds = reinterpret_cast<float *>(smem + NW * NF * MF * 1024);
-  char *x_lds = smem + NW * NF * MF * 1024 + (a.M * nk * 4 + 127) / 128 * 128;
+  float *xs_lds = reinterpret_cast<float *>(smem + NW * 1024);
+  char *x_lds = smem + NW * 1024 + (a.M * nk * 4 + 127) / 128 * 128;
 
-  const uint8_t *wp[NF];
-  const float *wsp[NF];
-#pragma unroll
-  for (int n = 0; n < NF; ++n) {
-    const int row = min(n0 + 16 * n + r16, a.N - 1);
-    wp[n] = a.W + static_cast<int64_t>(row) * a.K;
-    wsp[n] = a.Ws + static_cast<int64_t>(min(n0 + 16 * n, a.N - 1) >> 7) * nk;
-  }
-  const uint8_t *xp[MF];
-  const float *xsp[MF];
-#pragma unroll
-  for (int m = 0; m < MF; ++m) {
-    const int row = min(16 * m + r16, a.M - 1);
-    xp[m] = LDSX ? nullptr : a.X + static_cast<int64_t>(row) * a.K;
-    xsp[m] = LDSX ? nullptr : a.Xs + row * a.xs_row;
-  }
+  const uint8_t *wp = a.W + static_cast<int64_t>(min(n0 + r16, a.N - 1)) * a.K;
+  const float *wsp = a.Ws + static_cast<int64_t>(n0 >> 7) * nk;
+  const int xrow = min(r16, a.M - 1);
+  const uint8_t *xp = LDSX ? nullptr : a.X + static_cast<int64_t>(xrow) * a.K;
+  const float *xsp = LDSX ? nullptr : a.Xs + xrow * a.xs_row;
   auto frag = [&](const uint8_t *p, int k) {  // the lane's two chunks of block k; zeros past the row's end
     const bool last = tail && k == nk - 1;
     const bool in0 = !last || 16 * g < tail, in1 = !last || 64 + 16 * g < tail;
@@ -90,28 +78,22 @@ __global__ void __launch_bounds__(64 * NW) k_fp8_rows(const Fp8RowsArgs ra) {
     }
     return f;
   };
-  f4 acc[NF][MF];
-#pragma unroll
-  for (int n = 0; n < NF; ++n)
-#pragma unroll
-    for (int m = 0; m < MF; ++m) acc[n][m] = f4{0.f, 0.f, 0.f, 0.f};
+  f4 acc = {0.f, 0.f, 0.f, 0.f};
   bool ready = !LDSX;
   for (int k0 = wave; k0 < nk || !ready; k0 += NW * D) {
-    i8v wf[D][NF];
-    float ws[D][NF];
+    i8v wf[D];
+    float ws[D];
 #pragma unroll
     for (int d = 0; d < D; ++d) {
       const int k = k0 + NW * d;
-      if (k < nk)
-#pragma unroll
-        for (int n = 0; n < NF; ++n) {
-          wf[d][n] = frag(wp[n], k);
-          ws[d][n] = uniform_load(wsp[n], k);
-        }
+      if (k < nk) {
+        wf[d] = frag(wp, k);
+        ws[d] = uniform_load(wsp, k);
+      }
     }
     if constexpr (LDSX) {
       if (!ready) {
-        rows_quant<XDT < 0 ? 0 : XDT>(ra.x, ra.ldx, a.M, a.K, nk, x_lds, xs_lds, [](int r) { return r; });
+        rows_quant<XDT < 0 ? 0 : XDT>(ra.x, ra.ldx, a.M, a.K, nk, x_lds, xs_lds);
         __syncthreads();
         ready = true;
       }
@@ -120,46 +102,35 @@ __global__ void __launch_bounds__(64 * NW) k_fp8_rows(const Fp8RowsArgs ra) {
     for (int d = 0; d < D; ++d) {
       const int k = k0 + NW * d;
       if (k >= nk) break;
+      i8v xf;
+      float xs;
+      if constexpr (LDSX) {
+        const u4 c0 = *reinterpret_cast<const u4 *>(x_lds + rows_chunk(xrow, 8 * k + g, nk));
+        const u4 c1 = *reinterpret_cast<const u4 *>(x_lds + rows_chunk(xrow, 8 * k + 4 + g, nk));
 #pragma unroll
-      for (int m = 0; m < MF; ++m) {
-        i8v xf;
-        float xs;
-        if constexpr (LDSX) {
-          const int row = min(r16, a.M - 1);
-          const u4 c0 = *reinterpret_cast<const u4 *>(x_lds + rows_chunk(row, 8 * k + g, nk));
-          const u4 c1 = *reinterpret_cast<const u4 *>(x_lds + rows_chunk(row, 8 * k + 4 + g, nk));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            xf[j] = static_cast<int>(c0[j]);
-            xf[4 + j] = static_cast<int>(c1[j]);
-          }
-          xs = xs_lds[row * nk + k];
-        } else {
-          xf = frag(xp[m], k);
-          xs = xsp[m][k];
+        for (int j = 0; j < 4; ++j) {
+          xf[j] = static_cast<int>(c0[j]);
+          xf[4 + j] = static_cast<int>(c1[j]);
         }
-#pragma unroll
-        for (int n = 0; n < NF; ++n) {
-          const f4 t = fp8_block<HALF>(wf[d][n], xf);
-          const float s = xs * ws[d][n];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[n][m][i] = fmaf(t[i], s, acc[n][m][i]);
-        }
+        xs = xs_lds[xrow * nk + k];
+      } else {
+        xf = frag(xp, k);
+        xs = xsp[k];
       }
+      const f4 t = fp8_block<HALF>(wf[d], xf);
+      const float s = xs * ws[d];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = fmaf(t[i], s, acc[i]);
     }
   }
-#pragma unroll
-  for (int n = 0; n < NF; ++n)
-#pragma unroll
-    for (int m = 0; m < MF; ++m) red[(wave * NF * MF + n * MF + m) * 64 + lane] = acc[n][m];
+  red[wave * 64 + lane] = acc;
   __syncthreads();
-  if (wave < NF * MF) {  // wave n MF + m adds that fragment over the waves
-    f4 s = red[wave * 64 + lane];
+  if (wave == 0) {  // the sum over the waves
+    f4 s = red[lane];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) s += red[(w * NF * MF + wave) * 64 + lane];
-    const int n = wave / MF, m = wave % MF, row = 16 * m + r16, col = n0 + 16 * n + 4 * g;
-    const int left = row < a.M ? a.N - col : 0;
-    const int64_t at = static_cast<int64_t>(row) * a.ldy + col;
+    for (int w = 1; w < NW; ++w) s += red[w * 64 + lane];
+    const int col = n0 + 4 * g, left = r16 < a.M ? a.N - col : 0;
+    const int64_t at = static_cast<int64_t>(r16) * a.ldy + col;
     switch (a.ydt) {
       case VYBDQ_F32: fp8_put4<VYBDQ_F32>(a, at, left, s); break;
       case VYBDQ_F16: fp8_put4<VYBDQ_F16>(a, at, left, s); break;
@@ -170,20 +141,20 @@ __global__ void __launch_bounds__(64 * NW) k_fp8_rows(const Fp8RowsArgs ra) {
 }
 
 // LDS of a launch: the waves' sums, and X's scales and codes where they are made there
-inline int64_t fp8_rows_lds(int MF, int NF, int NW, bool ldsx, int64_t M, int64_t KB) {
-  return NW * NF * MF * 1024 + (ldsx ? (M * KB * 4 + 127) / 128 * 128 + M * KB * 128 : 0);
+inline int64_t fp8_rows_lds(int NW, bool ldsx, int64_t M, int64_t KB) {
+  return NW * 1024 + (ldsx ? (M * KB * 4 + 127) / 128 * 128 + M * KB * 128 : 0);
 }
 
-template <int MF, int NF, int NW, int D, int XDT, bool HALF>
+template <int NW, int D, int XDT, bool HALF>
 int fp8_rows_launch(const Fp8RowsArgs &a, hipStream_t s) {
-  const int64_t lds = fp8_rows_lds(MF, NF, NW, XDT >= 0, a.m.M, a.m.KB);
+  const int64_t lds = fp8_rows_lds(NW, XDT >= 0, a.m.M, a.m.KB);
   static std::atomic<uint64_t> raised{0};
-  auto *fn = &k_fp8_rows<MF, NF, NW, D, XDT, HALF>;
+  auto *fn = &k_fp8_rows<NW, D, XDT, HALF>;
   if (lds > 64 * 1024) {
     const int rc = ensure_lds_limit(reinterpret_cast<const void *>(fn), 160 * 1024, raised, "fp8 product (few rows)");
     if (rc) return rc;
   }
-  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>((a.m.N + 16 * NF - 1) / (16 * NF))), dim3(64 * NW), lds, s, a);
+  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>((a.m.N + 15) / 16)), dim3(64 * NW), lds, s, a);
   return check_launch("fp8 product (few rows)");
 }
 
