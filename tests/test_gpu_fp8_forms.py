@@ -1,5 +1,7 @@
 """8-bit floating-point weights on the GPU, form by form, on data whose result is known to the last bit or bounded by arithmetic: what
-may lie beside what, and what the e4m3 instruction drops."""
+may lie beside what, what the e4m3 instruction drops, and every kernel of the pipeline going on from tile to tile."""
+
+import math
 
 import numpy as np
 import pytest
@@ -122,3 +124,203 @@ def test_what_the_instruction_drops(dev, rng, monkeypatch, M, K, tile, y, kind):
     assert (np.abs(got - want) <= tol + last(want, tol)).all(), np.abs(got - want).max()
     tol += 0 if y == "f32" else f * fp8.e4m3_loss(xs, wc)
     assert (np.abs(got - exact) <= tol + last(exact, tol)).all()
+
+
+# ---- from tile to tile ------------------------------------------------------------------------------
+
+CUS = 256  # a tile of the pipeline fills a CU's LDS, so this many workgroups take all tiles in turn
+
+
+def force(monkeypatch, rows, splits, M, N, K, y, more=1.0):
+    """Force tiles of `rows` x 256 and splits of K, and see that the product takes them, more than `more` to a workgroup."""
+    nk = -(-K // 128)
+    assert nk // splits >= 4 and (rows < 192 or y in ("f16", "bf16")) and (rows != 192 or K % 128 == 0)
+    assert splits == 1 or (M <= 1024 and splits <= min(nk // 4, 16) and splits * M * N * 4 <= 1 << 26)
+    assert -(-M // rows) * -(-N // 256) * splits > more * CUS
+    monkeypatch.setenv("VYBDQ_FP8_TILE", f"{rows},{splits}")
+
+
+TILES = [(64, 1, 512, "bf16"), (64, 1, 528, "bf16"), (64, 1, 640, "f32"), (64, 1, 656, "f32"), (128, 1, 640, "bf16"), (128, 1, 624, "f16"),
+         (128, 1, 512, "f32"), (128, 1, 528, "f64"), (192, 1, 512, "f16"), (192, 1, 640, "bf16"), (192, 1, 896, "bf16"),
+         (256, 1, 512, "bf16"), (256, 1, 528, "bf16"), (256, 1, 640, "f16"), (256, 1, 1008, "bf16")]
+
+
+@pytest.mark.parametrize("N", [17988, 17989])
+@pytest.mark.parametrize("rows,splits,K,y", TILES)
+def test_product_from_tile_to_tile(dev, rng, monkeypatch, rows, splits, K, y, N):
+    M = 9 * rows + 5
+    force(monkeypatch, rows, splits, M, N, K, y, more=2.5)
+    W, Ws, X, Xs, want = whole_product(rng, M, N, K, dev)
+    r = torch.randint(-99, 100, (M, N), device=dev).to(DT[y])
+    got = ops.gemm_fp8(W, Ws, X, Xs, y_dtype=DT[y], residual=r)
+    assert torch.equal(got, (want + r.double()).to(DT[y]))
+    assert ops.gemm_fp8(W, Ws, X, Xs, y_dtype=DT[y], residual=r, out=r) is r and torch.equal(r, got)
+
+
+@pytest.mark.parametrize("N", [8988, 8990])
+@pytest.mark.parametrize("K", [1776, 1792])  # 14 blocks, 4, 5 and 5 to a split
+@pytest.mark.parametrize("rows,y", [(64, "bf16"), (64, "f32"), (128, "f16"), (128, "f64"), (192, "bf16"), (256, "bf16")])
+def test_split_product_from_tile_to_tile(dev, rng, monkeypatch, rows, y, K, N):
+    if rows == 192 and K % 128:
+        K = 1920  # (that tile takes whole blocks: 5 to each split)
+    M = 600
+    force(monkeypatch, rows, 3, M, N, K, y)
+    W, Ws, X, Xs, want = whole_product(rng, M, N, K, dev)
+    r = torch.randint(-99, 100, (M, N), device=dev).to(DT[y])
+    work = ops.Fp8Workspace([(M, N, K)], dev)
+    work.buf.fill_(0x7f)
+    got = ops.gemm_fp8(W, Ws, X, Xs, y_dtype=DT[y], residual=r, workspace=work)
+    assert torch.equal(got, (want + r.double()).to(DT[y]))
+
+
+def test_scales_far_apart(dev, rng):
+    """The scales' products are formed before they meet a sum: 2^100 and 2^-100 leave nothing behind."""
+    for M, N, K in ((1, 50, 640), (70, 300, 640), (300, 300, 256)):
+        W, Ws, X, Xs, want = whole_product(rng, M, N, K, dev)
+        for e in (100, -100):
+            for y in ("f32", "bf16"):
+                got = ops.gemm_fp8(W, Ws * 2.0 ** e, X, Xs * 2.0 ** -e, y_dtype=DT[y])
+                assert torch.equal(got, want.to(DT[y]))
+
+
+def test_products_of_one_workspace_in_a_graph(dev, rng, monkeypatch):
+    """Split products of two layers, one after the other through one workspace, captured and replayed with eager work between."""
+    M, K = 200, 2048
+    layers, wants = [], []
+    work = ops.Fp8Workspace([(M, K, K)], dev)
+    for _ in range(2):
+        W, Ws = whole(rng, K, K, 2, dev), powers(rng, (K // 128, K // 128), dev)
+        layers.append(ops.Fp8Linear(W, Ws, max_rows=M, workspace=work))
+    step = lambda v: layers[1](layers[0](v, y_dtype=torch.bfloat16), y_dtype=torch.bfloat16, residual=v)
+    x = torch.randn(3, M, K, device=dev).bfloat16()
+    for tile in ("64,3", "128,4"):
+        monkeypatch.setenv("VYBDQ_FP8_TILE", tile)
+        wants, v = [step(x[i]) for i in range(3)], x[0].clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = step(v)
+        for i in (0, 1, 2, 1):
+            v.copy_(x[i])
+            g.replay()
+            assert torch.equal(y, wants[i])
+            assert torch.equal(step(x[0]), wants[0])
+
+
+# ---- the experts' layer -----------------------------------------------------------------------------
+
+def sparse(rng, E, n, k):
+    """Codes [E, n, k] with three entries -1 or 1 to a row: products with whole numbers up to 3 are whole numbers up to 9."""
+    c = np.zeros((E * n, k), np.uint8)
+    first, step = rng.integers(0, k, E * n), rng.integers(1, k // 3, (2, E * n))
+    for at in (first, first + step[0], first + step[0] + step[1]):
+        c[np.arange(E * n), at % k] = np.where(rng.random(E * n) < 0.5, 0x38, 0xb8)
+    return c.reshape(E, n, k), np.ones((E, fp8.blocks(n), fp8.blocks(k)), np.float32)
+
+
+def normal(rng, E, n, k):
+    c = np.stack([fp8.e4m3_encode(np.clip(rng.standard_normal((n, k)) * 110, -448, 448)) for _ in range(E)])
+    return c, (rng.uniform(0.5, 1.5, (E, fp8.blocks(n), fp8.blocks(k))) / (110 * math.sqrt(k))).astype(np.float32)
+
+
+def on(dev, pair):
+    return torch.from_numpy(pair[0]).to(dev).view(E4M3), torch.from_numpy(pair[1]).to(dev)
+
+
+def weights64(pair, e, dev):
+    return torch.from_numpy(fp8.weights(pair[0][e], pair[1][e])).to(dev)
+
+
+def expert(x, gate, up, down, e, limit, out, dev):
+    """float64 output rows [t, H] of expert e, what separates the kernel's float32 rows from them, and their magnitude. No activation
+    may lie so near the border between two codes (4e-6 of it) that float32 could go either way."""
+    g, u = (x @ weights64(p, e, dev).t() for p in (gate, up))
+    g, u = g.clamp(max=limit), u.clamp(-limit, limit)
+    a = (g / (1 + torch.exp(-g)) * u).cpu().numpy()
+    codes, scales = fp8.quant(a)
+    for f in (1 - 4e-6, 1 + 4e-6):
+        c, s = fp8.quant(a * f)
+        assert (c == codes).all() and (s == scales).all()
+    a, w = torch.from_numpy(fp8.activations(codes, scales)).to(dev), weights64(down, e, dev)
+    tol = (130 + scales.shape[1]) * 2.0 ** -23 * (a.abs() @ w.abs().t())
+    if out != "f32":  # the instruction's loss: 2^-10 of the sum of magnitudes, subnormal codes counted as 2^-6
+        size = lambda c, s: np.where(c & 0x7f, np.maximum(np.abs(e4m3_decode(c)), 2.0 ** -6), 0) * s
+        sa = torch.from_numpy(size(codes, scales.astype(np.float64).repeat(128, 1))).to(dev)
+        sw = torch.from_numpy(size(down[0][e], down[1][e].astype(np.float64).repeat(128, 0).repeat(128, 1))).to(dev)
+        tol += 2.0 ** -10 * (sa @ sw.t())
+    y = a @ w.t()
+    return y, tol, y.abs()
+
+
+# tiles of 128 and of 64 rows, three blocks of K (the pipeline's least) and more, experts of a few rows and of many; `one`: all tokens
+# at the same experts
+LAYERS = [(6000, 4, 2, 384, 384, True, 128, ""), (5000, 5, 2, 896, 640, False, 128, ""), (2000, 64, 2, 384, 384, True, 64, ""),
+          (1500, 64, 2, 896, 640, False, 64, ""), (1500, 64, 2, 896, 640, True, 64, "one"), (200, 8, 2, 384, 384, False, 64, "one"),
+          (20, 8, 2, 640, 384, True, 16, "one")]
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("T,E,k,H,I,shared,rows,where", LAYERS)
+def test_layer_from_tile_to_tile(dev, rng, T, E, k, H, I, shared, rows, where, out):
+    n, hit, limit = T * k, min(E, T * k), 7.0
+    assert rows == (16 if n <= 8 * hit else 64 if n <= 64 * hit else 128)
+    logits = rng.standard_normal((T, E)).astype(np.float32) + np.linspace(-1.5, 1.5, E, dtype=np.float32)[rng.permutation(E)]
+    if where == "one":
+        logits[:, 3], logits[:, 6] = 9.0, 8.0
+    idx, w = fp8.route(logits, k, scale=1.5)
+    count = np.bincount(idx.reshape(-1), minlength=E)
+    if where == "" and T > 1000:
+        tiles = (-(-count // rows)).sum() + (-(-T // rows) if shared else 0)
+        assert tiles * (I // 128) > CUS and tiles * -(-H // 256) > CUS
+        assert count.max() > 128 and (rows == 128 or count[count > 0].min() < 32)
+    gate, up, down = sparse(rng, E + 1, I, H), sparse(rng, E + 1, I, H), normal(rng, E + 1, H, I)
+    x = rng.integers(-3, 4, (T, H)).astype(np.float32)
+    cut = [on(dev, (c[:E], s[:E])) for c, s in (gate, up, down)]
+    layer = ops.MoeFp8Layer(*cut, topk=k, shared=[on(dev, (c[E], s[E])) for c, s in (gate, up, down)] if shared else None, scale=1.5,
+                            limit=limit)
+    xd, ld = torch.from_numpy(x).to(dev), torch.from_numpy(logits).to(dev)
+    got, gi, gw = layer(xd, ld, out_dtype=DT[out], routing=True)
+    np.testing.assert_array_equal(gi.cpu().numpy(), idx)
+    np.testing.assert_allclose(gw.cpu().numpy(), w, rtol=2.0 ** -24 * 1.001)
+    want, tol, size = (torch.zeros(T, H, dtype=torch.float64, device=dev) for _ in range(3))
+    wd = gw.double().cpu().numpy()
+    for e in range(E + 1 if shared else E):
+        share = (wd * (idx == e)).sum(1) if e < E else np.ones(T)
+        t = torch.from_numpy(np.nonzero(share)[0]).to(dev)
+        if len(t):
+            f = torch.from_numpy(share).to(dev)[t, None]
+            for total, part in zip((want, tol, size), expert(xd[t].double(), gate, up, down, e, limit, out, dev)):
+                total[t] += f * part
+    tol += (k + 3) * 2.0 ** -24 * size  # the weighted sum, in float32
+    tol += HALF[out] * (want.abs() + tol)
+    err = (got.double() - want).abs()
+    assert (err <= tol).all(), (err / tol).max()
+    assert torch.equal(layer(xd, ld, out_dtype=DT[out]), got)  # whichever workgroup is the faster one
+
+
+@pytest.mark.parametrize("T,times", [(8, 10), (64, 4), (400, 1)])
+def test_activations_of_gate_and_up_keep_their_codes(dev, rng, T, times):
+    """Down is the identity and the one expert's weight 1, so the float32 output is the quantized activation itself. Gate and up on fp16
+    instructions are off by 1e-7 of their rms, exponential, division and products by 3e-7: an activation moves to the next code with
+    a probability of 4e-7 over a step of 1/8 to 1/16 of it, about 1 in 200000 (1 in 5000 had the e4m3 instruction taken the sums).
+    10 of 200000 are allowed, each by one code."""
+    H = I = 512
+    eye = np.zeros((1, H, I), np.uint8)
+    eye[0, np.arange(H), np.arange(H)] = 0x38
+    moved = total = 0
+    for _ in range(times):
+        gate, up = normal(rng, 1, I, H), normal(rng, 1, I, H)
+        layer = ops.MoeFp8Layer(on(dev, gate), on(dev, up), on(dev, (eye, np.ones((1, 4, 4), np.float32))), topk=1, scale=1.0)
+        x = rng.standard_normal((T, H)).astype(np.float32)
+        got, _, w = layer(torch.from_numpy(x).to(dev), torch.zeros(T, 1, device=dev), routing=True)
+        assert (w == 1).all()
+        xq = fp8.activations(*fp8.quant(x))
+        g, u = (xq @ fp8.weights(p[0][0], p[1][0]).T for p in (gate, up))
+        g, u = np.minimum(g, 10.0), np.clip(u, -10.0, 10.0)
+        codes, scales = fp8.quant(g / (1 + np.exp(-g)) * u)
+        scales = scales.astype(np.float64).repeat(128, 1)
+        have = fp8.e4m3_encode(got.double().cpu().numpy() / scales)
+        np.testing.assert_array_equal(e4m3_decode(have) * scales, got.double().cpu().numpy())
+        other = e4m3_decode(have) != e4m3_decode(codes)
+        assert (np.abs((have & 0x7f).astype(int) - (codes & 0x7f).astype(int))[other] == 1).all()
+        moved, total = moved + other.sum(), total + other.size
+    assert moved <= max(1, 10 * total // 200000), (moved, total)
