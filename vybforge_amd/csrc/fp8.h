@@ -92,6 +92,8 @@ inline bool fp8_overlap(Fp8Span a, Fp8Span b) {
   return false;
 }
 
+constexpr int64_t kFp8QuantBlocks = (int64_t(1) << 28) - 16;  // most blocks of a quantizer's launch: 16 threads each, below 2^32 in all
+
 int fp8_quant_rows(const void *X, int x_dt, int64_t M, int64_t K, int64_t ldx, uint8_t *Xq, float *Xs, hipStream_t s);
 
 }  // namespace vybdq

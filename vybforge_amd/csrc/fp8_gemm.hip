@@ -259,7 +259,7 @@ extern "C" int vybdq_linear_fp8(uint64_t W, uint64_t Ws, uint64_t X, int x_dt, i
   const int rc = fp8_check(__func__, M, N, K, W, Ws, Y, y_dt, ldy, RS);
   if (rc || M == 0) return rc;
   VYBDQ_REQUIRE(X, VYBDQ_ERR_ARG, "null buffer");
-  VYBDQ_REQUIRE(M * ((K + 127) / 128) < (int64_t(1) << 28), VYBDQ_ERR_SHAPE, "M ceil(K / 128) must be below 2^28");
+  VYBDQ_REQUIRE(M * ((K + 127) / 128) <= kFp8QuantBlocks, VYBDQ_ERR_SHAPE, "M ceil(K / 128) must be at most 2^28 - 16");
   VYBDQ_REQUIRE(M == 1 || ldx >= K, VYBDQ_ERR_SHAPE, "ldx is smaller than a row");
   VYBDQ_REQUIRE(X % 16 == 0 && (M == 1 || ldx * dt_size(x_dt) % 16 == 0), VYBDQ_ERR_ALIGN, "rows of X must be 16-byte aligned");
   VYBDQ_REQUIRE(ws && ws % 256 == 0 && ws_bytes >= vybdq_linear_fp8_workspace_size(M, N, K), VYBDQ_ERR_WORKSPACE,

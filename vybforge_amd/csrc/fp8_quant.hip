@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(256) k_fp8_quant(const void *__restrict__ X, u
   if ((threadIdx.x & 15) == 0) Xs[u] = sc;
 }
 
-// M ceil(K / 128) below 2^28: a grid holds less than 2^32 threads (the callers check)
+// M ceil(K / 128) is at most kFp8QuantBlocks (the callers check)
 int fp8_quant_rows(const void *X, int x_dt, int64_t M, int64_t K, int64_t ldx, uint8_t *Xq, float *Xs, hipStream_t s) {
   const int64_t KB = (K + 127) / 128, blocks = M * KB;
   const dim3 grid(static_cast<unsigned>((blocks + 15) / 16));
@@ -45,8 +45,8 @@ extern "C" int vybdq_quant_fp8(uint64_t X, int x_dt, int64_t ldx, uint64_t Xq, u
   VYBDQ_REQUIRE(dt_valid_in(x_dt), VYBDQ_ERR_ARG, "x_dt must be F32, F16 or BF16");
   VYBDQ_REQUIRE(M >= 0 && K >= 16 && K % 16 == 0 && K < (int64_t(1) << 23), VYBDQ_ERR_SHAPE,
                 "M must not be negative, K must be a multiple of 16 in 16 .. 2^23 - 16");
-  VYBDQ_REQUIRE(M < (int64_t(1) << 28) && M * ((K + 127) / 128) < (int64_t(1) << 28), VYBDQ_ERR_SHAPE,
-                "M ceil(K / 128) must be below 2^28");
+  VYBDQ_REQUIRE(M <= kFp8QuantBlocks && M * ((K + 127) / 128) <= kFp8QuantBlocks, VYBDQ_ERR_SHAPE,
+                "M ceil(K / 128) must be at most 2^28 - 16");
   if (M == 0) return VYBDQ_OK;
   VYBDQ_REQUIRE(X && Xq && Xs, VYBDQ_ERR_ARG, "null buffer");
   VYBDQ_REQUIRE(M == 1 || ldx >= K, VYBDQ_ERR_SHAPE, "ldx is smaller than a row");
