@@ -324,3 +324,108 @@ def test_activations_of_gate_and_up_keep_their_codes(dev, rng, T, times):
         assert (np.abs((have & 0x7f).astype(int) - (codes & 0x7f).astype(int))[other] == 1).all()
         moved, total = moved + other.sum(), total + other.size
     assert moved <= max(1, 10 * total // 200000), (moved, total)
+
+
+def small_layer(dev, rng, E, H, I, k, shared=True, **kw):
+    """A layer, its host pairs (E + 1 experts, the last one shared) and whole-number tokens for it."""
+    pairs = sparse(rng, E + 1, I, H), sparse(rng, E + 1, I, H), normal(rng, E + 1, H, I)
+    layer = ops.MoeFp8Layer(*[on(dev, (c[:E], s[:E])) for c, s in pairs], topk=k, limit=7.0,
+                            shared=[on(dev, (c[E], s[E])) for c, s in pairs] if shared else None, **kw)
+    return layer, pairs, lambda T: torch.from_numpy(rng.integers(-3, 4, (T, H)).astype(np.float32)).to(dev)
+
+
+@pytest.mark.parametrize("T", [2, 30, 200])
+def test_layer_inputs_of_every_type(dev, rng, T):
+    """Tokens and logits that every type holds give the same bits in every type; 16-bit outputs are one sum, rounded to each."""
+    layer, _, tokens = small_layer(dev, rng, 8, 384, 256, 3)
+    x, logits = tokens(T), torch.randn(T, 8, device=dev).bfloat16()
+    for out in ("f32", "f16", "bf16"):
+        want = layer(x, logits.float(), out_dtype=DT[out])
+        for a in (torch.float32, torch.float16, torch.bfloat16):
+            for b in (torch.float64, torch.float32, torch.float16, torch.bfloat16):
+                if b != torch.float16 or (logits.to(b).bfloat16() == logits).all():
+                    assert torch.equal(layer(x.to(a), logits.to(b), out_dtype=DT[out]), want), (a, b)
+    h, b = (layer(x, logits, out_dtype=DT[d]).double() for d in ("f16", "bf16"))
+    assert ((h - b).abs() <= (2.0 ** -8 + 2.0 ** -10) * b.abs() + 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("T", [1, 5, 40])
+def test_layer_gives_either_part_of_its_routing(dev, rng, T):
+    layer, _, tokens = small_layer(dev, rng, 8, 256, 128, 2, shared=False, scale=1.5)
+    x, logits = tokens(T), torch.randn(T, 8, device=dev)
+    want, idx, w = layer(x, logits, routing=True)
+    ws, n = layer._workspace(T)
+    for give_idx, give_w in ((True, False), (False, True), (False, False)):
+        out, i, v = torch.empty_like(want), torch.full_like(idx, -7), torch.full_like(w, -7)
+        ops.call("vybdq_moe_forward_fp8", x.data_ptr(), _lib.F32, logits.data_ptr(), _lib.F32, 0, *layer._w, out.data_ptr(), _lib.F32,
+                 i.data_ptr() if give_idx else 0, v.data_ptr() if give_w else 0, T, 256, 128, 8, 2, 1.5, 7.0, 0, 1, 1, 1, 2, ws, n, stream())
+        assert torch.equal(out, want)
+        assert torch.equal(i, idx if give_idx else torch.full_like(idx, -7))
+        assert torch.equal(v, w if give_w else torch.full_like(w, -7))
+
+
+@pytest.mark.parametrize("E,k,kw", [(1024, 64, {}), (1000, 8, dict(groups=8, top_groups=3)), (96, 1, {}), (1024, 1, dict(groups=64, top_groups=9))])
+@pytest.mark.parametrize("T", [1, 2, 9])
+def test_layer_of_many_experts(dev, rng, E, k, kw, T):
+    layer, pairs, tokens = small_layer(dev, rng, E, 128, 128, k, score="softmax", renorm=False, scale=2.0, **kw)
+    x, logits = tokens(T), rng.standard_normal((T, E)).astype(np.float32)
+    idx, w = fp8.route(logits, k, None, 2.0, softmax=True, renorm=False, **kw)
+    got, gi, gw = layer(x, torch.from_numpy(logits).to(dev), routing=True)
+    np.testing.assert_array_equal(gi.cpu().numpy(), idx)
+    np.testing.assert_allclose(gw.cpu().numpy(), w, rtol=2.0 ** -24 * 1.001)
+    want, tol, size = expert(x.double(), *pairs, E, 7.0, "f32", dev)
+    for t in range(T):
+        for s in range(k):
+            parts = expert(x[t:t + 1].double(), *pairs, int(idx[t, s]), 7.0, "f32", dev)
+            for total, part in zip((want, tol, size), parts):
+                total[t] += float(gw[t, s]) * part[0]
+    tol = tol + (k + 3) * 2.0 ** -24 * size
+    assert ((got.double() - want).abs() <= tol + HALF["f32"] * (want.abs() + tol)).all()
+
+
+def test_layers_on_two_streams_at_once(dev, rng):
+    """Two layers with workspaces of their own, call by call beside each other; then one of them moves to the other's stream and
+    grows there."""
+    made = [small_layer(dev, rng, 8, 512, 384, 2) for _ in range(2)]
+    xs = [[(tokens(T), torch.randn(T, 8, device=dev)) for T in (3, 100, 700, 50)] for _, _, tokens in made]
+    wants = [[layer(*a) for a in x] for (layer, _, _), x in zip(made, xs)]
+    fresh = [ops.MoeFp8Layer(*zip(layer.tensors[0:6:2], layer.tensors[1:6:2]), topk=2, limit=7.0,
+                             shared=list(zip(layer.tensors[6::2], layer.tensors[7::2]))) for layer, _, _ in made]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for j in range(4):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(fresh[i](*xs[i][j]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g, w in zip(got, wants) for a, b in zip(g, w))
+    layer = ops.MoeFp8Layer(*zip(made[0][0].tensors[0:6:2], made[0][0].tensors[1:6:2]), topk=2, limit=7.0,
+                            shared=list(zip(made[0][0].tensors[6::2], made[0][0].tensors[7::2])))
+    for j, s in ((1, streams[0]), (2, streams[1]), (3, streams[0])):
+        for other in streams:
+            s.wait_stream(other)
+        with torch.cuda.stream(s):
+            y = layer(*xs[0][j])
+            torch.empty(layer._ws.numel() // 2, dtype=torch.uint8, device=dev).fill_(0x7f)  # (where a freed workspace may have been)
+        s.synchronize()
+        assert torch.equal(y, wants[0][j])
+
+
+@pytest.mark.parametrize("M", [1, 3, 30, 140])
+def test_linear_with_every_output(dev, rng, M):
+    """Float64 outputs and residuals, one row of a wider matrix, an output in place of the residual."""
+    N, K = 201, 656
+    W, Ws, Xq, Xs, _ = whole_product(rng, M, N, K, dev)
+    x = values(Xq, torch.ones_like(Xs), 1)
+    want = x.double() @ values(W, Ws, 128).double().t()
+    layer = ops.Fp8Linear(W, Ws, max_rows=M)
+    wide = torch.full((M, 1024), 77.0, device=dev)
+    wide[:, 16:16 + K] = x
+    for y in ("f64", "f32", "f16", "bf16"):
+        r = torch.randint(-9, 10, (M, N), device=dev).to(DT[y])
+        for v in (wide[:, 16:16 + K], wide[:, 16:16 + K].half(), wide[M - 1:, 16:16 + K]):
+            rows = slice(M - len(v), M)
+            out = r[rows].clone()
+            assert layer(v, y_dtype=DT[y], residual=out, out=out) is out
+            assert torch.equal(out, (want[rows] + r[rows].double()).to(DT[y]))
