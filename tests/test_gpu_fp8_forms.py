@@ -9,8 +9,10 @@ import torch
 
 from oracle import fp8
 from oracle.kvcache import e4m3_decode
+from tests import st_writer
 from tests.e4m3_cases import hard_codes
 from vybforge_amd import _lib, ops
+from vybforge_amd.safetensors import Checkpoint
 
 pytestmark = pytest.mark.gpu
 
@@ -429,3 +431,28 @@ def test_linear_with_every_output(dev, rng, M):
             out = r[rows].clone()
             assert layer(v, y_dtype=DT[y], residual=out, out=out) is out
             assert torch.equal(out, (want[rows] + r[rows].double()).to(DT[y]))
+
+
+def test_layer_from_a_checkpoint(dev, rng, tmp_path):
+    """Experts that a checkpoint holds one tensor each, copied into stacked arrays as the integration guide has it."""
+    E, H, I = 4, 256, 128
+    pairs = [normal(rng, E, n, m) for n, m in ((I, H), (I, H), (H, I))]
+    tensors = []
+    for (c, s), proj in zip(pairs, ("gate_proj", "up_proj", "down_proj")):
+        for e in range(E):
+            tensors.append((f"mlp.experts.{e}.{proj}.weight", "F8_E4M3", list(c[e].shape), c[e].tobytes()))
+            tensors.append((f"mlp.experts.{e}.{proj}.scale", s[e]))
+    st_writer.write(tmp_path / "model.safetensors", tensors)
+    ckpt = Checkpoint(tmp_path)
+
+    def stacked(proj, N, K):
+        codes = torch.empty(E, N, K, dtype=E4M3, device=dev)
+        scales = torch.empty(E, N // 128, K // 128, device=dev)
+        for e in range(E):
+            codes[e].copy_(ckpt.to_device(f"mlp.experts.{e}.{proj}.weight", dev))
+            scales[e].copy_(ckpt.to_device(f"mlp.experts.{e}.{proj}.scale", dev))
+        return codes, scales
+
+    layer = ops.MoeFp8Layer(stacked("gate_proj", I, H), stacked("up_proj", I, H), stacked("down_proj", H, I), topk=2)
+    x, logits = torch.randn(9, H, device=dev), torch.randn(9, E, device=dev)
+    assert torch.equal(layer(x, logits), ops.MoeFp8Layer(*[on(dev, p) for p in pairs], topk=2)(x, logits))

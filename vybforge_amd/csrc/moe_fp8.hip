@@ -22,8 +22,8 @@ struct MoeFp8Lists {
   int4 *tiles;
 };
 
-// Few tokens (at most 64 rows) in one launch: workgroup 0 routes them and lists rows and tiles, the others quantize x (one token of
-// 6144 over 256 experts: 10 us against 18 of three launches).
+// Few tokens (at most 8, and 64 rows) in one launch: workgroup 0 routes them and lists rows and tiles, the others quantize x (one
+// token of 6144 over 256 experts: 7.1 to 8.3 us; quantizer, router and bucketing by themselves 2.0, 5.4 and 4.6, and two gaps).
 template <bool SOFTMAX, bool BIAS, int TOP, int ENT>
 __global__ void __launch_bounds__(256) k_moe_fp8_front(const RouteArgs r, const void *__restrict__ x, int x_dt, int H,
                                                        uint8_t *__restrict__ xq, float *__restrict__ xs, int BM, int shared,
@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256) k_moe_fp8_front(const RouteArgs r, const 
 
 // Many tokens, one workgroup: rows per expert, the first row and tile of each (thread e: expert e), then every (token, slot)'s row.
 // A row's place among its expert's comes from an atomic cursor: no result depends on it, each row is computed from its own token
-// alone and added through pos. 32768 rows: 21 us (70 with 256 threads).
+// alone and added through pos. One CU, so in proportion to the rows: 384 rows 4.6 us, 32768 rows 21 to 29 (70 with 256 threads).
 __global__ void __launch_bounds__(1024) k_moe_fp8_bucket(const int *__restrict__ idx, int T, int topk, int E, int BM, int shared,
                                                          const MoeFp8Lists l) {
   __shared__ int cnt[1024], wave_rows[16], wave_tiles[16];

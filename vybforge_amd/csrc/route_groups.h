@@ -76,7 +76,7 @@ __device__ __forceinline__ double wave_f64(double v, F op) {
 }
 
 // The same selection as route_select, for up to 8 entries a lane: each lane sorts its entries once (best first, ties to the lower
-// id), so a round compares the lanes' first entries and the winner's lane moves up (16384 tokens over 160
+// id; Batcher's odd-even merge), so a round compares the lanes' first entries and the winner's lane moves up (16384 tokens over 160
 // experts in groups, 6 to a token: 25.6 us with the entries compared anew each round, 22.3 to 23.7 so).
 template <int ENT>
 __device__ __forceinline__ uint32_t route_select_sorted(uint64_t (&key)[ENT], uint32_t (&eid)[ENT], int topk) {
