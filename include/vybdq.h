@@ -620,8 +620,9 @@ int vybdq_quant_fp8(uint64_t X, int x_dt, int64_t ldx, uint64_t Xq, uint64_t Xs,
    are float32. Scales are any float32 whose products Xs Ws float32 holds: it rounds them once, and one past its range makes the
    outputs infinite or NaN. For F16 and BF16 outputs a block's sum comes from the e4m3 matrix instruction, which cuts the products of
    every eight neighbouring k below 2^-13 of the largest of the eight, a subnormal code counted as 2^-6: 1.4e-5 of the sum's rms for
-   normal data, at most 2^-10 of the sum of the products' magnitudes so counted. (An F32 output has no such loss.) W and Xq 16-byte
-   aligned; Y must not overlap X, W, Ws or RS (RS may be Y itself), nor the part of ws that is used any of these.
+   normal data, 6e-5 where a few columns of X are thirty times the others, at most 2^-10 of the sum of the products' magnitudes so
+   counted. (An F32 output has no such loss.) W and Xq 16-byte aligned; Y must not overlap X, W, Ws or RS (RS may be Y itself), nor
+   the part of ws that is used any of these.
    ceil(M / 128) ceil(N / 128) below 2^22, M and N below 2^24.
    ws: 256-byte aligned, any contents, or 0; with vybdq_gemm_fp8_workspace_size(M, N, K) bytes (-1: unsupported; the size covers
    every smaller M; at most 64 MiB) calls whose tiles do not fill the GPU split K and add float32 sums in a second launch (last

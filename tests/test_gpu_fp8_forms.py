@@ -434,7 +434,7 @@ def test_linear_with_every_output(dev, rng, M):
 
 
 def test_layer_from_a_checkpoint(dev, rng, tmp_path):
-    """Experts that a checkpoint holds one tensor each, copied into stacked arrays as the integration guide has it."""
+    """Experts that a checkpoint holds one tensor each, copied into stacked arrays."""
     E, H, I = 4, 256, 128
     pairs = [normal(rng, E, n, m) for n, m in ((I, H), (I, H), (H, I))]
     tensors = []
