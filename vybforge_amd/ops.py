@@ -857,7 +857,8 @@ def gemm_fp8(W, Ws, Xq, Xs, y_dtype=torch.float32, residual=None, out=None, work
     """Y [M, N] = X W^T (+ residual) of e4m3 codes Xq [M, K], W [N, K] and their scales Xs [M, ceil(K / 128)],
     Ws [ceil(N / 128), ceil(K / 128)] (vybdq_gemm_fp8).
 
-    workspace: an Fp8Workspace (K split across workgroups) or None for the unsplit product."""
+    workspace: an Fp8Workspace (K split across workgroups) or None for the unsplit product. float16 and bfloat16 outputs take their
+    sums from the e4m3 matrix instruction, which drops a little of them (vybdq_gemm_fp8 says how much); float32 drops nothing."""
     N, K = _fp8_matrix(W, Ws, (), "W")
     M = Xq.shape[0]
     _need(Xq.dim() == 2 and Xq.shape[1] == K and Xq.dtype == E4M3, f"Xq must be float8_e4m3fn [M, {K}]")
@@ -891,7 +892,7 @@ class Fp8Workspace:
 
 class Fp8Linear:
     """x [M, K] -> y [M, N] through a matrix of e4m3 codes [N, K] with float32 scales [ceil(N / 128), ceil(K / 128)]: x is
-    quantized (quant_fp8) and multiplied (vybdq_linear_fp8), with a workspace for up to max_rows rows: its own, or an
+    quantized (quant_fp8) and multiplied (vybdq_linear_fp8; outputs as gemm_fp8's), with a workspace for up to max_rows rows: its own, or an
     Fp8Workspace that holds (max_rows, N, K). Calls that use one workspace must not overlap."""
 
     def __init__(self, W, Ws, max_rows=64, workspace=None):
